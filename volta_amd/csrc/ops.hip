@@ -1,0 +1,670 @@
+// Entry points of the feed-forward operators (include/volta_ops.h): argument
+// checks, workspaces, and the launches of a call in order.  Nothing here
+// keeps state between calls.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <exception>
+#include <string>
+#include <vector>
+
+#include "../../include/volta_ops.h"
+#include "../../include/volta_train.h"
+#include "ops_gemm.h"
+#include "ops_rows.h"
+#include "rt_lower.h"
+
+namespace volta {
+namespace ops {
+namespace {
+
+constexpr int64_t kMaxLd = int64_t{1} << 21;
+constexpr int64_t kMaxRows = int64_t{1} << 30;
+
+struct Refused {
+  std::string what;
+};
+[[noreturn]] void refuse(const std::string& m) { throw Refused{m}; }
+
+int elem_bytes(int type) { return type == VOLTA_OP_F32 ? 4 : type == VOLTA_OP_E4M3 ? 1 : 2; }
+int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+
+// Runs a call's body; every way it can end becomes the entry point's return.
+template <typename F>
+int32_t guarded(const char* call, F body) {
+  try {
+    body();
+    return 0;
+  } catch (const Refused& r) {
+    try { rt_set_error(std::string(call) + ": " + r.what); } catch (...) {}
+  } catch (const std::exception& e) {
+    try { rt_set_error(std::string(call) + ": " + e.what()); } catch (...) {}
+  } catch (...) {
+  }
+  return -1;
+}
+
+void check_hip(hipError_t e, const char* what) {
+  if (e != hipSuccess) refuse(std::string(what) + " launch failed: " + hipGetErrorString(e));
+}
+
+hipStream_t stream_of(void* stream) {
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  // NULL and the runtime's two named streams are the current device's
+  if ((uintptr_t)stream > 2) {
+    hipDevice_t of = 0;
+    int cur = 0;
+    hipError_t e = hipStreamGetDevice(st, &of);
+    if (e == hipSuccess) e = hipGetDevice(&cur);
+    if (e != hipSuccess) refuse(std::string("the stream's device: ") + hipGetErrorString(e));
+    if (of != cur)
+      refuse("the stream is of device " + std::to_string(of) + ", the current device is " + std::to_string(cur));
+  }
+  return st;
+}
+
+// A matrix of a call: `rows` x `cols` elements of `bytes`, `ld` apart.
+struct Mat {
+  const char* name;
+  const void* p;
+  int64_t rows, cols, ld;
+  int bytes;
+  bool out;
+  int64_t span() const { return p && rows > 0 ? ((rows - 1) * ld + cols) * bytes : 0; }
+  bool vec(int64_t n) const { return !p || ((uintptr_t)p % (n * bytes) == 0 && (rows <= 1 || ld % n == 0)); }
+};
+
+void check_dims(const char* what, int64_t n, int64_t lo, int64_t hi) {
+  if (n < lo || n > hi)
+    refuse(std::string(what) + " is " + std::to_string(n) + ", must be " + std::to_string(lo) + " to " +
+           std::to_string(hi));
+}
+int64_t ld_of(const char* what, int64_t ld, int64_t cols) {
+  if (ld == 0) ld = cols;
+  if (ld < cols || ld > kMaxLd)
+    refuse(std::string(what) + " is " + std::to_string(ld) + ", must be " + std::to_string(cols) + " to " +
+           std::to_string(kMaxLd) + " (0: packed)");
+  return ld;
+}
+void check_type(int type) {
+  if (type != VOLTA_OP_F32 && type != VOLTA_OP_BF16 && type != VOLTA_OP_F16)
+    refuse("type is " + std::to_string(type) + ", must be F32, BF16 or F16");
+}
+void check_act(int act) {
+  if (act != VOLTA_OP_ACT_NONE && (act < VOLTA_ACT_RELU || act > VOLTA_ACT_GELU))
+    refuse("act is " + std::to_string(act) + ", must be none (-1) or relu .. gelu (0 .. 5)");
+}
+
+struct Shared {  // two matrices of a call that may be the same one
+  const void *a, *b;
+};
+
+// Alignment of every pointer, and no output over anything else but where
+// `same` allows the two to be one matrix.
+void check_mats(const std::vector<Mat>& mats, const std::vector<Shared>& same, const void* workspace = nullptr,
+                int64_t workspace_bytes = 0) {
+  for (const Mat& m : mats)
+    if (m.p && (uintptr_t)m.p % m.bytes != 0) refuse(std::string(m.name) + " is not aligned to its element");
+  auto meet = [](const void* p, int64_t n, const void* q, int64_t k) {
+    const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
+    return n > 0 && k > 0 && a < b + (uintptr_t)k && b < a + (uintptr_t)n;
+  };
+  // Column ranges of one wider matrix: the later one starts behind the
+  // earlier one's columns and ends before its next row.
+  auto beside = [](const Mat& a, const Mat& b) {
+    const Mat &lo = (uintptr_t)a.p <= (uintptr_t)b.p ? a : b, &hi = &lo == &a ? b : a;
+    const int64_t apart = (int64_t)((uintptr_t)hi.p - (uintptr_t)lo.p);
+    if (a.ld != b.ld || a.bytes != b.bytes || apart % a.bytes != 0) return false;
+    const int64_t col = apart / a.bytes % a.ld;
+    return col >= lo.cols && col + hi.cols <= a.ld;
+  };
+  for (size_t i = 0; i < mats.size(); ++i) {
+    for (size_t j = i + 1; j < mats.size(); ++j) {
+      const Mat &a = mats[i], &b = mats[j];
+      if (!a.out && !b.out) continue;
+      if (!meet(a.p, a.span(), b.p, b.span()) || beside(a, b)) continue;
+      bool ok = false;
+      for (const Shared& s : same)
+        if (((s.a == a.p && s.b == b.p) || (s.a == b.p && s.b == a.p)) && a.p == b.p && a.ld == b.ld &&
+            a.cols == b.cols && a.bytes == b.bytes)
+          ok = true;
+      if (!ok) refuse(std::string(a.name) + " and " + b.name + " overlap");
+    }
+    if (meet(mats[i].p, mats[i].span(), workspace, workspace_bytes))
+      refuse(std::string(mats[i].name) + " overlaps the workspace");
+  }
+}
+void need(const void* p, const char* name) {
+  if (!p) refuse(std::string(name) + " is NULL");
+}
+void check_workspace(const void* p, int64_t have, int64_t want) {
+  if (want == 0) return;
+  if (!p || have < want)
+    refuse("the workspace holds " + std::to_string(p ? have : 0) + " bytes, needed are " + std::to_string(want));
+  if ((uintptr_t)p % 16 != 0) refuse("the workspace is not 16-byte aligned");
+}
+
+hipError_t gemm(int type, int layout, int kind, const OpPlan& plan, const OpGemm& g, hipStream_t st) {
+  return type == VOLTA_OP_F32    ? op_gemm_f32(layout, kind, plan, g, st)
+         : type == VOLTA_OP_BF16 ? op_gemm_bf16(layout, kind, plan, g, st)
+                                 : op_gemm_f16(layout, kind, plan, g, st);
+}
+
+// Rows of 16-byte chunks: what the direct loads need.
+bool chunked(const Mat& m) {
+  const int64_t e = 16 / m.bytes;
+  return m.vec(e) && m.cols % e == 0;
+}
+
+// The shape of a product: a plan depends on it and on `direct`, which the
+// pointers decide; the workspace holds either plan's partial sums.
+struct Shape {
+  int layout, kind;
+  int64_t M, N, K;
+  int pieces, outputs;
+};
+OpPlan plan_of(int type, const Shape& s, bool direct) {
+  return op_gemm_plan(elem_bytes(type), s.layout, s.kind, s.M, s.N, s.K, s.pieces, s.outputs, direct);
+}
+int64_t partial_bytes(int type, const Shape& s) {
+  int64_t n = 0;
+  for (bool direct : {false, true})
+    n = std::max(n, op_gemm_partial_bytes(plan_of(type, s, direct), s.kind, s.M, s.N, s.outputs));
+  return align256(n);
+}
+
+// One product of a call.
+void product(int type, const Shape& s, const std::vector<Mat>& ps, const std::vector<Mat>& qs, OpEpilogue epi,
+             const std::vector<Mat>& written, float* partial, hipStream_t st, const char* what) {
+  if (s.M == 0 || s.N == 0) return;
+  OpGemm g{};
+  bool direct = true;
+  for (size_t i = 0; i < 2; ++i) {
+    const Mat &p = ps[std::min(i, ps.size() - 1)], &q = qs[std::min(i, qs.size() - 1)];
+    g.p[i] = p.p;
+    g.q[i] = q.p;
+    direct = direct && chunked(p) && chunked(q);
+  }
+  g.ld_p = ps[0].ld;
+  g.ld_q = qs[0].ld;
+  g.M = (int32_t)s.M;
+  g.N = (int32_t)s.N;
+  g.K = (int32_t)s.K;
+  g.pieces = s.pieces;
+  g.outputs = s.outputs;
+  g.direct = direct;
+  g.partial = partial;
+  const OpPlan plan = plan_of(type, s, direct);
+  // a grid has fewer than 2^32 threads
+  if (op_gemm_blocks(plan, s.kind, s.M, s.N) > (int64_t{1} << 22)) refuse("rows * columns of a product are too many");
+  epi.vec = 1;
+  for (const Mat& m : written) epi.vec = epi.vec && m.vec(4);
+  g.epi = epi;
+  check_hip(gemm(type, s.layout, s.kind, plan, g, st), what);
+}
+
+// ---------------------------------------------------------------------------
+struct Linear {
+  volta_op_linear d;
+  Shape fwd, dx, dw;
+  int strips;
+  int64_t part_fwd, dp_bytes, sums_bytes, part_bwd;
+  int64_t forward_bytes() const { return part_fwd; }
+  int64_t backward_bytes() const { return dp_bytes + sums_bytes + part_bwd; }
+};
+
+Linear linear_of(const volta_op_linear* in) {
+  need(in, "the description");
+  Linear l{};
+  volta_op_linear& d = l.d;
+  d = *in;
+  check_type(d.type);
+  check_act(d.act);
+  check_dims("rows", d.rows, 0, kMaxRows);
+  check_dims("inputs", d.inputs, 1, kMaxLd);
+  check_dims("outputs", d.outputs, 1, kMaxLd);
+  d.ld_x = ld_of("ld_x", d.ld_x, d.inputs);
+  d.ld_w = ld_of("ld_w", d.ld_w, d.outputs);
+  d.ld_y = ld_of("ld_y", d.ld_y, d.outputs);
+  d.ld_residual = ld_of("ld_residual", d.ld_residual, d.outputs);
+  d.ld_pre = ld_of("ld_pre", d.ld_pre, d.outputs);
+  d.ld_dx = ld_of("ld_dx", d.ld_dx, d.inputs);
+  d.ld_dw = ld_of("ld_dw", d.ld_dw, d.outputs);
+  l.fwd = {OP_NN, OP_LINEAR, d.rows, d.outputs, d.inputs, 1, 1};
+  l.dx = {OP_NT, OP_STORE, d.rows, d.inputs, d.outputs, 1, 1};
+  l.dw = {OP_TN, OP_STORE, d.inputs, d.outputs, d.rows, 1, 1};
+  l.part_fwd = partial_bytes(d.type, l.fwd);
+  l.dp_bytes = d.act == VOLTA_OP_ACT_NONE ? 0 : align256(d.rows * d.outputs * elem_bytes(d.type));
+  l.strips = act_grad_strips(d.type, d.rows, d.outputs);
+  l.sums_bytes = align256(4 * l.strips * d.outputs);
+  l.part_bwd = std::max(partial_bytes(d.type, l.dx), partial_bytes(d.type, l.dw));
+  return l;
+}
+
+struct Gated {
+  volta_op_gated d;
+  Shape fwd, dx, dw;
+  int strips;
+  int64_t part_fwd, d_bytes, sums_bytes, part_bwd;
+  int64_t forward_bytes() const { return part_fwd; }
+  int64_t backward_bytes() const { return 2 * d_bytes + 2 * sums_bytes + part_bwd; }
+};
+
+Gated gated_of(const volta_op_gated* in) {
+  need(in, "the description");
+  Gated l{};
+  volta_op_gated& d = l.d;
+  d = *in;
+  check_type(d.type);
+  check_act(d.act);
+  check_dims("rows", d.rows, 0, kMaxRows);
+  check_dims("inputs", d.inputs, 1, kMaxLd);
+  check_dims("hidden", d.hidden, 1, kMaxLd);
+  d.ld_x = ld_of("ld_x", d.ld_x, d.inputs);
+  d.ld_w = ld_of("ld_w", d.ld_w, d.hidden);
+  d.ld_h = ld_of("ld_h", d.ld_h, d.hidden);
+  d.ld_pre = ld_of("ld_pre", d.ld_pre, d.hidden);
+  d.ld_dx = ld_of("ld_dx", d.ld_dx, d.inputs);
+  d.ld_dw = ld_of("ld_dw", d.ld_dw, d.hidden);
+  l.fwd = {OP_NN, OP_GATED, d.rows, d.hidden, d.inputs, 1, 1};
+  l.dx = {OP_NT, OP_STORE, d.rows, d.inputs, d.hidden, 2, 1};
+  l.dw = {OP_TN, OP_STORE, d.inputs, d.hidden, d.rows, 1, 2};
+  l.part_fwd = partial_bytes(d.type, l.fwd);
+  l.d_bytes = align256(d.rows * d.hidden * elem_bytes(d.type));
+  l.strips = act_grad_strips(d.type, d.rows, d.hidden);
+  l.sums_bytes = align256(4 * l.strips * d.hidden);
+  l.part_bwd = std::max(partial_bytes(d.type, l.dx), partial_bytes(d.type, l.dw));
+  return l;
+}
+
+struct Norm {
+  volta_op_rms_norm d;
+  int partial_rows;
+  int64_t backward_bytes() const { return align256(4 * partial_rows * d.cols); }
+};
+
+Norm norm_of(const volta_op_rms_norm* in, bool backward) {
+  need(in, "the description");
+  Norm n{};
+  volta_op_rms_norm& d = n.d;
+  d = *in;
+  check_type(d.type);
+  check_dims("rows", d.rows, 0, kMaxRows);
+  check_dims("cols", d.cols, 1, kMaxLd);
+  if (!(d.eps >= 0.0f) || !std::isfinite(d.eps)) refuse("eps is negative or not finite");
+  if (!backward) {
+    if (d.out_type != d.type && d.out_type != VOLTA_OP_E4M3) refuse("out_type must be type or E4M3");
+    if (d.group != 0 && (d.out_type != VOLTA_OP_E4M3 || d.group != 128))
+      refuse("group is " + std::to_string(d.group) + ", must be 0, or 128 with out_type E4M3");
+  }
+  d.ld_x = ld_of("ld_x", d.ld_x, d.cols);
+  d.ld_residual = ld_of("ld_residual", d.ld_residual, d.cols);
+  d.ld_sum = ld_of("ld_sum", d.ld_sum, d.cols);
+  d.ld_y = ld_of("ld_y", d.ld_y, d.cols);
+  d.ld_dx = ld_of("ld_dx", d.ld_dx, d.cols);
+  n.partial_rows = norm_grad_blocks(d.type, d.rows, d.cols);
+  return n;
+}
+
+template <typename F>
+int64_t bytes_of(const char* call, int32_t direction, F f) {
+  int64_t n = -1;
+  guarded(call, [&] {
+    if (direction != VOLTA_OP_FORWARD && direction != VOLTA_OP_BACKWARD)
+      refuse("direction is " + std::to_string(direction) + ", must be forward (0) or backward (1)");
+    n = f(direction == VOLTA_OP_BACKWARD);
+  });
+  return n;
+}
+
+}  // namespace
+}  // namespace ops
+}  // namespace volta
+
+using namespace volta;
+using namespace volta::ops;
+
+extern "C" {
+
+int64_t volta_op_linear_workspace(const volta_op_linear* d, int32_t direction) {
+  return bytes_of("volta_op_linear_workspace", direction, [&](bool backward) {
+    const Linear l = linear_of(d);
+    return backward ? l.backward_bytes() : l.forward_bytes();
+  });
+}
+
+int32_t volta_op_linear_forward(const volta_op_linear* in, const void* x, const void* w, const void* bias,
+                                const void* residual, void* y, void* pre, void* workspace, int64_t workspace_bytes,
+                                void* stream) {
+  return guarded("volta_op_linear_forward", [&] {
+    const Linear l = linear_of(in);
+    const volta_op_linear& d = l.d;
+    const int e = elem_bytes(d.type);
+    if (d.rows > 0) {
+      need(x, "x");
+      need(y, "y");
+    }
+    need(w, "w");
+    const Mat mx{"x", x, d.rows, d.inputs, d.ld_x, e, false}, mw{"w", w, d.inputs, d.outputs, d.ld_w, e, false};
+    const Mat mb{"bias", bias, 1, d.outputs, d.outputs, e, false};
+    const Mat mr{"residual", residual, d.rows, d.outputs, d.ld_residual, e, false};
+    const Mat my{"y", y, d.rows, d.outputs, d.ld_y, e, true}, mp{"pre", pre, d.rows, d.outputs, d.ld_pre, e, true};
+    check_workspace(workspace, workspace_bytes, l.forward_bytes());
+    check_mats({mx, mw, mb, mr, my, mp}, {{residual, y}}, workspace, l.forward_bytes());
+    const hipStream_t st = stream_of(stream);
+    OpEpilogue epi{};
+    epi.act = d.act;
+    epi.bias[0] = bias;
+    epi.residual = residual;
+    epi.out[0] = y;
+    epi.pre[0] = pre;
+    epi.ld_out = d.ld_y;
+    epi.ld_residual = d.ld_residual;
+    epi.ld_pre = d.ld_pre;
+    product(d.type, l.fwd, {mx}, {mw}, epi, {mb, mr, my, mp}, static_cast<float*>(workspace), st, "product");
+  });
+}
+
+int32_t volta_op_linear_backward(const volta_op_linear* in, const void* dy, const void* x, const void* w,
+                                 const void* pre, void* dx, void* dw, void* db, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
+  return guarded("volta_op_linear_backward", [&] {
+    const Linear l = linear_of(in);
+    const volta_op_linear& d = l.d;
+    const int e = elem_bytes(d.type);
+    const bool act = d.act != VOLTA_OP_ACT_NONE;
+    if (!dx && !dw && !db) refuse("dx, dw and db are all NULL");
+    if (d.rows > 0) {
+      need(dy, "dy");
+      if (act) need(pre, "pre");
+      if (dw) need(x, "x");
+    }
+    if (dx) need(w, "w");
+    const Mat mdy{"dy", dy, d.rows, d.outputs, d.ld_y, e, false}, mx{"x", x, d.rows, d.inputs, d.ld_x, e, false};
+    const Mat mw{"w", w, d.inputs, d.outputs, d.ld_w, e, false};
+    const Mat mp{"pre", act ? pre : nullptr, d.rows, d.outputs, d.ld_pre, e, false};
+    const Mat mdx{"dx", dx, d.rows, d.inputs, d.ld_dx, e, true}, mdw{"dw", dw, d.inputs, d.outputs, d.ld_dw, e, true};
+    const Mat mdb{"db", db, 1, d.outputs, d.outputs, e, true};
+    check_workspace(workspace, workspace_bytes, l.backward_bytes());
+    check_mats({mdy, mx, mw, mp, mdx, mdw, mdb}, {}, workspace, l.backward_bytes());
+    const hipStream_t st = stream_of(stream);
+    char* ws = static_cast<char*>(workspace);
+    float* sums = reinterpret_cast<float*>(ws + l.dp_bytes);
+    float* partial = reinterpret_cast<float*>(ws + l.dp_bytes + l.sums_bytes);
+    Mat mdp = mdy;  // without an activation dp is dy
+    if (act) mdp = {"dp", ws, d.rows, d.outputs, d.outputs, e, false};
+    if ((act && (dx || dw) && d.rows > 0) || db) {
+      ActGradArgs a{};
+      a.dy = dy;
+      a.pre[0] = act ? pre : nullptr;
+      a.d[0] = act && (dx || dw) ? ws : nullptr;
+      a.partial[0] = db ? sums : nullptr;
+      a.act = d.act;
+      a.rows = d.rows;
+      a.cols = (int32_t)d.outputs;
+      a.ld_dy = d.ld_y;
+      a.ld_pre = d.ld_pre;
+      check_hip(act_grad(d.type, false, a, st), "activation gradient");
+      if (db) check_hip(sum_partials(d.type, sums, l.strips, d.outputs, db, st), "bias gradient");
+    }
+    OpEpilogue epi{};
+    if (dx) {
+      epi.out[0] = dx;
+      epi.ld_out = d.ld_dx;
+      product(d.type, l.dx, {mdp}, {mw}, epi, {mdx}, partial, st, "dx");
+    }
+    if (dw) {
+      epi.out[0] = dw;
+      epi.ld_out = d.ld_dw;
+      product(d.type, l.dw, {mx}, {mdp}, epi, {mdw}, partial, st, "dw");
+    }
+  });
+}
+
+int64_t volta_op_gated_workspace(const volta_op_gated* d, int32_t direction) {
+  return bytes_of("volta_op_gated_workspace", direction, [&](bool backward) {
+    const Gated l = gated_of(d);
+    return backward ? l.backward_bytes() : l.forward_bytes();
+  });
+}
+
+int32_t volta_op_gated_forward(const volta_op_gated* in, const void* x, const void* w_gate, const void* w_up,
+                               const void* b_gate, const void* b_up, void* h, void* gate, void* up, void* workspace,
+                               int64_t workspace_bytes, void* stream) {
+  return guarded("volta_op_gated_forward", [&] {
+    const Gated l = gated_of(in);
+    const volta_op_gated& d = l.d;
+    const int e = elem_bytes(d.type);
+    if (d.rows > 0) {
+      need(x, "x");
+      need(h, "h");
+    }
+    need(w_gate, "w_gate");
+    need(w_up, "w_up");
+    if (!gate != !up) refuse("gate and up are kept both or neither");
+    const Mat mx{"x", x, d.rows, d.inputs, d.ld_x, e, false};
+    const Mat mg{"w_gate", w_gate, d.inputs, d.hidden, d.ld_w, e, false};
+    const Mat mu{"w_up", w_up, d.inputs, d.hidden, d.ld_w, e, false};
+    const Mat bg{"b_gate", b_gate, 1, d.hidden, d.hidden, e, false}, bu{"b_up", b_up, 1, d.hidden, d.hidden, e, false};
+    const Mat mh{"h", h, d.rows, d.hidden, d.ld_h, e, true};
+    const Mat pg{"gate", gate, d.rows, d.hidden, d.ld_pre, e, true}, pu{"up", up, d.rows, d.hidden, d.ld_pre, e, true};
+    check_workspace(workspace, workspace_bytes, l.forward_bytes());
+    check_mats({mx, mg, mu, bg, bu, mh, pg, pu}, {}, workspace, l.forward_bytes());
+    const hipStream_t st = stream_of(stream);
+    OpEpilogue epi{};
+    epi.act = d.act;
+    epi.bias[0] = b_gate;
+    epi.bias[1] = b_up;
+    epi.out[0] = h;
+    epi.pre[0] = gate;
+    epi.pre[1] = up;
+    epi.ld_out = d.ld_h;
+    epi.ld_pre = d.ld_pre;
+    product(d.type, l.fwd, {mx}, {mg, mu}, epi, {bg, bu, mh, pg, pu}, static_cast<float*>(workspace), st, "product");
+  });
+}
+
+int32_t volta_op_gated_backward(const volta_op_gated* in, const void* dh, const void* x, const void* w_gate,
+                                const void* w_up, const void* gate, const void* up, void* dx, void* dw_gate,
+                                void* dw_up, void* db_gate, void* db_up, void* workspace, int64_t workspace_bytes,
+                                void* stream) {
+  return guarded("volta_op_gated_backward", [&] {
+    const Gated l = gated_of(in);
+    const volta_op_gated& d = l.d;
+    const int e = elem_bytes(d.type);
+    if (!dw_gate != !dw_up) refuse("dw_gate and dw_up are wanted both or neither");
+    if (!dx && !dw_gate && !db_gate && !db_up) refuse("every gradient is NULL");
+    if (d.rows > 0) {
+      need(dh, "dh");
+      need(gate, "gate");
+      need(up, "up");
+      if (dw_gate) need(x, "x");
+    }
+    if (dx) {
+      need(w_gate, "w_gate");
+      need(w_up, "w_up");
+    }
+    const Mat mdh{"dh", dh, d.rows, d.hidden, d.ld_h, e, false}, mx{"x", x, d.rows, d.inputs, d.ld_x, e, false};
+    const Mat mg{"w_gate", w_gate, d.inputs, d.hidden, d.ld_w, e, false};
+    const Mat mu{"w_up", w_up, d.inputs, d.hidden, d.ld_w, e, false};
+    const Mat pg{"gate", gate, d.rows, d.hidden, d.ld_pre, e, false}, pu{"up", up, d.rows, d.hidden, d.ld_pre, e, false};
+    const Mat mdx{"dx", dx, d.rows, d.inputs, d.ld_dx, e, true};
+    const Mat wg{"dw_gate", dw_gate, d.inputs, d.hidden, d.ld_dw, e, true};
+    const Mat wu{"dw_up", dw_up, d.inputs, d.hidden, d.ld_dw, e, true};
+    const Mat bg{"db_gate", db_gate, 1, d.hidden, d.hidden, e, true}, bu{"db_up", db_up, 1, d.hidden, d.hidden, e, true};
+    check_workspace(workspace, workspace_bytes, l.backward_bytes());
+    check_mats({mdh, mx, mg, mu, pg, pu, mdx, wg, wu, bg, bu}, {}, workspace, l.backward_bytes());
+    const hipStream_t st = stream_of(stream);
+    char* ws = static_cast<char*>(workspace);
+    float* sums[2] = {reinterpret_cast<float*>(ws + 2 * l.d_bytes),
+                      reinterpret_cast<float*>(ws + 2 * l.d_bytes + l.sums_bytes)};
+    float* partial = reinterpret_cast<float*>(ws + 2 * (l.d_bytes + l.sums_bytes));
+    if (d.rows > 0 || db_gate || db_up) {
+      ActGradArgs a{};
+      a.dy = dh;
+      a.pre[0] = gate;
+      a.pre[1] = up;
+      a.d[0] = ws;
+      a.d[1] = ws + l.d_bytes;
+      a.partial[0] = db_gate ? sums[0] : nullptr;
+      a.partial[1] = db_up ? sums[1] : nullptr;
+      a.act = d.act;
+      a.rows = d.rows;
+      a.cols = (int32_t)d.hidden;
+      a.ld_dy = d.ld_h;
+      a.ld_pre = d.ld_pre;
+      check_hip(act_grad(d.type, true, a, st), "activation gradient");
+      if (db_gate) check_hip(sum_partials(d.type, sums[0], l.strips, d.hidden, db_gate, st), "bias gradient");
+      if (db_up) check_hip(sum_partials(d.type, sums[1], l.strips, d.hidden, db_up, st), "bias gradient");
+    }
+    const Mat dg{"dg", ws, d.rows, d.hidden, d.hidden, e, false};
+    const Mat du{"du", ws + l.d_bytes, d.rows, d.hidden, d.hidden, e, false};
+    OpEpilogue epi{};
+    if (dx) {
+      epi.out[0] = dx;
+      epi.ld_out = d.ld_dx;
+      product(d.type, l.dx, {dg, du}, {mg, mu}, epi, {mdx}, partial, st, "dx");
+    }
+    if (dw_gate) {
+      epi.out[0] = dw_gate;
+      epi.out[1] = dw_up;
+      epi.ld_out = d.ld_dw;
+      product(d.type, l.dw, {mx}, {dg, du}, epi, {wg, wu}, partial, st, "dw");
+    }
+  });
+}
+
+int64_t volta_op_rms_norm_workspace(const volta_op_rms_norm* d, int32_t direction) {
+  return bytes_of("volta_op_rms_norm_workspace", direction, [&](bool backward) {
+    const Norm n = norm_of(d, backward);
+    return backward ? n.backward_bytes() : (int64_t)0;
+  });
+}
+
+int32_t volta_op_rms_norm_forward(const volta_op_rms_norm* in, const void* x, const void* residual,
+                                  const void* weight, void* y, void* sum, float* rstd, float* scales, void* stream) {
+  return guarded("volta_op_rms_norm_forward", [&] {
+    const Norm n = norm_of(in, false);
+    const volta_op_rms_norm& d = n.d;
+    const int e = elem_bytes(d.type);
+    const bool e4m3 = d.out_type == VOLTA_OP_E4M3;
+    if (d.rows > 0) {
+      need(x, "x");
+      need(y, "y");
+      if (e4m3) need(scales, "scales");
+    }
+    if (!e4m3 && scales) refuse("scales are of out_type E4M3 alone");
+    const int64_t groups = d.group ? (d.cols + d.group - 1) / d.group : 1;
+    check_mats({{"x", x, d.rows, d.cols, d.ld_x, e, false},
+                {"residual", residual, d.rows, d.cols, d.ld_residual, e, false},
+                {"weight", weight, 1, d.cols, d.cols, e, false},
+                {"y", y, d.rows, d.cols, d.ld_y, elem_bytes(d.out_type), true},
+                {"sum", sum, d.rows, d.cols, d.ld_sum, e, true},
+                {"rstd", rstd, d.rows, 1, 1, 4, true},
+                {"scales", scales, d.rows, groups, groups, 4, true}},
+               {{sum, x}, {sum, residual}});
+    const hipStream_t st = stream_of(stream);
+    NormArgs a{};
+    a.x = x;
+    a.residual = residual;
+    a.weight = weight;
+    a.y = y;
+    a.sum = sum;
+    a.rstd = rstd;
+    a.scales = scales;
+    a.rows = d.rows;
+    a.cols = (int32_t)d.cols;
+    a.group = d.group ? d.group : (int32_t)d.cols;
+    a.ld_x = d.ld_x;
+    a.ld_residual = d.ld_residual;
+    a.ld_y = d.ld_y;
+    a.ld_sum = d.ld_sum;
+    a.eps = d.eps;
+    check_hip(norm_forward(d.type, e4m3, a, st), "norm");
+  });
+}
+
+int32_t volta_op_rms_norm_backward(const volta_op_rms_norm* in, const void* dy, const void* s, const float* rstd,
+                                   const void* weight, const void* dsum, void* dx, void* dweight, void* workspace,
+                                   int64_t workspace_bytes, void* stream) {
+  return guarded("volta_op_rms_norm_backward", [&] {
+    const Norm n = norm_of(in, true);
+    const volta_op_rms_norm& d = n.d;
+    const int e = elem_bytes(d.type);
+    if (!dx && !dweight) refuse("dx and dweight are both NULL");
+    if (d.rows > 0) {
+      need(dy, "dy");
+      need(s, "s");
+      need(rstd, "rstd");
+    }
+    if (dweight) check_workspace(workspace, workspace_bytes, n.backward_bytes());
+    check_mats({{"dy", dy, d.rows, d.cols, d.ld_y, e, false},
+                {"s", s, d.rows, d.cols, d.ld_x, e, false},
+                {"rstd", rstd, d.rows, 1, 1, 4, false},
+                {"weight", weight, 1, d.cols, d.cols, e, false},
+                {"dsum", dsum, d.rows, d.cols, d.ld_sum, e, false},
+                {"dx", dx, d.rows, d.cols, d.ld_dx, e, true},
+                {"dweight", dweight, 1, d.cols, d.cols, e, true}},
+               {{dsum, dx}}, dweight ? workspace : nullptr, n.backward_bytes());
+    const hipStream_t st = stream_of(stream);
+    NormGradArgs a{};
+    a.dy = dy;
+    a.s = s;
+    a.weight = weight;
+    a.dsum = dsum;
+    a.rstd = rstd;
+    a.dx = dx;
+    a.partial = dweight ? static_cast<float*>(workspace) : nullptr;
+    a.rows = d.rows;
+    a.cols = (int32_t)d.cols;
+    a.ld_dy = d.ld_y;
+    a.ld_s = d.ld_x;
+    a.ld_dsum = d.ld_sum;
+    a.ld_dx = d.ld_dx;
+    check_hip(norm_backward(d.type, a, st), "norm gradient");
+    if (dweight) check_hip(sum_partials(d.type, a.partial, n.partial_rows, d.cols, dweight, st), "weight gradient");
+  });
+}
+
+int32_t volta_op_dropout_forward(const volta_op_dropout* in, const void* x, const void* residual, void* y,
+                                 uint64_t seed, uint64_t offset, void* stream) {
+  return guarded("volta_op_dropout_forward", [&] {
+    need(in, "the description");
+    volta_op_dropout d = *in;
+    check_type(d.type);
+    check_dims("rows", d.rows, 0, kMaxRows);
+    check_dims("cols", d.cols, 1, kMaxLd);
+    if (!(d.p >= 0.0 && d.p < 1.0)) refuse("p must be at least 0 and below 1");
+    d.ld_x = ld_of("ld_x", d.ld_x, d.cols);
+    d.ld_residual = ld_of("ld_residual", d.ld_residual, d.cols);
+    d.ld_y = ld_of("ld_y", d.ld_y, d.cols);
+    const int e = elem_bytes(d.type);
+    if (d.rows > 0) {
+      need(x, "x");
+      need(y, "y");
+    }
+    check_mats({{"x", x, d.rows, d.cols, d.ld_x, e, false},
+                {"residual", residual, d.rows, d.cols, d.ld_residual, e, false},
+                {"y", y, d.rows, d.cols, d.ld_y, e, true}},
+               {{x, y}, {residual, y}});
+    const hipStream_t st = stream_of(stream);
+    DropoutArgs a{};
+    a.x = x;
+    a.residual = residual;
+    a.y = y;
+    a.rows = d.rows;
+    a.cols = d.cols;
+    a.ld_x = d.ld_x;
+    a.ld_residual = d.ld_residual;
+    a.ld_y = d.ld_y;
+    a.seed = seed;
+    a.offset = offset;
+    a.threshold = (uint32_t)(d.p * 4294967296.0);
+    a.scale = (float)(1.0 / (1.0 - d.p));
+    check_hip(dropout_forward(d.type, a, st), "dropout");
+  });
+}
+
+}  // extern "C"

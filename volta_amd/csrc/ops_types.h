@@ -1,0 +1,160 @@
+// Element types of the feed-forward operators (include/volta_ops.h): storage,
+// conversions, vector accesses, and their matrix instruction.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/volta_ops.h"
+#include "device_common.h"
+
+namespace volta {
+namespace ops {
+
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+
+// 16 bytes of a fragment or a chunk, whatever they hold.
+typedef uint32_t chunk16 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+struct alignas(4 * sizeof(T)) Quad {
+  T v[4];
+};
+
+template <typename T> __device__ __forceinline__ float to_f(T x) { return (float)x; }
+template <typename T> __device__ __forceinline__ T from_f(float x) { return (T)x; }  // to the nearest, ties to even
+
+// Four consecutive elements as floats: one access where `vec` says that the
+// address allows it, else the first `cnt` one by one (the rest 0).
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, bool vec, int cnt, float (&f)[4]) {
+  if (vec) {
+    const Quad<T> q = *reinterpret_cast<const Quad<T>*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = to_f(q.v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = i < cnt ? to_f(p[i]) : 0.0f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, bool vec, int cnt, const float (&f)[4]) {
+  if (vec) {
+    Quad<T> q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q.v[i] = from_f<T>(f[i]);
+    *reinterpret_cast<Quad<T>*>(p) = q;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < cnt) p[i] = from_f<T>(f[i]);
+  }
+}
+
+// f(x) and f'(x) of the layers' activations.  float32 results take the
+// training step's own functions (device_common.h).  16-bit results need a
+// relative error well under 2^-9 only: the hardware's exp2 and reciprocal (one
+// unit in the last place of 32 bits each) instead of the library's functions
+// and IEEE division, which would cost a gated layer's epilogue a fifth of its
+// products' time.  tanh(v) = 1 - 2 / (1 + e^2v) cancels near 0, where its
+// series takes over (|v| < 1/4: the next term, 17/315 v^7, is 1.3e-5 of v).
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
+__device__ __forceinline__ float fast_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + fast_exp(-x)); }
+__device__ __forceinline__ float fast_tanh(float v) {
+  const float big = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + fast_exp(2.0f * v));
+  const float v2 = v * v;
+  const float small = v * (1.0f - v2 * (0.333333333f - 0.133333333f * v2));
+  return fabsf(v) < 0.25f ? small : big;
+}
+constexpr float kGeluC = 0.7978845608f, kGeluK = 0.044715f;
+
+template <typename T>
+__device__ __forceinline__ float op_act(int act, float x) {
+  if constexpr (sizeof(T) == 4) {
+    return act_forward(act, x);
+  } else {
+    switch (act) {
+      case VOLTA_ACT_RELU: return x > 0.0f ? x : 0.0f;
+      case VOLTA_ACT_SIGMOID: return fast_sigmoid(x);
+      case VOLTA_ACT_TANH: return fast_tanh(x);
+      case VOLTA_ACT_LEAKY_RELU: return x > 0.0f ? x : 0.01f * x;
+      case VOLTA_ACT_SILU: return x * fast_sigmoid(x);
+      // 0.5 x (1 + tanh v) = x sigmoid(2v)
+      case VOLTA_ACT_GELU: return x * fast_sigmoid(2.0f * kGeluC * (x + kGeluK * x * x * x));
+      default: return x;
+    }
+  }
+}
+
+// f of four values: the activation is asked once.
+template <typename T>
+__device__ __forceinline__ void op_act4(int act, float (&x)[4]) {
+#define VOLTA_ACT4(A)                                       \
+  case A:                                                   \
+    _Pragma("unroll") for (int i = 0; i < 4; ++i) x[i] = op_act<T>(A, x[i]); \
+    break
+  switch (act) {
+    VOLTA_ACT4(VOLTA_ACT_RELU);
+    VOLTA_ACT4(VOLTA_ACT_SIGMOID);
+    VOLTA_ACT4(VOLTA_ACT_TANH);
+    VOLTA_ACT4(VOLTA_ACT_LEAKY_RELU);
+    VOLTA_ACT4(VOLTA_ACT_SILU);
+    VOLTA_ACT4(VOLTA_ACT_GELU);
+    default: break;
+  }
+#undef VOLTA_ACT4
+}
+
+// f and f' together (the gated layer's gradient needs both).
+template <typename T>
+__device__ __forceinline__ void op_act_both(int act, float x, float* f, float* slope) {
+  if constexpr (sizeof(T) == 4) {
+    *f = act_forward(act, x);
+    *slope = act == VOLTA_ACT_RELU ? (x > 0.0f ? 1.0f : 0.0f) : act_derivative(act, x, *f);
+  } else {
+    switch (act) {
+      case VOLTA_ACT_RELU:
+        *f = x > 0.0f ? x : 0.0f;
+        *slope = x > 0.0f ? 1.0f : 0.0f;
+        break;
+      case VOLTA_ACT_SIGMOID: {
+        const float q = fast_sigmoid(x);
+        *f = q;
+        *slope = q * fast_sigmoid(-x);
+        break;
+      }
+      case VOLTA_ACT_TANH: {
+        // 1 - tanh^2 = 4 q (1 - q), q = sigmoid(2x)
+        *f = fast_tanh(x);
+        *slope = 4.0f * fast_sigmoid(2.0f * x) * fast_sigmoid(-2.0f * x);
+        break;
+      }
+      case VOLTA_ACT_LEAKY_RELU:
+        *f = x > 0.0f ? x : 0.01f * x;
+        *slope = x > 0.0f ? 1.0f : 0.01f;
+        break;
+      case VOLTA_ACT_SILU: {
+        const float q = fast_sigmoid(x);
+        *f = x * q;
+        *slope = q + x * q * fast_sigmoid(-x);
+        break;
+      }
+      case VOLTA_ACT_GELU: {
+        const float v2 = 2.0f * kGeluC * (x + kGeluK * x * x * x);
+        const float q = fast_sigmoid(v2);
+        *f = x * q;
+        *slope = q + x * q * fast_sigmoid(-v2) * 2.0f * kGeluC * (1.0f + 3.0f * kGeluK * x * x);
+        break;
+      }
+      default:
+        *f = x;
+        *slope = 1.0f;
+    }
+  }
+}
+
+}  // namespace ops
+}  // namespace volta

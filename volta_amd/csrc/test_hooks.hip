@@ -5,6 +5,8 @@
 
 #include <algorithm>
 
+#include "../../include/volta_ops.h"
+#include "ops_gemm.h"
 #include "gemm.h"
 #include "spec.h"
 #include "step_kernels.h"
@@ -231,6 +233,73 @@ int32_t volta_hip_optimizer(int32_t kind, float* w, float* m, float* v, const fl
     return -1;
   }
   return 0;
+}
+
+// A product of the feed-forward operators on a given tile and number of
+// splits (ops_gemm.h), synchronously: D = sum over the pieces of P_i Q_i, or
+// the gated pair act(P Q_0) * (P Q_1) with the SiLU.  OP_LINEAR and OP_GATED
+// run without biases, residual and kept pre-activations.  Returns 0, or -1
+// for a plan that the operators would not make or a device error.
+int32_t volta_hip_op_product(int32_t type, int32_t layout, int32_t kind, int32_t tile, int32_t splits, int32_t direct,
+                             const void* p0, const void* p1, int64_t ld_p, const void* q0, const void* q1,
+                             int64_t ld_q, void* out0, void* out1, int64_t ld_out, int32_t M, int32_t N, int32_t K,
+                             int32_t pieces, int32_t outputs) {
+  using namespace volta::ops;
+  const int e = type == VOLTA_OP_F32 ? 4 : 2;
+  const int per_chunk = 16 / e, stages = pieces * ((K + op_stage_k(e) - 1) / op_stage_k(e));
+  const bool p_kc = layout != OP_TN, q_kc = layout == OP_NT;
+  const int p_len = p_kc ? K : M, q_len = q_kc ? K : N;
+  for (const void* x : {p0, p1, q0, q1})
+    if (direct && ((uintptr_t)x % 16 != 0)) return -1;
+  if (direct && (ld_p % per_chunk || ld_q % per_chunk || p_len % per_chunk || q_len % per_chunk)) return -1;
+  if (M < 1 || N < 1 || K < 0 || ld_p < p_len || ld_q < q_len || ld_out < N || splits < 1) return -1;
+  if (tile < OP_TILE_256 || tile > OP_TILE_SKINNY) return -1;
+  if (tile == OP_TILE_256 && (e == 4 || !direct)) return -1;
+  if (tile == OP_TILE_SKINNY && (M > 64 || layout == OP_TN)) return -1;
+  if ((pieces != 1 && (pieces != 2 || layout != OP_NT)) || (outputs != 1 && (outputs != 2 || layout != OP_TN))) return -1;
+  OpPlan plan{tile, 1, stages};
+  if (stages > 0) {
+    plan.stages_per_split = (stages + splits - 1) / splits;
+    plan.splits = (stages + plan.stages_per_split - 1) / plan.stages_per_split;
+  }
+  const int64_t bytes = op_gemm_partial_bytes(plan, kind, M, N, outputs);
+  void* ws = nullptr;
+  if (bytes && hipMalloc(&ws, bytes) != hipSuccess) return -1;
+  OpGemm g{};
+  g.p[0] = p0;
+  g.p[1] = p1;
+  g.q[0] = q0;
+  g.q[1] = q1;
+  g.ld_p = ld_p;
+  g.ld_q = ld_q;
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.pieces = pieces;
+  g.outputs = outputs;
+  g.direct = direct;
+  g.partial = static_cast<float*>(ws);
+  g.epi.act = kind == OP_GATED ? VOLTA_ACT_SILU : VOLTA_OP_ACT_NONE;
+  g.epi.vec = ld_out % 4 == 0 && (uintptr_t)out0 % (4 * e) == 0 && (uintptr_t)out1 % (4 * e) == 0;
+  g.epi.out[0] = out0;
+  g.epi.out[1] = out1;
+  g.epi.ld_out = ld_out;
+  hipError_t rc = type == VOLTA_OP_F32    ? op_gemm_f32(layout, kind, plan, g, nullptr)
+                  : type == VOLTA_OP_BF16 ? op_gemm_bf16(layout, kind, plan, g, nullptr)
+                                          : op_gemm_f16(layout, kind, plan, g, nullptr);
+  if (rc == hipSuccess) rc = hipStreamSynchronize(nullptr);
+  if (ws) (void)hipFree(ws);
+  return rc == hipSuccess ? 0 : -1;
+}
+
+// The plan of such a product: {tile, splits, stages of a split}.
+void volta_hip_op_plan(int32_t elem_bytes, int32_t layout, int32_t kind, int64_t M, int64_t N, int64_t K,
+                       int32_t pieces, int32_t outputs, int32_t direct, int32_t* plan) {
+  const volta::ops::OpPlan p =
+      volta::ops::op_gemm_plan(elem_bytes, layout, kind, M, N, K, pieces, outputs, direct != 0);
+  plan[0] = p.tile;
+  plan[1] = p.splits;
+  plan[2] = p.stages_per_split;
 }
 
 }  // extern "C"

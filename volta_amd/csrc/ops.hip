@@ -176,8 +176,8 @@ int64_t partial_bytes(int type, const Shape& s) {
 }
 
 // One product of a call.
-void product(int type, const Shape& s, const std::vector<Mat>& ps, const std::vector<Mat>& qs, OpEpilogue epi,
-             const std::vector<Mat>& written, float* partial, hipStream_t st, const char* what) {
+void product(int type, const Shape& s, const std::vector<Mat>& ps, const std::vector<Mat>& qs, const OpEpilogue& epi,
+             float* partial, hipStream_t st, const char* what) {
   if (s.M == 0 || s.N == 0) return;
   OpGemm g{};
   bool direct = true;
@@ -199,8 +199,6 @@ void product(int type, const Shape& s, const std::vector<Mat>& ps, const std::ve
   const OpPlan plan = plan_of(type, s, direct);
   // a grid has fewer than 2^32 threads
   if (op_gemm_blocks(plan, s.kind, s.M, s.N) > (int64_t{1} << 22)) refuse("rows * columns of a product are too many");
-  epi.vec = 1;
-  for (const Mat& m : written) epi.vec = epi.vec && m.vec(4);
   g.epi = epi;
   check_hip(gemm(type, s.layout, s.kind, plan, g, st), what);
 }
@@ -363,7 +361,7 @@ int32_t volta_op_linear_forward(const volta_op_linear* in, const void* x, const 
     epi.ld_out = d.ld_y;
     epi.ld_residual = d.ld_residual;
     epi.ld_pre = d.ld_pre;
-    product(d.type, l.fwd, {mx}, {mw}, epi, {mb, mr, my, mp}, static_cast<float*>(workspace), st, "product");
+    product(d.type, l.fwd, {mx}, {mw}, epi, static_cast<float*>(workspace), st, "product");
   });
 }
 
@@ -413,12 +411,12 @@ int32_t volta_op_linear_backward(const volta_op_linear* in, const void* dy, cons
     if (dx) {
       epi.out[0] = dx;
       epi.ld_out = d.ld_dx;
-      product(d.type, l.dx, {mdp}, {mw}, epi, {mdx}, partial, st, "dx");
+      product(d.type, l.dx, {mdp}, {mw}, epi, partial, st, "dx");
     }
     if (dw) {
       epi.out[0] = dw;
       epi.ld_out = d.ld_dw;
-      product(d.type, l.dw, {mx}, {mdp}, epi, {mdw}, partial, st, "dw");
+      product(d.type, l.dw, {mx}, {mdp}, epi, partial, st, "dw");
     }
   });
 }
@@ -462,7 +460,7 @@ int32_t volta_op_gated_forward(const volta_op_gated* in, const void* x, const vo
     epi.pre[1] = up;
     epi.ld_out = d.ld_h;
     epi.ld_pre = d.ld_pre;
-    product(d.type, l.fwd, {mx}, {mg, mu}, epi, {bg, bu, mh, pg, pu}, static_cast<float*>(workspace), st, "product");
+    product(d.type, l.fwd, {mx}, {mg, mu}, epi, static_cast<float*>(workspace), st, "product");
   });
 }
 
@@ -525,13 +523,13 @@ int32_t volta_op_gated_backward(const volta_op_gated* in, const void* dh, const 
     if (dx) {
       epi.out[0] = dx;
       epi.ld_out = d.ld_dx;
-      product(d.type, l.dx, {dg, du}, {mg, mu}, epi, {mdx}, partial, st, "dx");
+      product(d.type, l.dx, {dg, du}, {mg, mu}, epi, partial, st, "dx");
     }
     if (dw_gate) {
       epi.out[0] = dw_gate;
       epi.out[1] = dw_up;
       epi.ld_out = d.ld_dw;
-      product(d.type, l.dw, {mx}, {dg, du}, epi, {wg, wu}, partial, st, "dw");
+      product(d.type, l.dw, {mx}, {dg, du}, epi, partial, st, "dw");
     }
   });
 }

@@ -25,7 +25,6 @@ enum OpKind {
 
 struct OpEpilogue {
   int32_t act;
-  int32_t vec;  // rows of out, residual and pre, and the biases, allow 4-element accesses
   const void* bias[2];
   const void* residual;
   void* out[2];  // OP_STORE: one for each q (blockIdx.z)

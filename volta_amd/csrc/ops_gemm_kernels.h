@@ -28,6 +28,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "ops_gemm.h"
 #include "ops_types.h"
@@ -35,15 +36,10 @@
 namespace volta {
 namespace ops {
 
-typedef __attribute__((address_space(3))) void* LdsPtr;
 typedef __attribute__((address_space(3))) shortx4* LdsShort4;
 
 // What a direct load reads where k is past the end.
 static __device__ const __attribute__((aligned(16))) uint32_t op_zeros[4] = {0, 0, 0, 0};
-
-typedef uint32_t chunk16_by2 __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t chunk16_by4 __attribute__((ext_vector_type(4), aligned(4)));
-#define VOLTA_GLOBAL __attribute__((address_space(1)))
 
 template <typename T> struct Mfma;
 template <> struct Mfma<__bf16> {
@@ -70,8 +66,7 @@ template <> struct Mfma<float> {  // lane group g holds k = 4g .. 4g + 3 of 16: 
 // 16 bytes at any element address.
 template <typename T>
 __device__ __forceinline__ chunk16 load_unaligned(const T* p) {
-  if constexpr (sizeof(T) == 2) return *(const VOLTA_GLOBAL chunk16_by2*)p;
-  else return *(const VOLTA_GLOBAL chunk16_by4*)p;
+  return *(const VOLTA_GLOBAL typename Access<16, sizeof(T)>::type*)p;
 }
 // The first `cnt` elements of a chunk, the rest 0.
 template <typename T>
@@ -81,6 +76,27 @@ __device__ __forceinline__ chunk16 load_part(const T* p, int cnt) {
 #pragma unroll
   for (int i = 0; i < E; ++i) u.e[i] = i < cnt ? ((const VOLTA_GLOBAL T*)p)[i] : (T)0.0f;
   return u.c;
+}
+
+// 16 bytes a lane from global memory to LDS, lane after lane from byte `lds`
+// on; nothing passes through registers.  Written as asm because the compiler
+// keeps apart only a few such loads: with a ring of stages it no longer knows
+// which of them a read of LDS depends on, and waits for all before each read.
+// The kernels wait themselves (op_wait_loads), by counting: loads return in
+// order.  M0 takes a cycle to reach the load.
+__device__ __forceinline__ void op_load_lds(const char* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
+               "v"(off), "s"(base)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void op_load_lds(const char* from, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(
+                   __builtin_amdgcn_readfirstlane(lds)),
+               "v"(from)
+               : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t op_lds_byte(const char* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 }
 
 // One operand's tile of one stage: R rows (KC) or R columns (MC), loaded by NW
@@ -128,19 +144,17 @@ struct Tile {
   }
 
   // Direct: the stage at `base`, whose k are all inside, or the first `k_left` of them.
-  __device__ __forceinline__ void issue(const char* base, char* lds, int wave) const {
+  __device__ __forceinline__ void issue(const char* base, uint32_t lds, int wave) const {
 #pragma unroll
-    for (int t = 0; t < kLoads; ++t)
-      __builtin_amdgcn_global_load_lds((const void*)(base + off[t]), (LdsPtr)(lds + (wave + t * NW) * 1024), 16, 0, 0);
+    for (int t = 0; t < kLoads; ++t) op_load_lds(base, off[t], lds + (wave + t * NW) * 1024);
   }
-  __device__ __forceinline__ void issue_tail(const char* base, char* lds, int wave, int lane, int k_left) const {
+  __device__ __forceinline__ void issue_tail(const char* base, uint32_t lds, int wave, int lane, int k_left) const {
 #pragma unroll
     for (int t = 0; t < kLoads; ++t) {
       int r, c;
       place((wave + t * NW) * 64 + lane, &r, &c);
       const bool in = KC ? c * kE < k_left : r < k_left;
-      const char* a = in ? base + off[t] : reinterpret_cast<const char*>(op_zeros);
-      __builtin_amdgcn_global_load_lds((const void*)a, (LdsPtr)(lds + (wave + t * NW) * 1024), 16, 0, 0);
+      op_load_lds(in ? base + off[t] : reinterpret_cast<const char*>(op_zeros), lds + (wave + t * NW) * 1024);
     }
   }
 
@@ -193,57 +207,185 @@ struct Tile {
   }
 };
 
-// What a launch's epilogue has to do, in one word.
-constexpr int kHasBias0 = 1, kHasBias1 = 2, kHasPre = 4, kHasResidual = 8, kVec = 16, kActShift = 8;
-template <int KIND>
-__device__ __forceinline__ int op_epilogue_flags(const OpEpilogue& e) {
-  int f = e.vec ? kVec : 0;
+// The epilogue of V consecutive columns n .. of row m, cnt of them in the
+// matrix: d0 (and, gated, d1) are the sums, b0 and b1 the columns' biases.
+template <typename T, int KIND, int V>
+__device__ __forceinline__ void op_epilogue(const OpEpilogue& e, int z, int64_t m, int n, int cnt, float (&d0)[V],
+                                            float (&d1)[V], const float (&b0)[V], const float (&b1)[V]) {
   if constexpr (KIND != OP_STORE) {
-    f |= (e.bias[0] ? kHasBias0 : 0) | (e.pre[0] ? kHasPre : 0) | (e.act + 1) << kActShift;
-    if constexpr (KIND == OP_GATED) f |= e.bias[1] ? kHasBias1 : 0;
-    else f |= e.residual ? kHasResidual : 0;
+    float r[V];
+    const bool residual = KIND == OP_LINEAR && e.residual;
+    if (residual) load_vec(static_cast<const T*>(e.residual) + m * e.ld_residual + n, cnt, r);
+#pragma unroll
+    for (int i = 0; i < V; ++i) d0[i] += b0[i];
+    if constexpr (KIND == OP_GATED) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) d1[i] += b1[i];
+    }
+    if (e.pre[0]) {
+      store_vec(static_cast<T*>(e.pre[0]) + m * e.ld_pre + n, cnt, d0);
+      if constexpr (KIND == OP_GATED) store_vec(static_cast<T*>(e.pre[1]) + m * e.ld_pre + n, cnt, d1);
+    }
+    op_act_all<T>(e.act, d0);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if constexpr (KIND == OP_GATED) d0[i] *= d1[i];
+      else if (residual) d0[i] += r[i];
+    }
   }
-  return f;
+  store_vec(static_cast<T*>(e.out[z]) + m * e.ld_out + n, cnt, d0);
+}
+template <typename T, int KIND, int V>
+__device__ __forceinline__ void op_biases(const OpEpilogue& e, int n, int cnt, float (&b0)[V], float (&b1)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) b0[i] = b1[i] = 0.0f;
+  if constexpr (KIND != OP_STORE) {
+    if (e.bias[0]) load_vec(static_cast<const T*>(e.bias[0]) + n, cnt, b0);
+    if (KIND == OP_GATED && e.bias[1]) load_vec(static_cast<const T*>(e.bias[1]) + n, cnt, b1);
+  }
 }
 
-// The epilogue of four consecutive columns n .. of row m (cnt of them inside).
-template <typename T, int KIND>
-__device__ __forceinline__ void op_epilogue(const OpEpilogue& e, int flags, int z, int64_t m, int n, int cnt,
-                                            float (&d0)[4], float (&d1)[4]) {
-  const bool vec = (flags & kVec) && cnt == 4;
-  if constexpr (KIND != OP_STORE) {
-    float b[4];
-    if (flags & kHasBias0) {
-      load4(static_cast<const T*>(e.bias[0]) + n, vec, cnt, b);
+// A loop over 0 .. N - 1 whose index is a constant of its body.
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void op_unroll(F f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>());
+    op_unroll<N, I + 1>(f);
+  }
+}
+// Waits until at most N of the wave's loads are in flight (they return in
+// order), and the block's barrier, neither moved by the compiler.
+template <int N>
+__device__ __forceinline__ void op_wait_loads() {
+  static_assert(N < 64, "what the counter holds");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void op_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void op_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
+
+// A wave's sums (TM x TN blocks of 16x16; gated: the last half of the columns
+// belongs to the second matrix) to the outputs, or to the partial sums.  They
+// pass through `region`, LDS of the wave's own, 16 or 32 rows at a time, so
+// that a lane then has consecutive columns of one row: accesses of 16 bytes,
+// four lanes side by side on a row, and one small loop of code for all rows
+// (unrolled over the blocks, the epilogue is larger than the instruction
+// cache, and its loads wait for the stores before them).  A row in LDS is 4
+// floats longer than its columns, so that 16 rows' blocks meet no bank twice.
+template <int TM, int TN>
+constexpr int op_out_rows = TM % 2 == 0 ? 32 : 16;
+template <int TM, int TN>
+constexpr int op_region_bytes = op_out_rows<TM, TN> * (TN * 16 + 4) * 4;
+template <typename T, int KIND, int TM, int TN>
+__device__ __forceinline__ void op_write_out(const OpGemm& g, floatx4 (&acc)[TM][TN], char* region, int lane, int m0,
+                                             int n0, int z, int split) {
+  constexpr bool kGated = KIND == OP_GATED;
+  constexpr int kRows = op_out_rows<TM, TN>, RB = kRows / 16, kLd = TN * 16 + 4;
+  constexpr int kCols = kGated ? TN * 8 : TN * 16, V = kCols / 4;  // columns of D, and of them a lane's
+  float* lds = reinterpret_cast<float*>(region);
+  const int row = lane >> 2, col = (lane & 3) * V;
+  const int n = n0 + col, cnt = g.N - n;
+  float b0[V], b1[V];
+  if (g.splits <= 1) op_biases<T, KIND>(g.epi, n, cnt, b0, b1);
+#pragma unroll 1
+  for (int ph = 0; ph < TM / RB; ++ph) {
+    op_unroll<TM / RB>([&](auto I) {
+      int now = ph;  // opaque, or the compiler makes one indexed access of these and acc an array in memory
+      asm volatile("" : "+s"(now));
+      if (now == I) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) d0[i] += b[i];
-    }
-    if (flags & kHasPre) store4(static_cast<T*>(e.pre[0]) + m * e.ld_pre + n, vec, cnt, d0);
-    const int act = (flags >> kActShift) - 1;
-    if constexpr (KIND == OP_GATED) {
-      if (flags & kHasBias1) {
-        load4(static_cast<const T*>(e.bias[1]) + n, vec, cnt, b);
+        for (int b = 0; b < RB; ++b)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d1[i] += b[i];
+          for (int j = 0; j < TN; ++j)
+            *reinterpret_cast<floatx4*>(lds + (b * 16 + (lane & 15)) * kLd + j * 16 + (lane >> 4) * 4) =
+                acc[decltype(I)::value * RB + b][j];
       }
-      if (flags & kHasPre) store4(static_cast<T*>(e.pre[1]) + m * e.ld_pre + n, vec, cnt, d1);
-    }
-    op_act4<T>(act, d0);
-    if constexpr (KIND == OP_GATED) {
+    });
 #pragma unroll
-      for (int i = 0; i < 4; ++i) d0[i] *= d1[i];
-    } else if (flags & kHasResidual) {
-      load4(static_cast<const T*>(e.residual) + m * e.ld_residual + n, vec, cnt, b);
+    for (int b = 0; b < RB; ++b) {
+      const int m = m0 + ph * kRows + b * 16 + row;
+      const float* from = lds + (b * 16 + row) * kLd + col;
+      float d0[V], d1[V];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) d0[i] += b[i];
+      for (int c = 0; c < V; c += 4) {
+        const floatx4 x = *reinterpret_cast<const floatx4*>(from + c);
+        floatx4 y = {};
+        if constexpr (kGated) y = *reinterpret_cast<const floatx4*>(from + kCols + c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          d0[c + i] = x[i];
+          d1[c + i] = y[i];
+        }
+      }
+      if (m >= g.M || cnt <= 0) continue;
+      if (g.splits > 1) {
+        const int64_t planes = kGated ? 2 : g.outputs;
+        float* p = g.partial + ((split * planes + z) * g.M + m) * (int64_t)g.N + n;
+        store_vec(p, cnt, d0);
+        if constexpr (kGated) store_vec(p + (int64_t)g.M * g.N, cnt, d1);
+      } else {
+        op_epilogue<T, KIND>(g.epi, z, m, n, cnt, d0, d1, b0, b1);
+      }
     }
   }
-  store4(static_cast<T*>(e.out[z]) + m * e.ld_out + n, vec, cnt, d0);
 }
 
-__device__ __forceinline__ void store_partial(float* p, int N, int cnt, const float (&d)[4]) {
-  store4<float>(p, (N & 3) == 0 && cnt == 4, cnt, d);
+// Where a stage of an operand starts: row or column x0, k.
+template <typename T, bool KC>
+__device__ __forceinline__ const char* op_stage_base(const void* p, int64_t ld, int x0, int k) {
+  const int64_t e = KC ? (int64_t)x0 * ld + k : (int64_t)k * ld + x0;
+  return static_cast<const char*>(p) + e * (int64_t)sizeof(T);
 }
+
+// Where the next stage to load starts, in every operand (a block's loop takes
+// every `step`-th stage): advanced by additions, since a stage's address
+// computed anew costs a wave more time than its loads.
+template <typename T, int LAYOUT, bool GATED>
+struct Cursor {
+  static constexpr bool P_KC = LAYOUT != OP_TN, Q_KC = LAYOUT == OP_NT;
+  static constexpr int kSubs = GATED ? 2 : 1, kStageK = 128 / (int)sizeof(T);
+  const char* p;
+  const char* q[kSubs];
+  int64_t dp, dq;  // bytes of a step
+  int k, dk;       // in this piece
+  int piece, m0, n0, z;
+
+  __device__ __forceinline__ void place(const OpGemm& g) {
+    p = op_stage_base<T, P_KC>(g.p[piece], g.ld_p, m0, k);
+#pragma unroll
+    for (int i = 0; i < kSubs; ++i)
+      q[i] = op_stage_base<T, Q_KC>(g.q[GATED ? i : LAYOUT == OP_TN ? z : piece], g.ld_q, n0, k);
+  }
+  __device__ __forceinline__ int piece_k(const OpGemm& g) const { return (g.K + kStageK - 1) / kStageK * kStageK; }
+  __device__ __forceinline__ void init(const OpGemm& g, int m0_, int n0_, int z_, int s, int step) {
+    m0 = m0_;
+    n0 = n0_;
+    z = z_;
+    dk = step * kStageK;
+    dp = (P_KC ? (int64_t)dk : dk * g.ld_p) * (int64_t)sizeof(T);
+    dq = (Q_KC ? (int64_t)dk : dk * g.ld_q) * (int64_t)sizeof(T);
+    k = s * kStageK;
+    piece = LAYOUT == OP_NT && g.pieces > 1 && k >= piece_k(g) ? 1 : 0;
+    if (piece) k -= piece_k(g);
+    place(g);
+  }
+  __device__ __forceinline__ void advance(const OpGemm& g) {
+    k += dk;
+    p += dp;
+#pragma unroll
+    for (int i = 0; i < kSubs; ++i) q[i] += dq;
+    if (LAYOUT == OP_NT && g.pieces > 1 && piece == 0 && k >= piece_k(g)) {
+      piece = 1;
+      k -= piece_k(g);
+      place(g);
+    }
+  }
+};
 
 // Block -> tile.  Blocks go to the 8 XCDs in turn; each XCD takes a run of
 // consecutive tiles, in groups of `kGroup` rows of tiles walked column by
@@ -262,10 +404,11 @@ __device__ __forceinline__ void op_tile_of(int b, int tiles_m, int tiles_n, int*
 }
 
 // ---------------------------------------------------------------------------
-// Tiled product: BM x BN of D per block, WGM x WGN waves, two stages in LDS --
-// the loads of stage s + 1 are issued before stage s is multiplied.
+// Tiled product: BM x BN of D per block, WGM x WGN waves, a ring of NST stages
+// in LDS -- the loads of stage s + NST - 1 are issued before stage s is
+// multiplied, so a stage's loads have NST - 1 stages' time to arrive.
 // ---------------------------------------------------------------------------
-template <typename T, int LAYOUT, int KIND, int BM, int BN, int WGM, int WGN, bool DIRECT>
+template <typename T, int LAYOUT, int KIND, int BM, int BN, int WGM, int WGN, int NST, bool DIRECT>
 __global__ void __launch_bounds__(WGM* WGN * 64) op_gemm_tiled(OpGemm g) {
   constexpr int NW = WGM * WGN, WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
   constexpr bool kGated = KIND == OP_GATED;
@@ -274,13 +417,11 @@ __global__ void __launch_bounds__(WGM* WGN * 64) op_gemm_tiled(OpGemm g) {
   constexpr bool P_KC = LAYOUT != OP_TN, Q_KC = LAYOUT == OP_NT;
   using PT = Tile<T, BM, P_KC, NW>;
   using QT = Tile<T, SN, Q_KC, NW>;
-  constexpr int kStageK = PT::kStageK;
-  // one array for each operand and stage: the compiler sees that the loads
-  // into one do not touch what is read from the other
-  __shared__ __attribute__((aligned(16))) char lds_p0[PT::kBytes];
-  __shared__ __attribute__((aligned(16))) char lds_q0[QT::kBytes * kSubs];
-  __shared__ __attribute__((aligned(16))) char lds_p1[PT::kBytes];
-  __shared__ __attribute__((aligned(16))) char lds_q1[QT::kBytes * kSubs];
+  constexpr int kStageK = PT::kStageK, kStageBytes = PT::kBytes + QT::kBytes * kSubs;
+  constexpr int kStageLoads = PT::kLoads + QT::kLoads * kSubs;
+  static_assert(NST >= 2 && NST <= 4 && (DIRECT || NST == 2), "ring");
+  __shared__ __attribute__((aligned(16))) char lds[NST * kStageBytes];
+  auto stage = [&](auto i) { return lds + decltype(i)::value % NST * kStageBytes; };
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -299,41 +440,28 @@ __global__ void __launch_bounds__(WGM* WGN * 64) op_gemm_tiled(OpGemm g) {
   const int s_begin = split * g.stages_per_split;
   const int s_end = min(per_piece * g.pieces, s_begin + g.stages_per_split);
 
-  auto base_of = [&](const void* p, int64_t ld, bool kc, int x0, int k) {
-    const int64_t e = kc ? (int64_t)x0 * ld + k : (int64_t)k * ld + x0;
-    return static_cast<const char*>(p) + e * (int64_t)sizeof(T);
-  };
+  Cursor<T, LAYOUT, kGated> next;
+  next.init(g, m0, n0, z, s_begin, 1);
   chunk16 rp[DIRECT ? 1 : PT::kLoads], rq[kSubs][DIRECT ? 1 : QT::kLoads];
-  auto load = [&](int s, char* lp, char* lq) {
-    const int piece = s >= per_piece ? 1 : 0;
-    const int k = (s - piece * per_piece) * kStageK, k_left = g.K - k;
-    const char* bp = base_of(g.p[piece], g.ld_p, P_KC, m0, k);
-    const char* bq[kSubs];
-#pragma unroll
-    for (int i = 0; i < kSubs; ++i)
-      bq[i] = base_of(g.q[kGated ? i : LAYOUT == OP_TN ? z : piece], g.ld_q, Q_KC, n0, k);
+  auto load = [&](char* to) {  // the next stage
+    const int k_left = g.K - next.k;
     if constexpr (DIRECT) {
+      const uint32_t lp = op_lds_byte(to), lq = lp + PT::kBytes;
       if (k_left >= kStageK) {
-        pt.issue(bp, lp, wave);
+        pt.issue(next.p, lp, wave);
 #pragma unroll
-        for (int i = 0; i < kSubs; ++i) qt.issue(bq[i], lq + i * QT::kBytes, wave);
+        for (int i = 0; i < kSubs; ++i) qt.issue(next.q[i], lq + i * QT::kBytes, wave);
       } else {
-        pt.issue_tail(bp, lp, wave, lane, k_left);
+        pt.issue_tail(next.p, lp, wave, lane, k_left);
 #pragma unroll
-        for (int i = 0; i < kSubs; ++i) qt.issue_tail(bq[i], lq + i * QT::kBytes, wave, lane, k_left);
+        for (int i = 0; i < kSubs; ++i) qt.issue_tail(next.q[i], lq + i * QT::kBytes, wave, lane, k_left);
       }
     } else {
-      pt.fetch(bp, rp, wave, lane, p_left, k_left);
+      pt.fetch(next.p, rp, wave, lane, p_left, k_left);
 #pragma unroll
-      for (int i = 0; i < kSubs; ++i) qt.fetch(bq[i], rq[i], wave, lane, q_left, k_left);
+      for (int i = 0; i < kSubs; ++i) qt.fetch(next.q[i], rq[i], wave, lane, q_left, k_left);
     }
-  };
-  auto put = [&](char* lp, char* lq) {
-    if constexpr (!DIRECT) {
-      pt.put(rp, lp, wave, lane);
-#pragma unroll
-      for (int i = 0; i < kSubs; ++i) qt.put(rq[i], lq + i * QT::kBytes, wave, lane);
-    }
+    next.advance(g);
   };
 
   floatx4 acc[TM][TN];
@@ -342,7 +470,8 @@ __global__ void __launch_bounds__(WGM* WGN * 64) op_gemm_tiled(OpGemm g) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  auto compute = [&](const char* lp, const char* lq) {
+  auto compute = [&](const char* from) {
+    const char* lq = from + PT::kBytes;
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
       chunk16 fp[TM], fq[TN];
@@ -350,87 +479,259 @@ __global__ void __launch_bounds__(WGM* WGN * 64) op_gemm_tiled(OpGemm g) {
       for (int j = 0; j < TN; ++j)
         fq[j] = QT::frag(lq + (j / TNS) * QT::kBytes, (wn * TNS + j % TNS) * 16, kk, lane);
 #pragma unroll
-      for (int i = 0; i < TM; ++i) fp[i] = PT::frag(lp, wm * WM + i * 16, kk, lane);
+      for (int i = 0; i < TM; ++i) fp[i] = PT::frag(from, wm * WM + i * 16, kk, lane);
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = Mfma<T>::mul(fq[j], fp[i], acc[i][j]);
     }
   };
-  // Stage s has arrived (its loads, or its chunks from registers), and every
-  // wave has finished reading the other pair of arrays.
-  auto arrived = [&](char* lp, char* lq) {
-    if constexpr (DIRECT) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    } else {
-      put(lp, lq);
+
+  if constexpr (DIRECT) {
+    op_unroll<NST - 1>([&](auto i) {
+      if (s_begin + i < s_end) load(stage(i));
+    });
+    for (int s0 = s_begin; s0 < s_end; s0 += NST) {
+      op_unroll<NST>([&](auto i) {
+        const int s = s0 + i;
+        if (s >= s_end) return;
+        // stage s is there once only the newer stages' loads are in flight;
+        // behind the barrier it is there for every wave, and every wave has
+        // finished reading stage s - 1, whose place the next loads take
+        if (s + NST - 2 < s_end) op_wait_loads<(NST - 2) * kStageLoads>();
+        else op_wait_loads<0>();
+        op_wait_lds();
+        op_barrier();
+        if (s + NST - 1 < s_end) load(stage(std::integral_constant<int, decltype(i)::value + NST - 1>()));
+        __builtin_amdgcn_sched_barrier(0);
+        compute(stage(i));
+      });
     }
-    __syncthreads();
+  } else {
+    auto put = [&](char* to) {
+      pt.put(rp, to, wave, lane);
+#pragma unroll
+      for (int i = 0; i < kSubs; ++i) qt.put(rq[i], to + PT::kBytes + i * QT::kBytes, wave, lane);
+      __syncthreads();
+    };
+    if (s_begin < s_end) load(lds);
+    for (int s0 = s_begin; s0 < s_end; s0 += 2) {
+      op_unroll<2>([&](auto i) {
+        const int s = s0 + i;
+        if (s >= s_end) return;
+        put(stage(i));
+        if (s + 1 < s_end) load(lds);
+        __builtin_amdgcn_sched_barrier(0);
+        compute(stage(i));
+      });
+    }
+  }
+
+  __syncthreads();  // the ring is free
+  static_assert(NW * op_region_bytes<TM, TN> <= NST * kStageBytes, "regions fit the ring");
+  op_write_out<T, KIND>(g, acc, lds + wave * op_region_bytes<TM, TN>, lane, m0 + wm * WM, n0 + wn * (TNS * 16), z, split);
+}
+
+// ---------------------------------------------------------------------------
+// Large product, 16 bits: 256x256 of D per block, eight waves (2 x 4, each
+// 128x64), two stages of k in LDS in four regions each -- the halves of P's
+// rows and Q's columns that a wave multiplies apart:
+//
+//   region P0, P1: rows 0..63 and 64..127 of each of the two wave rows
+//   region Q0, Q1: columns 0..31 and 32..63 of each of the four wave columns
+//                  (gated: the gate's and the up matrix's 32 columns)
+//
+// A stage is two phases of 32 matrix instructions; each reads what it
+// multiplies, issues the loads that overwrite regions read two phases ago or
+// in the one before, and multiplies:
+//
+//   phase   reads             loads                  multiplies
+//     0     P0, Q0, Q1 of s   Q1 and P1 of s + 1     P0 by Q0, Q1
+//     1     P1 of s           Q0 and P0 of s + 2     P1 by Q0, Q1
+//
+// The waves of the second row start half a phase later, so that of the two
+// waves of a SIMD one reads LDS while the other multiplies.  Behind a region
+// that is to be read, three or four more regions' loads stay in flight (48 or
+// 64 KB); the wait is for the older ones alone.  (Four phases of 16
+// instructions with a region each measured 4 to 12 % slower: the barrier
+// between two phases costs about 90 cycles.)
+// ---------------------------------------------------------------------------
+template <typename T, bool KC, int BLK, int STRIDE>
+struct Region : Tile<T, 128, KC, 8> {
+  using Base = Tile<T, 128, KC, 8>;
+  // Row or column j of the region is x0 + (j / BLK) STRIDE + j % BLK of the matrix.
+  __device__ __forceinline__ void init(int64_t ld, int x0, int left, int wave, int lane) {
+#pragma unroll
+    for (int t = 0; t < Base::kLoads; ++t) {
+      int r, c;
+      Base::place((wave + t * 8) * 64 + lane, &r, &c);
+      if constexpr (KC) {
+        r = min(x0 + r / BLK * STRIDE + r % BLK, left - 1);
+        this->off[t] = (uint32_t)r * (uint32_t)(ld * Base::kElem) + (uint32_t)c * 16u;
+      } else {
+        const int j = c * Base::kE;
+        c = min(x0 + j / BLK * STRIDE + j % BLK, (left - 1) / Base::kE * Base::kE);
+        this->off[t] = (uint32_t)r * (uint32_t)(ld * Base::kElem) + (uint32_t)(c * Base::kElem);
+      }
+    }
+  }
+};
+
+template <typename T, int LAYOUT, int KIND>
+__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) op_gemm_large(OpGemm g) {
+  constexpr bool kGated = KIND == OP_GATED, P_KC = LAYOUT != OP_TN, Q_KC = LAYOUT == OP_NT;
+  constexpr int kRegion = 128 * 128, kStageK = 64, SN = kGated ? 128 : 256;
+  using PR = Region<T, P_KC, 64, 128>;
+  using QR = Region<T, Q_KC, kGated ? 128 : 32, kGated ? 128 : 64>;
+  static_assert(PR::kBytes == kRegion && PR::kLoads == 2, "two loads a wave and region");
+  __shared__ __attribute__((aligned(16))) char lds[8 * kRegion];  // [stage & 1][P0, P1, Q0, Q1]
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 2, wn = wave & 3;
+  int tm, tn;
+  op_tile_of(blockIdx.x, g.tiles_m, g.tiles_n, &tm, &tn);
+  const int m0 = tm * 256, n0 = tn * SN;
+  const int z = g.outputs > 1 ? blockIdx.z : 0, split = blockIdx.y;
+  PR pr[2];
+  QR qr[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    pr[h].init(g.ld_p, h * 64, g.M - m0, wave, lane);
+    qr[h].init(g.ld_q, kGated ? 0 : h * 32, g.N - n0, wave, lane);
+  }
+  const int per_piece = (g.K + kStageK - 1) / kStageK;
+  const int s_begin = split * g.stages_per_split;
+  const int S = min(per_piece * g.pieces, s_begin + g.stages_per_split) - s_begin;
+
+  auto at = [&](int buf, int region) { return lds + (buf * 4 + region) * kRegion; };
+  // two cursors: the halves are loaded in different phases
+  Cursor<T, LAYOUT, kGated> next[2];
+  next[0].init(g, m0, n0, z, s_begin, 1);
+  next[1].init(g, m0, n0, z, s_begin, 1);
+  // P and Q halves h of the next stage of their cursor
+  auto load = [&](int buf, auto half) {
+    constexpr int h = decltype(half)::value;
+    const uint32_t tp = op_lds_byte(at(buf, h)), tq = op_lds_byte(at(buf, 2 + h));
+    const int k_left = g.K - next[h].k;
+    const char* q = next[h].q[kGated ? h : 0];
+    if (k_left >= kStageK) {
+      qr[h].issue(q, tq, wave);
+      pr[h].issue(next[h].p, tp, wave);
+    } else {
+      qr[h].issue_tail(q, tq, wave, lane, k_left);
+      pr[h].issue_tail(next[h].p, tp, wave, lane, k_left);
+    }
+    next[h].advance(g);
+  };
+  floatx4 acc[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  chunk16 fp[4][2], fq[4][2];
+
+  auto read_p = [&](const char* from) {
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) fp[i][kk] = PR::frag(from, wm * 64 + i * 16, kk, lane);
+  };
+  auto read_q = [&](const char* from, int h) {
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) fq[2 * h + j][kk] = QR::frag(from, wn * 32 + j * 16, kk, lane);
+  };
+  auto mul = [&](int half, int h) {
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 2 * h; j < 2 * h + 2; ++j)
+          acc[half * 4 + i][j] = Mfma<T>::mul(fq[j][kk], fp[i][kk], acc[half * 4 + i][j]);
+  };
+#define VOLTA_N(X) std::integral_constant<int, X>()
+  auto stage = [&](int s, auto buf) {
+    constexpr int B = decltype(buf)::value;
+    const int left = S - 1 - s;  // stages behind this one
+    read_q(at(B, 2), 0);
+    read_p(at(B, 0));
+    if (left >= 1) {
+      load(1 - B, VOLTA_N(1));
+      op_wait_loads<8>();  // P1 of s is there
+    } else {
+      op_wait_loads<0>();
+    }
+    op_wait_lds();
+    op_barrier();
+    read_q(at(B, 3), 1);  // arrives while Q0 is multiplied
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+    mul(0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    mul(0, 1);
+    __builtin_amdgcn_s_setprio(0);
+    op_barrier();
+    read_p(at(B, 1));
+    if (left >= 2) {
+      load(B, VOLTA_N(0));
+      op_wait_loads<6>();  // P0, Q0 and Q1 of s + 1 are there
+    } else {
+      op_wait_loads<2>();
+    }
+    op_wait_lds();
+    op_barrier();
+    __builtin_amdgcn_s_setprio(1);
+    mul(1, 0);
+    mul(1, 1);
+    __builtin_amdgcn_s_setprio(0);
+    op_barrier();
   };
 
-  if (s_begin < s_end) load(s_begin, lds_p0, lds_q0);
-  for (int s = s_begin; s < s_end; s += 2) {
-    arrived(lds_p0, lds_q0);
-    if (s + 1 < s_end) load(s + 1, lds_p1, lds_q1);
-    __builtin_amdgcn_sched_barrier(0);
-    compute(lds_p0, lds_q0);
-    if (s + 1 < s_end) {
-      arrived(lds_p1, lds_q1);
-      if (s + 2 < s_end) load(s + 2, lds_p0, lds_q0);
-      __builtin_amdgcn_sched_barrier(0);
-      compute(lds_p1, lds_q1);
+  if (S > 0) {
+    load(0, VOLTA_N(0));
+    load(0, VOLTA_N(1));
+    if (S > 1) {
+      load(1, VOLTA_N(0));
+      op_wait_loads<6>();  // P0, Q0 and Q1 of the first stage are there
+    } else {
+      op_wait_loads<2>();
     }
-  }
-
-  // Lane: row l % 16 of its block, columns 4 (l / 16) ..
-  const int all_flags = op_epilogue_flags<KIND>(g.epi);
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int m = m0 + wm * WM + i * 16 + (lane & 15);
-    if (m >= g.M) continue;
-#pragma unroll
-    for (int j = 0; j < TNS; ++j) {
-      const int n = n0 + (wn * TNS + j) * 16 + (lane >> 4) * 4, cnt = min(4, g.N - n);
-      if (cnt <= 0) continue;
-      float d0[4], d1[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        d0[r] = acc[i][j][r];
-        d1[r] = kGated ? acc[i][j + TNS * (kSubs - 1)][r] : 0.0f;
-      }
-      // asked anew for each block: the compiler would else make a copy of all
-      // blocks' epilogues for each answer, and spill the sums on the way there
-      int flags = all_flags;
-      asm volatile("" : "+s"(flags));
-      if (g.splits > 1) {
-        const int64_t planes = kGated ? 2 : g.outputs;
-        float* p = g.partial + ((split * planes + z) * g.M + m) * (int64_t)g.N + n;
-        store_partial(p, g.N, cnt, d0);
-        if constexpr (kGated) store_partial(p + (int64_t)g.M * g.N, g.N, cnt, d1);
-      } else {
-        op_epilogue<T, KIND>(g.epi, flags, z, m, n, cnt, d0, d1);
-      }
-      __builtin_amdgcn_sched_barrier(0);  // one block's values in flight
+    op_barrier();
+    if (wm == 1) op_barrier();
+    for (int s = 0; s < S; s += 2) {
+      stage(s, VOLTA_N(0));
+      if (s + 1 < S) stage(s + 1, VOLTA_N(1));
     }
+    if (wm == 0) op_barrier();
   }
+#undef VOLTA_N
+  __syncthreads();  // the regions are free
+  static_assert(8 * op_region_bytes<8, 4> <= 8 * kRegion, "output regions fit");
+  op_write_out<T, KIND>(g, acc, lds + wave * op_region_bytes<8, 4>, lane, m0 + wm * 128, n0 + wn * (kGated ? 32 : 64), z,
+                        split);
 }
 
 // ---------------------------------------------------------------------------
 // Skinny product, M <= 16 MT: each weight is read once and bounds the time.
 // A block takes 32 columns (of each weight matrix) and its waves take turns
-// over the stages of k, each with stages of its own in LDS (no barrier before
-// the end); the waves' sums are added at the end, in wave order.
+// over the stages of k, each with a ring of its own in LDS for both operands
+// (no barrier before the end); the waves' sums are added at the end, in wave
+// order.
 // ---------------------------------------------------------------------------
 template <typename T, int LAYOUT, int KIND, int MT, int NW, int NST, bool DIRECT>
 __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
   constexpr bool kGated = KIND == OP_GATED, Q_KC = LAYOUT == OP_NT;
   constexpr int kSubs = kGated ? 2 : 1, BN = 32, TN = 2 * kSubs;
+  using PT = Tile<T, 16 * MT, true, 1>;
   using QT = Tile<T, BN, Q_KC, 1>;
-  constexpr int kStageK = QT::kStageK, kE = QT::kE;
-  constexpr int kWaveBytes = QT::kBytes * kSubs;
-  constexpr int kSumBytes = NW * MT * TN * 1024;
-  constexpr int kLds = NW * NST * kWaveBytes;
-  __shared__ __attribute__((aligned(16))) char lds[kLds > kSumBytes ? kLds : kSumBytes];
+  constexpr int kStageK = QT::kStageK;
+  constexpr int kWaveBytes = PT::kBytes + QT::kBytes * kSubs;
+  constexpr int kStageLoads = PT::kLoads + QT::kLoads * kSubs;
+  static_assert(DIRECT ? NST >= 2 : NST == 1, "ring");
+  __shared__ __attribute__((aligned(16))) char lds[NST * NW * kWaveBytes];
 
   const int tid = threadIdx.x, lane = tid & 63, l = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -438,51 +739,38 @@ __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
   int tm, tn;
   op_tile_of(blockIdx.x, 1, g.tiles_n, &tm, &tn);
   const int n0 = tn * BN, split = blockIdx.y, q_left = g.N - n0;
+  PT pt;
   QT qt;
+  pt.init(g.ld_p, g.M, 0, lane);
   qt.init(g.ld_q, q_left, 0, lane);
   const int per_piece = (g.K + kStageK - 1) / kStageK;
   const int s_begin = split * g.stages_per_split;
   const int s_end = min(per_piece * g.pieces, s_begin + g.stages_per_split);
   char* mine = lds + wave * (NST * kWaveBytes);
+  auto ring = [&](auto turn) { return mine + decltype(turn)::value % NST * kWaveBytes; };
 
-  int64_t p_row[MT];
+  chunk16 rp[DIRECT ? 1 : PT::kLoads], rq[kSubs][DIRECT ? 1 : QT::kLoads];
+  Cursor<T, LAYOUT, kGated> next;
+  next.init(g, 0, n0, 0, s_begin + wave, NW);
+  auto load = [&](auto turn) {  // this wave's next stage
+    const int k_left = g.K - next.k;
+    if constexpr (DIRECT) {
+      const uint32_t lp = op_lds_byte(ring(turn)), lq = lp + PT::kBytes;
+      if (k_left >= kStageK) {
 #pragma unroll
-  for (int i = 0; i < MT; ++i) p_row[i] = (int64_t)min(i * 16 + l, g.M - 1) * g.ld_p;
-
-  chunk16 fp[NST][MT][2];
-  chunk16 rq[DIRECT ? 1 : NST][kSubs][DIRECT ? 1 : QT::kLoads];
-  auto load = [&](int s, int slot) {
-    const int piece = s >= per_piece ? 1 : 0;
-    const int k = (s - piece * per_piece) * kStageK, k_left = g.K - k;
-    char* to = mine + slot * kWaveBytes;
-#pragma unroll
-    for (int i = 0; i < kSubs; ++i) {
-      const char* base = static_cast<const char*>(g.q[kGated ? i : piece]) +
-                         (Q_KC ? (int64_t)n0 * g.ld_q + k : (int64_t)k * g.ld_q + n0) * (int64_t)sizeof(T);
-      if constexpr (DIRECT) {
-        if (k_left >= kStageK) qt.issue(base, to + i * QT::kBytes, 0);
-        else qt.issue_tail(base, to + i * QT::kBytes, 0, lane, k_left);
+        for (int i = 0; i < kSubs; ++i) qt.issue(next.q[i], lq + i * QT::kBytes, 0);
+        pt.issue(next.p, lp, 0);
       } else {
-        qt.fetch(base, rq[slot][i], 0, lane, q_left, k_left);
+#pragma unroll
+        for (int i = 0; i < kSubs; ++i) qt.issue_tail(next.q[i], lq + i * QT::kBytes, 0, lane, k_left);
+        pt.issue_tail(next.p, lp, 0, lane, k_left);
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kSubs; ++i) qt.fetch(next.q[i], rq[i], 0, lane, q_left, k_left);
+      pt.fetch(next.p, rp, 0, lane, g.M, k_left);
     }
-    const T* p = static_cast<const T*>(g.p[piece]) + k;
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        const int c = (4 * kk + lg) * kE, have = k_left - c;
-        const T* a = p + p_row[i] + c;
-        if constexpr (DIRECT) {
-          // always one load, so that the loads in flight can be counted
-          const void* from = have > 0 ? (const void*)a : (const void*)op_zeros;
-          fp[slot][i][kk] = *(const VOLTA_GLOBAL chunk16*)from;
-        } else {
-          if (have >= kE) fp[slot][i][kk] = load_unaligned(a);
-          else if (have <= 0) fp[slot][i][kk] = chunk16{0, 0, 0, 0};
-          else fp[slot][i][kk] = load_part(a, have);
-        }
-      }
+    next.advance(g);
   };
 
   floatx4 acc[MT][TN];
@@ -491,74 +779,78 @@ __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  auto compute = [&](int slot) {
-    char* from = mine + slot * kWaveBytes;
-    if constexpr (!DIRECT) {
-#pragma unroll
-      for (int i = 0; i < kSubs; ++i) qt.put(rq[slot][i], from + i * QT::kBytes, 0, lane);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
+  auto compute = [&](const char* from) {
+    const char* lq = from + PT::kBytes;
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
-      chunk16 fq[TN];
+      chunk16 fq[TN], fp[MT];
 #pragma unroll
-      for (int j = 0; j < TN; ++j) fq[j] = QT::frag(from + (j >> 1) * QT::kBytes, (j & 1) * 16, kk, lane);
+      for (int j = 0; j < TN; ++j) fq[j] = QT::frag(lq + (j >> 1) * QT::kBytes, (j & 1) * 16, kk, lane);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) fp[i] = PT::frag(from, i * 16, kk, lane);
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = Mfma<T>::mul(fq[j], fp[slot][i][kk], acc[i][j]);
+        for (int j = 0; j < TN; ++j) acc[i][j] = Mfma<T>::mul(fq[j], fp[i], acc[i][j]);
     }
   };
 
-  // This wave's stages: s_begin + wave, + NW, ...  NST - 1 of them in flight.
-  int next = s_begin + wave;
-#pragma unroll
-  for (int i = 0; i < NST - 1; ++i, next += NW)
-    if (next < s_end) load(next, i);
-  for (int s = s_begin + wave; s < s_end; s += NST * NW) {
-#pragma unroll
-    for (int i = 0; i < NST; ++i) {
-      const int cur = s + i * NW;
-      if (cur < s_end) {
-        // the slot this overwrites was read one turn ago
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        const bool more = next < s_end;
-        if (more) load(next, (i + NST - 1) % NST);
-        next += NW;
-        if constexpr (DIRECT) {
-          // loads return in order: all but the newer stages' have to be back
-          constexpr int kOps = kSubs * QT::kLoads + MT * 2;
-          if (next - NW < s_end) {  // a full ring is in flight
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * kOps) : "memory");
-          } else {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-          }
+  // This wave's stages: s_begin + wave, + NW, ...
+  if constexpr (DIRECT) {  // NST - 1 of them in flight
+    op_unroll<NST - 1>([&](auto i) {
+      if (s_begin + wave + i * NW < s_end) load(i);
+    });
+    for (int s0 = s_begin + wave; s0 < s_end; s0 += NST * NW) {
+      op_unroll<NST>([&](auto i) {
+        const int s = s0 + i * NW;
+        if (s >= s_end) return;
+        op_wait_lds();  // what the next loads overwrite was read one turn ago
+        __builtin_amdgcn_sched_barrier(0);
+        // the stage is there once only the newer stages' loads are in flight
+        if (s + (NST - 1) * NW < s_end) {
+          load(std::integral_constant<int, decltype(i)::value + NST - 1>());
+          op_wait_loads<(NST - 1) * kStageLoads>();
+        } else {
+          op_wait_loads<0>();
         }
-        compute(i);
-      }
+        __builtin_amdgcn_sched_barrier(0);
+        compute(ring(i));
+      });
+    }
+  } else {
+    constexpr auto only = std::integral_constant<int, 0>();
+    if (s_begin + wave < s_end) load(only);
+    for (int s = s_begin + wave; s < s_end; s += NW) {
+      pt.put(rp, mine, 0, lane);
+#pragma unroll
+      for (int i = 0; i < kSubs; ++i) qt.put(rq[i], mine + PT::kBytes + i * QT::kBytes, 0, lane);
+      if (s + NW < s_end) load(only);
+      __builtin_amdgcn_sched_barrier(0);
+      compute(mine);
     }
   }
 
-  // Add the waves' sums: [wave][block][lane] of four floats.
-  __syncthreads();
+  // Add the waves' sums, 16 rows at a time: [wave][block][lane] of four floats.
   floatx4* sums = reinterpret_cast<floatx4*>(lds);
+  const int j = tid >> 6 & 1, n = n0 + j * 16 + lg * 4, cnt = g.N - n;  // of the threads that add
+  float b0[4], b1[4];
+  if (g.splits <= 1) op_biases<T, KIND>(g.epi, n, cnt, b0, b1);
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+  for (int i = 0; i < MT; ++i) {
+    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < TN; ++j) sums[((wave * MT + i) * TN + j) * 64 + lane] = acc[i][j];
-  __syncthreads();
-  for (int t = tid; t < MT * 2 * 64; t += NW * 64) {
-    const int ln = t & 63, j = (t >> 6) & 1, i = t >> 7;
-    floatx4 a = sums[(i * TN + j) * 64 + ln], b = {};
+    for (int c = 0; c < TN; ++c) sums[(wave * TN + c) * 64 + lane] = acc[i][c];
+    __syncthreads();
+    const int m = i * 16 + l;
+    if (tid >= 128 || m >= g.M || cnt <= 0) continue;
+    floatx4 a = sums[j * 64 + lane], b = {};
 #pragma unroll
-    for (int w = 1; w < NW; ++w) a = a + sums[((w * MT + i) * TN + j) * 64 + ln];
+    for (int w = 1; w < NW; ++w) a = a + sums[(w * TN + j) * 64 + lane];
     if constexpr (kGated) {
-      b = sums[(i * TN + j + 2) * 64 + ln];
+      b = sums[(j + 2) * 64 + lane];
 #pragma unroll
-      for (int w = 1; w < NW; ++w) b = b + sums[((w * MT + i) * TN + j + 2) * 64 + ln];
+      for (int w = 1; w < NW; ++w) b = b + sums[(w * TN + j + 2) * 64 + lane];
     }
-    const int m = i * 16 + (ln & 15), n = n0 + j * 16 + (ln >> 4) * 4, cnt = min(4, g.N - n);
-    if (m >= g.M || cnt <= 0) continue;
     float d0[4], d1[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -567,65 +859,91 @@ __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
     }
     if (g.splits > 1) {
       float* p = g.partial + ((int64_t)(split * kSubs) * g.M + m) * g.N + n;
-      store_partial(p, g.N, cnt, d0);
-      if constexpr (kGated) store_partial(p + (int64_t)g.M * g.N, g.N, cnt, d1);
+      store_vec(p, cnt, d0);
+      if constexpr (kGated) store_vec(p + (int64_t)g.M * g.N, cnt, d1);
     } else {
-      op_epilogue<T, KIND>(g.epi, op_epilogue_flags<KIND>(g.epi), 0, m, n, cnt, d0, d1);
+      op_epilogue<T, KIND>(g.epi, 0, m, n, cnt, d0, d1, b0, b1);
     }
   }
 }
 
 // The splits' partial sums, added in order, and the epilogue: a thread for
-// four columns of a row.
+// four columns of a row.  Eight splits' sums are loaded at a time.
 template <typename T, int KIND>
 __global__ void __launch_bounds__(256) op_gemm_reduce(OpGemm g) {
   const int quads = (g.N + 3) / 4, z = blockIdx.y;
   const int64_t t = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
   if (t >= (int64_t)g.M * quads) return;
   const int64_t m = t / quads;
-  const int n = (int)(t - m * quads) * 4, cnt = min(4, g.N - n);
-  const bool vec = (g.N & 3) == 0;
+  const int n = (int)(t - m * quads) * 4, cnt = g.N - n;
   const int64_t plane = (int64_t)g.M * g.N, planes = KIND == OP_GATED ? 2 : g.outputs;
   const float* p = g.partial + z * plane + m * g.N + n;
-  float d0[4], d1[4] = {}, v[4];
-  load4(p, vec, cnt, d0);
-  if constexpr (KIND == OP_GATED) load4(p + plane, vec, cnt, d1);
-  for (int s = 1; s < g.splits; ++s) {
-    p += planes * plane;
-    load4(p, vec, cnt, v);
+  float d0[4] = {}, d1[4] = {}, b0[4], b1[4];
+  op_biases<T, KIND>(g.epi, n, cnt, b0, b1);
+  for (int s = 0; s < g.splits; s += 8) {
+    float v[8][4], w[8][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) d0[i] += v[i];
-    if constexpr (KIND == OP_GATED) {
-      load4(p + plane, vec, cnt, v);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) d1[i] += v[i];
+    for (int i = 0; i < 8; ++i) {
+      const bool in = s + i < g.splits;
+      const float* q = p + (in ? (s + i) * (planes * plane) : 0);
+      load_vec(q, cnt, v[i]);
+      if constexpr (KIND == OP_GATED) load_vec(q + plane, cnt, w[i]);
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (s + i < g.splits) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          d0[c] += v[i][c];
+          if constexpr (KIND == OP_GATED) d1[c] += w[i][c];
+        }
+      }
   }
-  op_epilogue<T, KIND>(g.epi, op_epilogue_flags<KIND>(g.epi), z, m, n, cnt, d0, d1);
+  op_epilogue<T, KIND>(g.epi, z, m, n, cnt, d0, d1, b0, b1);
 }
 
 // ---------------------------------------------------------------------------
-template <typename T, int LAYOUT, int KIND, int BM, int BN, int WGM, int WGN, bool DIRECT>
+template <typename T, int LAYOUT, int KIND, int BM, int BN, int WGM, int WGN, int NST, bool DIRECT>
 hipError_t launch_tiled(OpGemm& g, hipStream_t st) {
   constexpr int SN = KIND == OP_GATED ? BN / 2 : BN;
   g.tiles_m = (g.M + BM - 1) / BM;
   g.tiles_n = (g.N + SN - 1) / SN;
-  hipLaunchKernelGGL((op_gemm_tiled<T, LAYOUT, KIND, BM, BN, WGM, WGN, DIRECT>),
+  hipLaunchKernelGGL((op_gemm_tiled<T, LAYOUT, KIND, BM, BN, WGM, WGN, NST, DIRECT>),
                      dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits, (unsigned)g.outputs),
                      dim3(WGM * WGN * 64), 0, st, g);
   return hipGetLastError();
 }
 
-template <typename T, int LAYOUT, int KIND, int MT, bool DIRECT>
-hipError_t launch_skinny(OpGemm& g, hipStream_t st) {
-  g.tiles_m = 1;
-  g.tiles_n = (g.N + 31) / 32;
-  constexpr int NW = KIND == OP_GATED ? 4 : 8, NST = KIND == OP_GATED || !DIRECT ? 2 : 4;
-  hipLaunchKernelGGL((op_gemm_skinny<T, LAYOUT, KIND, MT, NW, NST, DIRECT>),
-                     dim3((unsigned)g.tiles_n, (unsigned)g.splits), dim3(NW * 64), 0, st, g);
+template <typename T, int LAYOUT, int KIND>
+hipError_t launch_large(OpGemm& g, hipStream_t st) {
+  constexpr int SN = KIND == OP_GATED ? 128 : 256;
+  g.tiles_m = (g.M + 255) / 256;
+  g.tiles_n = (g.N + SN - 1) / SN;
+  hipLaunchKernelGGL((op_gemm_large<T, LAYOUT, KIND>),
+                     dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits, (unsigned)g.outputs), dim3(512), 0, st,
+                     g);
   return hipGetLastError();
 }
 
+// Waves and ring of the skinny form: what fits a CU's 160 KB of LDS.
+template <int KIND, int MT, bool DIRECT>
+struct SkinnyShape {
+  static constexpr int kWaves = KIND == OP_GATED || MT > 1 ? 4 : 8;
+  static constexpr int kStages = !DIRECT ? 1 : KIND == OP_GATED ? (MT == 4 ? 2 : 3) : (MT == 2 ? 4 : 3);
+};
+template <typename T, int LAYOUT, int KIND, int MT, bool DIRECT>
+hipError_t launch_skinny(OpGemm& g, hipStream_t st) {
+  using S = SkinnyShape<KIND, MT, DIRECT>;
+  g.tiles_m = 1;
+  g.tiles_n = (g.N + 31) / 32;
+  hipLaunchKernelGGL((op_gemm_skinny<T, LAYOUT, KIND, MT, S::kWaves, S::kStages, DIRECT>),
+                     dim3((unsigned)g.tiles_n, (unsigned)g.splits), dim3(S::kWaves * 64), 0, st, g);
+  return hipGetLastError();
+}
+
+#ifndef VOLTA_NST128
+#define VOLTA_NST128 2
+#endif
 template <typename T, int LAYOUT, int KIND>
 hipError_t launch(const OpPlan& plan, OpGemm& g, hipStream_t st) {
   g.splits = plan.splits;
@@ -646,14 +964,14 @@ hipError_t launch(const OpPlan& plan, OpGemm& g, hipStream_t st) {
                       : launch_skinny<T, LAYOUT, KIND, 4, false>(g, st);
     }
   } else if (plan.tile == OP_TILE_256 && g.direct) {
-    if constexpr (sizeof(T) == 2) e = launch_tiled<T, LAYOUT, KIND, 256, 256, 2, 4, true>(g, st);
+    if constexpr (sizeof(T) == 2) e = launch_large<T, LAYOUT, KIND>(g, st);
     else return hipErrorInvalidValue;
   } else if (plan.tile == OP_TILE_64) {
-    e = g.direct ? launch_tiled<T, LAYOUT, KIND, 64, 64, 2, 2, true>(g, st)
-                 : launch_tiled<T, LAYOUT, KIND, 64, 64, 2, 2, false>(g, st);
+    e = g.direct ? launch_tiled<T, LAYOUT, KIND, 64, 64, 2, 2, 4, true>(g, st)
+                 : launch_tiled<T, LAYOUT, KIND, 64, 64, 2, 2, 2, false>(g, st);
   } else {
-    e = g.direct ? launch_tiled<T, LAYOUT, KIND, 128, 128, 2, 2, true>(g, st)
-                 : launch_tiled<T, LAYOUT, KIND, 128, 128, 2, 2, false>(g, st);
+    e = g.direct ? launch_tiled<T, LAYOUT, KIND, 128, 128, 2, 2, VOLTA_NST128, true>(g, st)
+                 : launch_tiled<T, LAYOUT, KIND, 128, 128, 2, 2, 2, false>(g, st);
   }
   if (e != hipSuccess || g.splits <= 1) return e;
   const int64_t quads = (int64_t)g.M * ((g.N + 3) / 4);

@@ -39,7 +39,7 @@ OpPlan op_gemm_plan(int elem_bytes, int layout, int kind, int64_t M, int64_t N, 
   if (M <= 64 && layout != OP_TN) {
     // A block's waves share its stages out; with few column blocks the sum is
     // split over blocks too, as long as every wave keeps four stages.
-    const int64_t blocks = ceil_div(N, 32), waves = kind == OP_GATED ? 4 : 8;
+    const int64_t blocks = ceil_div(N, 32), waves = kind == OP_GATED || M > 16 ? 4 : 8;
     const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(128 / blocks, stages / (4 * waves)));
     return split_plan(OP_TILE_SKINNY, splits);
   }

@@ -13,9 +13,6 @@ namespace volta {
 namespace ops {
 namespace {
 
-#define VOLTA_GLOBAL __attribute__((address_space(1)))
-typedef uint32_t chunk16_by2 __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t chunk16_by4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t chunk8_by1 __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint32_t chunk4_by1 __attribute__((aligned(1)));
 
@@ -30,47 +27,13 @@ __device__ __forceinline__ int64_t block_id() { return (int64_t)blockIdx.y * gri
 // The elements of one 16-byte access.
 template <typename T> constexpr int kChunk = 16 / (int)sizeof(T);
 
-// Elements p[0 .. cnt) as floats, the rest 0 (cnt <= 0: nothing is read).
 template <typename T>
 __device__ __forceinline__ void load_row(const T* p, int cnt, float (&f)[kChunk<T>]) {
-  constexpr int E = kChunk<T>;
-  union { chunk16 c; T e[E]; } u;
-  if (cnt >= E) {
-    if constexpr (sizeof(T) == 2) u.c = *(const VOLTA_GLOBAL chunk16_by2*)p;
-    else u.c = *(const VOLTA_GLOBAL chunk16_by4*)p;
-#pragma unroll
-    for (int i = 0; i < E; ++i) f[i] = to_f(u.e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < E; ++i) f[i] = i < cnt ? to_f(((const VOLTA_GLOBAL T*)p)[i]) : 0.0f;
-  }
+  load_vec(p, cnt, f);
 }
 template <typename T>
 __device__ __forceinline__ void store_row(T* p, int cnt, const float (&f)[kChunk<T>]) {
-  constexpr int E = kChunk<T>;
-  if (cnt >= E) {
-    union { chunk16 c; T e[E]; } u;
-#pragma unroll
-    for (int i = 0; i < E; ++i) u.e[i] = from_f<T>(f[i]);
-    if constexpr (sizeof(T) == 2) *(VOLTA_GLOBAL chunk16_by2*)p = u.c;
-    else *(VOLTA_GLOBAL chunk16_by4*)p = u.c;
-  } else {
-#pragma unroll
-    for (int i = 0; i < E; ++i)
-      if (i < cnt) ((VOLTA_GLOBAL T*)p)[i] = from_f<T>(f[i]);
-  }
-}
-// cnt floats of a row of 32-bit sums.
-template <int E>
-__device__ __forceinline__ void store_sums(float* p, int cnt, const float (&f)[E]) {
-  if (cnt >= E) {
-#pragma unroll
-    for (int i = 0; i < E / 4; ++i) store4u(p + 4 * i, floatx4{f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]});
-  } else {
-#pragma unroll
-    for (int i = 0; i < E; ++i)
-      if (i < cnt) p[i] = f[i];
-  }
+  store_vec(p, cnt, f);
 }
 // E (4 or 8) values as e4m3 codes, to the nearest.
 template <int E>
@@ -355,7 +318,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_grad_kernel(NormGr
   // a row of partial sums for each block's row in flight
   float* p = a.partial + ((int64_t)blockIdx.x * RPB + threadIdx.x / TPR) * a.cols;
 #pragma unroll
-  for (int k = 0; k < NCH; ++k) store_sums<E>(p + (t + k * TPR) * E, a.cols - (t + k * TPR) * E, dw[k]);
+  for (int k = 0; k < NCH; ++k) store_vec(p + (t + k * TPR) * E, a.cols - (t + k * TPR) * E, dw[k]);
 }
 
 // Rows too long for registers: dx row by row, read twice, and dweight column
@@ -418,7 +381,7 @@ __device__ __forceinline__ void strip_store(float (*lds)[64][kChunk<T>], const f
     float v[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) v[i] = ((lds[0][lane][i] + lds[1][lane][i]) + lds[2][lane][i]) + lds[3][lane][i];
-    store_sums<E>(partial + (int64_t)blockIdx.y * cols + c, cols - c, v);
+    store_vec(partial + (int64_t)blockIdx.y * cols + c, cols - c, v);
   }
 }
 

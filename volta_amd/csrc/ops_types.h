@@ -18,39 +18,55 @@ typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 // 16 bytes of a fragment or a chunk, whatever they hold.
 typedef uint32_t chunk16 __attribute__((ext_vector_type(4)));
 
-template <typename T>
-struct alignas(4 * sizeof(T)) Quad {
-  T v[4];
-};
-
 template <typename T> __device__ __forceinline__ float to_f(T x) { return (float)x; }
 template <typename T> __device__ __forceinline__ T from_f(float x) { return (T)x; }  // to the nearest, ties to even
 
-// Four consecutive elements as floats: one access where `vec` says that the
-// address allows it, else the first `cnt` one by one (the rest 0).
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, bool vec, int cnt, float (&f)[4]) {
-  if (vec) {
-    const Quad<T> q = *reinterpret_cast<const Quad<T>*>(p);
+// N consecutive elements of a row as floats, N a power of two, at any element
+// address (the memory pipeline takes unaligned accesses of up to 16 bytes);
+// only the first cnt are inside the row: the rest reads 0 and is not written.
+#define VOLTA_GLOBAL __attribute__((address_space(1)))
+template <int BYTES, int ALIGN> struct Access;
+#define VOLTA_ACCESS(BYTES, ALIGN, BASE, N) \
+  template <> struct Access<BYTES, ALIGN> { typedef BASE type __attribute__((ext_vector_type(N), aligned(ALIGN))); }
+VOLTA_ACCESS(16, 4, uint32_t, 4);
+VOLTA_ACCESS(16, 2, uint32_t, 4);
+VOLTA_ACCESS(8, 4, uint32_t, 2);
+VOLTA_ACCESS(8, 2, uint32_t, 2);
+VOLTA_ACCESS(4, 2, uint32_t, 1);
+#undef VOLTA_ACCESS
+template <typename T, int N>
+__device__ __forceinline__ void load_vec(const T* p, int cnt, float (&f)[N]) {
+  constexpr int B = N * (int)sizeof(T) < 16 ? N * (int)sizeof(T) : 16, E = B / (int)sizeof(T);
+  typedef typename Access<B, sizeof(T)>::type V;
+  if (cnt >= N) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = to_f(q.v[i]);
+    for (int c = 0; c < N / E; ++c) {
+      union { V v; T e[E]; } u;
+      u.v = *(const VOLTA_GLOBAL V*)(p + c * E);
+#pragma unroll
+      for (int i = 0; i < E; ++i) f[c * E + i] = to_f(u.e[i]);
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = i < cnt ? to_f(p[i]) : 0.0f;
+    for (int i = 0; i < N; ++i) f[i] = i < cnt ? to_f(((const VOLTA_GLOBAL T*)p)[i]) : 0.0f;
   }
 }
-
-template <typename T>
-__device__ __forceinline__ void store4(T* p, bool vec, int cnt, const float (&f)[4]) {
-  if (vec) {
-    Quad<T> q;
+template <typename T, int N>
+__device__ __forceinline__ void store_vec(T* p, int cnt, const float (&f)[N]) {
+  constexpr int B = N * (int)sizeof(T) < 16 ? N * (int)sizeof(T) : 16, E = B / (int)sizeof(T);
+  typedef typename Access<B, sizeof(T)>::type V;
+  if (cnt >= N) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) q.v[i] = from_f<T>(f[i]);
-    *reinterpret_cast<Quad<T>*>(p) = q;
+    for (int c = 0; c < N / E; ++c) {
+      union { V v; T e[E]; } u;
+#pragma unroll
+      for (int i = 0; i < E; ++i) u.e[i] = from_f<T>(f[c * E + i]);
+      *(VOLTA_GLOBAL V*)(p + c * E) = u.v;
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < cnt) p[i] = from_f<T>(f[i]);
+    for (int i = 0; i < N; ++i)
+      if (i < cnt) ((VOLTA_GLOBAL T*)p)[i] = from_f<T>(f[i]);
   }
 }
 
@@ -89,23 +105,23 @@ __device__ __forceinline__ float op_act(int act, float x) {
   }
 }
 
-// f of four values: the activation is asked once.
-template <typename T>
-__device__ __forceinline__ void op_act4(int act, float (&x)[4]) {
-#define VOLTA_ACT4(A)                                       \
+// f of N values: the activation is asked once.
+template <typename T, int N>
+__device__ __forceinline__ void op_act_all(int act, float (&x)[N]) {
+#define VOLTA_ACT_ALL(A)                                       \
   case A:                                                   \
-    _Pragma("unroll") for (int i = 0; i < 4; ++i) x[i] = op_act<T>(A, x[i]); \
+    _Pragma("unroll") for (int i = 0; i < N; ++i) x[i] = op_act<T>(A, x[i]); \
     break
   switch (act) {
-    VOLTA_ACT4(VOLTA_ACT_RELU);
-    VOLTA_ACT4(VOLTA_ACT_SIGMOID);
-    VOLTA_ACT4(VOLTA_ACT_TANH);
-    VOLTA_ACT4(VOLTA_ACT_LEAKY_RELU);
-    VOLTA_ACT4(VOLTA_ACT_SILU);
-    VOLTA_ACT4(VOLTA_ACT_GELU);
+    VOLTA_ACT_ALL(VOLTA_ACT_RELU);
+    VOLTA_ACT_ALL(VOLTA_ACT_SIGMOID);
+    VOLTA_ACT_ALL(VOLTA_ACT_TANH);
+    VOLTA_ACT_ALL(VOLTA_ACT_LEAKY_RELU);
+    VOLTA_ACT_ALL(VOLTA_ACT_SILU);
+    VOLTA_ACT_ALL(VOLTA_ACT_GELU);
     default: break;
   }
-#undef VOLTA_ACT4
+#undef VOLTA_ACT_ALL
 }
 
 // f and f' together (the gated layer's gradient needs both).

@@ -280,7 +280,6 @@ int32_t volta_hip_op_product(int32_t type, int32_t layout, int32_t kind, int32_t
   g.direct = direct;
   g.partial = static_cast<float*>(ws);
   g.epi.act = kind == OP_GATED ? VOLTA_ACT_SILU : VOLTA_OP_ACT_NONE;
-  g.epi.vec = ld_out % 4 == 0 && (uintptr_t)out0 % (4 * e) == 0 && (uintptr_t)out1 % (4 * e) == 0;
   g.epi.out[0] = out0;
   g.epi.out[1] = out1;
   g.epi.ld_out = ld_out;

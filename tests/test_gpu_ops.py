@@ -21,7 +21,7 @@ from volta_amd import load_hip, ops
 
 pytestmark = pytest.mark.gpu
 
-TILES = {"256": 0, "128": 1, "64": 2, "skinny": 3}
+TILES = {"256": 0, "128": 1, "64": 2, "skinny": 3, "64x128": 4}
 NN, NT, TN = 0, 1, 2
 LINEAR, GATED, STORE = 0, 1, 2
 U32 = 2.0**-24
@@ -97,7 +97,7 @@ def _forms(t):
         for kind in kinds:
             for tile in TILES:
                 for direct in (False, True):
-                    if tile == "256" and (t == "f32" or not direct):
+                    if (tile == "256" and t == "f32") or (tile in ("256", "64x128") and not direct):
                         continue
                     if tile == "skinny" and layout == TN:
                         continue

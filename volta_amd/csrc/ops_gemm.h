@@ -49,7 +49,7 @@ struct OpGemm {
 
 // Tiles, by rows x columns of D.  OP_TILE_SKINNY takes up to 64 rows and 32
 // columns (of each weight matrix), the sum over k shared out over its waves.
-enum OpTile { OP_TILE_256 = 0, OP_TILE_128 = 1, OP_TILE_64 = 2, OP_TILE_SKINNY = 3 };
+enum OpTile { OP_TILE_256 = 0, OP_TILE_128 = 1, OP_TILE_64 = 2, OP_TILE_SKINNY = 3, OP_TILE_64X128 = 4 };
 
 struct OpPlan {
   int32_t tile;

@@ -374,16 +374,24 @@ struct Cursor {
     if (piece) k -= piece_k(g);
     place(g);
   }
-  __device__ __forceinline__ void advance(const OpGemm& g) {
+  // Inside the piece, or into the next one.
+  __device__ __forceinline__ void step() {
     k += dk;
     p += dp;
 #pragma unroll
     for (int i = 0; i < kSubs; ++i) q[i] += dq;
+  }
+  __device__ __forceinline__ void cross(const OpGemm& g) {
     if (LAYOUT == OP_NT && g.pieces > 1 && piece == 0 && k >= piece_k(g)) {
       piece = 1;
       k -= piece_k(g);
       place(g);
     }
+  }
+  // Steps from here on whose stages are whole.
+  __device__ __forceinline__ int whole_steps(const OpGemm& g) const {
+    const int stages = (g.K - k) / kStageK;
+    return stages > 0 ? (stages - 1) / (dk / kStageK) + 1 : 0;
   }
 };
 
@@ -461,7 +469,8 @@ __global__ void __launch_bounds__(WGM* WGN * 64) op_gemm_tiled(OpGemm g) {
 #pragma unroll
       for (int i = 0; i < kSubs; ++i) qt.fetch(next.q[i], rq[i], wave, lane, q_left, k_left);
     }
-    next.advance(g);
+    next.step();
+    next.cross(g);
   };
 
   floatx4 acc[TM][TN];
@@ -604,25 +613,27 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) o
   const int s_begin = split * g.stages_per_split;
   const int S = min(per_piece * g.pieces, s_begin + g.stages_per_split) - s_begin;
 
-  auto at = [&](int buf, int region) { return lds + (buf * 4 + region) * kRegion; };
   // two cursors: the halves are loaded in different phases
   Cursor<T, LAYOUT, kGated> next[2];
   next[0].init(g, m0, n0, z, s_begin, 1);
   next[1].init(g, m0, n0, z, s_begin, 1);
-  // P and Q halves h of the next stage of their cursor
-  auto load = [&](int buf, auto half) {
+  // P and Q halves h of the next stage of their cursor to the stage at byte
+  // `to` of LDS; `whole`: it is, and in one piece
+  auto load = [&](uint32_t to, auto half, auto whole) {
     constexpr int h = decltype(half)::value;
-    const uint32_t tp = op_lds_byte(at(buf, h)), tq = op_lds_byte(at(buf, 2 + h));
-    const int k_left = g.K - next[h].k;
+    constexpr bool W = decltype(whole)::value;
+    const uint32_t tp = to + h * kRegion, tq = to + (2 + h) * kRegion;
+    const int k_left = W ? kStageK : g.K - next[h].k;
     const char* q = next[h].q[kGated ? h : 0];
-    if (k_left >= kStageK) {
+    if (W || k_left >= kStageK) {
       qr[h].issue(q, tq, wave);
       pr[h].issue(next[h].p, tp, wave);
     } else {
       qr[h].issue_tail(q, tq, wave, lane, k_left);
       pr[h].issue_tail(next[h].p, tp, wave, lane, k_left);
     }
-    next[h].advance(g);
+    next[h].step();
+    if constexpr (!W) next[h].cross(g);
   };
   floatx4 acc[8][4];
 #pragma unroll
@@ -652,21 +663,26 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) o
         for (int j = 2 * h; j < 2 * h + 2; ++j)
           acc[half * 4 + i][j] = Mfma<T>::mul(fq[j][kk], fp[i][kk], acc[half * 4 + i][j]);
   };
-#define VOLTA_N(X) std::integral_constant<int, X>()
-  auto stage = [&](int s, auto buf) {
-    constexpr int B = decltype(buf)::value;
+  constexpr auto H0 = std::integral_constant<int, 0>();
+  constexpr auto H1 = std::integral_constant<int, 1>();
+  const uint32_t lds_byte = op_lds_byte(lds);
+  int from = 0;  // byte of the stage in LDS
+  auto stage = [&](int s, auto whole) {
+    constexpr bool W = decltype(whole)::value;
+    const char* at = lds + from;
     const int left = S - 1 - s;  // stages behind this one
-    read_q(at(B, 2), 0);
-    read_p(at(B, 0));
-    if (left >= 1) {
-      load(1 - B, VOLTA_N(1));
+    read_q(at + 2 * kRegion, 0);
+    read_p(at);
+    __builtin_amdgcn_sched_barrier(0);
+    if (W || left >= 1) {
+      load(lds_byte + (from ^ 4 * kRegion), H1, whole);
       op_wait_loads<8>();  // P1 of s is there
     } else {
       op_wait_loads<0>();
     }
     op_wait_lds();
     op_barrier();
-    read_q(at(B, 3), 1);  // arrives while Q0 is multiplied
+    read_q(at + 3 * kRegion, 1);  // arrives while Q0 is multiplied
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(1);
     mul(0, 0);
@@ -674,13 +690,15 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) o
     mul(0, 1);
     __builtin_amdgcn_s_setprio(0);
     op_barrier();
-    read_p(at(B, 1));
-    if (left >= 2) {
-      load(B, VOLTA_N(0));
+    read_p(at + kRegion);
+    __builtin_amdgcn_sched_barrier(0);
+    if (W || left >= 2) {
+      load(lds_byte + from, H0, whole);
       op_wait_loads<6>();  // P0, Q0 and Q1 of s + 1 are there
     } else {
       op_wait_loads<2>();
     }
+    from ^= 4 * kRegion;
     op_wait_lds();
     op_barrier();
     __builtin_amdgcn_s_setprio(1);
@@ -691,27 +709,160 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) o
   };
 
   if (S > 0) {
-    load(0, VOLTA_N(0));
-    load(0, VOLTA_N(1));
+    constexpr auto any = std::false_type();
+    load(lds_byte, H0, any);
+    load(lds_byte, H1, any);
     if (S > 1) {
-      load(1, VOLTA_N(0));
+      load(lds_byte + 4 * kRegion, H0, any);
       op_wait_loads<6>();  // P0, Q0 and Q1 of the first stage are there
     } else {
       op_wait_loads<2>();
     }
     op_barrier();
     if (wm == 1) op_barrier();
-    for (int s = 0; s < S; s += 2) {
-      stage(s, VOLTA_N(0));
-      if (s + 1 < S) stage(s + 1, VOLTA_N(1));
+    for (int s = 0; s < S; ++s) {
+      // whole stages in a loop without a branch, the others one by one
+      for (int n = min(min(next[0].whole_steps(g), next[1].whole_steps(g)), S - 2 - s); n > 0; --n, ++s)
+        stage(s, std::true_type());
+      next[0].cross(g);
+      next[1].cross(g);
+      if (s < S) stage(s, any);
     }
     if (wm == 0) op_barrier();
   }
-#undef VOLTA_N
   __syncthreads();  // the regions are free
   static_assert(8 * op_region_bytes<8, 4> <= 8 * kRegion, "output regions fit");
   op_write_out<T, KIND>(g, acc, lds + wave * op_region_bytes<8, 4>, lane, m0 + wm * 128, n0 + wn * (kGated ? 32 : 64), z,
                         split);
+}
+
+// ---------------------------------------------------------------------------
+// Middle-sized product: BM x BN of D per block, eight waves (WGM x WGN), a
+// ring of NST stages of KS times 128 bytes of k in LDS.  As in the large form
+// the waves 4 to 7 run half a stage behind the waves 0 to 3, so that of a
+// SIMD's two waves one reads LDS while the other multiplies; a stage is one
+// phase.
+// ---------------------------------------------------------------------------
+template <typename T, int LAYOUT, int KIND, int BM, int BN, int WGM, int WGN, int KS, int NST>
+__global__ void __launch_bounds__(512) op_gemm_middle(OpGemm g) {
+  static_assert(WGM * WGN == 8, "eight waves");
+  constexpr int WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
+  constexpr bool kGated = KIND == OP_GATED, P_KC = LAYOUT != OP_TN, Q_KC = LAYOUT == OP_NT;
+  constexpr int kSubs = kGated ? 2 : 1, SN = BN / kSubs, TNS = TN / kSubs;
+  // 32 columns of each weight matrix are four load instructions: half of the waves load each
+  constexpr bool kHalves = kGated && SN < 64;
+  using PT = Tile<T, BM, P_KC, 8>;
+  using QT = Tile<T, SN, Q_KC, kHalves ? 4 : 8>;
+  constexpr int kStageK = PT::kStageK, kPart = PT::kBytes + QT::kBytes * kSubs, kStageBytes = KS * kPart;
+  constexpr int kStageLoads = KS * (PT::kLoads + QT::kLoads * (kHalves ? 1 : kSubs));
+  __shared__ __attribute__((aligned(16))) char lds[NST * kStageBytes];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WGN, wn = wave % WGN;
+  int tm, tn;
+  op_tile_of(blockIdx.x, g.tiles_m, g.tiles_n, &tm, &tn);
+  const int m0 = tm * BM, n0 = tn * SN;
+  const int z = g.outputs > 1 ? blockIdx.z : 0, split = blockIdx.y;
+  PT pt;
+  QT qt;
+  pt.init(g.ld_p, g.M - m0, wave, lane);
+  qt.init(g.ld_q, g.N - n0, kHalves ? wave & 3 : wave, lane);
+  const int s_begin = split * g.stages_per_split;
+  int parts = min((g.K + kStageK - 1) / kStageK * g.pieces, s_begin + g.stages_per_split) - s_begin;
+  const int S = (parts + KS - 1) / KS;
+  Cursor<T, LAYOUT, kGated> next;
+  next.init(g, m0, n0, z, s_begin, 1);
+  // The next stage to byte `to` of LDS; `whole`: it is, and in one piece.
+  auto load = [&](uint32_t to, auto whole) {
+    constexpr bool W = decltype(whole)::value;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      const int k_left = W ? kStageK : parts > i ? g.K - next.k : 0;  // a part behind the last one is zeros
+      const uint32_t lp = to + i * kPart, lq = lp + PT::kBytes;
+      if constexpr (kHalves) {
+        const char* q = wave < 4 ? next.q[0] : next.q[kSubs - 1];
+        const uint32_t half = lq + (wave < 4 ? 0 : QT::kBytes);
+        if (W || k_left >= kStageK) qt.issue(q, half, wave & 3);
+        else qt.issue_tail(q, half, wave & 3, lane, k_left);
+      } else {
+#pragma unroll
+        for (int w = 0; w < kSubs; ++w) {
+          if (W || k_left >= kStageK) qt.issue(next.q[w], lq + w * QT::kBytes, wave);
+          else qt.issue_tail(next.q[w], lq + w * QT::kBytes, wave, lane, k_left);
+        }
+      }
+      if (W || k_left >= kStageK) pt.issue(next.p, lp, wave);
+      else pt.issue_tail(next.p, lp, wave, lane, k_left);
+      next.step();
+      if constexpr (!W) next.cross(g);
+    }
+    parts -= KS;
+  };
+
+  floatx4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  chunk16 fp[TM][2 * KS], fq[TN][2 * KS];
+
+  // One stage, read at byte `from` of LDS; the next loads go where the stage
+  // before was, which every wave has read.
+  int from = 0, to = (NST - 1) * kStageBytes;
+  const uint32_t lds_byte = op_lds_byte(lds);
+  auto stage = [&](int s, auto whole) {
+    constexpr bool W = decltype(whole)::value;
+#pragma unroll
+    for (int kk = 0; kk < 2 * KS; ++kk) {
+      const char* part = lds + from + (kk >> 1) * kPart;
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        fq[j][kk] = QT::frag(part + PT::kBytes + (j / TNS) * QT::kBytes, (wn * TNS + j % TNS) * 16, kk & 1, lane);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) fp[i][kk] = PT::frag(part, wm * WM + i * 16, kk & 1, lane);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (W || s + NST - 1 < S) {
+      load(lds_byte + to, whole);
+      op_wait_loads<(NST - 2) * kStageLoads>();  // stage s + 1 is there
+    } else {
+      op_wait_loads<0>();
+    }
+    to = from;
+    from = from == (NST - 1) * kStageBytes ? 0 : from + kStageBytes;
+    op_wait_lds();
+    op_barrier();
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int kk = 0; kk < 2 * KS; ++kk)
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = Mfma<T>::mul(fq[j][kk], fp[i][kk], acc[i][j]);
+    __builtin_amdgcn_s_setprio(0);
+    op_barrier();
+  };
+
+  if (S > 0) {
+#pragma unroll 1
+    for (int i = 0; i < NST - 1 && i < S; ++i) load(lds_byte + i * kStageBytes, std::false_type());
+    if (S >= NST - 1) op_wait_loads<(NST - 2) * kStageLoads>();
+    else op_wait_loads<0>();
+    op_barrier();
+    if (wave >= 4) op_barrier();
+    for (int s = 0; s < S; ++s) {
+      // whole stages in a loop without a branch, the others one by one
+      for (int n = min(min(next.whole_steps(g), parts) / KS, S - (NST - 1) - s); n > 0; --n, ++s)
+        stage(s, std::true_type());
+      next.cross(g);
+      if (s < S) stage(s, std::false_type());
+    }
+    if (wave < 4) op_barrier();
+  }
+  __syncthreads();  // the ring is free
+  static_assert(8 * op_region_bytes<TM, TN> <= NST * kStageBytes, "output regions fit the ring");
+  op_write_out<T, KIND>(g, acc, lds + wave * op_region_bytes<TM, TN>, lane, m0 + wm * WM, n0 + wn * (TNS * 16), z, split);
 }
 
 // ---------------------------------------------------------------------------
@@ -721,10 +872,10 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) o
 // (no barrier before the end); the waves' sums are added at the end, in wave
 // order.
 // ---------------------------------------------------------------------------
-template <typename T, int LAYOUT, int KIND, int MT, int NW, int NST, bool DIRECT>
+template <typename T, int LAYOUT, int KIND, int MT, int BN, int NW, int NST, bool DIRECT>
 __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
   constexpr bool kGated = KIND == OP_GATED, Q_KC = LAYOUT == OP_NT;
-  constexpr int kSubs = kGated ? 2 : 1, BN = 32, TN = 2 * kSubs;
+  constexpr int kSubs = kGated ? 2 : 1, TNS = BN / 16, TN = TNS * kSubs;
   using PT = Tile<T, 16 * MT, true, 1>;
   using QT = Tile<T, BN, Q_KC, 1>;
   constexpr int kStageK = QT::kStageK;
@@ -747,30 +898,32 @@ __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
   const int s_begin = split * g.stages_per_split;
   const int s_end = min(per_piece * g.pieces, s_begin + g.stages_per_split);
   char* mine = lds + wave * (NST * kWaveBytes);
-  auto ring = [&](auto turn) { return mine + decltype(turn)::value % NST * kWaveBytes; };
 
   chunk16 rp[DIRECT ? 1 : PT::kLoads], rq[kSubs][DIRECT ? 1 : QT::kLoads];
   Cursor<T, LAYOUT, kGated> next;
   next.init(g, 0, n0, 0, s_begin + wave, NW);
-  auto load = [&](auto turn) {  // this wave's next stage
-    const int k_left = g.K - next.k;
+  // This wave's next stage, to byte `to` of LDS; `whole`: it is, and in one piece.
+  auto load = [&](uint32_t to, auto whole) {
+    constexpr bool W = decltype(whole)::value;
+    const int k_left = W ? kStageK : g.K - next.k;
     if constexpr (DIRECT) {
-      const uint32_t lp = op_lds_byte(ring(turn)), lq = lp + PT::kBytes;
-      if (k_left >= kStageK) {
+      const uint32_t lq = to + PT::kBytes;
+      if (W || k_left >= kStageK) {
 #pragma unroll
         for (int i = 0; i < kSubs; ++i) qt.issue(next.q[i], lq + i * QT::kBytes, 0);
-        pt.issue(next.p, lp, 0);
+        pt.issue(next.p, to, 0);
       } else {
 #pragma unroll
         for (int i = 0; i < kSubs; ++i) qt.issue_tail(next.q[i], lq + i * QT::kBytes, 0, lane, k_left);
-        pt.issue_tail(next.p, lp, 0, lane, k_left);
+        pt.issue_tail(next.p, to, 0, lane, k_left);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < kSubs; ++i) qt.fetch(next.q[i], rq[i], 0, lane, q_left, k_left);
       pt.fetch(next.p, rp, 0, lane, g.M, k_left);
     }
-    next.advance(g);
+    next.step();
+    if constexpr (!W) next.cross(g);
   };
 
   floatx4 acc[MT][TN];
@@ -785,7 +938,7 @@ __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
     for (int kk = 0; kk < 2; ++kk) {
       chunk16 fq[TN], fp[MT];
 #pragma unroll
-      for (int j = 0; j < TN; ++j) fq[j] = QT::frag(lq + (j >> 1) * QT::kBytes, (j & 1) * 16, kk, lane);
+      for (int j = 0; j < TN; ++j) fq[j] = QT::frag(lq + (j / TNS) * QT::kBytes, (j % TNS) * 16, kk, lane);
 #pragma unroll
       for (int i = 0; i < MT; ++i) fp[i] = PT::frag(from, i * 16, kk, lane);
 #pragma unroll
@@ -796,35 +949,41 @@ __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
   };
 
   // This wave's stages: s_begin + wave, + NW, ...
+  const int S = s_end > s_begin + wave ? (s_end - s_begin - wave + NW - 1) / NW : 0;
   if constexpr (DIRECT) {  // NST - 1 of them in flight
-    op_unroll<NST - 1>([&](auto i) {
-      if (s_begin + wave + i * NW < s_end) load(i);
-    });
-    for (int s0 = s_begin + wave; s0 < s_end; s0 += NST * NW) {
-      op_unroll<NST>([&](auto i) {
-        const int s = s0 + i * NW;
-        if (s >= s_end) return;
-        op_wait_lds();  // what the next loads overwrite was read one turn ago
-        __builtin_amdgcn_sched_barrier(0);
-        // the stage is there once only the newer stages' loads are in flight
-        if (s + (NST - 1) * NW < s_end) {
-          load(std::integral_constant<int, decltype(i)::value + NST - 1>());
-          op_wait_loads<(NST - 1) * kStageLoads>();
-        } else {
-          op_wait_loads<0>();
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        compute(ring(i));
-      });
+    const uint32_t lds_byte = op_lds_byte(mine);
+    int from = 0, to = (NST - 1) * kWaveBytes;
+    auto stage = [&](int s, auto whole) {
+      constexpr bool W = decltype(whole)::value;
+      op_wait_lds();  // what the next loads overwrite was read one turn ago
+      __builtin_amdgcn_sched_barrier(0);
+      // the stage is there once only the newer stages' loads are in flight
+      if (W || s + NST - 1 < S) {
+        load(lds_byte + to, whole);
+        op_wait_loads<(NST - 1) * kStageLoads>();
+      } else {
+        op_wait_loads<0>();
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      compute(mine + from);
+      to = from;
+      from = from == (NST - 1) * kWaveBytes ? 0 : from + kWaveBytes;
+    };
+#pragma unroll 1
+    for (int i = 0; i < NST - 1 && i < S; ++i) load(lds_byte + i * kWaveBytes, std::false_type());
+    for (int s = 0; s < S; ++s) {
+      for (int n = min(next.whole_steps(g), S - (NST - 1) - s); n > 0; --n, ++s) stage(s, std::true_type());
+      next.cross(g);
+      if (s < S) stage(s, std::false_type());
     }
   } else {
-    constexpr auto only = std::integral_constant<int, 0>();
-    if (s_begin + wave < s_end) load(only);
-    for (int s = s_begin + wave; s < s_end; s += NW) {
+    constexpr auto any = std::false_type();
+    if (S > 0) load(0, any);
+    for (int s = 0; s < S; ++s) {
       pt.put(rp, mine, 0, lane);
 #pragma unroll
       for (int i = 0; i < kSubs; ++i) qt.put(rq[i], mine + PT::kBytes + i * QT::kBytes, 0, lane);
-      if (s + NW < s_end) load(only);
+      if (s + 1 < S) load(0, any);
       __builtin_amdgcn_sched_barrier(0);
       compute(mine);
     }
@@ -832,9 +991,9 @@ __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
 
   // Add the waves' sums, 16 rows at a time: [wave][block][lane] of four floats.
   floatx4* sums = reinterpret_cast<floatx4*>(lds);
-  const int j = tid >> 6 & 1, n = n0 + j * 16 + lg * 4, cnt = g.N - n;  // of the threads that add
-  float b0[4], b1[4];
-  if (g.splits <= 1) op_biases<T, KIND>(g.epi, n, cnt, b0, b1);
+  // a wave adds the blocks wave, wave + NW, ... of the 16 columns each
+  constexpr int kTurns = (TNS + NW - 1) / NW;
+  static_assert(NW * TN * 1024 <= NST * NW * kWaveBytes, "sums fit the ring");
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     __syncthreads();
@@ -842,27 +1001,33 @@ __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
     for (int c = 0; c < TN; ++c) sums[(wave * TN + c) * 64 + lane] = acc[i][c];
     __syncthreads();
     const int m = i * 16 + l;
-    if (tid >= 128 || m >= g.M || cnt <= 0) continue;
-    floatx4 a = sums[j * 64 + lane], b = {};
+    if (m >= g.M) continue;
 #pragma unroll
-    for (int w = 1; w < NW; ++w) a = a + sums[(w * TN + j) * 64 + lane];
-    if constexpr (kGated) {
-      b = sums[(j + 2) * 64 + lane];
+    for (int u = 0; u < kTurns; ++u) {
+      const int j = wave + u * NW, n = n0 + j * 16 + lg * 4, cnt = g.N - n;
+      if (j >= TNS || cnt <= 0) continue;
+      floatx4 a = sums[j * 64 + lane], b = {};
 #pragma unroll
-      for (int w = 1; w < NW; ++w) b = b + sums[(w * TN + j + 2) * 64 + lane];
-    }
-    float d0[4], d1[4];
+      for (int w = 1; w < NW; ++w) a = a + sums[(w * TN + j) * 64 + lane];
+      if constexpr (kGated) {
+        b = sums[(j + TNS) * 64 + lane];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      d0[r] = a[r];
-      d1[r] = b[r];
-    }
-    if (g.splits > 1) {
-      float* p = g.partial + ((int64_t)(split * kSubs) * g.M + m) * g.N + n;
-      store_vec(p, cnt, d0);
-      if constexpr (kGated) store_vec(p + (int64_t)g.M * g.N, cnt, d1);
-    } else {
-      op_epilogue<T, KIND>(g.epi, 0, m, n, cnt, d0, d1, b0, b1);
+        for (int w = 1; w < NW; ++w) b = b + sums[(w * TN + j + TNS) * 64 + lane];
+      }
+      float d0[4], d1[4], b0[4], b1[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        d0[r] = a[r];
+        d1[r] = b[r];
+      }
+      if (g.splits > 1) {
+        float* p = g.partial + ((int64_t)(split * kSubs) * g.M + m) * g.N + n;
+        store_vec(p, cnt, d0);
+        if constexpr (kGated) store_vec(p + (int64_t)g.M * g.N, cnt, d1);
+      } else {
+        op_biases<T, KIND>(g.epi, n, cnt, b0, b1);
+        op_epilogue<T, KIND>(g.epi, 0, m, n, cnt, d0, d1, b0, b1);
+      }
     }
   }
 }
@@ -914,6 +1079,17 @@ hipError_t launch_tiled(OpGemm& g, hipStream_t st) {
   return hipGetLastError();
 }
 
+template <typename T, int LAYOUT, int KIND, int BM, int BN, int WGM, int WGN, int KS, int NST>
+hipError_t launch_middle(OpGemm& g, hipStream_t st) {
+  constexpr int SN = KIND == OP_GATED ? BN / 2 : BN;
+  g.tiles_m = (g.M + BM - 1) / BM;
+  g.tiles_n = (g.N + SN - 1) / SN;
+  hipLaunchKernelGGL((op_gemm_middle<T, LAYOUT, KIND, BM, BN, WGM, WGN, KS, NST>),
+                     dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits, (unsigned)g.outputs), dim3(512), 0, st,
+                     g);
+  return hipGetLastError();
+}
+
 template <typename T, int LAYOUT, int KIND>
 hipError_t launch_large(OpGemm& g, hipStream_t st) {
   constexpr int SN = KIND == OP_GATED ? 128 : 256;
@@ -926,24 +1102,29 @@ hipError_t launch_large(OpGemm& g, hipStream_t st) {
 }
 
 // Waves and ring of the skinny form: what fits a CU's 160 KB of LDS.
+#ifndef SK_BN
+#define SK_BN 32
+#define SK_W 8
+#define SK_S 3
+#define SK_GW 4
+#define SK_GS 3
+#endif
 template <int KIND, int MT, bool DIRECT>
 struct SkinnyShape {
-  static constexpr int kWaves = KIND == OP_GATED || MT > 1 ? 4 : 8;
-  static constexpr int kStages = !DIRECT ? 1 : KIND == OP_GATED ? (MT == 4 ? 2 : 3) : (MT == 2 ? 4 : 3);
+  static constexpr int kCols = SK_BN;
+  static constexpr int kWaves = KIND == OP_GATED ? (MT == 4 ? 2 : SK_GW) : MT > 1 ? 4 : SK_W;
+  static constexpr int kStages = !DIRECT ? 1 : KIND == OP_GATED ? (MT == 4 ? 2 : SK_GS) : (MT == 2 ? 3 : MT == 4 ? 2 : SK_S);
 };
 template <typename T, int LAYOUT, int KIND, int MT, bool DIRECT>
 hipError_t launch_skinny(OpGemm& g, hipStream_t st) {
   using S = SkinnyShape<KIND, MT, DIRECT>;
   g.tiles_m = 1;
-  g.tiles_n = (g.N + 31) / 32;
-  hipLaunchKernelGGL((op_gemm_skinny<T, LAYOUT, KIND, MT, S::kWaves, S::kStages, DIRECT>),
+  g.tiles_n = (g.N + S::kCols - 1) / S::kCols;
+  hipLaunchKernelGGL((op_gemm_skinny<T, LAYOUT, KIND, MT, S::kCols, S::kWaves, S::kStages, DIRECT>),
                      dim3((unsigned)g.tiles_n, (unsigned)g.splits), dim3(S::kWaves * 64), 0, st, g);
   return hipGetLastError();
 }
 
-#ifndef VOLTA_NST128
-#define VOLTA_NST128 2
-#endif
 template <typename T, int LAYOUT, int KIND>
 hipError_t launch(const OpPlan& plan, OpGemm& g, hipStream_t st) {
   g.splits = plan.splits;
@@ -967,10 +1148,13 @@ hipError_t launch(const OpPlan& plan, OpGemm& g, hipStream_t st) {
     if constexpr (sizeof(T) == 2) e = launch_large<T, LAYOUT, KIND>(g, st);
     else return hipErrorInvalidValue;
   } else if (plan.tile == OP_TILE_64) {
-    e = g.direct ? launch_tiled<T, LAYOUT, KIND, 64, 64, 2, 2, 4, true>(g, st)
+    constexpr int WGM = KIND == OP_GATED ? 4 : 2;  // a wave has columns of both weight matrices
+    e = g.direct ? launch_middle<T, LAYOUT, KIND, 64, 64, WGM, 8 / WGM, 2, 4>(g, st)
                  : launch_tiled<T, LAYOUT, KIND, 64, 64, 2, 2, 2, false>(g, st);
+  } else if (plan.tile == OP_TILE_64X128 && g.direct) {
+    e = launch_middle<T, LAYOUT, KIND, 64, 128, 2, 4, 1, 4>(g, st);
   } else {
-    e = g.direct ? launch_tiled<T, LAYOUT, KIND, 128, 128, 2, 2, VOLTA_NST128, true>(g, st)
+    e = g.direct ? launch_middle<T, LAYOUT, KIND, 128, 128, 2, 4, 1, 4>(g, st)
                  : launch_tiled<T, LAYOUT, KIND, 128, 128, 2, 2, 2, false>(g, st);
   }
   if (e != hipSuccess || g.splits <= 1) return e;

@@ -17,7 +17,8 @@ struct TileCost {
   double rate16, rate32;  // share of the matrix rate that a full CU reaches
 };
 // Measured on large products (bf16, float32).
-constexpr TileCost kTiles[3] = {{256, 256, 1, 0.50, 0.85}, {128, 128, 2, 0.40, 0.85}, {64, 64, 4, 0.22, 0.75}};
+constexpr TileCost kTiles[5] = {
+    {256, 256, 1, 0.50, 0.85}, {128, 128, 2, 0.40, 0.85}, {64, 64, 4, 0.22, 0.75}, {64, 32, 1, 1, 1}, {64, 128, 1, .3, .8}};
 constexpr double kCuFlops16 = 9.8e6, kCuFlops32 = 0.61e6;  // of one CU in a microsecond
 constexpr double kStageUs = 0.6;                           // a stage's loads, when nothing else hides them
 constexpr double kReduceUs = 4.0, kReduceBytesPerUs = 3e6; // the launch that adds the partial sums

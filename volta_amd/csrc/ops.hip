@@ -73,7 +73,6 @@ struct Mat {
   int bytes;
   bool out;
   int64_t span() const { return p && rows > 0 ? ((rows - 1) * ld + cols) * bytes : 0; }
-  bool vec(int64_t n) const { return !p || ((uintptr_t)p % (n * bytes) == 0 && (rows <= 1 || ld % n == 0)); }
 };
 
 void check_dims(const char* what, int64_t n, int64_t lo, int64_t hi) {
@@ -152,54 +151,110 @@ hipError_t gemm(int type, int layout, int kind, const OpPlan& plan, const OpGemm
                                  : op_gemm_f16(layout, kind, plan, g, st);
 }
 
-// Rows of 16-byte chunks: what the direct loads need.
-bool chunked(const Mat& m) {
-  const int64_t e = 16 / m.bytes;
-  return m.vec(e) && m.cols % e == 0;
+// An operand of a product as its description gives it: rows of `len`
+// contiguous elements, `ld` apart.
+struct Operand {
+  int64_t rows, len, ld;
+  int count;  // matrices of it
+};
+bool whole_chunks(int type, const Operand& o) {
+  const int64_t e = 16 / elem_bytes(type);
+  return o.len % e == 0 && o.ld % e == 0;
+}
+int64_t packed_ld(int type, int64_t len) {
+  const int64_t e = 16 / elem_bytes(type);
+  return (len + e - 1) / e * e;
+}
+int64_t packed_bytes(int type, const Operand& o) {
+  return align256(o.rows * packed_ld(type, o.len) * elem_bytes(type));
 }
 
-// The shape of a product: a plan depends on it and on `direct`, which the
-// pointers decide; the workspace holds either plan's partial sums.
+// The shape of a product, and what follows for it from the description alone:
+// whether operands are laid out anew in rows of whole chunks, and the
+// workspace.  (Where a pointer turns out not to be 16-byte aligned, the
+// product takes the loads through registers.)
 struct Shape {
   int layout, kind;
   int64_t M, N, K;
   int pieces, outputs;
+  Operand p, q;
+  bool pack_p, pack_q;
+  int64_t partial_bytes, pack_bytes;  // partial sums, then the copies
+  int64_t bytes() const { return partial_bytes + pack_bytes; }
 };
 OpPlan plan_of(int type, const Shape& s, bool direct) {
   return op_gemm_plan(elem_bytes(type), s.layout, s.kind, s.M, s.N, s.K, s.pieces, s.outputs, direct);
 }
-int64_t partial_bytes(int type, const Shape& s) {
-  int64_t n = 0;
+Shape shape_of(int type, int layout, int kind, int64_t M, int64_t N, int64_t K, int pieces, int outputs, Operand p,
+               Operand q) {
+  Shape s{layout, kind, M, N, K, pieces, outputs, p, q, !whole_chunks(type, p), !whole_chunks(type, q), 0, 0};
+  if (s.pack_p || s.pack_q) {
+    s.pack_bytes = (s.pack_p ? p.count * packed_bytes(type, p) : 0) + (s.pack_q ? q.count * packed_bytes(type, q) : 0);
+    if (!op_gemm_pack(elem_bytes(type), layout, kind, M, N, K, pieces, outputs, s.pack_bytes)) {
+      s.pack_p = s.pack_q = false;
+      s.pack_bytes = 0;
+    }
+  }
   for (bool direct : {false, true})
-    n = std::max(n, op_gemm_partial_bytes(plan_of(type, s, direct), s.kind, s.M, s.N, s.outputs));
-  return align256(n);
+    s.partial_bytes =
+        std::max(s.partial_bytes, align256(op_gemm_partial_bytes(plan_of(type, s, direct), kind, M, N, outputs)));
+  return s;
 }
 
-// One product of a call.
-void product(int type, const Shape& s, const std::vector<Mat>& ps, const std::vector<Mat>& qs, const OpEpilogue& epi,
-             float* partial, hipStream_t st, const char* what) {
+// One product of a call: its operands' matrices (one, or p.count / q.count
+// different ones), epilogue and workspace.
+void product(int type, const Shape& s, const void* const* ps, const void* const* qs, const OpEpilogue& epi,
+             char* workspace, hipStream_t st, const char* what) {
   if (s.M == 0 || s.N == 0) return;
   OpGemm g{};
+  PackArgs pack{};
+  char* at = workspace + s.partial_bytes;
   bool direct = true;
-  for (size_t i = 0; i < 2; ++i) {
-    const Mat &p = ps[std::min(i, ps.size() - 1)], &q = qs[std::min(i, qs.size() - 1)];
-    g.p[i] = p.p;
-    g.q[i] = q.p;
-    direct = direct && chunked(p) && chunked(q);
+  auto operand = [&](const Operand& o, const void* const* from, bool packs, const void** to, int64_t* ld) {
+    *ld = packs ? packed_ld(type, o.len) : o.ld;
+    for (int i = 0; i < 2; ++i) {
+      if (i >= o.count) {
+        to[i] = to[0];
+        continue;
+      }
+      to[i] = from[i];
+      if (packs) {
+        pack.from[pack.n] = from[i];
+        pack.to[pack.n] = at;
+        pack.rows[pack.n] = o.rows;
+        pack.cols[pack.n] = (int32_t)o.len;
+        pack.ld_from[pack.n] = o.ld;
+        pack.ld_to[pack.n] = *ld;
+        ++pack.n;
+        to[i] = at;
+        at += packed_bytes(type, o);
+      }
+      direct = direct && (uintptr_t)to[i] % 16 == 0 && (packs || whole_chunks(type, o));
+    }
+  };
+  operand(s.p, ps, s.pack_p, g.p, &g.ld_p);
+  operand(s.q, qs, s.pack_q, g.q, &g.ld_q);
+  if (pack.n && !direct) {  // one operand would still not do: none is laid out anew
+    pack.n = 0;
+    for (int i = 0; i < 2; ++i) {
+      g.p[i] = ps[std::min(i, s.p.count - 1)];
+      g.q[i] = qs[std::min(i, s.q.count - 1)];
+    }
+    g.ld_p = s.p.ld;
+    g.ld_q = s.q.ld;
   }
-  g.ld_p = ps[0].ld;
-  g.ld_q = qs[0].ld;
   g.M = (int32_t)s.M;
   g.N = (int32_t)s.N;
   g.K = (int32_t)s.K;
   g.pieces = s.pieces;
   g.outputs = s.outputs;
   g.direct = direct;
-  g.partial = partial;
+  g.partial = reinterpret_cast<float*>(workspace);
+  g.epi = epi;
   const OpPlan plan = plan_of(type, s, direct);
   // a grid has fewer than 2^32 threads
   if (op_gemm_blocks(plan, s.kind, s.M, s.N) > (int64_t{1} << 22)) refuse("rows * columns of a product are too many");
-  g.epi = epi;
+  if (pack.n) check_hip(pack_rows(type, pack, st), "layout");
   check_hip(gemm(type, s.layout, s.kind, plan, g, st), what);
 }
 
@@ -208,9 +263,9 @@ struct Linear {
   volta_op_linear d;
   Shape fwd, dx, dw;
   int strips;
-  int64_t part_fwd, dp_bytes, sums_bytes, part_bwd;
-  int64_t forward_bytes() const { return part_fwd; }
-  int64_t backward_bytes() const { return dp_bytes + sums_bytes + part_bwd; }
+  int64_t ld_dp, dp_bytes, sums_bytes;
+  int64_t forward_bytes() const { return fwd.bytes(); }
+  int64_t backward_bytes() const { return dp_bytes + sums_bytes + std::max(dx.bytes(), dw.bytes()); }
 };
 
 Linear linear_of(const volta_op_linear* in) {
@@ -230,14 +285,16 @@ Linear linear_of(const volta_op_linear* in) {
   d.ld_pre = ld_of("ld_pre", d.ld_pre, d.outputs);
   d.ld_dx = ld_of("ld_dx", d.ld_dx, d.inputs);
   d.ld_dw = ld_of("ld_dw", d.ld_dw, d.outputs);
-  l.fwd = {OP_NN, OP_LINEAR, d.rows, d.outputs, d.inputs, 1, 1};
-  l.dx = {OP_NT, OP_STORE, d.rows, d.inputs, d.outputs, 1, 1};
-  l.dw = {OP_TN, OP_STORE, d.inputs, d.outputs, d.rows, 1, 1};
-  l.part_fwd = partial_bytes(d.type, l.fwd);
-  l.dp_bytes = d.act == VOLTA_OP_ACT_NONE ? 0 : align256(d.rows * d.outputs * elem_bytes(d.type));
+  // without an activation dp is dy itself
+  l.ld_dp = d.act == VOLTA_OP_ACT_NONE ? d.ld_y : packed_ld(d.type, d.outputs);
+  l.dp_bytes = d.act == VOLTA_OP_ACT_NONE ? 0 : packed_bytes(d.type, {d.rows, d.outputs, 0, 1});
+  const int64_t dp_len = d.act == VOLTA_OP_ACT_NONE ? d.outputs : l.ld_dp;
+  const Operand x{d.rows, d.inputs, d.ld_x, 1}, w{d.inputs, d.outputs, d.ld_w, 1}, dp{d.rows, dp_len, l.ld_dp, 1};
+  l.fwd = shape_of(d.type, OP_NN, OP_LINEAR, d.rows, d.outputs, d.inputs, 1, 1, x, w);
+  l.dx = shape_of(d.type, OP_NT, OP_STORE, d.rows, d.inputs, d.outputs, 1, 1, dp, w);
+  l.dw = shape_of(d.type, OP_TN, OP_STORE, d.inputs, d.outputs, d.rows, 1, 1, x, dp);
   l.strips = act_grad_strips(d.type, d.rows, d.outputs);
   l.sums_bytes = align256(4 * l.strips * d.outputs);
-  l.part_bwd = std::max(partial_bytes(d.type, l.dx), partial_bytes(d.type, l.dw));
   return l;
 }
 
@@ -245,9 +302,9 @@ struct Gated {
   volta_op_gated d;
   Shape fwd, dx, dw;
   int strips;
-  int64_t part_fwd, d_bytes, sums_bytes, part_bwd;
-  int64_t forward_bytes() const { return part_fwd; }
-  int64_t backward_bytes() const { return 2 * d_bytes + 2 * sums_bytes + part_bwd; }
+  int64_t ld_d, d_bytes, sums_bytes;
+  int64_t forward_bytes() const { return fwd.bytes(); }
+  int64_t backward_bytes() const { return 2 * (d_bytes + sums_bytes) + std::max(dx.bytes(), dw.bytes()); }
 };
 
 Gated gated_of(const volta_op_gated* in) {
@@ -266,14 +323,14 @@ Gated gated_of(const volta_op_gated* in) {
   d.ld_pre = ld_of("ld_pre", d.ld_pre, d.hidden);
   d.ld_dx = ld_of("ld_dx", d.ld_dx, d.inputs);
   d.ld_dw = ld_of("ld_dw", d.ld_dw, d.hidden);
-  l.fwd = {OP_NN, OP_GATED, d.rows, d.hidden, d.inputs, 1, 1};
-  l.dx = {OP_NT, OP_STORE, d.rows, d.inputs, d.hidden, 2, 1};
-  l.dw = {OP_TN, OP_STORE, d.inputs, d.hidden, d.rows, 1, 2};
-  l.part_fwd = partial_bytes(d.type, l.fwd);
-  l.d_bytes = align256(d.rows * d.hidden * elem_bytes(d.type));
+  l.ld_d = packed_ld(d.type, d.hidden);
+  l.d_bytes = packed_bytes(d.type, {d.rows, d.hidden, 0, 1});
+  const Operand x{d.rows, d.inputs, d.ld_x, 1}, w{d.inputs, d.hidden, d.ld_w, 2}, dg{d.rows, l.ld_d, l.ld_d, 2};
+  l.fwd = shape_of(d.type, OP_NN, OP_GATED, d.rows, d.hidden, d.inputs, 1, 1, x, w);
+  l.dx = shape_of(d.type, OP_NT, OP_STORE, d.rows, d.inputs, d.hidden, 2, 1, dg, w);
+  l.dw = shape_of(d.type, OP_TN, OP_STORE, d.inputs, d.hidden, d.rows, 1, 2, x, dg);
   l.strips = act_grad_strips(d.type, d.rows, d.hidden);
   l.sums_bytes = align256(4 * l.strips * d.hidden);
-  l.part_bwd = std::max(partial_bytes(d.type, l.dx), partial_bytes(d.type, l.dw));
   return l;
 }
 
@@ -361,7 +418,7 @@ int32_t volta_op_linear_forward(const volta_op_linear* in, const void* x, const 
     epi.ld_out = d.ld_y;
     epi.ld_residual = d.ld_residual;
     epi.ld_pre = d.ld_pre;
-    product(d.type, l.fwd, {mx}, {mw}, epi, static_cast<float*>(workspace), st, "product");
+    product(d.type, l.fwd, &x, &w, epi, static_cast<char*>(workspace), st, "product");
   });
 }
 
@@ -390,9 +447,8 @@ int32_t volta_op_linear_backward(const volta_op_linear* in, const void* dy, cons
     const hipStream_t st = stream_of(stream);
     char* ws = static_cast<char*>(workspace);
     float* sums = reinterpret_cast<float*>(ws + l.dp_bytes);
-    float* partial = reinterpret_cast<float*>(ws + l.dp_bytes + l.sums_bytes);
-    Mat mdp = mdy;  // without an activation dp is dy
-    if (act) mdp = {"dp", ws, d.rows, d.outputs, d.outputs, e, false};
+    char* rest = ws + l.dp_bytes + l.sums_bytes;
+    const void* dp = act ? ws : dy;
     if ((act && (dx || dw) && d.rows > 0) || db) {
       ActGradArgs a{};
       a.dy = dy;
@@ -404,6 +460,7 @@ int32_t volta_op_linear_backward(const volta_op_linear* in, const void* dy, cons
       a.cols = (int32_t)d.outputs;
       a.ld_dy = d.ld_y;
       a.ld_pre = d.ld_pre;
+      a.ld_d = l.ld_dp;
       check_hip(act_grad(d.type, false, a, st), "activation gradient");
       if (db) check_hip(sum_partials(d.type, sums, l.strips, d.outputs, db, st), "bias gradient");
     }
@@ -411,12 +468,12 @@ int32_t volta_op_linear_backward(const volta_op_linear* in, const void* dy, cons
     if (dx) {
       epi.out[0] = dx;
       epi.ld_out = d.ld_dx;
-      product(d.type, l.dx, {mdp}, {mw}, epi, partial, st, "dx");
+      product(d.type, l.dx, &dp, &w, epi, rest, st, "dx");
     }
     if (dw) {
       epi.out[0] = dw;
       epi.ld_out = d.ld_dw;
-      product(d.type, l.dw, {mx}, {mdp}, epi, partial, st, "dw");
+      product(d.type, l.dw, &x, &dp, epi, rest, st, "dw");
     }
   });
 }
@@ -460,7 +517,8 @@ int32_t volta_op_gated_forward(const volta_op_gated* in, const void* x, const vo
     epi.pre[1] = up;
     epi.ld_out = d.ld_h;
     epi.ld_pre = d.ld_pre;
-    product(d.type, l.fwd, {mx}, {mg, mu}, epi, static_cast<float*>(workspace), st, "product");
+    const void* w[2] = {w_gate, w_up};
+    product(d.type, l.fwd, &x, w, epi, static_cast<char*>(workspace), st, "product");
   });
 }
 
@@ -498,7 +556,7 @@ int32_t volta_op_gated_backward(const volta_op_gated* in, const void* dh, const 
     char* ws = static_cast<char*>(workspace);
     float* sums[2] = {reinterpret_cast<float*>(ws + 2 * l.d_bytes),
                       reinterpret_cast<float*>(ws + 2 * l.d_bytes + l.sums_bytes)};
-    float* partial = reinterpret_cast<float*>(ws + 2 * (l.d_bytes + l.sums_bytes));
+    char* rest = ws + 2 * (l.d_bytes + l.sums_bytes);
     if (d.rows > 0 || db_gate || db_up) {
       ActGradArgs a{};
       a.dy = dh;
@@ -513,23 +571,23 @@ int32_t volta_op_gated_backward(const volta_op_gated* in, const void* dh, const 
       a.cols = (int32_t)d.hidden;
       a.ld_dy = d.ld_h;
       a.ld_pre = d.ld_pre;
+      a.ld_d = l.ld_d;
       check_hip(act_grad(d.type, true, a, st), "activation gradient");
       if (db_gate) check_hip(sum_partials(d.type, sums[0], l.strips, d.hidden, db_gate, st), "bias gradient");
       if (db_up) check_hip(sum_partials(d.type, sums[1], l.strips, d.hidden, db_up, st), "bias gradient");
     }
-    const Mat dg{"dg", ws, d.rows, d.hidden, d.hidden, e, false};
-    const Mat du{"du", ws + l.d_bytes, d.rows, d.hidden, d.hidden, e, false};
+    const void *dgu[2] = {ws, ws + l.d_bytes}, *w[2] = {w_gate, w_up};
     OpEpilogue epi{};
     if (dx) {
       epi.out[0] = dx;
       epi.ld_out = d.ld_dx;
-      product(d.type, l.dx, {dg, du}, {mg, mu}, epi, partial, st, "dx");
+      product(d.type, l.dx, dgu, w, epi, rest, st, "dx");
     }
     if (dw_gate) {
       epi.out[0] = dw_gate;
       epi.out[1] = dw_up;
       epi.ld_out = d.ld_dw;
-      product(d.type, l.dw, {mx}, {dg, du}, epi, partial, st, "dw");
+      product(d.type, l.dw, &x, dgu, epi, rest, st, "dw");
     }
   });
 }

@@ -47,14 +47,24 @@ struct OpGemm {
   OpEpilogue epi;
 };
 
-// Tiles, by rows x columns of D.  OP_TILE_SKINNY takes up to 64 rows and 32
-// columns (of each weight matrix), the sum over k shared out over its waves.
-enum OpTile { OP_TILE_256 = 0, OP_TILE_128 = 1, OP_TILE_64 = 2, OP_TILE_SKINNY = 3, OP_TILE_64X128 = 4 };
+// Tiles, by rows x columns of D (gated: half the columns of each weight
+// matrix).  The skinny ones take 16, 32 or 64 rows and 32 columns (of each
+// weight matrix), the sum over k shared out over a block's waves.
+enum OpTile {
+  OP_TILE_256 = 0,
+  OP_TILE_128 = 1,
+  OP_TILE_64X128 = 2,
+  OP_TILE_64 = 3,
+  OP_TILE_SKINNY16 = 4,
+  OP_TILE_SKINNY32 = 5,
+  OP_TILE_SKINNY64 = 6
+};
 
 struct OpPlan {
   int32_t tile;
   int32_t splits;
   int32_t stages_per_split;
+  double us;  // what the model gives it
 };
 
 // k elements of one stage (128 bytes of every row).
@@ -64,6 +74,10 @@ inline int op_stage_k(int elem_bytes) { return 128 / elem_bytes; }
 // workspace can be asked for without a device.
 OpPlan op_gemm_plan(int elem_bytes, int layout, int kind, int64_t M, int64_t N, int64_t K, int pieces, int outputs,
                     bool direct);
+// Whether it pays to lay out operands of `pack_bytes` anew, in rows of whole
+// 16-byte chunks, for the direct loads.
+bool op_gemm_pack(int elem_bytes, int layout, int kind, int64_t M, int64_t N, int64_t K, int pieces, int outputs,
+                  int64_t pack_bytes);
 // Bytes of partial sums that the plan needs.
 int64_t op_gemm_partial_bytes(const OpPlan& plan, int kind, int64_t M, int64_t N, int outputs);
 

@@ -43,23 +43,28 @@ static __device__ const __attribute__((aligned(16))) uint32_t op_zeros[4] = {0, 
 
 template <typename T> struct Mfma;
 template <> struct Mfma<__bf16> {
-  static __device__ __forceinline__ floatx4 mul(chunk16 a, chunk16 b, floatx4 c) {
+  static constexpr int kSteps = 1;
+  static __device__ __forceinline__ floatx4 mul(int, chunk16 a, chunk16 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
                                                    0, 0);
   }
 };
 template <> struct Mfma<_Float16> {
-  static __device__ __forceinline__ floatx4 mul(chunk16 a, chunk16 b, floatx4 c) {
+  static constexpr int kSteps = 1;
+  static __device__ __forceinline__ floatx4 mul(int, chunk16 a, chunk16 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(halfx8, a), __builtin_bit_cast(halfx8, b), c, 0,
                                                   0, 0);
   }
 };
-template <> struct Mfma<float> {  // lane group g holds k = 4g .. 4g + 3 of 16: step j takes 4g + j
-  static __device__ __forceinline__ floatx4 mul(chunk16 a, chunk16 b, floatx4 c) {
+// Float fragments take four instructions: lane group g holds k = 4g .. 4g + 3
+// of 16, and step j takes 4g + j.  They are issued step by step over all
+// blocks, not block by block: one that adds to the sum of the one before it
+// waits for it.
+template <> struct Mfma<float> {
+  static constexpr int kSteps = 4;
+  static __device__ __forceinline__ floatx4 mul(int step, chunk16 a, chunk16 b, floatx4 c) {
     const floatx4 x = __builtin_bit_cast(floatx4, a), y = __builtin_bit_cast(floatx4, b);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
-    return c;
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(x[step], y[step], c, 0, 0, 0);
   }
 };
 
@@ -490,9 +495,11 @@ __global__ void __launch_bounds__(WGM* WGN * 64) op_gemm_tiled(OpGemm g) {
 #pragma unroll
       for (int i = 0; i < TM; ++i) fp[i] = PT::frag(from, wm * WM + i * 16, kk, lane);
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+      for (int st = 0; st < Mfma<T>::kSteps; ++st)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = Mfma<T>::mul(fq[j], fp[i], acc[i][j]);
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[i][j] = Mfma<T>::mul(st, fq[j], fp[i], acc[i][j]);
     }
   };
 
@@ -542,7 +549,7 @@ __global__ void __launch_bounds__(WGM* WGN * 64) op_gemm_tiled(OpGemm g) {
 }
 
 // ---------------------------------------------------------------------------
-// Large product, 16 bits: 256x256 of D per block, eight waves (2 x 4, each
+// Large product: 256x256 of D per block, eight waves (2 x 4, each
 // 128x64), two stages of k in LDS in four regions each -- the halves of P's
 // rows and Q's columns that a wave multiplies apart:
 //
@@ -589,7 +596,7 @@ struct Region : Tile<T, 128, KC, 8> {
 template <typename T, int LAYOUT, int KIND>
 __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) op_gemm_large(OpGemm g) {
   constexpr bool kGated = KIND == OP_GATED, P_KC = LAYOUT != OP_TN, Q_KC = LAYOUT == OP_NT;
-  constexpr int kRegion = 128 * 128, kStageK = 64, SN = kGated ? 128 : 256;
+  constexpr int kRegion = 128 * 128, kStageK = 128 / (int)sizeof(T), SN = kGated ? 128 : 256;
   using PR = Region<T, P_KC, 64, 128>;
   using QR = Region<T, Q_KC, kGated ? 128 : 32, kGated ? 128 : 64>;
   static_assert(PR::kBytes == kRegion && PR::kLoads == 2, "two loads a wave and region");
@@ -658,10 +665,12 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) o
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int st = 0; st < Mfma<T>::kSteps; ++st)
 #pragma unroll
-        for (int j = 2 * h; j < 2 * h + 2; ++j)
-          acc[half * 4 + i][j] = Mfma<T>::mul(fq[j][kk], fp[i][kk], acc[half * 4 + i][j]);
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 2 * h; j < 2 * h + 2; ++j)
+            acc[half * 4 + i][j] = Mfma<T>::mul(st, fq[j][kk], fp[i][kk], acc[half * 4 + i][j]);
   };
   constexpr auto H0 = std::integral_constant<int, 0>();
   constexpr auto H1 = std::integral_constant<int, 1>();
@@ -837,9 +846,11 @@ __global__ void __launch_bounds__(512) op_gemm_middle(OpGemm g) {
 #pragma unroll
     for (int kk = 0; kk < 2 * KS; ++kk)
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+      for (int st = 0; st < Mfma<T>::kSteps; ++st)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = Mfma<T>::mul(fq[j][kk], fp[i][kk], acc[i][j]);
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[i][j] = Mfma<T>::mul(st, fq[j][kk], fp[i][kk], acc[i][j]);
     __builtin_amdgcn_s_setprio(0);
     op_barrier();
   };
@@ -866,8 +877,8 @@ __global__ void __launch_bounds__(512) op_gemm_middle(OpGemm g) {
 }
 
 // ---------------------------------------------------------------------------
-// Skinny product, M <= 16 MT: each weight is read once and bounds the time.
-// A block takes 32 columns (of each weight matrix) and its waves take turns
+// Skinny product, few rows: reading the weights bounds the time.  A block
+// takes 16 MT rows and BN columns (of each weight matrix) and its waves take turns
 // over the stages of k, each with a ring of its own in LDS for both operands
 // (no barrier before the end); the waves' sums are added at the end, in wave
 // order.
@@ -888,11 +899,11 @@ __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // blocks next to each other share cache lines of W: one XCD takes a run of them
   int tm, tn;
-  op_tile_of(blockIdx.x, 1, g.tiles_n, &tm, &tn);
-  const int n0 = tn * BN, split = blockIdx.y, q_left = g.N - n0;
+  op_tile_of(blockIdx.x, g.tiles_m, g.tiles_n, &tm, &tn);
+  const int m0 = tm * (16 * MT), n0 = tn * BN, split = blockIdx.y, p_left = g.M - m0, q_left = g.N - n0;
   PT pt;
   QT qt;
-  pt.init(g.ld_p, g.M, 0, lane);
+  pt.init(g.ld_p, p_left, 0, lane);
   qt.init(g.ld_q, q_left, 0, lane);
   const int per_piece = (g.K + kStageK - 1) / kStageK;
   const int s_begin = split * g.stages_per_split;
@@ -901,7 +912,7 @@ __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
 
   chunk16 rp[DIRECT ? 1 : PT::kLoads], rq[kSubs][DIRECT ? 1 : QT::kLoads];
   Cursor<T, LAYOUT, kGated> next;
-  next.init(g, 0, n0, 0, s_begin + wave, NW);
+  next.init(g, m0, n0, 0, s_begin + wave, NW);
   // This wave's next stage, to byte `to` of LDS; `whole`: it is, and in one piece.
   auto load = [&](uint32_t to, auto whole) {
     constexpr bool W = decltype(whole)::value;
@@ -920,7 +931,7 @@ __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
     } else {
 #pragma unroll
       for (int i = 0; i < kSubs; ++i) qt.fetch(next.q[i], rq[i], 0, lane, q_left, k_left);
-      pt.fetch(next.p, rp, 0, lane, g.M, k_left);
+      pt.fetch(next.p, rp, 0, lane, p_left, k_left);
     }
     next.step();
     if constexpr (!W) next.cross(g);
@@ -942,9 +953,11 @@ __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
 #pragma unroll
       for (int i = 0; i < MT; ++i) fp[i] = PT::frag(from, i * 16, kk, lane);
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int st = 0; st < Mfma<T>::kSteps; ++st)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = Mfma<T>::mul(fq[j], fp[i], acc[i][j]);
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[i][j] = Mfma<T>::mul(st, fq[j], fp[i], acc[i][j]);
     }
   };
 
@@ -1000,7 +1013,7 @@ __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
 #pragma unroll
     for (int c = 0; c < TN; ++c) sums[(wave * TN + c) * 64 + lane] = acc[i][c];
     __syncthreads();
-    const int m = i * 16 + l;
+    const int m = m0 + i * 16 + l;
     if (m >= g.M) continue;
 #pragma unroll
     for (int u = 0; u < kTurns; ++u) {
@@ -1101,27 +1114,21 @@ hipError_t launch_large(OpGemm& g, hipStream_t st) {
   return hipGetLastError();
 }
 
-// Waves and ring of the skinny form: what fits a CU's 160 KB of LDS.
-#ifndef SK_BN
-#define SK_BN 32
-#define SK_W 8
-#define SK_S 3
-#define SK_GW 4
-#define SK_GS 3
-#endif
+// Columns, waves and ring of the skinny form: what fits a CU's 160 KB of LDS.
+// (64 columns, or half the waves, measured the same within 5 %.)
 template <int KIND, int MT, bool DIRECT>
 struct SkinnyShape {
-  static constexpr int kCols = SK_BN;
-  static constexpr int kWaves = KIND == OP_GATED ? (MT == 4 ? 2 : SK_GW) : MT > 1 ? 4 : SK_W;
-  static constexpr int kStages = !DIRECT ? 1 : KIND == OP_GATED ? (MT == 4 ? 2 : SK_GS) : (MT == 2 ? 3 : MT == 4 ? 2 : SK_S);
+  static constexpr int kCols = 32;
+  static constexpr int kWaves = KIND == OP_GATED || MT > 1 ? 4 : 8;
+  static constexpr int kStages = !DIRECT ? 1 : KIND == OP_GATED ? (MT == 4 ? 2 : 3) : (MT == 2 ? 4 : 3);
 };
 template <typename T, int LAYOUT, int KIND, int MT, bool DIRECT>
 hipError_t launch_skinny(OpGemm& g, hipStream_t st) {
   using S = SkinnyShape<KIND, MT, DIRECT>;
-  g.tiles_m = 1;
+  g.tiles_m = (g.M + 16 * MT - 1) / (16 * MT);
   g.tiles_n = (g.N + S::kCols - 1) / S::kCols;
   hipLaunchKernelGGL((op_gemm_skinny<T, LAYOUT, KIND, MT, S::kCols, S::kWaves, S::kStages, DIRECT>),
-                     dim3((unsigned)g.tiles_n, (unsigned)g.splits), dim3(S::kWaves * 64), 0, st, g);
+                     dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits), dim3(S::kWaves * 64), 0, st, g);
   return hipGetLastError();
 }
 
@@ -1130,23 +1137,20 @@ hipError_t launch(const OpPlan& plan, OpGemm& g, hipStream_t st) {
   g.splits = plan.splits;
   g.stages_per_split = plan.stages_per_split;
   hipError_t e;
-  if (plan.tile == OP_TILE_SKINNY) {
+  if (plan.tile >= OP_TILE_SKINNY16) {
     if constexpr (LAYOUT == OP_TN) {
       return hipErrorInvalidValue;
+    } else if (g.direct) {
+      e = plan.tile == OP_TILE_SKINNY16   ? launch_skinny<T, LAYOUT, KIND, 1, true>(g, st)
+          : plan.tile == OP_TILE_SKINNY32 ? launch_skinny<T, LAYOUT, KIND, 2, true>(g, st)
+                                          : launch_skinny<T, LAYOUT, KIND, 4, true>(g, st);
     } else {
-      const int mt = (g.M + 15) / 16;
-      if (g.direct)
-        e = mt <= 1   ? launch_skinny<T, LAYOUT, KIND, 1, true>(g, st)
-            : mt == 2 ? launch_skinny<T, LAYOUT, KIND, 2, true>(g, st)
-                      : launch_skinny<T, LAYOUT, KIND, 4, true>(g, st);
-      else
-        e = mt <= 1   ? launch_skinny<T, LAYOUT, KIND, 1, false>(g, st)
-            : mt == 2 ? launch_skinny<T, LAYOUT, KIND, 2, false>(g, st)
-                      : launch_skinny<T, LAYOUT, KIND, 4, false>(g, st);
+      e = plan.tile == OP_TILE_SKINNY16   ? launch_skinny<T, LAYOUT, KIND, 1, false>(g, st)
+          : plan.tile == OP_TILE_SKINNY32 ? launch_skinny<T, LAYOUT, KIND, 2, false>(g, st)
+                                          : launch_skinny<T, LAYOUT, KIND, 4, false>(g, st);
     }
   } else if (plan.tile == OP_TILE_256 && g.direct) {
-    if constexpr (sizeof(T) == 2) e = launch_large<T, LAYOUT, KIND>(g, st);
-    else return hipErrorInvalidValue;
+    e = launch_large<T, LAYOUT, KIND>(g, st);
   } else if (plan.tile == OP_TILE_64) {
     constexpr int WGM = KIND == OP_GATED ? 4 : 2;  // a wave has columns of both weight matrices
     e = g.direct ? launch_middle<T, LAYOUT, KIND, 64, 64, WGM, 8 / WGM, 2, 4>(g, st)

@@ -1,5 +1,6 @@
 // Which tile a product of the feed-forward operators takes (ops_gemm.h), and
-// over how many blocks its sum over k is split.  Host code without a device.
+// over how many blocks its sum over k is split: the one of least time by a
+// model of a block's time, measured tile by tile.  Host code without a device.
 #include <algorithm>
 #include <cstdint>
 
@@ -11,17 +12,24 @@ namespace {
 
 constexpr int64_t kCus = 256;  // of an MI355X
 
+// A block's time in microseconds: `fixed` for its start, its first loads and
+// its epilogue, and `stage` for 128 bytes of k, or more where the matrix
+// instructions of float32 take longer (`flops_us`: of a CU in a microsecond).
 struct TileCost {
-  int bm, bn;        // rows and columns of D
-  int resident;      // blocks a CU holds
-  double rate16, rate32;  // share of the matrix rate that a full CU reaches
+  int bm, bn;      // rows and columns of D (gated: half the columns of each weight matrix)
+  double fixed, stage;
 };
-// Measured on large products (bf16, float32).
-constexpr TileCost kTiles[5] = {
-    {256, 256, 1, 0.50, 0.85}, {128, 128, 2, 0.40, 0.85}, {64, 64, 4, 0.22, 0.75}, {64, 32, 1, 1, 1}, {64, 128, 1, .3, .8}};
-constexpr double kCuFlops16 = 9.8e6, kCuFlops32 = 0.61e6;  // of one CU in a microsecond
-constexpr double kStageUs = 0.6;                           // a stage's loads, when nothing else hides them
-constexpr double kReduceUs = 4.0, kReduceBytesPerUs = 3e6; // the launch that adds the partial sums
+// Measured on an MI355X, bf16.
+constexpr TileCost kTiles[7] = {
+    {256, 256, 6.0, 0.95}, {128, 128, 3.2, 0.43}, {64, 128, 2.4, 0.33}, {64, 64, 2.2, 0.23},
+    {16, 32, 1.0, 0.0},    {32, 32, 1.0, 0.0},    {64, 32, 1.2, 0.0},
+};
+constexpr double kFlops32 = 0.55e6;                        // float32, of one CU in a microsecond
+constexpr double kSkinnyBytes = 60e3;                      // what a CU's waves load in a microsecond
+constexpr double kReadBytes = 5.5e6;                       // what the chip reads in a microsecond
+constexpr double kLaunchUs = 2.2;                          // of a launch, whatever it does
+constexpr double kReduceUs = 5.0, kReduceBytes = 4e6;      // the launch that adds the partial sums
+constexpr double kPackUs = 3.0;                            // the launch that lays operands out again, at the same rate
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -30,44 +38,49 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 OpPlan op_gemm_plan(int elem_bytes, int layout, int kind, int64_t M, int64_t N, int64_t K, int pieces, int outputs,
                     bool direct) {
   const int64_t stages = pieces * ceil_div(K, op_stage_k(elem_bytes));
-  const int planes = kind == OP_GATED ? 2 : outputs;
-  OpPlan best{OP_TILE_128, 1, (int32_t)stages};
+  const int planes = kind == OP_GATED ? 2 : outputs, subs = kind == OP_GATED ? 2 : 1;
+  OpPlan best{OP_TILE_128, 1, (int32_t)stages, 0.0};
   if (stages == 0 || M == 0) return best;
-  auto split_plan = [&](int tile, int64_t splits) {
-    const int64_t per = ceil_div(stages, splits);
-    return OpPlan{tile, (int32_t)ceil_div(stages, per), (int32_t)per};
-  };
-  if (M <= 64 && layout != OP_TN) {
-    // A block's waves share its stages out; with few column blocks the sum is
-    // split over blocks too, as long as every wave keeps four stages.
-    const int64_t blocks = ceil_div(N, 32), waves = kind == OP_GATED || M > 16 ? 4 : 8;
-    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(128 / blocks, stages / (4 * waves)));
-    return split_plan(OP_TILE_SKINNY, splits);
-  }
-  const double cu = elem_bytes == 4 ? kCuFlops32 : kCuFlops16;
+  // every product reads both operands, from memory at the rate of memory
+  const double read_us = (double)elem_bytes * pieces * K * ((double)M + (double)subs * N * outputs) / kReadBytes;
   double best_us = 1e30;
-  for (int t = 0; t < 3; ++t) {
+  for (int t = 0; t < 7; ++t) {
     const TileCost& c = kTiles[t];
-    if (c.bm == 256 && (!direct || elem_bytes == 4)) continue;
-    const int64_t sn = kind == OP_GATED ? c.bn / 2 : c.bn;
+    const bool skinny = t >= OP_TILE_SKINNY16;
+    if (skinny && (layout == OP_TN || M > 512)) continue;
+    if (!direct && (t == OP_TILE_256 || t == OP_TILE_64X128)) continue;
+    const int64_t sn = skinny ? 32 : kind == OP_GATED ? c.bn / 2 : c.bn;
     const int64_t tiles = ceil_div(M, c.bm) * ceil_div(N, sn) * outputs;
-    const double stage_us = 2.0 * c.bm * c.bn * op_stage_k(elem_bytes) / (cu * (elem_bytes == 4 ? c.rate32 : c.rate16));
-    for (int64_t splits = 1; splits <= 64 && splits <= std::max<int64_t>(1, stages / 2); splits *= 2) {
-      const OpPlan p = split_plan(t, splits);
-      const int64_t blocks = tiles * p.splits, room = kCus * c.resident;
-      const int64_t rounds = blocks / room, rest = ceil_div(blocks - rounds * room, kCus);
-      // a full CU works at its rate; a part-full one at least as fast as its loads come
-      const double full = std::max(c.resident * stage_us, kStageUs);
-      const double part = rest == 0 ? 0.0 : std::max(rest * stage_us, kStageUs);
-      double us = p.stages_per_split * (rounds * full + part) + (rounds + (rest > 0)) * 1.5;
-      if (p.splits > 1) us += kReduceUs + 8.0 * p.splits * planes * (double)M * (double)N / kReduceBytesPerUs;
-      if (us < best_us) {
+    const int waves = skinny ? (kind == OP_GATED || c.bm > 16 ? 4 : 8) : 1;
+    double stage_us = c.stage;
+    if (skinny) {
+      // a turn of the waves: W in rows of 64 bytes counts for more, as whole cache lines are fetched
+      const double w = layout == OP_NN && elem_bytes == 2 ? 1.6 : 1.0;
+      stage_us = waves * 128.0 * (32 * subs * w + c.bm) / kSkinnyBytes;
+    }
+    if (elem_bytes == 4)
+      stage_us = std::max(stage_us, 2.0 * c.bm * sn * subs * op_stage_k(4) * waves / kFlops32);
+    // through registers, one stage ahead
+    if (!direct) stage_us = skinny ? 1.1 * stage_us + 0.5 : stage_us * (t == OP_TILE_64 ? 2.0 : 4.0);
+    for (int64_t splits = 1; splits <= 32 && (splits == 1 || stages / splits >= 4 * waves); splits *= 2) {
+      const int64_t per = ceil_div(stages, splits), used = ceil_div(stages, per);
+      const double rounds = (double)ceil_div(tiles * used, kCus);
+      double us = kLaunchUs + rounds * c.fixed + std::max(rounds * ceil_div(per, waves) * stage_us, read_us);
+      if (used > 1) us += kReduceUs + 8.0 * used * planes * (double)M * (double)N / kReduceBytes;
+      if (us < best_us * (splits > 1 ? 0.93 : 1.0)) {
         best_us = us;
-        best = p;
+        best = OpPlan{t, (int32_t)used, (int32_t)per, us};
       }
     }
   }
   return best;
+}
+
+bool op_gemm_pack(int elem_bytes, int layout, int kind, int64_t M, int64_t N, int64_t K, int pieces, int outputs,
+                  int64_t pack_bytes) {
+  const double staged = op_gemm_plan(elem_bytes, layout, kind, M, N, K, pieces, outputs, false).us;
+  const double direct = op_gemm_plan(elem_bytes, layout, kind, M, N, K, pieces, outputs, true).us;
+  return direct + kPackUs + 2.0 * (double)pack_bytes / kReduceBytes < staged;
 }
 
 int64_t op_gemm_partial_bytes(const OpPlan& plan, int kind, int64_t M, int64_t N, int outputs) {
@@ -77,9 +90,9 @@ int64_t op_gemm_partial_bytes(const OpPlan& plan, int kind, int64_t M, int64_t N
 }
 
 int64_t op_gemm_blocks(const OpPlan& plan, int kind, int64_t M, int64_t N) {
-  if (plan.tile == OP_TILE_SKINNY) return ceil_div(N, 32);
   const TileCost& c = kTiles[plan.tile];
-  return ceil_div(M, c.bm) * ceil_div(N, kind == OP_GATED ? c.bn / 2 : c.bn);
+  const int64_t sn = plan.tile >= OP_TILE_SKINNY16 ? 32 : kind == OP_GATED ? c.bn / 2 : c.bn;
+  return ceil_div(M, c.bm) * ceil_div(N, sn);
 }
 
 }  // namespace ops

@@ -41,15 +41,27 @@ hipError_t sum_partials(int type, const float* partial, int n, int64_t cols, voi
 struct ActGradArgs {
   const void* dy;
   const void* pre[2];  // gated: gate and up
-  void* d[2];          // dp, or dg and du (packed rows), or NULL: column sums of dy alone
+  void* d[2];          // dp, or dg and du, or NULL: column sums of dy alone
   float* partial[2];   // column sums of dp, or of dg and du, [act_grad_strips][cols]; NULL where not wanted
   int32_t act;
   int64_t rows;
   int32_t cols;
   int64_t ld_dy, ld_pre;
+  int64_t ld_d;        // whole 16-byte chunks; what a row's last chunk has behind its columns is set to 0
 };
 int act_grad_strips(int type, int64_t rows, int64_t cols);
 hipError_t act_grad(int type, bool gated, const ActGradArgs& a, hipStream_t st);
+
+// Copies up to three matrices into rows of whole 16-byte chunks, zeros behind
+// a row's columns.
+struct PackArgs {
+  const void* from[3];
+  void* to[3];
+  int64_t rows[3], ld_from[3], ld_to[3];
+  int32_t cols[3];
+  int32_t n;
+};
+hipError_t pack_rows(int type, const PackArgs& a, hipStream_t st);
 
 struct DropoutArgs {
   const void *x, *residual;

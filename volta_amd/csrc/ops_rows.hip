@@ -441,12 +441,14 @@ __global__ void __launch_bounds__(256) act_grad_kernel(ActGradArgs a, int per) {
         s0[i] += u[i];
         s1[i] += d[i];
       }
-      store_row(static_cast<T*>(a.d[0]) + r * a.cols + c, cnt, u);
-      store_row(static_cast<T*>(a.d[1]) + r * a.cols + c, cnt, d);
+      if (cnt > 0) {  // what is behind the columns came out as 0
+        store_row(static_cast<T*>(a.d[0]) + r * a.ld_d + c, E, u);
+        store_row(static_cast<T*>(a.d[1]) + r * a.ld_d + c, E, d);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < E; ++i) s0[i] += d[i];
-      if (a.d[0]) store_row(static_cast<T*>(a.d[0]) + r * a.cols + c, cnt, d);
+      if (a.d[0] && cnt > 0) store_row(static_cast<T*>(a.d[0]) + r * a.ld_d + c, E, d);
     }
   }
   if (a.partial[0]) strip_store<T>(lds, s0, a.partial[0], a.cols, c, lane, wave);
@@ -475,6 +477,19 @@ __global__ void __launch_bounds__(1024) sum_partials_kernel(const float* partial
     for (int w = 1; w < 16; ++w) s += lds[w][lane];
     out[c] = from_f<T>(s);
   }
+}
+
+// A thread for 16 bytes of a row of the copy.
+template <typename T>
+__global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
+  constexpr int E = kChunk<T>;
+  const int i = blockIdx.z;
+  const int64_t chunks = a.ld_to[i] / E, id = block_id() * 256 + threadIdx.x, row = id / chunks;
+  if (row >= a.rows[i]) return;
+  const int c = (int)(id - row * chunks) * E;
+  float f[E];
+  load_row(static_cast<const T*>(a.from[i]) + row * a.ld_from[i] + c, a.cols[i] - c, f);
+  store_row(static_cast<T*>(a.to[i]) + row * a.ld_to[i] + c, E, f);
 }
 
 // ---------------------------------------------------------------------------
@@ -613,6 +628,18 @@ hipError_t act_grad(int type, bool gated, const ActGradArgs& a, hipStream_t st) 
     using T = decltype(t);
     if (gated) hipLaunchKernelGGL((act_grad_kernel<T, true>), grid, dim3(256), 0, st, a, per);
     else hipLaunchKernelGGL((act_grad_kernel<T, false>), grid, dim3(256), 0, st, a, per);
+    return hipGetLastError();
+  });
+}
+
+hipError_t pack_rows(int type, const PackArgs& a, hipStream_t st) {
+  return with_type(type, [&](auto t) {
+    using T = decltype(t);
+    int64_t blocks = 1;
+    for (int i = 0; i < a.n; ++i) blocks = std::max(blocks, (a.rows[i] * (a.ld_to[i] / kChunk<T>)+255) / 256);
+    dim3 grid = grid_of(blocks);
+    grid.z = (unsigned)a.n;
+    hipLaunchKernelGGL((pack_kernel<T>), grid, dim3(256), 0, st, a);
     return hipGetLastError();
   });
 }

@@ -57,7 +57,8 @@ enum OpTile {
   OP_TILE_64 = 3,
   OP_TILE_SKINNY16 = 4,
   OP_TILE_SKINNY32 = 5,
-  OP_TILE_SKINNY64 = 6
+  OP_TILE_SKINNY64 = 6,
+  OP_TILES = 7
 };
 
 struct OpPlan {

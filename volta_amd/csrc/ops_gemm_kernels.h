@@ -1115,7 +1115,8 @@ hipError_t launch_large(OpGemm& g, hipStream_t st) {
 }
 
 // Columns, waves and ring of the skinny form: what fits a CU's 160 KB of LDS.
-// (64 columns, or half the waves, measured the same within 5 %.)
+// (64 columns, a whole cache line of 16-bit W, measured as fast as the 64x64
+// tile where W comes from memory, and slower where it is small.)
 template <int KIND, int MT, bool DIRECT>
 struct SkinnyShape {
   static constexpr int kCols = 32;

@@ -14,18 +14,18 @@ constexpr int64_t kCus = 256;  // of an MI355X
 
 // A block's time in microseconds: `fixed` for its start, its first loads and
 // its epilogue, and `stage` for 128 bytes of k, or more where the matrix
-// instructions of float32 take longer (`flops_us`: of a CU in a microsecond).
+// instructions of float32 take longer.
 struct TileCost {
   int bm, bn;      // rows and columns of D (gated: half the columns of each weight matrix)
   double fixed, stage;
+  double flops32;  // float32 flops of a CU in a microsecond
 };
-// Measured on an MI355X, bf16.
-constexpr TileCost kTiles[7] = {
-    {256, 256, 6.0, 0.95}, {128, 128, 3.2, 0.43}, {64, 128, 2.4, 0.33}, {64, 64, 2.2, 0.23},
-    {16, 32, 1.0, 0.0},    {32, 32, 1.0, 0.0},    {64, 32, 1.2, 0.0},
+// Measured on an MI355X.
+constexpr TileCost kTiles[OP_TILES] = {
+    {256, 256, 6.0, 0.95, 0.55e6}, {128, 128, 3.2, 0.43, 0.47e6}, {64, 128, 2.4, 0.33, 0.42e6}, {64, 64, 2.2, 0.23, 0.38e6},
+    {16, 32, 1.0, 0.0, 0.45e6},    {32, 32, 1.0, 0.0, 0.45e6},    {64, 32, 1.2, 0.0, 0.45e6},
 };
-constexpr double kFlops32 = 0.55e6;                        // float32, of one CU in a microsecond
-constexpr double kSkinnyBytes = 60e3;                      // what a CU's waves load in a microsecond
+constexpr double kSkinnyBytes = 80e3;                      // what a CU's waves load in a microsecond
 constexpr double kReadBytes = 5.5e6;                       // what the chip reads in a microsecond
 constexpr double kLaunchUs = 2.2;                          // of a launch, whatever it does
 constexpr double kReduceUs = 5.0, kReduceBytes = 4e6;      // the launch that adds the partial sums
@@ -44,28 +44,27 @@ OpPlan op_gemm_plan(int elem_bytes, int layout, int kind, int64_t M, int64_t N, 
   // every product reads both operands, from memory at the rate of memory
   const double read_us = (double)elem_bytes * pieces * K * ((double)M + (double)subs * N * outputs) / kReadBytes;
   double best_us = 1e30;
-  for (int t = 0; t < 7; ++t) {
+  for (int t = 0; t < OP_TILES; ++t) {
     const TileCost& c = kTiles[t];
     const bool skinny = t >= OP_TILE_SKINNY16;
     if (skinny && (layout == OP_TN || M > 512)) continue;
     if (!direct && (t == OP_TILE_256 || t == OP_TILE_64X128)) continue;
-    const int64_t sn = skinny ? 32 : kind == OP_GATED ? c.bn / 2 : c.bn;
+    const int64_t sn = skinny ? c.bn : kind == OP_GATED ? c.bn / 2 : c.bn;
     const int64_t tiles = ceil_div(M, c.bm) * ceil_div(N, sn) * outputs;
-    const int waves = skinny ? (kind == OP_GATED || c.bm > 16 ? 4 : 8) : 1;
-    double stage_us = c.stage;
-    if (skinny) {
-      // a turn of the waves: W in rows of 64 bytes counts for more, as whole cache lines are fetched
-      const double w = layout == OP_NN && elem_bytes == 2 ? 1.6 : 1.0;
-      stage_us = waves * 128.0 * (32 * subs * w + c.bm) / kSkinnyBytes;
-    }
+    const int waves = !skinny ? 1 : kind == OP_GATED || c.bm > 16 ? 4 : 8;
+    double stage_us = c.stage, tile_read_us = read_us;
+    // half cache lines of W: whole ones are fetched (134 MB of W from memory: 40 us in 64-byte pieces, 29 in 128)
+    const bool halves = layout == OP_NN && sn * elem_bytes < 128;
+    if (halves) tile_read_us *= 1.45;
+    if (skinny) stage_us = waves * 128.0 * ((double)sn * subs * (halves ? 1.6 : 1.0) + c.bm) / kSkinnyBytes;  // a turn
     if (elem_bytes == 4)
-      stage_us = std::max(stage_us, 2.0 * c.bm * sn * subs * op_stage_k(4) * waves / kFlops32);
+      stage_us = std::max(stage_us, 2.0 * c.bm * sn * subs * op_stage_k(4) * waves / c.flops32);
     // through registers, one stage ahead
     if (!direct) stage_us = skinny ? 1.1 * stage_us + 0.5 : stage_us * (t == OP_TILE_64 ? 2.0 : 4.0);
-    for (int64_t splits = 1; splits <= 32 && (splits == 1 || stages / splits >= 4 * waves); splits *= 2) {
+    for (int64_t splits = 1; splits <= 32 && (splits == 1 || stages / splits >= 2 * waves); splits *= 2) {
       const int64_t per = ceil_div(stages, splits), used = ceil_div(stages, per);
       const double rounds = (double)ceil_div(tiles * used, kCus);
-      double us = kLaunchUs + rounds * c.fixed + std::max(rounds * ceil_div(per, waves) * stage_us, read_us);
+      double us = kLaunchUs + rounds * c.fixed + std::max(rounds * ceil_div(per, waves) * stage_us, tile_read_us);
       if (used > 1) us += kReduceUs + 8.0 * used * planes * (double)M * (double)N / kReduceBytes;
       if (us < best_us * (splits > 1 ? 0.93 : 1.0)) {
         best_us = us;
@@ -91,7 +90,7 @@ int64_t op_gemm_partial_bytes(const OpPlan& plan, int kind, int64_t M, int64_t N
 
 int64_t op_gemm_blocks(const OpPlan& plan, int kind, int64_t M, int64_t N) {
   const TileCost& c = kTiles[plan.tile];
-  const int64_t sn = plan.tile >= OP_TILE_SKINNY16 ? 32 : kind == OP_GATED ? c.bn / 2 : c.bn;
+  const int64_t sn = plan.tile >= OP_TILE_SKINNY16 ? c.bn : kind == OP_GATED ? c.bn / 2 : c.bn;
   return ceil_div(M, c.bm) * ceil_div(N, sn);
 }
 

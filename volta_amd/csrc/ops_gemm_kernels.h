@@ -417,13 +417,13 @@ __device__ __forceinline__ void op_tile_of(int b, int tiles_m, int tiles_n, int*
 }
 
 // ---------------------------------------------------------------------------
-// Tiled product: BM x BN of D per block, WGM x WGN waves, a ring of NST stages
-// in LDS -- the loads of stage s + NST - 1 are issued before stage s is
-// multiplied, so a stage's loads have NST - 1 stages' time to arrive.
+// Staged product, for operands whose rows direct loads cannot take: BM x BN of
+// D per block, 2 x 2 waves.  A stage goes through registers into one of two
+// places in LDS; the loads of the next are in flight while it is multiplied.
 // ---------------------------------------------------------------------------
-template <typename T, int LAYOUT, int KIND, int BM, int BN, int WGM, int WGN, int NST, bool DIRECT>
-__global__ void __launch_bounds__(WGM* WGN * 64) op_gemm_tiled(OpGemm g) {
-  constexpr int NW = WGM * WGN, WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
+template <typename T, int LAYOUT, int KIND, int BM, int BN>
+__global__ void __launch_bounds__(256) op_gemm_staged(OpGemm g) {
+  constexpr int NW = 4, WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16;
   constexpr bool kGated = KIND == OP_GATED;
   constexpr int kSubs = kGated ? 2 : 1, SN = BN / kSubs;  // gated: half the columns of each weight matrix
   constexpr int TNS = TN / kSubs;
@@ -431,14 +431,11 @@ __global__ void __launch_bounds__(WGM* WGN * 64) op_gemm_tiled(OpGemm g) {
   using PT = Tile<T, BM, P_KC, NW>;
   using QT = Tile<T, SN, Q_KC, NW>;
   constexpr int kStageK = PT::kStageK, kStageBytes = PT::kBytes + QT::kBytes * kSubs;
-  constexpr int kStageLoads = PT::kLoads + QT::kLoads * kSubs;
-  static_assert(NST >= 2 && NST <= 4 && (DIRECT || NST == 2), "ring");
-  __shared__ __attribute__((aligned(16))) char lds[NST * kStageBytes];
-  auto stage = [&](auto i) { return lds + decltype(i)::value % NST * kStageBytes; };
+  __shared__ __attribute__((aligned(16))) char lds[2 * kStageBytes];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave / WGN, wn = wave % WGN;
+  const int wm = wave >> 1, wn = wave & 1;
   int tm, tn;
   op_tile_of(blockIdx.x, g.tiles_m, g.tiles_n, &tm, &tn);
   const int m0 = tm * BM, n0 = tn * SN;
@@ -455,27 +452,22 @@ __global__ void __launch_bounds__(WGM* WGN * 64) op_gemm_tiled(OpGemm g) {
 
   Cursor<T, LAYOUT, kGated> next;
   next.init(g, m0, n0, z, s_begin, 1);
-  chunk16 rp[DIRECT ? 1 : PT::kLoads], rq[kSubs][DIRECT ? 1 : QT::kLoads];
-  auto load = [&](char* to) {  // the next stage
+  chunk16 rp[PT::kLoads], rq[kSubs][QT::kLoads];
+  auto fetch = [&]() {  // the next stage
     const int k_left = g.K - next.k;
-    if constexpr (DIRECT) {
-      const uint32_t lp = op_lds_byte(to), lq = lp + PT::kBytes;
-      if (k_left >= kStageK) {
-        pt.issue(next.p, lp, wave);
+    pt.fetch(next.p, rp, wave, lane, p_left, k_left);
 #pragma unroll
-        for (int i = 0; i < kSubs; ++i) qt.issue(next.q[i], lq + i * QT::kBytes, wave);
-      } else {
-        pt.issue_tail(next.p, lp, wave, lane, k_left);
-#pragma unroll
-        for (int i = 0; i < kSubs; ++i) qt.issue_tail(next.q[i], lq + i * QT::kBytes, wave, lane, k_left);
-      }
-    } else {
-      pt.fetch(next.p, rp, wave, lane, p_left, k_left);
-#pragma unroll
-      for (int i = 0; i < kSubs; ++i) qt.fetch(next.q[i], rq[i], wave, lane, q_left, k_left);
-    }
+    for (int i = 0; i < kSubs; ++i) qt.fetch(next.q[i], rq[i], wave, lane, q_left, k_left);
     next.step();
     next.cross(g);
+  };
+  // A wave writes a place again only behind the barrier that every wave
+  // reached after it had read it.
+  auto put = [&](char* to) {
+    pt.put(rp, to, wave, lane);
+#pragma unroll
+    for (int i = 0; i < kSubs; ++i) qt.put(rq[i], to + PT::kBytes + i * QT::kBytes, wave, lane);
+    __syncthreads();
   };
 
   floatx4 acc[TM][TN];
@@ -503,48 +495,21 @@ __global__ void __launch_bounds__(WGM* WGN * 64) op_gemm_tiled(OpGemm g) {
     }
   };
 
-  if constexpr (DIRECT) {
-    op_unroll<NST - 1>([&](auto i) {
-      if (s_begin + i < s_end) load(stage(i));
+  if (s_begin < s_end) fetch();
+  for (int s0 = s_begin; s0 < s_end; s0 += 2) {
+    op_unroll<2>([&](auto i) {
+      const int s = s0 + i;
+      if (s >= s_end) return;
+      char* at = lds + decltype(i)::value * kStageBytes;
+      put(at);
+      if (s + 1 < s_end) fetch();
+      __builtin_amdgcn_sched_barrier(0);
+      compute(at);
     });
-    for (int s0 = s_begin; s0 < s_end; s0 += NST) {
-      op_unroll<NST>([&](auto i) {
-        const int s = s0 + i;
-        if (s >= s_end) return;
-        // stage s is there once only the newer stages' loads are in flight;
-        // behind the barrier it is there for every wave, and every wave has
-        // finished reading stage s - 1, whose place the next loads take
-        if (s + NST - 2 < s_end) op_wait_loads<(NST - 2) * kStageLoads>();
-        else op_wait_loads<0>();
-        op_wait_lds();
-        op_barrier();
-        if (s + NST - 1 < s_end) load(stage(std::integral_constant<int, decltype(i)::value + NST - 1>()));
-        __builtin_amdgcn_sched_barrier(0);
-        compute(stage(i));
-      });
-    }
-  } else {
-    auto put = [&](char* to) {
-      pt.put(rp, to, wave, lane);
-#pragma unroll
-      for (int i = 0; i < kSubs; ++i) qt.put(rq[i], to + PT::kBytes + i * QT::kBytes, wave, lane);
-      __syncthreads();
-    };
-    if (s_begin < s_end) load(lds);
-    for (int s0 = s_begin; s0 < s_end; s0 += 2) {
-      op_unroll<2>([&](auto i) {
-        const int s = s0 + i;
-        if (s >= s_end) return;
-        put(stage(i));
-        if (s + 1 < s_end) load(lds);
-        __builtin_amdgcn_sched_barrier(0);
-        compute(stage(i));
-      });
-    }
   }
 
-  __syncthreads();  // the ring is free
-  static_assert(NW * op_region_bytes<TM, TN> <= NST * kStageBytes, "regions fit the ring");
+  __syncthreads();  // both places are free
+  static_assert(NW * op_region_bytes<TM, TN> <= 2 * kStageBytes, "output regions fit");
   op_write_out<T, KIND>(g, acc, lds + wave * op_region_bytes<TM, TN>, lane, m0 + wm * WM, n0 + wn * (TNS * 16), z, split);
 }
 
@@ -1081,14 +1046,14 @@ __global__ void __launch_bounds__(256) op_gemm_reduce(OpGemm g) {
 }
 
 // ---------------------------------------------------------------------------
-template <typename T, int LAYOUT, int KIND, int BM, int BN, int WGM, int WGN, int NST, bool DIRECT>
-hipError_t launch_tiled(OpGemm& g, hipStream_t st) {
+template <typename T, int LAYOUT, int KIND, int BM, int BN>
+hipError_t launch_staged(OpGemm& g, hipStream_t st) {
   constexpr int SN = KIND == OP_GATED ? BN / 2 : BN;
   g.tiles_m = (g.M + BM - 1) / BM;
   g.tiles_n = (g.N + SN - 1) / SN;
-  hipLaunchKernelGGL((op_gemm_tiled<T, LAYOUT, KIND, BM, BN, WGM, WGN, NST, DIRECT>),
-                     dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits, (unsigned)g.outputs),
-                     dim3(WGM * WGN * 64), 0, st, g);
+  hipLaunchKernelGGL((op_gemm_staged<T, LAYOUT, KIND, BM, BN>),
+                     dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits, (unsigned)g.outputs), dim3(256), 0, st,
+                     g);
   return hipGetLastError();
 }
 
@@ -1155,12 +1120,12 @@ hipError_t launch(const OpPlan& plan, OpGemm& g, hipStream_t st) {
   } else if (plan.tile == OP_TILE_64) {
     constexpr int WGM = KIND == OP_GATED ? 4 : 2;  // a wave has columns of both weight matrices
     e = g.direct ? launch_middle<T, LAYOUT, KIND, 64, 64, WGM, 8 / WGM, 2, 4>(g, st)
-                 : launch_tiled<T, LAYOUT, KIND, 64, 64, 2, 2, 2, false>(g, st);
+                 : launch_staged<T, LAYOUT, KIND, 64, 64>(g, st);
   } else if (plan.tile == OP_TILE_64X128 && g.direct) {
     e = launch_middle<T, LAYOUT, KIND, 64, 128, 2, 4, 1, 4>(g, st);
   } else {
     e = g.direct ? launch_middle<T, LAYOUT, KIND, 128, 128, 2, 4, 1, 4>(g, st)
-                 : launch_tiled<T, LAYOUT, KIND, 128, 128, 2, 2, 2, false>(g, st);
+                 : launch_staged<T, LAYOUT, KIND, 128, 128>(g, st);
   }
   if (e != hipSuccess || g.splits <= 1) return e;
   const int64_t quads = (int64_t)g.M * ((g.N + 3) / 4);

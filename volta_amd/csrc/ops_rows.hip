@@ -315,8 +315,25 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_grad_kernel(NormGr
     }
   }
   if (!a.partial) return;
-  // a row of partial sums for each block's row in flight
-  float* p = a.partial + ((int64_t)blockIdx.x * RPB + threadIdx.x / TPR) * a.cols;
+  float* p = a.partial + (int64_t)blockIdx.x * a.cols;
+  if constexpr (RPB > 1) {  // the block's waves' sums, in wave order
+    __shared__ float sums[RPB - 1][NCH][E][TPR];
+    const int w = threadIdx.x / TPR;
+    if (w > 0) {
+#pragma unroll
+      for (int k = 0; k < NCH; ++k)
+#pragma unroll
+        for (int i = 0; i < E; ++i) sums[w - 1][k][i][t] = dw[k][i];
+    }
+    __syncthreads();
+    if (w > 0) return;
+#pragma unroll
+    for (int u = 0; u < RPB - 1; ++u)
+#pragma unroll
+      for (int k = 0; k < NCH; ++k)
+#pragma unroll
+        for (int i = 0; i < E; ++i) dw[k][i] += sums[u][k][i][t];
+  }
 #pragma unroll
   for (int k = 0; k < NCH; ++k) store_vec(p + (t + k * TPR) * E, a.cols - (t + k * TPR) * E, dw[k]);
 }
@@ -552,9 +569,8 @@ int chunks_of(int type, int64_t cols) {
 constexpr int kNormGradHeld = 2048;  // chunks of a row that the gradient's kernel holds at most
 
 template <typename T, int TPR, int NCH>
-hipError_t norm_grad_launch(const NormGradArgs& a, int partial_rows, hipStream_t st) {
-  constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
-  hipLaunchKernelGGL((norm_grad_kernel<T, TPR, NCH>), dim3((unsigned)(partial_rows / RPB)), dim3(TPR * RPB), 0, st, a);
+hipError_t norm_grad_launch(const NormGradArgs& a, int blocks, hipStream_t st) {
+  hipLaunchKernelGGL((norm_grad_kernel<T, TPR, NCH>), dim3((unsigned)blocks), dim3(TPR < 256 ? 256 : TPR), 0, st, a);
   return hipGetLastError();
 }
 
@@ -581,8 +597,10 @@ hipError_t norm_forward(int type, bool e4m3, const NormArgs& a, hipStream_t st) 
 int norm_grad_blocks(int type, int64_t rows, int64_t cols) {
   const int chunks = chunks_of(type, cols);
   if (chunks > kNormGradHeld) return strips_of(chunks, rows);
+  // as many blocks as the chip holds: 8192 x 4096 bf16 took 84 us with 512 blocks, 57 with 1024, 61 with 2048
+  // (and 4 us more for the sum of their partial sums)
   const int rpb = chunks <= 128 ? 4 : 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>((rows + rpb - 1) / rpb, 512)) * rpb;
+  return (int)std::max<int64_t>(1, std::min<int64_t>((rows + rpb - 1) / rpb, chunks <= 512 ? 1024 : 512));
 }
 
 hipError_t norm_backward(int type, const NormGradArgs& a, hipStream_t st) {

@@ -17,13 +17,16 @@
  *     step.  ld_* is a matrix's distance between rows in elements; 0 means
  *     packed.  A matrix of rows that overlap (ld below the row's length) is
  *     refused, and so is an ld over 2^21.
- *   - Pointers are device pointers, aligned to their element.  Rows that are
- *     16-byte aligned (pointer and ld) and a multiple of 16 bytes long take
- *     the fast loads; others are correct and slower.
+ *   - Pointers are device pointers, aligned to their element.  A product's
+ *     operands whose rows are 16-byte aligned (pointer and ld) and a multiple
+ *     of 16 bytes long take the fast loads; operands of other lengths or ld
+ *     are copied into the workspace where that pays, and else read through
+ *     registers, as are misaligned pointers.
  *   - The call enqueues its kernels on `stream` (a hipStream_t; NULL: the
  *     default stream) of the current device and returns.  It allocates
  *     nothing and waits for nothing, so it can be captured into a graph.  A
- *     stream of another device is refused.
+ *     stream or memory of another device is refused, and so is memory that
+ *     no device reads.
  *   - `workspace` is device memory of at least the bytes that the operator's
  *     *_workspace call gives for the same description (0: NULL is fine),
  *     16-byte aligned.  Its contents do not matter before and after.  Calls

@@ -722,3 +722,110 @@ def test_rows_far_into_a_large_matrix(lib):
         assert np.array_equal(back.bits(), packed.bits())
     finally:
         lib.lib.volta_hip_device_free(int(p))
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_misaligned_beside_an_operand_laid_out_anew(lib, t):
+    """x's rows are not whole chunks, so it would be copied; W's are, but W
+    starts at an odd element, so neither takes the direct loads: the sums are
+    whole numbers, so the result is exact."""
+    M, K, N = 1600, 1001, 1504
+    rng = np.random.default_rng(78)
+    x, w = whole(rng, M, K), whole(rng, K, N)
+    op = ops.Linear(M, K, N, t)
+    for lead in (0, 1):
+        mx, mw, my = Mat(lib, t, M, K, x), Mat(lib, t, K, N, w, lead=lead), Mat(lib, t, M, N)
+        ws = Space(lib, op)
+        op.forward(mx, mw, my, workspace=ws)
+        ws.check()
+        assert np.array_equal(my.bits().view(R.STORE[t]), R.pack(x @ w, t)), lead
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_one_matrix_as_gate_and_up(lib, t):
+    """Wg and Wu may be the same matrix, odd rows of it among them."""
+    for M, K, N in ((3, 40, 24), (70, 33, 41), (1600, 1001, 1501)):
+        rng = np.random.default_rng(M)
+        x, w = draws(rng, t, M, K), draws(rng, t, K, N)
+        mx, m1, m2 = Mat(lib, t, M, K, x), Mat(lib, t, K, N, w), Mat(lib, t, K, N, w)
+        op = ops.GatedFF(M, K, N, t)
+        ws, wsb = Space(lib, op), Space(lib, op, True)
+        got = []
+        for up in (m1, m2):
+            h, g, u, dx = Mat(lib, t, M, N), Mat(lib, t, M, N), Mat(lib, t, M, N), Mat(lib, t, M, K)
+            op.forward(mx, m1, up, h, gate=g, up=u, workspace=ws)
+            op.backward(h, mx, m1, up, g, u, dx=dx, workspace=wsb)
+            got.append([m.bits() for m in (h, g, u, dx)])
+        ws.check()
+        wsb.check()
+        assert np.array_equal(got[0][1], got[0][2])
+        assert all(np.array_equal(a, b) for a, b in zip(*got))
+
+
+def test_blocks_on_two_streams_at_once(lib):
+    """Two blocks enqueued on two streams, a workspace each, one of them in
+    the forms for a few rows: the bits they have alone."""
+    hip = _hip(lib)
+    blocks = [Block(lib, "bf16", 300, 512, 1024), Block(lib, "bf16", 5, 2048, 4096, seed=12)]
+    want = []
+    for b in blocks:
+        b.run()
+        want.append(b.bits())
+    streams = [C.c_void_p(), C.c_void_p()]
+    for st in streams:
+        assert hip.hipStreamCreate(C.byref(st)) == 0
+    for _ in range(3):
+        for b in blocks:
+            for k in Block.OUT:  # spoil the last outputs
+                m = b.m[k]
+                lib.lib.volta_hip_copy(m.dev.ptr, m.before.ctypes.data, m.before.nbytes, 1)
+        assert hip.hipDeviceSynchronize() == 0
+        for _ in range(4):
+            for b, st in zip(blocks, streams):
+                b.run(stream=st.value)
+        for st in streams:
+            assert hip.hipStreamSynchronize(st) == 0
+        for b, w in zip(blocks, want):
+            assert all(np.array_equal(v, w[k]) for k, v in b.bits().items())
+    for st in streams:
+        assert hip.hipStreamDestroy(st) == 0
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_dropout_at_the_end_of_the_stream(lib, t):
+    """Outputs are counted modulo 2^64."""
+    M, N, p = 3, 37, 0.5
+    rng = np.random.default_rng(4)
+    x = draws(rng, t, M, N)
+    mx, my = Mat(lib, t, M, N, x), Mat(lib, t, M, N)
+    for seed, offset in (((1 << 64) - 1, (1 << 64) - 7), (5, (1 << 64) - 1), (0, 1 << 63)):
+        ops.Dropout(M, N, t, p).forward(mx, my, seed=seed, offset=offset)
+        want = np.where(R.splitmix_keep(M * N, seed, offset, p).reshape(M, N), 2 * x, 0)
+        assert np.array_equal(my.bits().view(R.STORE[t]), R.pack(want, t))
+
+
+def test_host_memory_refused(lib):
+    """A matrix or workspace that is not memory a device reads is refused on
+    the host, and nothing is enqueued."""
+    M, K, N = 300, 64, 64
+    m = {k: Mat(lib, "f32", *s) for k, s in {"x": (M, K), "w": (K, N), "y": (M, N), "dw": (K, N), "r": (1, M)}.items()}
+    host = np.zeros(M * N + 4, np.float32)
+    h = host.ctypes.data + -host.ctypes.data % 16
+    lin, nrm, drp = ops.Linear(M, K, N, act="relu"), ops.RmsNorm(M, K), ops.Dropout(M, K)
+    ws = Space(lib, lin, True)
+
+    def refused(name, call):
+        with pytest.raises(ops.OperatorError) as e:
+            call()
+        assert name + " is not memory" in str(e.value), str(e.value)
+
+    refused("x", lambda: lin.forward(h, m["w"], m["y"], workspace=ws))
+    refused("w", lambda: lin.forward(m["x"], h, m["y"], workspace=ws))
+    refused("y", lambda: lin.forward(m["x"], m["w"], h, workspace=ws))
+    refused("bias", lambda: lin.forward(m["x"], m["w"], m["y"], bias=h, workspace=ws))
+    refused("dw", lambda: lin.backward(m["y"], m["x"], m["w"], pre=m["y"], dw=h, workspace=ws))
+    refused("the workspace", lambda: lin.backward(m["y"], m["x"], m["w"], pre=m["y"], dw=m["dw"], workspace=h))
+    refused("weight", lambda: nrm.forward(m["x"], m["y"], weight=h))
+    refused("rstd", lambda: nrm.forward(m["x"], m["y"], rstd=h))
+    refused("y", lambda: drp.forward(m["x"], h))
+    assert all(v.untouched() for v in m.values()) and not host.any()

@@ -159,3 +159,12 @@ def test_host_types():
     assert v[0x7E] == 448 and v[1] == 2.0**-9 and v[0x88] == -(2.0**-6) and np.isnan(v[0x7F]) and np.isnan(v[0xFF])
     assert list(R.splitmix_keep(4, 0, 0, 0.5)) == [bool(b >= 1 << 31) for z in (0xE220A8397B1DCDAF, 0x6E789E6AA1B965F4)
                                                    for b in (z & 0xFFFFFFFF, z >> 32)]
+
+
+def test_products_of_too_many_blocks_refused():
+    """Whatever the direction: by the workspace's call already."""
+    for op in (ops.Linear(1 << 30, 64, 64, "bf16"), ops.GatedFF(1 << 30, 64, 64, "bf16"),
+               ops.Linear(1 << 30, 63, 65, "f32", act="gelu")):
+        for backward in (False, True):
+            refused(lambda: op.workspace_bytes(backward=backward), "too many")
+    assert ops.Linear(1 << 24, 64, 64, "bf16").workspace_bytes(backward=True) > 0

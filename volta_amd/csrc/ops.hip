@@ -7,8 +7,8 @@
 #include <cmath>
 #include <cstdint>
 #include <exception>
+#include <initializer_list>
 #include <string>
-#include <vector>
 
 #include "../../include/volta_ops.h"
 #include "../../include/volta_train.h"
@@ -22,6 +22,7 @@ namespace {
 
 constexpr int64_t kMaxLd = int64_t{1} << 21;
 constexpr int64_t kMaxRows = int64_t{1} << 30;
+constexpr int64_t kMaxBlocks = int64_t{1} << 22;  // a dimension of a grid has fewer than 2^32 threads
 
 struct Refused {
   std::string what;
@@ -48,21 +49,6 @@ int32_t guarded(const char* call, F body) {
 
 void check_hip(hipError_t e, const char* what) {
   if (e != hipSuccess) refuse(std::string(what) + " launch failed: " + hipGetErrorString(e));
-}
-
-hipStream_t stream_of(void* stream) {
-  const hipStream_t st = static_cast<hipStream_t>(stream);
-  // NULL and the runtime's two named streams are the current device's
-  if ((uintptr_t)stream > 2) {
-    hipDevice_t of = 0;
-    int cur = 0;
-    hipError_t e = hipStreamGetDevice(st, &of);
-    if (e == hipSuccess) e = hipGetDevice(&cur);
-    if (e != hipSuccess) refuse(std::string("the stream's device: ") + hipGetErrorString(e));
-    if (of != cur)
-      refuse("the stream is of device " + std::to_string(of) + ", the current device is " + std::to_string(cur));
-  }
-  return st;
 }
 
 // A matrix of a call: `rows` x `cols` elements of `bytes`, `ld` apart.
@@ -102,9 +88,10 @@ struct Shared {  // two matrices of a call that may be the same one
 
 // Alignment of every pointer, and no output over anything else but where
 // `same` allows the two to be one matrix.
-void check_mats(const std::vector<Mat>& mats, const std::vector<Shared>& same, const void* workspace = nullptr,
-                int64_t workspace_bytes = 0) {
-  for (const Mat& m : mats)
+void check_mats(std::initializer_list<Mat> list, std::initializer_list<Shared> same, const void* workspace,
+                int64_t workspace_bytes) {
+  const Mat* mats = list.begin();
+  for (const Mat& m : list)
     if (m.p && (uintptr_t)m.p % m.bytes != 0) refuse(std::string(m.name) + " is not aligned to its element");
   auto meet = [](const void* p, int64_t n, const void* q, int64_t k) {
     const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
@@ -119,8 +106,8 @@ void check_mats(const std::vector<Mat>& mats, const std::vector<Shared>& same, c
     const int64_t col = apart / a.bytes % a.ld;
     return col >= lo.cols && col + hi.cols <= a.ld;
   };
-  for (size_t i = 0; i < mats.size(); ++i) {
-    for (size_t j = i + 1; j < mats.size(); ++j) {
+  for (size_t i = 0; i < list.size(); ++i) {
+    for (size_t j = i + 1; j < list.size(); ++j) {
       const Mat &a = mats[i], &b = mats[j];
       if (!a.out && !b.out) continue;
       if (!meet(a.p, a.span(), b.p, b.span()) || beside(a, b)) continue;
@@ -134,6 +121,38 @@ void check_mats(const std::vector<Mat>& mats, const std::vector<Shared>& same, c
     if (meet(mats[i].p, mats[i].span(), workspace, workspace_bytes))
       refuse(std::string(mats[i].name) + " overlaps the workspace");
   }
+}
+// Memory of another device or of the host's own would be a fault of the GPU.
+void check_memory(const char* name, const void* p, int device) {
+  hipPointerAttribute_t at{};
+  if (hipPointerGetAttributes(&at, p) != hipSuccess || at.type == hipMemoryTypeUnregistered) {
+    (void)hipGetLastError();
+    refuse(std::string(name) + " is not memory that the device reads");
+  }
+  if (at.type == hipMemoryTypeDevice && at.device != device)
+    refuse(std::string(name) + " is of device " + std::to_string(at.device) + ", the current device is " +
+           std::to_string(device));
+}
+
+// What every call checks of its matrices, workspace and stream.
+hipStream_t check_call(std::initializer_list<Mat> mats, std::initializer_list<Shared> same, const void* workspace,
+                       int64_t workspace_bytes, void* stream) {
+  check_mats(mats, same, workspace, workspace_bytes);
+  int device = 0;
+  hipError_t e = hipGetDevice(&device);
+  if (e != hipSuccess) refuse(std::string("the current device: ") + hipGetErrorString(e));
+  // NULL and the runtime's two named streams are the current device's
+  if ((uintptr_t)stream > 2) {
+    hipDevice_t of = 0;
+    e = hipStreamGetDevice(static_cast<hipStream_t>(stream), &of);
+    if (e != hipSuccess) refuse(std::string("the stream's device: ") + hipGetErrorString(e));
+    if (of != device)
+      refuse("the stream is of device " + std::to_string(of) + ", the current device is " + std::to_string(device));
+  }
+  for (const Mat& m : mats)
+    if (m.span() > 0) check_memory(m.name, m.p, device);
+  if (workspace_bytes > 0) check_memory("the workspace", workspace, device);
+  return static_cast<hipStream_t>(stream);
 }
 void need(const void* p, const char* name) {
   if (!p) refuse(std::string(name) + " is NULL");
@@ -180,14 +199,19 @@ struct Shape {
   Operand p, q;
   bool pack_p, pack_q;
   int64_t partial_bytes, pack_bytes;  // partial sums, then the copies
-  int64_t bytes() const { return partial_bytes + pack_bytes; }
+  int64_t blocks;                     // of D's tiles, at most
+  // The workspace of a call with this product.
+  int64_t bytes() const {
+    if (blocks > kMaxBlocks) refuse("the rows and columns of a product are too many");
+    return partial_bytes + pack_bytes;
+  }
 };
 OpPlan plan_of(int type, const Shape& s, bool direct) {
   return op_gemm_plan(elem_bytes(type), s.layout, s.kind, s.M, s.N, s.K, s.pieces, s.outputs, direct);
 }
 Shape shape_of(int type, int layout, int kind, int64_t M, int64_t N, int64_t K, int pieces, int outputs, Operand p,
                Operand q) {
-  Shape s{layout, kind, M, N, K, pieces, outputs, p, q, !whole_chunks(type, p), !whole_chunks(type, q), 0, 0};
+  Shape s{layout, kind, M, N, K, pieces, outputs, p, q, !whole_chunks(type, p), !whole_chunks(type, q), 0, 0, 0};
   if (s.pack_p || s.pack_q) {
     s.pack_bytes = (s.pack_p ? p.count * packed_bytes(type, p) : 0) + (s.pack_q ? q.count * packed_bytes(type, q) : 0);
     if (!op_gemm_pack(elem_bytes(type), layout, kind, M, N, K, pieces, outputs, s.pack_bytes)) {
@@ -195,9 +219,11 @@ Shape shape_of(int type, int layout, int kind, int64_t M, int64_t N, int64_t K, 
       s.pack_bytes = 0;
     }
   }
-  for (bool direct : {false, true})
-    s.partial_bytes =
-        std::max(s.partial_bytes, align256(op_gemm_partial_bytes(plan_of(type, s, direct), kind, M, N, outputs)));
+  for (bool direct : {false, true}) {
+    const OpPlan plan = plan_of(type, s, direct);
+    s.partial_bytes = std::max(s.partial_bytes, align256(op_gemm_partial_bytes(plan, kind, M, N, outputs)));
+    s.blocks = std::max(s.blocks, op_gemm_blocks(plan, kind, M, N));
+  }
   return s;
 }
 
@@ -252,8 +278,6 @@ void product(int type, const Shape& s, const void* const* ps, const void* const*
   g.partial = reinterpret_cast<float*>(workspace);
   g.epi = epi;
   const OpPlan plan = plan_of(type, s, direct);
-  // a grid has fewer than 2^32 threads
-  if (op_gemm_blocks(plan, s.kind, s.M, s.N) > (int64_t{1} << 22)) refuse("rows * columns of a product are too many");
   if (pack.n) check_hip(pack_rows(type, pack, st), "layout");
   check_hip(gemm(type, s.layout, s.kind, plan, g, st), what);
 }
@@ -407,8 +431,7 @@ int32_t volta_op_linear_forward(const volta_op_linear* in, const void* x, const 
     const Mat mr{"residual", residual, d.rows, d.outputs, d.ld_residual, e, false};
     const Mat my{"y", y, d.rows, d.outputs, d.ld_y, e, true}, mp{"pre", pre, d.rows, d.outputs, d.ld_pre, e, true};
     check_workspace(workspace, workspace_bytes, l.forward_bytes());
-    check_mats({mx, mw, mb, mr, my, mp}, {{residual, y}}, workspace, l.forward_bytes());
-    const hipStream_t st = stream_of(stream);
+    const hipStream_t st = check_call({mx, mw, mb, mr, my, mp}, {{residual, y}}, workspace, l.forward_bytes(), stream);
     OpEpilogue epi{};
     epi.act = d.act;
     epi.bias[0] = bias;
@@ -443,8 +466,7 @@ int32_t volta_op_linear_backward(const volta_op_linear* in, const void* dy, cons
     const Mat mdx{"dx", dx, d.rows, d.inputs, d.ld_dx, e, true}, mdw{"dw", dw, d.inputs, d.outputs, d.ld_dw, e, true};
     const Mat mdb{"db", db, 1, d.outputs, d.outputs, e, true};
     check_workspace(workspace, workspace_bytes, l.backward_bytes());
-    check_mats({mdy, mx, mw, mp, mdx, mdw, mdb}, {}, workspace, l.backward_bytes());
-    const hipStream_t st = stream_of(stream);
+    const hipStream_t st = check_call({mdy, mx, mw, mp, mdx, mdw, mdb}, {}, workspace, l.backward_bytes(), stream);
     char* ws = static_cast<char*>(workspace);
     float* sums = reinterpret_cast<float*>(ws + l.dp_bytes);
     char* rest = ws + l.dp_bytes + l.sums_bytes;
@@ -506,8 +528,7 @@ int32_t volta_op_gated_forward(const volta_op_gated* in, const void* x, const vo
     const Mat mh{"h", h, d.rows, d.hidden, d.ld_h, e, true};
     const Mat pg{"gate", gate, d.rows, d.hidden, d.ld_pre, e, true}, pu{"up", up, d.rows, d.hidden, d.ld_pre, e, true};
     check_workspace(workspace, workspace_bytes, l.forward_bytes());
-    check_mats({mx, mg, mu, bg, bu, mh, pg, pu}, {}, workspace, l.forward_bytes());
-    const hipStream_t st = stream_of(stream);
+    const hipStream_t st = check_call({mx, mg, mu, bg, bu, mh, pg, pu}, {}, workspace, l.forward_bytes(), stream);
     OpEpilogue epi{};
     epi.act = d.act;
     epi.bias[0] = b_gate;
@@ -551,8 +572,8 @@ int32_t volta_op_gated_backward(const volta_op_gated* in, const void* dh, const 
     const Mat wu{"dw_up", dw_up, d.inputs, d.hidden, d.ld_dw, e, true};
     const Mat bg{"db_gate", db_gate, 1, d.hidden, d.hidden, e, true}, bu{"db_up", db_up, 1, d.hidden, d.hidden, e, true};
     check_workspace(workspace, workspace_bytes, l.backward_bytes());
-    check_mats({mdh, mx, mg, mu, pg, pu, mdx, wg, wu, bg, bu}, {}, workspace, l.backward_bytes());
-    const hipStream_t st = stream_of(stream);
+    const hipStream_t st = check_call({mdh, mx, mg, mu, pg, pu, mdx, wg, wu, bg, bu}, {}, workspace,
+                                      l.backward_bytes(), stream);
     char* ws = static_cast<char*>(workspace);
     float* sums[2] = {reinterpret_cast<float*>(ws + 2 * l.d_bytes),
                       reinterpret_cast<float*>(ws + 2 * l.d_bytes + l.sums_bytes)};
@@ -613,15 +634,15 @@ int32_t volta_op_rms_norm_forward(const volta_op_rms_norm* in, const void* x, co
     }
     if (!e4m3 && scales) refuse("scales are of out_type E4M3 alone");
     const int64_t groups = d.group ? (d.cols + d.group - 1) / d.group : 1;
-    check_mats({{"x", x, d.rows, d.cols, d.ld_x, e, false},
-                {"residual", residual, d.rows, d.cols, d.ld_residual, e, false},
-                {"weight", weight, 1, d.cols, d.cols, e, false},
-                {"y", y, d.rows, d.cols, d.ld_y, elem_bytes(d.out_type), true},
-                {"sum", sum, d.rows, d.cols, d.ld_sum, e, true},
-                {"rstd", rstd, d.rows, 1, 1, 4, true},
-                {"scales", scales, d.rows, groups, groups, 4, true}},
-               {{sum, x}, {sum, residual}});
-    const hipStream_t st = stream_of(stream);
+    const hipStream_t st = check_call(
+        {{"x", x, d.rows, d.cols, d.ld_x, e, false},
+         {"residual", residual, d.rows, d.cols, d.ld_residual, e, false},
+         {"weight", weight, 1, d.cols, d.cols, e, false},
+         {"y", y, d.rows, d.cols, d.ld_y, elem_bytes(d.out_type), true},
+         {"sum", sum, d.rows, d.cols, d.ld_sum, e, true},
+         {"rstd", rstd, d.rows, 1, 1, 4, true},
+         {"scales", scales, d.rows, groups, groups, 4, true}},
+        {{sum, x}, {sum, residual}}, nullptr, 0, stream);
     NormArgs a{};
     a.x = x;
     a.residual = residual;
@@ -656,15 +677,15 @@ int32_t volta_op_rms_norm_backward(const volta_op_rms_norm* in, const void* dy, 
       need(rstd, "rstd");
     }
     if (dweight) check_workspace(workspace, workspace_bytes, n.backward_bytes());
-    check_mats({{"dy", dy, d.rows, d.cols, d.ld_y, e, false},
-                {"s", s, d.rows, d.cols, d.ld_x, e, false},
-                {"rstd", rstd, d.rows, 1, 1, 4, false},
-                {"weight", weight, 1, d.cols, d.cols, e, false},
-                {"dsum", dsum, d.rows, d.cols, d.ld_sum, e, false},
-                {"dx", dx, d.rows, d.cols, d.ld_dx, e, true},
-                {"dweight", dweight, 1, d.cols, d.cols, e, true}},
-               {{dsum, dx}}, dweight ? workspace : nullptr, n.backward_bytes());
-    const hipStream_t st = stream_of(stream);
+    const hipStream_t st = check_call(
+        {{"dy", dy, d.rows, d.cols, d.ld_y, e, false},
+         {"s", s, d.rows, d.cols, d.ld_x, e, false},
+         {"rstd", rstd, d.rows, 1, 1, 4, false},
+         {"weight", weight, 1, d.cols, d.cols, e, false},
+         {"dsum", dsum, d.rows, d.cols, d.ld_sum, e, false},
+         {"dx", dx, d.rows, d.cols, d.ld_dx, e, true},
+         {"dweight", dweight, 1, d.cols, d.cols, e, true}},
+        {{dsum, dx}}, workspace, dweight ? n.backward_bytes() : 0, stream);
     NormGradArgs a{};
     a.dy = dy;
     a.s = s;
@@ -701,11 +722,11 @@ int32_t volta_op_dropout_forward(const volta_op_dropout* in, const void* x, cons
       need(x, "x");
       need(y, "y");
     }
-    check_mats({{"x", x, d.rows, d.cols, d.ld_x, e, false},
-                {"residual", residual, d.rows, d.cols, d.ld_residual, e, false},
-                {"y", y, d.rows, d.cols, d.ld_y, e, true}},
-               {{x, y}, {residual, y}});
-    const hipStream_t st = stream_of(stream);
+    const hipStream_t st = check_call(
+        {{"x", x, d.rows, d.cols, d.ld_x, e, false},
+         {"residual", residual, d.rows, d.cols, d.ld_residual, e, false},
+         {"y", y, d.rows, d.cols, d.ld_y, e, true}},
+        {{x, y}, {residual, y}}, nullptr, 0, stream);
     DropoutArgs a{};
     a.x = x;
     a.residual = residual;

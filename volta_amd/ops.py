@@ -17,6 +17,7 @@ library raises OperatorError with its message.
 from __future__ import annotations
 
 import ctypes as C
+from operator import attrgetter
 
 from .abi import ACTIVATIONS
 
@@ -81,12 +82,22 @@ def bind(cdll: C.CDLL) -> C.CDLL:
     return cdll
 
 
+_READERS: dict = {}
+
+
+def _reader(t):
+    """How a matrix of type t gives its device address."""
+    read = int if issubclass(t, int) else t.data_ptr if hasattr(t, "data_ptr") else attrgetter("ptr")
+    _READERS[t] = read
+    return read
+
+
 def _address(m):
     """A matrix's device address; None stays None."""
-    if m is None or isinstance(m, int):
-        return m
-    ptr = getattr(m, "ptr", None)
-    return ptr if ptr is not None else m.data_ptr()
+    if m is None:
+        return None
+    t = type(m)
+    return (_READERS.get(t) or _reader(t))(m)
 
 
 def _bytes(m) -> int:

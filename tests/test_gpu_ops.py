@@ -21,7 +21,7 @@ from volta_amd import load_hip, ops
 
 pytestmark = pytest.mark.gpu
 
-TILES = {"256": 0, "128": 1, "64x128": 2, "64": 3, "skinny16": 4, "skinny32": 5, "skinny64": 6}
+TILES = {"256": 0, "256x128": 1, "128": 2, "64x128": 3, "64": 4, "skinny16": 5, "skinny32": 6, "skinny64": 7}
 NN, NT, TN = 0, 1, 2
 LINEAR, GATED, STORE = 0, 1, 2
 U32 = 2.0**-24
@@ -97,7 +97,7 @@ def _forms(t):
         for kind in kinds:
             for tile in TILES:
                 for direct in (False, True):
-                    if tile in ("256", "64x128") and not direct:
+                    if tile in ("256", "256x128", "64x128") and not direct:
                         continue
                     if tile.startswith("skinny") and layout == TN:
                         continue

@@ -52,13 +52,14 @@ struct OpGemm {
 // weight matrix), the sum over k shared out over a block's waves.
 enum OpTile {
   OP_TILE_256 = 0,
-  OP_TILE_128 = 1,
-  OP_TILE_64X128 = 2,
-  OP_TILE_64 = 3,
-  OP_TILE_SKINNY16 = 4,
-  OP_TILE_SKINNY32 = 5,
-  OP_TILE_SKINNY64 = 6,
-  OP_TILES = 7
+  OP_TILE_256X128 = 1,
+  OP_TILE_128 = 2,
+  OP_TILE_64X128 = 3,
+  OP_TILE_64 = 4,
+  OP_TILE_SKINNY16 = 5,
+  OP_TILE_SKINNY32 = 6,
+  OP_TILE_SKINNY64 = 7,
+  OP_TILES = 8
 };
 
 struct OpPlan {

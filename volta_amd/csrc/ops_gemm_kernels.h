@@ -1121,6 +1121,8 @@ hipError_t launch(const OpPlan& plan, OpGemm& g, hipStream_t st) {
     constexpr int WGM = KIND == OP_GATED ? 4 : 2;  // a wave has columns of both weight matrices
     e = g.direct ? launch_middle<T, LAYOUT, KIND, 64, 64, WGM, 8 / WGM, 2, 4>(g, st)
                  : launch_staged<T, LAYOUT, KIND, 64, 64>(g, st);
+  } else if (plan.tile == OP_TILE_256X128 && g.direct) {
+    e = launch_middle<T, LAYOUT, KIND, 256, 128, 4, 2, 1, 3>(g, st);
   } else if (plan.tile == OP_TILE_64X128 && g.direct) {
     e = launch_middle<T, LAYOUT, KIND, 64, 128, 2, 4, 1, 4>(g, st);
   } else {

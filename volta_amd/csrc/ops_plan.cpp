@@ -22,7 +22,7 @@ struct TileCost {
 };
 // Measured on an MI355X.
 constexpr TileCost kTiles[OP_TILES] = {
-    {256, 256, 6.0, 0.95, 0.55e6}, {128, 128, 3.2, 0.43, 0.47e6}, {64, 128, 2.4, 0.33, 0.42e6}, {64, 64, 2.2, 0.23, 0.38e6},
+    {256, 256, 6.0, 0.95, 0.55e6}, {256, 128, 4.4, 0.80, 0.52e6}, {128, 128, 3.2, 0.43, 0.47e6}, {64, 128, 2.4, 0.33, 0.42e6}, {64, 64, 2.2, 0.23, 0.38e6},
     {16, 32, 1.0, 0.0, 0.45e6},    {32, 32, 1.0, 0.0, 0.45e6},    {64, 32, 1.2, 0.0, 0.45e6},
 };
 constexpr double kSkinnyBytes = 80e3;                      // what a CU's waves load in a microsecond
@@ -48,7 +48,7 @@ OpPlan op_gemm_plan(int elem_bytes, int layout, int kind, int64_t M, int64_t N, 
     const TileCost& c = kTiles[t];
     const bool skinny = t >= OP_TILE_SKINNY16;
     if (skinny && (layout == OP_TN || M > 512)) continue;
-    if (!direct && (t == OP_TILE_256 || t == OP_TILE_64X128)) continue;
+    if (!direct && (t == OP_TILE_256 || t == OP_TILE_256X128 || t == OP_TILE_64X128)) continue;
     const int64_t sn = skinny ? c.bn : kind == OP_GATED ? c.bn / 2 : c.bn;
     const int64_t tiles = ceil_div(M, c.bm) * ceil_div(N, sn) * outputs;
     const int waves = !skinny ? 1 : kind == OP_GATED || c.bm > 16 ? 4 : 8;

@@ -419,7 +419,10 @@ __device__ __forceinline__ void op_tile_of(int b, int tiles_m, int tiles_n, int*
 // ---------------------------------------------------------------------------
 // Staged product, for operands whose rows direct loads cannot take: BM x BN of
 // D per block, 2 x 2 waves.  A stage goes through registers into one of two
-// places in LDS; the loads of the next are in flight while it is multiplied.
+// places in LDS; the loads of the next are in flight while it is multiplied,
+// one stage ahead, and their latency bounds it.  bf16 2048^3: 128x128 40.8 us
+// and 64x64, of which more fit a CU, 37.1, against 23.2 of the direct
+// 128x128; so operands are laid out anew where that copy takes less.
 // ---------------------------------------------------------------------------
 template <typename T, int LAYOUT, int KIND, int BM, int BN>
 __global__ void __launch_bounds__(256) op_gemm_staged(OpGemm g) {
@@ -536,6 +539,11 @@ __global__ void __launch_bounds__(256) op_gemm_staged(OpGemm g) {
 // 64 KB); the wait is for the older ones alone.  (Four phases of 16
 // instructions with a region each measured 4 to 12 % slower: the barrier
 // between two phases costs about 90 cycles.)
+//
+// Bound by the matrix instructions, which are busy 70 to 76 % of the cycles,
+// and by the chip's power, which lowers the clock on sums this large.  8192^3
+// in bf16 from memory: x W 821 us (1339 TFLOP/s), dp W^T 746 (1475), x^T dp
+// 810 (1357); 4096^3 in float32 1067 us (129).
 // ---------------------------------------------------------------------------
 template <typename T, bool KC, int BLK, int STRIDE>
 struct Region : Tile<T, 128, KC, 8> {
@@ -716,6 +724,17 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) o
 // the waves 4 to 7 run half a stage behind the waves 0 to 3, so that of a
 // SIMD's two waves one reads LDS while the other multiplies; a stage is one
 // phase.
+//
+// Tiles for grids that 256x256 would leave CUs idle in; what bounds them is
+// the time of a stage from barrier to barrier, 0.8 us (256x128), 0.45 to 0.55
+// (128x128), 0.35 and 0.25, and how evenly the tiles fill the CUs.  In bf16:
+//   256x128  gated, 1024 rows, 2048 to 4096   33.7 us, 1019 TFLOP/s (128x128 41.8)
+//   128x128  2048^3                           22.4 us,  768 TFLOP/s (256x128 30.7)
+//    64x128  gated, 1 row, 4096 to 16384      54.5 us, 4.9 TB/s of weights
+//    64x64   256 rows, 4096 to 2048           18 us (128x128 33.6, 64x128 26.3)
+// Tried and no faster: rings of 5 and 6 stages, two parts of k a stage at
+// 64x128, and half of the waves on either half of a stage's k, which reads a
+// third less of LDS and pays 1 to 2 us for adding the halves.
 // ---------------------------------------------------------------------------
 template <typename T, int LAYOUT, int KIND, int BM, int BN, int WGM, int WGN, int KS, int NST>
 __global__ void __launch_bounds__(512) op_gemm_middle(OpGemm g) {
@@ -846,7 +865,10 @@ __global__ void __launch_bounds__(512) op_gemm_middle(OpGemm g) {
 // takes 16 MT rows and BN columns (of each weight matrix) and its waves take turns
 // over the stages of k, each with a ring of its own in LDS for both operands
 // (no barrier before the end); the waves' sums are added at the end, in wave
-// order.
+// order.  float32, 64 rows, 1024 to 1024: 6 us (a launch that does nothing
+// takes 2); bf16, 1 row, 4096 to 4096: 11.7 us.  Columns of W in 64-byte
+// pieces cost it bandwidth where W is large and comes from memory: bf16, 16
+// rows, 4096 to 16384, 134 MB: 41 us, and 29 on 64x64 tiles.
 // ---------------------------------------------------------------------------
 template <typename T, int LAYOUT, int KIND, int MT, int BN, int NW, int NST, bool DIRECT>
 __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
@@ -1011,7 +1033,9 @@ __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
 }
 
 // The splits' partial sums, added in order, and the epilogue: a thread for
-// four columns of a row.  Eight splits' sums are loaded at a time.
+// four columns of a row.  Eight splits' sums are loaded at a time.  Bound by
+// its launch and one latency of memory at few rows (8 splits of 16 x 4096:
+// 4.7 us), by memory at many.
 template <typename T, int KIND>
 __global__ void __launch_bounds__(256) op_gemm_reduce(OpGemm g) {
   const int quads = (g.N + 3) / 4, z = blockIdx.y;

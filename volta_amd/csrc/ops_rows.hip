@@ -97,7 +97,9 @@ __device__ __forceinline__ float scale_of(float largest) {
 // ---------------------------------------------------------------------------
 // RMS norm.  TPR threads a row (a wave, or a block), which hold the row in
 // registers between the sum and the output: chunk t + i TPR for i < NCH.
-// NCH = 0: rows too long for that, read again for each pass.
+// NCH = 0: rows too long for that, read again for each pass (from L2).
+// 8192 x 4096 bf16 with a residual and its sum, 268 MB: 51 us, 5.25 TB/s, a
+// large copy's rate; 512 x 65536 (NCH = 0) 30 us, 4.5 TB/s.
 // ---------------------------------------------------------------------------
 template <typename T, bool E4M3, int TPR, int NCH>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_kernel(NormArgs a) {
@@ -256,6 +258,8 @@ hipError_t norm_launch(const NormArgs& a, hipStream_t st) {
 // ---------------------------------------------------------------------------
 // Gradients of the norm: block b takes rows b, b + blocks, ... and keeps the
 // sums of dweight of its rows in registers, a partial sum for each block.
+// 8192 x 4096 bf16 with dsum, 268 MB and 17 MB of partial sums: 57 us, 5.0
+// TB/s, and 5 us for the launch that adds the partial sums.
 // ---------------------------------------------------------------------------
 template <typename T, int TPR, int NCH>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_grad_kernel(NormGradArgs a) {
@@ -339,7 +343,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_grad_kernel(NormGr
 }
 
 // Rows too long for registers: dx row by row, read twice, and dweight column
-// by column.
+// by column.  512 x 65536 bf16: 50 + 24 us.
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_grad_wide_dx(NormGradArgs a) {
   constexpr int E = kChunk<T>;
@@ -424,7 +428,11 @@ __global__ void __launch_bounds__(256) norm_grad_wide_dw(NormGradArgs a, int per
 // ---------------------------------------------------------------------------
 // What a layer's gradients need before their products, with the columns'
 // sums, from 32 bits: linear, dp = dy f'(pre); gated, dg = dh u f'(g) and
-// du = dh f(g).
+// du = dh f(g).  dp, dg and du are rounded to the type, once: the matrix
+// instructions take no wider operands, and the two products read half the
+// bytes.  Kept apart from the products, which read each element many times
+// and would form it anew each time.  Gated, 8192 x 16384 bf16, 1.34 GB: 254
+// us, 5.3 TB/s.
 // ---------------------------------------------------------------------------
 template <typename T, bool GATED>
 __global__ void __launch_bounds__(256) act_grad_kernel(ActGradArgs a, int per) {
@@ -473,7 +481,8 @@ __global__ void __launch_bounds__(256) act_grad_kernel(ActGradArgs a, int per) {
 }
 
 // Partial sums of 64 columns: 16 waves take a sixteenth of the rows each, in
-// order, and their sums are added in wave order.
+// order, and their sums are added in wave order.  1024 rows of 4096: 5 us, a
+// launch and the latency of eight loads after another.
 template <typename T>
 __global__ void __launch_bounds__(1024) sum_partials_kernel(const float* partial, int n, int64_t cols, T* out) {
   __shared__ float lds[16][64];
@@ -496,7 +505,8 @@ __global__ void __launch_bounds__(1024) sum_partials_kernel(const float* partial
   }
 }
 
-// A thread for 16 bytes of a row of the copy.
+// A thread for 16 bytes of a row of the copy.  10 MB: 5 to 6 us, of which a
+// launch is 2.
 template <typename T>
 __global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
   constexpr int E = kChunk<T>;
@@ -512,7 +522,9 @@ __global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
 // ---------------------------------------------------------------------------
 // Dropout: a thread for 16 bytes of a row.  Element i's 32 bits are half of
 // output i/2 of the stream: E/2 outputs for a chunk that starts at an even i,
-// one more for an odd one.
+// one more for an odd one.  The counter replaces a stored mask's bytes; its
+// arithmetic, two 64-bit products for two elements, stays below the memory's
+// time: 8192 x 4096 bf16 with a residual, 201 MB, 38 us, 5.3 TB/s.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ uint64_t stream_output(uint64_t seed, uint64_t n) {
   uint64_t z = seed + (n + 1) * 0x9E3779B97F4A7C15ull;
@@ -654,7 +666,7 @@ hipError_t pack_rows(int type, const PackArgs& a, hipStream_t st) {
   return with_type(type, [&](auto t) {
     using T = decltype(t);
     int64_t blocks = 1;
-    for (int i = 0; i < a.n; ++i) blocks = std::max(blocks, (a.rows[i] * (a.ld_to[i] / kChunk<T>)+255) / 256);
+    for (int i = 0; i < a.n; ++i) blocks = std::max(blocks, (a.rows[i] * (a.ld_to[i] / kChunk<T>) + 255) / 256);
     dim3 grid = grid_of(blocks);
     grid.z = (unsigned)a.n;
     hipLaunchKernelGGL((pack_kernel<T>), grid, dim3(256), 0, st, a);

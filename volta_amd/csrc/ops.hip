@@ -286,7 +286,6 @@ void product(int type, const Shape& s, const void* const* ps, const void* const*
 struct Linear {
   volta_op_linear d;
   Shape fwd, dx, dw;
-  int strips;
   int64_t ld_dp, dp_bytes, sums_bytes;
   int64_t forward_bytes() const { return fwd.bytes(); }
   int64_t backward_bytes() const { return dp_bytes + sums_bytes + std::max(dx.bytes(), dw.bytes()); }
@@ -317,15 +316,13 @@ Linear linear_of(const volta_op_linear* in) {
   l.fwd = shape_of(d.type, OP_NN, OP_LINEAR, d.rows, d.outputs, d.inputs, 1, 1, x, w);
   l.dx = shape_of(d.type, OP_NT, OP_STORE, d.rows, d.inputs, d.outputs, 1, 1, dp, w);
   l.dw = shape_of(d.type, OP_TN, OP_STORE, d.inputs, d.outputs, d.rows, 1, 1, x, dp);
-  l.strips = act_grad_strips(d.type, d.rows, d.outputs);
-  l.sums_bytes = align256(4 * l.strips * d.outputs);
+  l.sums_bytes = align256(4 * act_grad_strips(d.type, d.rows, d.outputs) * d.outputs);
   return l;
 }
 
 struct Gated {
   volta_op_gated d;
   Shape fwd, dx, dw;
-  int strips;
   int64_t ld_d, d_bytes, sums_bytes;
   int64_t forward_bytes() const { return fwd.bytes(); }
   int64_t backward_bytes() const { return 2 * (d_bytes + sums_bytes) + std::max(dx.bytes(), dw.bytes()); }
@@ -353,8 +350,7 @@ Gated gated_of(const volta_op_gated* in) {
   l.fwd = shape_of(d.type, OP_NN, OP_GATED, d.rows, d.hidden, d.inputs, 1, 1, x, w);
   l.dx = shape_of(d.type, OP_NT, OP_STORE, d.rows, d.inputs, d.hidden, 2, 1, dg, w);
   l.dw = shape_of(d.type, OP_TN, OP_STORE, d.inputs, d.hidden, d.rows, 1, 2, x, dg);
-  l.strips = act_grad_strips(d.type, d.rows, d.hidden);
-  l.sums_bytes = align256(4 * l.strips * d.hidden);
+  l.sums_bytes = align256(4 * act_grad_strips(d.type, d.rows, d.hidden) * d.hidden);
   return l;
 }
 
@@ -476,7 +472,8 @@ int32_t volta_op_linear_backward(const volta_op_linear* in, const void* dy, cons
       a.dy = dy;
       a.pre[0] = act ? pre : nullptr;
       a.d[0] = act && (dx || dw) ? ws : nullptr;
-      a.partial[0] = db ? sums : nullptr;
+      a.sums[0] = db;
+      a.partial[0] = sums;
       a.act = d.act;
       a.rows = d.rows;
       a.cols = (int32_t)d.outputs;
@@ -484,7 +481,6 @@ int32_t volta_op_linear_backward(const volta_op_linear* in, const void* dy, cons
       a.ld_pre = d.ld_pre;
       a.ld_d = l.ld_dp;
       check_hip(act_grad(d.type, false, a, st), "activation gradient");
-      if (db) check_hip(sum_partials(d.type, sums, l.strips, d.outputs, db, st), "bias gradient");
     }
     OpEpilogue epi{};
     if (dx) {
@@ -585,8 +581,10 @@ int32_t volta_op_gated_backward(const volta_op_gated* in, const void* dh, const 
       a.pre[1] = up;
       a.d[0] = ws;
       a.d[1] = ws + l.d_bytes;
-      a.partial[0] = db_gate ? sums[0] : nullptr;
-      a.partial[1] = db_up ? sums[1] : nullptr;
+      a.sums[0] = db_gate;
+      a.sums[1] = db_up;
+      a.partial[0] = sums[0];
+      a.partial[1] = sums[1];
       a.act = d.act;
       a.rows = d.rows;
       a.cols = (int32_t)d.hidden;
@@ -594,8 +592,6 @@ int32_t volta_op_gated_backward(const volta_op_gated* in, const void* dh, const 
       a.ld_pre = d.ld_pre;
       a.ld_d = l.ld_d;
       check_hip(act_grad(d.type, true, a, st), "activation gradient");
-      if (db_gate) check_hip(sum_partials(d.type, sums[0], l.strips, d.hidden, db_gate, st), "bias gradient");
-      if (db_up) check_hip(sum_partials(d.type, sums[1], l.strips, d.hidden, db_up, st), "bias gradient");
     }
     const void *dgu[2] = {ws, ws + l.d_bytes}, *w[2] = {w_gate, w_up};
     OpEpilogue epi{};
@@ -701,7 +697,10 @@ int32_t volta_op_rms_norm_backward(const volta_op_rms_norm* in, const void* dy, 
     a.ld_dsum = d.ld_sum;
     a.ld_dx = d.ld_dx;
     check_hip(norm_backward(d.type, a, st), "norm gradient");
-    if (dweight) check_hip(sum_partials(d.type, a.partial, n.partial_rows, d.cols, dweight, st), "weight gradient");
+    if (dweight) {
+      const SumArgs s{{a.partial, nullptr}, {dweight, nullptr}, 1, n.partial_rows, d.cols};
+      check_hip(sum_partials(d.type, s, st), "weight gradient");
+    }
   });
 }
 

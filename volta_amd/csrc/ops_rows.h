@@ -35,20 +35,29 @@ struct NormGradArgs {
 int norm_grad_blocks(int type, int64_t rows, int64_t cols);
 hipError_t norm_backward(int type, const NormGradArgs& a, hipStream_t st);
 
-// out[c] = the sum over i < n of partial[i][c], in order, rounded to the type.
-hipError_t sum_partials(int type, const float* partial, int n, int64_t cols, void* out, hipStream_t st);
+// out[c] = the sum over i < n of partial[i][c], in order, rounded to the type;
+// up to two such sums.
+struct SumArgs {
+  const float* partial[2];
+  void* out[2];
+  int32_t count, n;
+  int64_t cols;
+};
+hipError_t sum_partials(int type, const SumArgs& a, hipStream_t st);
 
 struct ActGradArgs {
   const void* dy;
   const void* pre[2];  // gated: gate and up
   void* d[2];          // dp, or dg and du, or NULL: column sums of dy alone
-  float* partial[2];   // column sums of dp, or of dg and du, [act_grad_strips][cols]; NULL where not wanted
+  void* sums[2];       // column sums of dp, or of dg and du, rounded to the type; NULL where not wanted
+  float* partial[2];   // for each that is wanted, [act_grad_strips][cols] (0 of them: not read)
   int32_t act;
   int64_t rows;
   int32_t cols;
   int64_t ld_dy, ld_pre;
   int64_t ld_d;        // whole 16-byte chunks; what a row's last chunk has behind its columns is set to 0
 };
+// Rows of partial sums; 0 where the sums need none.
 int act_grad_strips(int type, int64_t rows, int64_t cols);
 hipError_t act_grad(int type, bool gated, const ActGradArgs& a, hipStream_t st);
 

@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_grad_kernel(NormGr
 }
 
 // Rows too long for registers: dx row by row, read twice, and dweight column
-// by column.  512 x 65536 bf16: 50 + 24 us.
+// by column.  512 x 65536 bf16: 50 + 23 us.
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_grad_wide_dx(NormGradArgs a) {
   constexpr int E = kChunk<T>;
@@ -387,12 +387,16 @@ __global__ void __launch_bounds__(1024) norm_grad_wide_dx(NormGradArgs a) {
   }
 }
 
-// Column strips: a block takes 64 chunks of columns of `per` rows, its four
-// waves a quarter of them each (row r0 + wave, + 4, ...), and adds the waves'
-// sums in wave order.
+// Column strips: a block takes 64 chunks of columns of `per` rows, its waves
+// the rows r0 + wave, + kStripWaves, ..., and adds the waves' sums in wave
+// order, to a row of partial sums or (one strip) to the output.
+// Sixteen, because a row's loads and activation take a wave 1.7 us one after
+// another: gradients of 256 rows of 1024 with biases took 11.3 us with 4 waves
+// of 4 rows, and take 8.5.
+constexpr int kStripWaves = 16;
 template <typename T>
 __device__ __forceinline__ void strip_store(float (*lds)[64][kChunk<T>], const float (&acc)[kChunk<T>], float* partial,
-                                            int cols, int c, int lane, int wave) {
+                                            T* out, int cols, int c, int lane, int wave) {
   constexpr int E = kChunk<T>;
   __syncthreads();
 #pragma unroll
@@ -401,20 +405,25 @@ __device__ __forceinline__ void strip_store(float (*lds)[64][kChunk<T>], const f
   if (wave == 0 && c < cols) {
     float v[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = ((lds[0][lane][i] + lds[1][lane][i]) + lds[2][lane][i]) + lds[3][lane][i];
-    store_vec(partial + (int64_t)blockIdx.y * cols + c, cols - c, v);
+    for (int i = 0; i < E; ++i) {
+      v[i] = lds[0][lane][i];
+#pragma unroll
+      for (int w = 1; w < kStripWaves; ++w) v[i] += lds[w][lane][i];
+    }
+    if (out) store_vec(out + c, cols - c, v);
+    else store_vec(partial + (int64_t)blockIdx.y * cols + c, cols - c, v);
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) norm_grad_wide_dw(NormGradArgs a, int per) {
+__global__ void __launch_bounds__(kStripWaves * 64) norm_grad_wide_dw(NormGradArgs a, int per) {
   constexpr int E = kChunk<T>;
-  __shared__ float lds[4][64][E];
+  __shared__ float lds[kStripWaves][64][E];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = (blockIdx.x * 64 + lane) * E, cnt = a.cols - c;
   const int64_t r0 = (int64_t)blockIdx.y * per, r1 = min(a.rows, r0 + per);
   float acc[E] = {};
-  for (int64_t r = r0 + wave; r < r1; r += 4) {
+  for (int64_t r = r0 + wave; r < r1; r += kStripWaves) {
     float dv[E], sv[E];
     load_row(static_cast<const T*>(a.dy) + r * a.ld_dy + c, cnt, dv);
     load_row(static_cast<const T*>(a.s) + r * a.ld_s + c, cnt, sv);
@@ -422,7 +431,7 @@ __global__ void __launch_bounds__(256) norm_grad_wide_dw(NormGradArgs a, int per
 #pragma unroll
     for (int i = 0; i < E; ++i) acc[i] = fmaf(dv[i], sv[i] * rstd, acc[i]);
   }
-  strip_store<T>(lds, acc, a.partial, a.cols, c, lane, wave);
+  strip_store<T>(lds, acc, a.partial, nullptr, a.cols, c, lane, wave);
 }
 
 // ---------------------------------------------------------------------------
@@ -435,14 +444,14 @@ __global__ void __launch_bounds__(256) norm_grad_wide_dw(NormGradArgs a, int per
 // us, 5.3 TB/s.
 // ---------------------------------------------------------------------------
 template <typename T, bool GATED>
-__global__ void __launch_bounds__(256) act_grad_kernel(ActGradArgs a, int per) {
+__global__ void __launch_bounds__(kStripWaves * 64) act_grad_kernel(ActGradArgs a, int per) {
   constexpr int E = kChunk<T>;
-  __shared__ float lds[4][64][E];
+  __shared__ float lds[kStripWaves][64][E];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = (blockIdx.x * 64 + lane) * E, cnt = a.cols - c;
   const int64_t r0 = (int64_t)blockIdx.y * per, r1 = min(a.rows, r0 + per);
   float s0[E] = {}, s1[E] = {};
-  for (int64_t r = r0 + wave; r < r1; r += 4) {
+  for (int64_t r = r0 + wave; r < r1; r += kStripWaves) {
     float d[E], g[E], u[E];
     load_row(static_cast<const T*>(a.dy) + r * a.ld_dy + c, cnt, d);
     if (a.pre[0]) load_row(static_cast<const T*>(a.pre[0]) + r * a.ld_pre + c, cnt, g);
@@ -476,32 +485,35 @@ __global__ void __launch_bounds__(256) act_grad_kernel(ActGradArgs a, int per) {
       if (a.d[0] && cnt > 0) store_row(static_cast<T*>(a.d[0]) + r * a.ld_d + c, E, d);
     }
   }
-  if (a.partial[0]) strip_store<T>(lds, s0, a.partial[0], a.cols, c, lane, wave);
-  if (GATED && a.partial[1]) strip_store<T>(lds, s1, a.partial[1], a.cols, c, lane, wave);
+  const bool one = gridDim.y == 1;
+  if (a.sums[0])
+    strip_store<T>(lds, s0, a.partial[0], one ? static_cast<T*>(a.sums[0]) : nullptr, a.cols, c, lane, wave);
+  if (GATED && a.sums[1])
+    strip_store<T>(lds, s1, a.partial[1], one ? static_cast<T*>(a.sums[1]) : nullptr, a.cols, c, lane, wave);
 }
 
 // Partial sums of 64 columns: 16 waves take a sixteenth of the rows each, in
 // order, and their sums are added in wave order.  1024 rows of 4096: 5 us, a
 // launch and the latency of eight loads after another.
 template <typename T>
-__global__ void __launch_bounds__(1024) sum_partials_kernel(const float* partial, int n, int64_t cols, T* out) {
+__global__ void __launch_bounds__(1024) sum_partials_kernel(SumArgs a) {
   __shared__ float lds[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t c = (int64_t)blockIdx.x * 64 + lane;
-  const int per = (n + 15) / 16, i0 = wave * per, i1 = min(n, i0 + per);
+  const int per = (a.n + 15) / 16, i0 = wave * per, i1 = min(a.n, i0 + per);
   float s = 0.0f;
-  if (c < cols) {
-    const float* p = partial + c;
+  if (c < a.cols) {
+    const float* p = a.partial[blockIdx.y] + c;
 #pragma unroll 8
-    for (int i = i0; i < i1; ++i) s += p[(int64_t)i * cols];
+    for (int i = i0; i < i1; ++i) s += p[(int64_t)i * a.cols];
   }
   lds[wave][lane] = s;
   __syncthreads();
-  if (wave == 0 && c < cols) {
+  if (wave == 0 && c < a.cols) {
     s = lds[0][lane];
 #pragma unroll
     for (int w = 1; w < 16; ++w) s += lds[w][lane];
-    out[c] = from_f<T>(s);
+    static_cast<T*>(a.out[blockIdx.y])[c] = from_f<T>(s);
   }
 }
 
@@ -586,10 +598,11 @@ hipError_t norm_grad_launch(const NormGradArgs& a, int blocks, hipStream_t st) {
   return hipGetLastError();
 }
 
-// Rows of a column strip and strips, for about 1024 blocks.
+// Rows of a column strip and strips, for about 512 blocks (gradients of 2000
+// rows of 2 x 3000: 21.6 us, and 23.8 for about 1024).
 int strip_rows(int chunks, int64_t rows) {
   const int64_t across = (chunks + 63) / 64;
-  const int64_t strips = std::max<int64_t>(1, std::min<int64_t>((rows + 15) / 16, 1024 / across));
+  const int64_t strips = std::max<int64_t>(1, std::min<int64_t>((rows + 15) / 16, 512 / across));
   return (int)std::max<int64_t>(1, (rows + strips - 1) / strips);
 }
 int strips_of(int chunks, int64_t rows) {
@@ -632,34 +645,53 @@ hipError_t norm_backward(int type, const NormGradArgs& a, hipStream_t st) {
       e = hipGetLastError();
     }
     if (e == hipSuccess && a.partial) {
-      hipLaunchKernelGGL((norm_grad_wide_dw<T>), dim3((unsigned)((chunks + 63) / 64), (unsigned)rows), dim3(256), 0, st,
-                         a, strip_rows(chunks, a.rows));
+      hipLaunchKernelGGL((norm_grad_wide_dw<T>), dim3((unsigned)((chunks + 63) / 64), (unsigned)rows),
+                         dim3(kStripWaves * 64), 0, st, a, strip_rows(chunks, a.rows));
       e = hipGetLastError();
     }
     return e;
   });
 }
 
-hipError_t sum_partials(int type, const float* partial, int n, int64_t cols, void* out, hipStream_t st) {
+hipError_t sum_partials(int type, const SumArgs& a, hipStream_t st) {
   return with_type(type, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL((sum_partials_kernel<T>), dim3((unsigned)((cols + 63) / 64)), dim3(1024), 0, st, partial, n,
-                       cols, static_cast<T*>(out));
+    hipLaunchKernelGGL((sum_partials_kernel<T>), dim3((unsigned)((a.cols + 63) / 64), (unsigned)a.count), dim3(1024), 0,
+                       st, a);
     return hipGetLastError();
   });
 }
 
-int act_grad_strips(int type, int64_t rows, int64_t cols) { return strips_of(chunks_of(type, cols), rows); }
+// Up to 32 rows are one strip, which stores the sums themselves: 7.5 us for 32
+// rows of 1024 with biases, 8.5 with a launch that adds two strips' (64 rows:
+// 11.1 and 8.5).
+int act_grad_rows(int chunks, int64_t rows) { return rows <= 32 ? 32 : strip_rows(chunks, rows); }
+
+int act_grad_strips(int type, int64_t rows, int64_t cols) {
+  const int per = act_grad_rows(chunks_of(type, cols), rows);
+  return rows <= per ? 0 : (int)((rows + per - 1) / per);
+}
 
 hipError_t act_grad(int type, bool gated, const ActGradArgs& a, hipStream_t st) {
-  const int chunks = chunks_of(type, a.cols), per = strip_rows(chunks, a.rows);
-  const dim3 grid((unsigned)((chunks + 63) / 64), (unsigned)strips_of(chunks, a.rows));
-  return with_type(type, [&](auto t) {
+  const int chunks = chunks_of(type, a.cols), per = act_grad_rows(chunks, a.rows);
+  const int strips = act_grad_strips(type, a.rows, a.cols);
+  const dim3 grid((unsigned)((chunks + 63) / 64), (unsigned)std::max(1, strips));
+  const hipError_t e = with_type(type, [&](auto t) {
     using T = decltype(t);
-    if (gated) hipLaunchKernelGGL((act_grad_kernel<T, true>), grid, dim3(256), 0, st, a, per);
-    else hipLaunchKernelGGL((act_grad_kernel<T, false>), grid, dim3(256), 0, st, a, per);
+    if (gated) hipLaunchKernelGGL((act_grad_kernel<T, true>), grid, dim3(kStripWaves * 64), 0, st, a, per);
+    else hipLaunchKernelGGL((act_grad_kernel<T, false>), grid, dim3(kStripWaves * 64), 0, st, a, per);
     return hipGetLastError();
   });
+  if (e != hipSuccess || strips == 0) return e;
+  SumArgs s{};
+  for (int i = 0; i < 2; ++i) {
+    if (!a.sums[i]) continue;
+    s.partial[s.count] = a.partial[i];
+    s.out[s.count++] = a.sums[i];
+  }
+  s.n = strips;
+  s.cols = a.cols;
+  return s.count ? sum_partials(type, s, st) : hipSuccess;
 }
 
 hipError_t pack_rows(int type, const PackArgs& a, hipStream_t st) {

@@ -97,7 +97,11 @@ int32_t volta_op_linear_forward(const volta_op_linear* d, const void* x, const v
  * an activation (and not read otherwise); dx, dw, db may be NULL where not
  * wanted (at least one is); x is read for dw, w for dx.  act' is the training
  * step's: 0 at 0 for ReLU.  dp is rounded to the type before its products, as
- * matrix instructions take their operands in it; db sums it before that. */
+ * matrix instructions take their operands in it (a half step of each dp, so dx
+ * and dw are off by about as much again as by their own rounding), and without
+ * loss of range: float16 holds dp in units of a power of two, which puts the
+ * largest magnitude of dp in [2^14, 2^15); only what is under 2^-28 of that
+ * loses bits.  db sums dp before its rounding. */
 int32_t volta_op_linear_backward(const volta_op_linear* d, const void* dy, const void* x, const void* w,
                                  const void* pre, void* dx, void* dw, void* db, void* workspace,
                                  int64_t workspace_bytes, void* stream);
@@ -125,8 +129,8 @@ int32_t volta_op_gated_forward(const volta_op_gated* d, const void* x, const voi
 /* From dh: dg = dh u act'(g); du = dh act(g); dx = dg Wg^T + du Wu^T;
  * dw_gate = x^T dg; dw_up = x^T du; db_gate, db_up = the column sums.  dx may
  * be NULL; so may dw_gate and dw_up (both or neither), and db_gate and db_up
- * (each).  dg and du are rounded to the type before their products, as
- * above. */
+ * (each).  dg and du are rounded to the type before their products, as dp
+ * above (float16: in units common to both). */
 int32_t volta_op_gated_backward(const volta_op_gated* d, const void* dh, const void* x, const void* w_gate,
                                 const void* w_up, const void* gate, const void* up, void* dx, void* dw_gate,
                                 void* dw_up, void* db_gate, void* db_up, void* workspace, int64_t workspace_bytes,

@@ -1,0 +1,135 @@
+"""The feed-forward operators' gradients (include/volta_ops.h) where their
+inputs are far from 1: float16 pre-activation gradients past its largest value
+or below its smallest normal one.  Bounds as in tests/test_gpu_ops.py."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from tests import ops_ref as R
+from tests.ops_ref import HALF, Mat, act, act_error, check, rounded
+from tests.test_gpu_ops import Space, U32, draws, sum_error
+from volta_amd import load_hip, ops
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return load_hip()
+
+
+SHAPES = [(1, 40, 24), (7, 33, 65), (40, 64, 136), (300, 256, 128), (1100, 1000, 1501)]
+# (what dy or dh, up, x and W are multiplied by): past 65504 with results well inside, and where
+# float16 has one to five bits left
+SCALES = {"large": (30000.0, 40.0, 2.0**-12, 2.0**-12), "small": (2.0**-20, 0.25, 64.0, 64.0)}
+
+
+def _product_error(p, d, ed, K, want, t):
+    """Of p @ d, d off by ed and rounded to t in units in which its largest
+    magnitude is at least 2^14: half a step of a subnormal is then 2^-25 2^-14
+    of that magnitude."""
+    e = ed + HALF[t] * (np.abs(d) + ed) + (np.abs(d) + ed).max() * 2.0**-39
+    return 1.001 * (np.abs(p) @ e + sum_error(p, np.abs(d) + e, K) + rounded(want, t)) + 1e-37
+
+
+@pytest.mark.parametrize("size", SCALES)
+@pytest.mark.parametrize("t", R.TYPES)
+def test_gated_gradients_far_from_one(lib, t, size):
+    """dg = dh u act'(g) is over 65504, or under 2^-14, in most places; dx and
+    dW are ordinary numbers of the type."""
+    sd, su, sx, sw = SCALES[size]
+    for n, (M, K, N) in enumerate(SHAPES):
+        a, rng = ("silu", "gelu", "relu")[n % 3], np.random.default_rng(500 + n)
+        print(t, size, a, M, K, N, flush=True)
+        x, wg, wu = draws(rng, t, M, K, scale=sx), draws(rng, t, K, N, scale=sw), draws(rng, t, K, N, scale=sw)
+        dh, g, u = np.clip(draws(rng, t, M, N, scale=sd), -60000, 60000), draws(rng, t, M, N), draws(rng, t, M, N, scale=su)
+        dh = R.unpack(R.pack(dh, t), t)
+        op = ops.GatedFF(M, K, N, t, a)
+        ws = Space(lib, op, True)
+        m = [Mat(lib, t, *v.shape, v) for v in (dh, x, wg, wu, g, u)]
+        out = {"dx": Mat(lib, t, M, K), "dw_gate": Mat(lib, t, K, N), "dw_up": Mat(lib, t, K, N)}
+        op.backward(*m, workspace=ws, **out)
+        f, slope = act(a, g)
+        ef, es = act_error(t, g) if a != "relu" else (0, 0)
+        dg, du = dh * u * slope, dh * f
+        eg = np.abs(dh * u) * es + 3 * U32 * np.abs(dg)
+        eu = np.abs(dh) * ef + 3 * U32 * np.abs(du)
+        cat, ecat, wcat = np.hstack([dg, du]), np.hstack([eg, eu]), np.hstack([wg, wu])
+        want = dg @ wg.T + du @ wu.T
+        assert np.abs(want).max() < 60000
+        check(out["dx"].get(), want, _product_error(wcat, cat.T, ecat.T, 2 * N, want.T, t).T, "dx")
+        top = np.abs(cat).max() * 2.0**-39  # both matrices in the same units
+        for name, d, ed in (("dw_gate", dg, eg), ("dw_up", du, eu)):
+            want = x.T @ d
+            assert np.abs(want).max() < 60000
+            check(out[name].get(), want, _product_error(x.T, d, ed + top, M, want, t), name)
+        ws.check()
+        for some in (["dx"], ["dw_gate", "dw_up"]):  # alone, the same bits
+            again = {k: Mat(lib, t, out[k].rows, out[k].cols) for k in some}
+            op.backward(*m, workspace=ws, **again)
+            assert all(np.array_equal(again[k].bits(), out[k].bits()) for k in some)
+
+
+@pytest.mark.parametrize("size", SCALES)
+@pytest.mark.parametrize("t", R.TYPES)
+def test_linear_gradients_far_from_one(lib, t, size):
+    """dp = dy act'(p): GELU's slope is up to 1.13, so dp passes 65504 where dy
+    nearly does."""
+    sd, su, sx, sw = SCALES[size]
+    for n, (M, K, N) in enumerate(SHAPES):
+        rng = np.random.default_rng(550 + n)
+        print(t, size, M, K, N, flush=True)
+        x, w, p = draws(rng, t, M, K, scale=sx), draws(rng, t, K, N, scale=sw), draws(rng, t, M, N, scale=1.5)
+        dy = np.copysign(rng.uniform(60000, 65000, (M, N)), rng.standard_normal((M, N))) if size == "large" else \
+            sd * su * rng.standard_normal((M, N))
+        dy = R.unpack(R.pack(dy, t), t)
+        op = ops.Linear(M, K, N, t, "gelu")
+        ws = Space(lib, op, True)
+        m = [Mat(lib, t, *v.shape, v) for v in (dy, x, w, p)]
+        dx, dw = Mat(lib, t, M, K), Mat(lib, t, K, N)
+        op.backward(m[0], m[1], m[2], pre=m[3], dx=dx, dw=dw, workspace=ws)
+        slope = act("gelu", p)[1]
+        d = dy * slope
+        ed = np.abs(dy) * act_error(t, p)[1] + 2 * U32 * np.abs(d)
+        want = d @ w.T
+        check(dx.get(), want, _product_error(w, d.T, ed.T, N, want.T, t).T, "dx")
+        want = x.T @ d
+        check(dw.get(), want, _product_error(x.T, d, ed, M, want, t), "dw")
+        ws.check()
+
+
+def test_infinity_keeps_to_its_row_in_dx(lib):
+    """A row of dy with an infinity or a NaN spoils its own row of dx alone, and
+    rows of zeros stay zeros."""
+    M, K, N = 70, 48, 40
+    rng = np.random.default_rng(60)
+    for bad in (np.inf, np.nan):
+        x, w, p, dy = (draws(rng, "f16", *s) for s in ((M, K), (K, N), (M, N), (M, N)))
+        dy[5] = 0
+        clean = dy.copy()
+        dy[3, 7] = bad
+        op = ops.Linear(M, K, N, "f16", "silu")
+        ws, dx = Space(lib, op, True), Mat(lib, "f16", M, K)
+        m = [Mat(lib, "f16", *v.shape, v) for v in (dy, x, w, p)]
+        op.backward(m[0], m[1], m[2], pre=m[3], dx=dx, workspace=ws)
+        got, d = dx.get(), clean * act("silu", p)[1]
+        want = d @ w.T
+        tol = _product_error(w, d.T, (np.abs(clean) * act_error("f16", p)[1]).T, N, want.T, "f16").T
+        # units of a matrix with an infinity are the type's own: its subnormals end at 2^-25
+        tol = tol + np.abs(np.ones((M, N)) @ np.abs(w.T)) * 2.0**-25
+        rest = np.arange(M) != 3
+        check(got[rest], want[rest], tol[rest], "dx")
+        assert not np.isfinite(got[3]).any() and (got[5] == 0).all()
+
+
+def test_gradients_of_zeros_are_zeros(lib):
+    M, K, N = 20, 16, 24
+    rng = np.random.default_rng(61)
+    op = ops.GatedFF(M, K, N, "f16")
+    ws = Space(lib, op, True)
+    m = [Mat(lib, "f16", *v.shape, v) for v in (np.zeros((M, N)), draws(rng, "f16", M, K), draws(rng, "f16", K, N),
+                                                draws(rng, "f16", K, N), draws(rng, "f16", M, N), draws(rng, "f16", M, N))]
+    dx, dg, du = Mat(lib, "f16", M, K), Mat(lib, "f16", K, N), Mat(lib, "f16", K, N)
+    op.backward(*m, dx=dx, dw_gate=dg, dw_up=du, workspace=ws)
+    assert all((v.get() == 0).all() for v in (dx, dg, du))

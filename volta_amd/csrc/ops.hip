@@ -286,9 +286,9 @@ void product(int type, const Shape& s, const void* const* ps, const void* const*
 struct Linear {
   volta_op_linear d;
   Shape fwd, dx, dw;
-  int64_t ld_dp, dp_bytes, sums_bytes;
+  int64_t ld_dp, dp_bytes, sums_bytes, unit_bytes;
   int64_t forward_bytes() const { return fwd.bytes(); }
-  int64_t backward_bytes() const { return dp_bytes + sums_bytes + std::max(dx.bytes(), dw.bytes()); }
+  int64_t backward_bytes() const { return dp_bytes + sums_bytes + unit_bytes + std::max(dx.bytes(), dw.bytes()); }
 };
 
 Linear linear_of(const volta_op_linear* in) {
@@ -317,15 +317,16 @@ Linear linear_of(const volta_op_linear* in) {
   l.dx = shape_of(d.type, OP_NT, OP_STORE, d.rows, d.inputs, d.outputs, 1, 1, dp, w);
   l.dw = shape_of(d.type, OP_TN, OP_STORE, d.inputs, d.outputs, d.rows, 1, 1, x, dp);
   l.sums_bytes = align256(4 * act_grad_strips(d.type, d.rows, d.outputs) * d.outputs);
+  l.unit_bytes = d.act == VOLTA_OP_ACT_NONE ? 0 : align256(4 * act_grad_units(d.type, d.rows, d.outputs));
   return l;
 }
 
 struct Gated {
   volta_op_gated d;
   Shape fwd, dx, dw;
-  int64_t ld_d, d_bytes, sums_bytes;
+  int64_t ld_d, d_bytes, sums_bytes, unit_bytes;
   int64_t forward_bytes() const { return fwd.bytes(); }
-  int64_t backward_bytes() const { return 2 * (d_bytes + sums_bytes) + std::max(dx.bytes(), dw.bytes()); }
+  int64_t backward_bytes() const { return 2 * (d_bytes + sums_bytes) + unit_bytes + std::max(dx.bytes(), dw.bytes()); }
 };
 
 Gated gated_of(const volta_op_gated* in) {
@@ -351,6 +352,7 @@ Gated gated_of(const volta_op_gated* in) {
   l.dx = shape_of(d.type, OP_NT, OP_STORE, d.rows, d.inputs, d.hidden, 2, 1, dg, w);
   l.dw = shape_of(d.type, OP_TN, OP_STORE, d.inputs, d.hidden, d.rows, 1, 2, x, dg);
   l.sums_bytes = align256(4 * act_grad_strips(d.type, d.rows, d.hidden) * d.hidden);
+  l.unit_bytes = align256(4 * act_grad_units(d.type, d.rows, d.hidden));
   return l;
 }
 
@@ -465,7 +467,8 @@ int32_t volta_op_linear_backward(const volta_op_linear* in, const void* dy, cons
     const hipStream_t st = check_call({mdy, mx, mw, mp, mdx, mdw, mdb}, {}, workspace, l.backward_bytes(), stream);
     char* ws = static_cast<char*>(workspace);
     float* sums = reinterpret_cast<float*>(ws + l.dp_bytes);
-    char* rest = ws + l.dp_bytes + l.sums_bytes;
+    float* unit = l.unit_bytes && (dx || dw) ? reinterpret_cast<float*>(ws + l.dp_bytes + l.sums_bytes) : nullptr;
+    char* rest = ws + l.dp_bytes + l.sums_bytes + l.unit_bytes;
     const void* dp = act ? ws : dy;
     if ((act && (dx || dw) && d.rows > 0) || db) {
       ActGradArgs a{};
@@ -474,6 +477,7 @@ int32_t volta_op_linear_backward(const volta_op_linear* in, const void* dy, cons
       a.d[0] = act && (dx || dw) ? ws : nullptr;
       a.sums[0] = db;
       a.partial[0] = sums;
+      a.unit = unit;
       a.act = d.act;
       a.rows = d.rows;
       a.cols = (int32_t)d.outputs;
@@ -483,6 +487,7 @@ int32_t volta_op_linear_backward(const volta_op_linear* in, const void* dy, cons
       check_hip(act_grad(d.type, false, a, st), "activation gradient");
     }
     OpEpilogue epi{};
+    epi.unit = unit;
     if (dx) {
       epi.out[0] = dx;
       epi.ld_out = d.ld_dx;
@@ -573,7 +578,9 @@ int32_t volta_op_gated_backward(const volta_op_gated* in, const void* dh, const 
     char* ws = static_cast<char*>(workspace);
     float* sums[2] = {reinterpret_cast<float*>(ws + 2 * l.d_bytes),
                       reinterpret_cast<float*>(ws + 2 * l.d_bytes + l.sums_bytes)};
-    char* rest = ws + 2 * (l.d_bytes + l.sums_bytes);
+    float* unit =
+        l.unit_bytes && (dx || dw_gate) ? reinterpret_cast<float*>(ws + 2 * (l.d_bytes + l.sums_bytes)) : nullptr;
+    char* rest = ws + 2 * (l.d_bytes + l.sums_bytes) + l.unit_bytes;
     if (d.rows > 0 || db_gate || db_up) {
       ActGradArgs a{};
       a.dy = dh;
@@ -585,6 +592,7 @@ int32_t volta_op_gated_backward(const volta_op_gated* in, const void* dh, const 
       a.sums[1] = db_up;
       a.partial[0] = sums[0];
       a.partial[1] = sums[1];
+      a.unit = unit;
       a.act = d.act;
       a.rows = d.rows;
       a.cols = (int32_t)d.hidden;
@@ -595,6 +603,7 @@ int32_t volta_op_gated_backward(const volta_op_gated* in, const void* dh, const 
     }
     const void *dgu[2] = {ws, ws + l.d_bytes}, *w[2] = {w_gate, w_up};
     OpEpilogue epi{};
+    epi.unit = unit;
     if (dx) {
       epi.out[0] = dx;
       epi.ld_out = d.ld_dx;

@@ -30,6 +30,7 @@ struct OpEpilogue {
   void* out[2];  // OP_STORE: one for each q (blockIdx.z)
   void* pre[2];
   int64_t ld_out, ld_residual, ld_pre;
+  const float* unit;  // OP_STORE in float16: one number on the device, what the sums are multiplied by; NULL: 1
 };
 
 struct OpGemm {

@@ -250,6 +250,23 @@ __device__ __forceinline__ void op_biases(const OpEpilogue& e, int n, int cnt, f
   }
 }
 
+// Sums alone in float16 may be in units of an operand's (act_grad_kernel).
+template <typename T, int KIND>
+constexpr bool kOpUnits = KIND == OP_STORE && std::is_same<T, _Float16>::value;
+template <typename T, int KIND>
+__device__ __forceinline__ float op_unit(const OpEpilogue& e) {
+  if constexpr (kOpUnits<T, KIND>)
+    if (e.unit) return *e.unit;
+  return 1.0f;
+}
+template <typename T, int KIND, int V>
+__device__ __forceinline__ void op_in_units(float unit, float (&d)[V]) {
+  if constexpr (kOpUnits<T, KIND>) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) d[i] *= unit;
+  }
+}
+
 // A loop over 0 .. N - 1 whose index is a constant of its body.
 template <int N, int I = 0, typename F>
 __device__ __forceinline__ void op_unroll(F f) {
@@ -301,8 +318,11 @@ __device__ __forceinline__ void op_write_out(const OpGemm& g, floatx4 (&acc)[TM]
   float* lds = reinterpret_cast<float*>(region);
   const int row = lane / kLanes, col = lane % kLanes * V;
   const int n = n0 + col, cnt = g.N - n;
-  float b0[V], b1[V];
-  if (g.splits <= 1) op_biases<T, KIND>(g.epi, n, cnt, b0, b1);
+  float b0[V], b1[V], unit = 1.0f;
+  if (g.splits <= 1) {
+    op_biases<T, KIND>(g.epi, n, cnt, b0, b1);
+    unit = op_unit<T, KIND>(g.epi);
+  }
 #pragma unroll 1
   for (int ph = 0; ph < TM / RB; ++ph) {
     op_unroll<TM / RB>([&](auto I) {
@@ -340,6 +360,7 @@ __device__ __forceinline__ void op_write_out(const OpGemm& g, floatx4 (&acc)[TM]
         store_vec(p, cnt, d0);
         if constexpr (kGated) store_vec(p + (int64_t)g.M * g.N, cnt, d1);
       } else {
+        op_in_units<T, KIND>(unit, d0);
         op_epilogue<T, KIND>(g.epi, z, m, n, cnt, d0, d1, b0, b1);
       }
     }
@@ -1032,6 +1053,7 @@ __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
         if constexpr (kGated) store_vec(p + (int64_t)g.M * g.N, cnt, d1);
       } else {
         op_biases<T, KIND>(g.epi, n, cnt, b0, b1);
+        op_in_units<T, KIND>(op_unit<T, KIND>(g.epi), d0);
         op_epilogue<T, KIND>(g.epi, 0, m, n, cnt, d0, d1, b0, b1);
       }
     }
@@ -1072,6 +1094,7 @@ __global__ void __launch_bounds__(256) op_gemm_reduce(OpGemm g) {
         }
       }
   }
+  op_in_units<T, KIND>(op_unit<T, KIND>(g.epi), d0);
   op_epilogue<T, KIND>(g.epi, z, m, n, cnt, d0, d1, b0, b1);
 }
 

@@ -51,6 +51,7 @@ struct ActGradArgs {
   void* d[2];          // dp, or dg and du, or NULL: column sums of dy alone
   void* sums[2];       // column sums of dp, or of dg and du, rounded to the type; NULL where not wanted
   float* partial[2];   // for each that is wanted, [act_grad_strips][cols] (0 of them: not read)
+  float* unit;         // float16: [act_grad_units]; unit[0] receives what 1 in d stands for.  NULL: 1
   int32_t act;
   int64_t rows;
   int32_t cols;
@@ -59,6 +60,8 @@ struct ActGradArgs {
 };
 // Rows of partial sums; 0 where the sums need none.
 int act_grad_strips(int type, int64_t rows, int64_t cols);
+// Floats of `unit`; 0 where the type needs none.
+int64_t act_grad_units(int type, int64_t rows, int64_t cols);
 hipError_t act_grad(int type, bool gated, const ActGradArgs& a, hipStream_t st);
 
 // Copies up to three matrices into rows of whole 16-byte chunks, zeros behind

@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "ops_types.h"
 
@@ -442,7 +443,92 @@ __global__ void __launch_bounds__(kStripWaves * 64) norm_grad_wide_dw(NormGradAr
 // bytes.  Kept apart from the products, which read each element many times
 // and would form it anew each time.  Gated, 8192 x 16384 bf16, 1.34 GB: 254
 // us, 5.3 TB/s.
+//
+// float16 ends at 65504 and has all of its bits from 2^-14 on, and dh u f'(g)
+// leaves that range where dx and dW do not.  So its d are held in a common
+// unit, the power of two that puts the largest magnitude of d between 2^14 and
+// 2^15 (found by a pass of its own, act_grad_largest), and the products'
+// epilogues multiply their sums by it: exact but for what is under 2^-28 of
+// the largest.  That pass is 5 us of a linear layer's gradients of 16 rows of
+// 1024 (12.0 without it, 17.4 with it), and 167 of a gated layer's of 8192 rows
+// of 4096 and 16384 (3433 and 3600).
 // ---------------------------------------------------------------------------
+// Chunk c of row r: dp in d, or dg in u and du in d.  What is behind the
+// columns comes out as 0.
+template <typename T, bool GATED>
+__device__ __forceinline__ void act_grad_chunk(const ActGradArgs& a, int64_t r, int c, int cnt, float (&d)[kChunk<T>],
+                                               float (&u)[kChunk<T>]) {
+  constexpr int E = kChunk<T>;
+  float g[E];
+  load_row(static_cast<const T*>(a.dy) + r * a.ld_dy + c, cnt, d);
+  if (a.pre[0]) load_row(static_cast<const T*>(a.pre[0]) + r * a.ld_pre + c, cnt, g);
+  if constexpr (GATED) load_row(static_cast<const T*>(a.pre[1]) + r * a.ld_pre + c, cnt, u);
+  if (!a.pre[0]) return;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    float f, slope;
+    op_act_both<T>(a.act, g[i], &f, &slope);
+    if constexpr (GATED) {
+      u[i] = d[i] * u[i] * slope;  // dg
+      d[i] = d[i] * f;             // du
+    } else {
+      d[i] = d[i] * slope;
+    }
+  }
+}
+
+// The largest of a block's values, on every thread.
+__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* lds) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, off, kWave));
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = lds[0];
+#pragma unroll
+  for (int w = 1; w < kStripWaves; ++w) v = max(v, lds[w]);
+  return v;
+}
+
+// unit[1 + block]: the bits of the largest magnitude among the d that the
+// block of act_grad_kernel's grid forms (an infinity or a NaN is larger than
+// any number).  Reads what that kernel reads again, from the memory-side
+// cache where it fits.
+template <bool GATED>
+__global__ void __launch_bounds__(kStripWaves * 64) act_grad_largest(ActGradArgs a, int per) {
+  using T = _Float16;
+  constexpr int E = kChunk<T>;
+  __shared__ uint32_t lds[kStripWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = (blockIdx.x * 64 + lane) * E, cnt = a.cols - c;
+  const int64_t r0 = (int64_t)blockIdx.y * per, r1 = min(a.rows, r0 + per);
+  uint32_t m = 0;
+  for (int64_t r = r0 + wave; r < r1; r += kStripWaves) {
+    float d[E], u[E];
+    act_grad_chunk<T, GATED>(a, r, c, cnt, d, u);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      m = max(m, __float_as_uint(fabsf(d[i])));
+      if constexpr (GATED) m = max(m, __float_as_uint(fabsf(u[i])));
+    }
+  }
+  m = block_max(m, lds);
+  if (threadIdx.x == 0) a.unit[1 + (int64_t)blockIdx.y * gridDim.x + blockIdx.x] = __uint_as_float(m);
+}
+
+// What 1 / unit multiplies d by, from the blocks' largest magnitudes; the
+// first block leaves unit[0].  All zeros, and an infinity or a NaN among them:
+// 1.  The exponents stay inside those of normal numbers.
+__device__ __forceinline__ float per_unit(const ActGradArgs& a, uint32_t* lds) {
+  const int n = (int)(gridDim.x * gridDim.y);
+  uint32_t m = 0;
+  for (int i = threadIdx.x; i < n; i += kStripWaves * 64) m = max(m, __float_as_uint(a.unit[1 + i]));
+  m = block_max(m, lds);
+  int up = 0;
+  if (m != 0 && m < 0x7f800000u) up = min(14 - (max((int)(m >> 23), 1) - 127), 126);
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.unit[0] = __uint_as_float((uint32_t)(127 - up) << 23);
+  return __uint_as_float((uint32_t)(127 + up) << 23);
+}
+
 template <typename T, bool GATED>
 __global__ void __launch_bounds__(kStripWaves * 64) act_grad_kernel(ActGradArgs a, int per) {
   constexpr int E = kChunk<T>;
@@ -450,38 +536,35 @@ __global__ void __launch_bounds__(kStripWaves * 64) act_grad_kernel(ActGradArgs 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = (blockIdx.x * 64 + lane) * E, cnt = a.cols - c;
   const int64_t r0 = (int64_t)blockIdx.y * per, r1 = min(a.rows, r0 + per);
-  float s0[E] = {}, s1[E] = {};
+  float s0[E] = {}, s1[E] = {}, up = 1.0f;
+  constexpr bool kUnits = std::is_same<T, _Float16>::value;
+  if constexpr (kUnits) {
+    __shared__ uint32_t top[kStripWaves];
+    if (a.unit) up = per_unit(a, top);
+  }
   for (int64_t r = r0 + wave; r < r1; r += kStripWaves) {
-    float d[E], g[E], u[E];
-    load_row(static_cast<const T*>(a.dy) + r * a.ld_dy + c, cnt, d);
-    if (a.pre[0]) load_row(static_cast<const T*>(a.pre[0]) + r * a.ld_pre + c, cnt, g);
-    if constexpr (GATED) load_row(static_cast<const T*>(a.pre[1]) + r * a.ld_pre + c, cnt, u);
-    if (a.pre[0]) {
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        float f, slope;
-        op_act_both<T>(a.act, g[i], &f, &slope);
-        if constexpr (GATED) {
-          u[i] = d[i] * u[i] * slope;  // dg
-          d[i] = d[i] * f;             // du
-        } else {
-          d[i] = d[i] * slope;
-        }
-      }
-    }
+    float d[E], u[E];
+    act_grad_chunk<T, GATED>(a, r, c, cnt, d, u);
     if constexpr (GATED) {
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         s0[i] += u[i];
         s1[i] += d[i];
+        if constexpr (kUnits) {
+          u[i] *= up;
+          d[i] *= up;
+        }
       }
-      if (cnt > 0) {  // what is behind the columns came out as 0
+      if (cnt > 0) {
         store_row(static_cast<T*>(a.d[0]) + r * a.ld_d + c, E, u);
         store_row(static_cast<T*>(a.d[1]) + r * a.ld_d + c, E, d);
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < E; ++i) s0[i] += d[i];
+      for (int i = 0; i < E; ++i) {
+        s0[i] += d[i];
+        if constexpr (kUnits) d[i] *= up;
+      }
       if (a.d[0] && cnt > 0) store_row(static_cast<T*>(a.d[0]) + r * a.ld_d + c, E, d);
     }
   }
@@ -672,10 +755,21 @@ int act_grad_strips(int type, int64_t rows, int64_t cols) {
   return rows <= per ? 0 : (int)((rows + per - 1) / per);
 }
 
+int64_t act_grad_units(int type, int64_t rows, int64_t cols) {
+  if (type != VOLTA_OP_F16 || rows == 0) return 0;
+  return 1 + (chunks_of(type, cols) + 63) / 64 * (int64_t)std::max(1, act_grad_strips(type, rows, cols));
+}
+
 hipError_t act_grad(int type, bool gated, const ActGradArgs& a, hipStream_t st) {
   const int chunks = chunks_of(type, a.cols), per = act_grad_rows(chunks, a.rows);
   const int strips = act_grad_strips(type, a.rows, a.cols);
   const dim3 grid((unsigned)((chunks + 63) / 64), (unsigned)std::max(1, strips));
+  if (a.unit) {
+    if (gated) hipLaunchKernelGGL((act_grad_largest<true>), grid, dim3(kStripWaves * 64), 0, st, a, per);
+    else hipLaunchKernelGGL((act_grad_largest<false>), grid, dim3(kStripWaves * 64), 0, st, a, per);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
   const hipError_t e = with_type(type, [&](auto t) {
     using T = decltype(t);
     if (gated) hipLaunchKernelGGL((act_grad_kernel<T, true>), grid, dim3(kStripWaves * 64), 0, st, a, per);

@@ -29,7 +29,7 @@ SOURCES = ["gemm.hip", "skinny.hip", "step_kernels.hip", "extras.hip", "runtime.
            "ops_gemm_f32.hip", "ops_gemm_bf16.hip", "ops_gemm_f16.hip", "ops_plan.cpp"]
 HEADERS = ["gemm.h", "skinny.h", "step_kernels.h", "extras.h", "device_common.h", "recorder.h", "spec.h",
            "narrow_dw.h", "out_head.h", "vt_frontend.h", "rt_lower.h", "ops_types.h", "ops_gemm.h",
-           "ops_gemm_kernels.h", "ops_rows.h"]
+           "ops_gemm_kernels.h", "ops_rows.h", "ops_launch.h"]
 CLI = os.path.join(PKG, "volta-hip")
 CLI_SOURCES = ["volta_hip_cli.cpp", "vt_frontend.cpp", "spec.cpp"]
 CXX = os.environ.get("CXX", "g++")

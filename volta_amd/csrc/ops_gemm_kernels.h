@@ -31,6 +31,7 @@
 #include <type_traits>
 
 #include "ops_gemm.h"
+#include "ops_launch.h"
 #include "ops_types.h"
 
 namespace volta {
@@ -1104,10 +1105,8 @@ hipError_t launch_staged(OpGemm& g, hipStream_t st) {
   constexpr int SN = KIND == OP_GATED ? BN / 2 : BN;
   g.tiles_m = (g.M + BM - 1) / BM;
   g.tiles_n = (g.N + SN - 1) / SN;
-  hipLaunchKernelGGL((op_gemm_staged<T, LAYOUT, KIND, BM, BN>),
-                     dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits, (unsigned)g.outputs), dim3(256), 0, st,
-                     g);
-  return hipGetLastError();
+  return op_launch(op_gemm_staged<T, LAYOUT, KIND, BM, BN>,
+                   dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits, (unsigned)g.outputs), dim3(256), st, g);
 }
 
 template <typename T, int LAYOUT, int KIND, int BM, int BN, int WGM, int WGN, int KS, int NST>
@@ -1115,10 +1114,8 @@ hipError_t launch_middle(OpGemm& g, hipStream_t st) {
   constexpr int SN = KIND == OP_GATED ? BN / 2 : BN;
   g.tiles_m = (g.M + BM - 1) / BM;
   g.tiles_n = (g.N + SN - 1) / SN;
-  hipLaunchKernelGGL((op_gemm_middle<T, LAYOUT, KIND, BM, BN, WGM, WGN, KS, NST>),
-                     dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits, (unsigned)g.outputs), dim3(512), 0, st,
-                     g);
-  return hipGetLastError();
+  return op_launch(op_gemm_middle<T, LAYOUT, KIND, BM, BN, WGM, WGN, KS, NST>,
+                   dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits, (unsigned)g.outputs), dim3(512), st, g);
 }
 
 template <typename T, int LAYOUT, int KIND>
@@ -1126,10 +1123,8 @@ hipError_t launch_large(OpGemm& g, hipStream_t st) {
   constexpr int SN = KIND == OP_GATED ? 128 : 256;
   g.tiles_m = (g.M + 255) / 256;
   g.tiles_n = (g.N + SN - 1) / SN;
-  hipLaunchKernelGGL((op_gemm_large<T, LAYOUT, KIND>),
-                     dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits, (unsigned)g.outputs), dim3(512), 0, st,
-                     g);
-  return hipGetLastError();
+  return op_launch(op_gemm_large<T, LAYOUT, KIND>,
+                   dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits, (unsigned)g.outputs), dim3(512), st, g);
 }
 
 // Columns, waves and ring of the skinny form: what fits a CU's 160 KB of LDS.
@@ -1146,9 +1141,8 @@ hipError_t launch_skinny(OpGemm& g, hipStream_t st) {
   using S = SkinnyShape<KIND, MT, DIRECT>;
   g.tiles_m = (g.M + 16 * MT - 1) / (16 * MT);
   g.tiles_n = (g.N + S::kCols - 1) / S::kCols;
-  hipLaunchKernelGGL((op_gemm_skinny<T, LAYOUT, KIND, MT, S::kCols, S::kWaves, S::kStages, DIRECT>),
-                     dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits), dim3(S::kWaves * 64), 0, st, g);
-  return hipGetLastError();
+  return op_launch(op_gemm_skinny<T, LAYOUT, KIND, MT, S::kCols, S::kWaves, S::kStages, DIRECT>,
+                   dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits), dim3(S::kWaves * 64), st, g);
 }
 
 template <typename T, int LAYOUT, int KIND>
@@ -1185,9 +1179,8 @@ hipError_t launch(const OpPlan& plan, OpGemm& g, hipStream_t st) {
   if (e != hipSuccess || g.splits <= 1) return e;
   const int64_t quads = (int64_t)g.M * ((g.N + 3) / 4);
   const int64_t blocks = (quads + 255) / 256, x = std::min<int64_t>(blocks, int64_t{1} << 20);
-  hipLaunchKernelGGL((op_gemm_reduce<T, KIND>),
-                     dim3((unsigned)x, (unsigned)g.outputs, (unsigned)((blocks + x - 1) / x)), dim3(256), 0, st, g);
-  return hipGetLastError();
+  return op_launch(op_gemm_reduce<T, KIND>,
+                   dim3((unsigned)x, (unsigned)g.outputs, (unsigned)((blocks + x - 1) / x)), dim3(256), st, g);
 }
 
 template <typename T>

@@ -8,6 +8,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "ops_launch.h"
 #include "ops_types.h"
 
 namespace volta {
@@ -241,19 +242,18 @@ hipError_t norm_launch(const NormArgs& a, hipStream_t st) {
   if (a.rows == 0) return hipSuccess;
   constexpr int E = kChunk<T>;
   const int chunks = (a.cols + E - 1) / E;
-#define VOLTA_NORM(TPR, NCH)                                                                              \
-  hipLaunchKernelGGL((norm_kernel<T, E4M3, TPR, NCH>), grid_of(TPR == 64 ? (a.rows + 3) / 4 : a.rows), \
-                     dim3(TPR < 256 ? 256 : TPR), 0, st, a)
+#define VOLTA_NORM(TPR, NCH)                                                                             \
+  return op_launch(norm_kernel<T, E4M3, TPR, NCH>, grid_of(TPR == 64 ? (a.rows + 3) / 4 : a.rows), \
+                   dim3(TPR < 256 ? 256 : TPR), st, a)
   if (chunks <= 64) VOLTA_NORM(64, 1);
-  else if (chunks <= 128) VOLTA_NORM(64, 2);
-  else if (chunks <= 256) VOLTA_NORM(256, 1);
-  else if (chunks <= 512) VOLTA_NORM(256, 2);
-  else if (chunks <= 1024) VOLTA_NORM(256, 4);
-  else if (chunks <= 2048) VOLTA_NORM(1024, 2);
-  else if (chunks <= 4096) VOLTA_NORM(1024, 4);
-  else VOLTA_NORM(1024, 0);
+  if (chunks <= 128) VOLTA_NORM(64, 2);
+  if (chunks <= 256) VOLTA_NORM(256, 1);
+  if (chunks <= 512) VOLTA_NORM(256, 2);
+  if (chunks <= 1024) VOLTA_NORM(256, 4);
+  if (chunks <= 2048) VOLTA_NORM(1024, 2);
+  if (chunks <= 4096) VOLTA_NORM(1024, 4);
+  VOLTA_NORM(1024, 0);
 #undef VOLTA_NORM
-  return hipGetLastError();
 }
 
 // ---------------------------------------------------------------------------
@@ -677,8 +677,7 @@ constexpr int kNormGradHeld = 2048;  // chunks of a row that the gradient's kern
 
 template <typename T, int TPR, int NCH>
 hipError_t norm_grad_launch(const NormGradArgs& a, int blocks, hipStream_t st) {
-  hipLaunchKernelGGL((norm_grad_kernel<T, TPR, NCH>), dim3((unsigned)blocks), dim3(TPR < 256 ? 256 : TPR), 0, st, a);
-  return hipGetLastError();
+  return op_launch(norm_grad_kernel<T, TPR, NCH>, dim3((unsigned)blocks), dim3(TPR < 256 ? 256 : TPR), st, a);
 }
 
 // Rows of a column strip and strips, for about 512 blocks (gradients of 2000
@@ -723,15 +722,10 @@ hipError_t norm_backward(int type, const NormGradArgs& a, hipStream_t st) {
     if (chunks <= 1024) return norm_grad_launch<T, 256, 4>(a, rows, st);
     if (chunks <= kNormGradHeld) return norm_grad_launch<T, 1024, 2>(a, rows, st);
     hipError_t e = hipSuccess;
-    if (a.dx && a.rows > 0) {
-      hipLaunchKernelGGL((norm_grad_wide_dx<T>), grid_of(a.rows), dim3(1024), 0, st, a);
-      e = hipGetLastError();
-    }
-    if (e == hipSuccess && a.partial) {
-      hipLaunchKernelGGL((norm_grad_wide_dw<T>), dim3((unsigned)((chunks + 63) / 64), (unsigned)rows),
-                         dim3(kStripWaves * 64), 0, st, a, strip_rows(chunks, a.rows));
-      e = hipGetLastError();
-    }
+    if (a.dx && a.rows > 0) e = op_launch(norm_grad_wide_dx<T>, grid_of(a.rows), dim3(1024), st, a);
+    if (e == hipSuccess && a.partial)
+      e = op_launch(norm_grad_wide_dw<T>, dim3((unsigned)((chunks + 63) / 64), (unsigned)rows), dim3(kStripWaves * 64),
+                    st, a, strip_rows(chunks, a.rows));
     return e;
   });
 }
@@ -739,9 +733,7 @@ hipError_t norm_backward(int type, const NormGradArgs& a, hipStream_t st) {
 hipError_t sum_partials(int type, const SumArgs& a, hipStream_t st) {
   return with_type(type, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL((sum_partials_kernel<T>), dim3((unsigned)((a.cols + 63) / 64), (unsigned)a.count), dim3(1024), 0,
-                       st, a);
-    return hipGetLastError();
+    return op_launch(sum_partials_kernel<T>, dim3((unsigned)((a.cols + 63) / 64), (unsigned)a.count), dim3(1024), st, a);
   });
 }
 
@@ -765,16 +757,14 @@ hipError_t act_grad(int type, bool gated, const ActGradArgs& a, hipStream_t st) 
   const int strips = act_grad_strips(type, a.rows, a.cols);
   const dim3 grid((unsigned)((chunks + 63) / 64), (unsigned)std::max(1, strips));
   if (a.unit) {
-    if (gated) hipLaunchKernelGGL((act_grad_largest<true>), grid, dim3(kStripWaves * 64), 0, st, a, per);
-    else hipLaunchKernelGGL((act_grad_largest<false>), grid, dim3(kStripWaves * 64), 0, st, a, per);
-    const hipError_t e = hipGetLastError();
+    const hipError_t e =
+        op_launch(gated ? act_grad_largest<true> : act_grad_largest<false>, grid, dim3(kStripWaves * 64), st, a, per);
     if (e != hipSuccess) return e;
   }
   const hipError_t e = with_type(type, [&](auto t) {
     using T = decltype(t);
-    if (gated) hipLaunchKernelGGL((act_grad_kernel<T, true>), grid, dim3(kStripWaves * 64), 0, st, a, per);
-    else hipLaunchKernelGGL((act_grad_kernel<T, false>), grid, dim3(kStripWaves * 64), 0, st, a, per);
-    return hipGetLastError();
+    return op_launch(gated ? act_grad_kernel<T, true> : act_grad_kernel<T, false>, grid, dim3(kStripWaves * 64), st, a,
+                     per);
   });
   if (e != hipSuccess || strips == 0) return e;
   SumArgs s{};
@@ -795,8 +785,7 @@ hipError_t pack_rows(int type, const PackArgs& a, hipStream_t st) {
     for (int i = 0; i < a.n; ++i) blocks = std::max(blocks, (a.rows[i] * (a.ld_to[i] / kChunk<T>) + 255) / 256);
     dim3 grid = grid_of(blocks);
     grid.z = (unsigned)a.n;
-    hipLaunchKernelGGL((pack_kernel<T>), grid, dim3(256), 0, st, a);
-    return hipGetLastError();
+    return op_launch(pack_kernel<T>, grid, dim3(256), st, a);
   });
 }
 
@@ -810,8 +799,7 @@ hipError_t dropout_forward(int type, const DropoutArgs& in, hipStream_t st) {
   return with_type(type, [&](auto t) {
     using T = decltype(t);
     const int64_t per_row = (a.cols + kChunk<T> - 1) / kChunk<T>;
-    hipLaunchKernelGGL((dropout_kernel<T>), grid_of((per_row * a.rows + 255) / 256), dim3(256), 0, st, a, per_row);
-    return hipGetLastError();
+    return op_launch(dropout_kernel<T>, grid_of((per_row * a.rows + 255) / 256), dim3(256), st, a, per_row);
   });
 }
 

@@ -152,7 +152,8 @@ int64_t volta_op_rms_norm_workspace(const volta_op_rms_norm* d, int32_t directio
 
 /* residual, weight [cols] (NULL: ones), sum and rstd (float [rows]) may be
  * NULL.  sum receives s, and may be x or residual.  y is normalised from s
- * before its rounding to `sum`.  With out_type E4M3, scales receives
+ * before its rounding to `sum`.  The squares' mean is a float too: of rows past
+ * about 1e19 it is infinite, rstd 0 and y 0.  With out_type E4M3, scales receives
  * [rows x ceil(cols / group)] floats, packed (one a row for group 0): for the
  * values v of a group, scale = max(max|v| / 448, 2^-126) and y = e4m3(v * (1 /
  * scale)), so v is about y * scale; a NaN among them makes the scale NaN and
@@ -161,7 +162,8 @@ int32_t volta_op_rms_norm_forward(const volta_op_rms_norm* d, const void* x, con
                                   const void* weight, void* y, void* sum, float* rstd, float* scales, void* stream);
 
 /* From dy, the forward's s (sum, or x without a residual) and rstd:
- * dx = rstd w dy - s rstd^3 mean(w dy s) + dsum, the gradient of x and of the
+ * dx = rstd w dy - s rstd^3 mean(w dy s) + dsum (formed without the cube, which
+ * leaves 32 bits long before dx does), the gradient of x and of the
  * residual alike; dsum, the gradient that reaches s by the residual stream,
  * may be NULL, and may be dx.  dweight [cols] = the column sums of dy s rstd
  * may be NULL, and so may dx, not both.  out_type and group are not read. */

@@ -1,6 +1,7 @@
 """The feed-forward operators' gradients (include/volta_ops.h) where their
 inputs are far from 1: float16 pre-activation gradients past its largest value
-or below its smallest normal one.  Bounds as in tests/test_gpu_ops.py."""
+or below its smallest normal one, rows of the norm whose 1/rms has no cube in 32
+bits.  Bounds as in tests/test_gpu_ops.py."""
 from __future__ import annotations
 
 import numpy as np
@@ -133,3 +134,38 @@ def test_gradients_of_zeros_are_zeros(lib):
     dx, dg, du = Mat(lib, "f16", M, K), Mat(lib, "f16", K, N), Mat(lib, "f16", K, N)
     op.backward(*m, dx=dx, dw_gate=dg, dw_up=du, workspace=ws)
     assert all((v.get() == 0).all() for v in (dx, dg, du))
+
+
+# ---------------------------------------------------------------------------
+# The norm's gradient.
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("eps,scale", [(1e-6, 1e15), (1e-6, 1e16), (0.0, 1e-15), (0.0, 1e-17), (0.0, 1.0)])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_norm_gradients_of_rows_far_from_one(lib, t, eps, scale):
+    """The cube of rstd, which the formula has, leaves 32 bits from rows of
+    1e13 or 1e-13 on; dx and its two terms do not.  Rows held in registers, of
+    a wave and of a block, and those read twice."""
+    for n, (M, D) in enumerate([(3, 7), (5, 512), (4, 1000), (3, 2056), (2, 9000), (2, 34001)]):
+        rng = np.random.default_rng(600 + n)
+        print(t, eps, scale, M, D, flush=True)
+        dy, s, w = draws(rng, t, M, D, scale=0.1), draws(rng, t, M, D, scale=scale), draws(rng, t, D)
+        # the gradient that reaches s by the residual stream, of dx's own size
+        ds = draws(rng, t, M, D, scale=0.1 / scale) if n % 2 else None
+        rstd32 = (1 / np.sqrt((s**2).mean(1) + eps)).astype(np.float32)
+        rstd = rstd32.astype(np.float64)[:, None]
+        op = ops.RmsNorm(M, D, t, eps)
+        ws = Space(lib, op, True)
+        dx, dw = Mat(lib, t, M, D), Mat(lib, t, 1, D)
+        op.backward(Mat(lib, t, M, D, dy), Mat(lib, t, M, D, s), Mat(lib, "f32", 1, M, rstd32[None]), dx=dx,
+                    weight=Mat(lib, t, 1, D, w), dsum=Mat(lib, t, M, D, ds) if ds is not None else None, dweight=dw,
+                    workspace=ws)
+        hat, wdy = s * rstd, w * dy
+        c = (wdy * hat).mean(1, keepdims=True)
+        ec = (D + 6) * U32 * np.abs(wdy * hat).mean(1, keepdims=True)
+        want = rstd * (wdy - hat * c) + (ds if ds is not None else 0)
+        tol = rstd * (4 * U32 * np.abs(wdy) + np.abs(hat) * (ec + 8 * U32 * np.abs(c))) + 3 * U32 * np.abs(want)
+        check(dx.get(), want, 1.01 * tol + rounded(want, t) * 1.01, "dx")
+        want = (dy * hat).sum(0)[None]
+        tol = (M + 4) * U32 * np.abs(dy * hat).sum(0)[None]
+        check(dw.get(), want, 1.01 * tol + rounded(want, t) * 1.01, "dweight")
+        ws.check()

@@ -1,7 +1,8 @@
 """The feed-forward operators' gradients (include/volta_ops.h) where their
 inputs are far from 1: float16 pre-activation gradients past its largest value
 or below its smallest normal one, rows of the norm whose 1/rms has no cube in 32
-bits.  Bounds as in tests/test_gpu_ops.py."""
+bits, pre-activations whose square is infinite.  Bounds as in
+tests/test_gpu_ops.py."""
 from __future__ import annotations
 
 import numpy as np
@@ -169,3 +170,34 @@ def test_norm_gradients_of_rows_far_from_one(lib, t, eps, scale):
         tol = (M + 4) * U32 * np.abs(dy * hat).sum(0)[None]
         check(dw.get(), want, 1.01 * tol + rounded(want, t) * 1.01, "dweight")
         ws.check()
+
+
+# ---------------------------------------------------------------------------
+# Slopes of activations.
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("t", R.TYPES)
+def test_gelu_slope_of_large_values(lib, t):
+    """1 on the right, 0 on the left, also where x^2 leaves 32 bits; f is x and
+    0.  Of one row the biases' gradients are dp, dg and du themselves."""
+    big = [40.0, 1000.0, 6e4] + ([1e13, 1e18, 2e19, 1e30, 3e38] if t != "f16" else [])
+    x = R.unpack(R.pack([v for b in big for v in (b, -b)], t), t)[None]
+    N = x.size
+    one, dy = Mat(lib, t, 1, N, np.ones((1, N))), Mat(lib, t, 1, N, np.ones((1, N)))
+    pre, inp, w = Mat(lib, t, 1, N, x), Mat(lib, t, 1, 8, np.zeros((1, 8))), Mat(lib, t, 8, N, np.zeros((8, N)))
+    lin, gat = ops.Linear(1, 8, N, t, "gelu"), ops.GatedFF(1, 8, N, t, "gelu")
+    db, dbg, dbu = Mat(lib, t, 1, N), Mat(lib, t, 1, N), Mat(lib, t, 1, N)
+    lin.backward(dy, inp, w, pre=pre, db=db, workspace=Space(lib, lin, True))
+    gat.backward(dy, inp, w, w, pre, one, db_gate=dbg, db_up=dbu, workspace=Space(lib, gat, True))
+    assert np.array_equal(db.get(), (x > 0) * 1.0) and np.array_equal(dbg.get(), (x > 0) * 1.0)
+    assert np.array_equal(dbu.get(), np.where(x > 0, x, 0.0))
+
+
+@pytest.mark.parametrize("t", R.TYPES)
+def test_gelu_slope_of_nan_is_nan(lib, t):
+    N = 8
+    pre = Mat(lib, t, 1, N, np.where(np.arange(N) == 3, np.nan, 1.0)[None])
+    m = [Mat(lib, t, 1, N, np.ones((1, N))) for _ in range(2)]
+    w, db = Mat(lib, t, N, N, np.zeros((N, N))), Mat(lib, t, 1, N)
+    lin = ops.Linear(1, N, N, t, "gelu")
+    lin.backward(m[0], m[1], w, pre=pre, db=db, workspace=Space(lib, lin, True))
+    assert np.array_equal(np.isnan(db.get()[0]), np.arange(N) == 3)

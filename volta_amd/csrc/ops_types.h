@@ -124,12 +124,18 @@ __device__ __forceinline__ void op_act_all(int act, float (&x)[N]) {
 #undef VOLTA_ACT_ALL
 }
 
+// Where GELU's slope is 1 or 0 to the last bit of 32: from there on x^2 has no
+// say in it, and past 2^64, where x^2 is infinite, would make it 0 times that.
+// A NaN stays.
+__device__ __forceinline__ float gelu_slope_at(float x) { return fabsf(x) > 32.0f ? copysignf(32.0f, x) : x; }
+
 // f and f' together (the gated layer's gradient needs both).
 template <typename T>
 __device__ __forceinline__ void op_act_both(int act, float x, float* f, float* slope) {
   if constexpr (sizeof(T) == 4) {
     *f = act_forward(act, x);
-    *slope = act == VOLTA_ACT_RELU ? (x > 0.0f ? 1.0f : 0.0f) : act_derivative(act, x, *f);
+    *slope = act == VOLTA_ACT_RELU ? (x > 0.0f ? 1.0f : 0.0f)
+                                   : act_derivative(act, act == VOLTA_ACT_GELU ? gelu_slope_at(x) : x, *f);
   } else {
     switch (act) {
       case VOLTA_ACT_RELU:
@@ -159,10 +165,11 @@ __device__ __forceinline__ void op_act_both(int act, float x, float* f, float* s
         break;
       }
       case VOLTA_ACT_GELU: {
-        const float v2 = 2.0f * kGeluC * (x + kGeluK * x * x * x);
+        const float s = gelu_slope_at(x);
+        const float v2 = 2.0f * kGeluC * (s + kGeluK * s * s * s);
         const float q = fast_sigmoid(v2);
         *f = x * q;
-        *slope = q + x * q * fast_sigmoid(-v2) * 2.0f * kGeluC * (1.0f + 3.0f * kGeluK * x * x);
+        *slope = q + s * q * fast_sigmoid(-v2) * 2.0f * kGeluC * (1.0f + 3.0f * kGeluK * s * s);
         break;
       }
       default:

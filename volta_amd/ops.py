@@ -5,10 +5,15 @@ backward, in float32 ("f32"), bfloat16 ("bf16") and float16 ("f16").
 An operator object holds the description of its matrices (sizes, types, row
 distances); a call takes the matrices themselves, as raw device addresses,
 DeviceArrays or anything with data_ptr() (a torch tensor), enqueues its
-kernels on `stream` (a hipStream_t as an integer; 0: the default stream) of
-the current device and returns.  Outputs, and a workspace of
-workspace_bytes() where that is not 0, are the caller's.  An error of the
-library raises OperatorError with its message.
+kernels on `stream` (a hipStream_t as an integer; 0: the default stream, also
+where torch's current one is another: pass its cuda_stream) of the current
+device and returns.  Outputs, and a workspace of workspace_bytes() where that
+is not 0, are the caller's.
+
+A torch tensor's type, shape and strides have to fit the description (rows of
+its last dimension, or a flat buffer; as many rows or more), a DeviceArray's
+bytes too; nothing is known of a raw address.  What does not fit, and an error
+of the library, raises OperatorError with a message.
 
     op = Linear(rows, inputs, outputs, "bf16", act="gelu")
     op.forward(x, w, y, bias=b, pre=pre, workspace=ws)
@@ -17,7 +22,6 @@ library raises OperatorError with its message.
 from __future__ import annotations
 
 import ctypes as C
-from operator import attrgetter
 
 from .abi import ACTIVATIONS
 
@@ -28,7 +32,7 @@ MASK64 = (1 << 64) - 1
 
 
 class OperatorError(RuntimeError):
-    """The library's message."""
+    """A refused call: the library's message, or which matrix does not fit the description."""
 
 
 class LinearDesc(C.Structure):
@@ -82,22 +86,96 @@ def bind(cdll: C.CDLL) -> C.CDLL:
     return cdll
 
 
-_READERS: dict = {}
+# What torch tensors may hold a type, by the names of torch's types; what an
+# element takes.
+_TORCH = {0: ("float32",), 1: ("bfloat16",), 2: ("float16",), 3: ("float8_e4m3fn", "uint8")}
+_SIZE = {0: 4, 1: 2, 2: 2, 3: 1}
+_NAMES = {v: k for k, v in TYPES.items()}
 
 
-def _reader(t):
-    """How a matrix of type t gives its device address."""
-    read = int if issubclass(t, int) else t.data_ptr if hasattr(t, "data_ptr") else attrgetter("ptr")
-    _READERS[t] = read
-    return read
+def _lies(shape, strides, rows, cols, ld) -> bool:
+    """Whether a tensor of this shape and these strides holds `rows` rows of
+    `cols` elements `ld` apart, or more of them: its last dimension is a row,
+    those before it count the rows; one dimension alone is a flat buffer."""
+    if rows <= 0:
+        return True
+    dims = [(n, s) for n, s in zip(shape, strides) if n != 1]
+    if any(n == 0 for n, _ in dims):
+        return False
+    if len(dims) <= 1 and (not dims or dims[0][1] == 1):
+        n = dims[0][0] if dims else 1
+        if n >= (rows - 1) * ld + cols:
+            return True
+    if cols != 1:
+        if not dims or dims[-1] != (cols, 1):
+            return False
+        dims.pop()
+    if rows == 1:
+        return True
+    have, apart = 1, ld
+    for n, s in reversed(dims):  # rows of rows, each `apart` from the next
+        if s != apart:
+            return False
+        have, apart = have * n, apart * n
+    return have >= rows
+
+
+def _matrix(name, type, rows, cols, ld=0):
+    """Returns how the address of matrix `name` of a call is taken: of a raw
+    address or of None as it is; of a torch tensor once its type, shape and
+    strides fit the description; of a DeviceArray once its bytes do."""
+    ld, dtype = ld or cols, None  # dtype: torch's, once a tensor has come by
+    shape, nbytes = (rows, cols) if ld == cols else None, rows * cols * _SIZE.get(type, 0)
+
+    def compare(m):
+        nonlocal dtype
+        if isinstance(m, int):
+            return m
+        if hasattr(m, "data_ptr"):
+            if hasattr(m, "dtype") and hasattr(m, "stride"):
+                if str(m.dtype).rpartition(".")[2] not in _TORCH.get(type, ()):
+                    raise OperatorError("%s is of %s, the description says %s"
+                                        % (name, m.dtype, _NAMES.get(type, type)))
+                dtype = m.dtype
+                if not _lies(tuple(m.shape), tuple(m.stride()), rows, cols, ld):
+                    raise OperatorError("%s has shape %s and strides %s, the description says %d rows of %d, %d apart"
+                                        % (name, tuple(m.shape), tuple(m.stride()), rows, cols, ld))
+            return m.data_ptr()
+        need = ((rows - 1) * ld + cols) * _SIZE.get(type, 0) if rows > 0 else 0
+        if getattr(m, "nbytes", need) < need:
+            raise OperatorError("%s holds %d bytes, the description says %d" % (name, m.nbytes, need))
+        return m.ptr
+
+    # The usual tensor, compared in the fewest steps (a call takes a few
+    # microseconds); of a row alone its bytes say as much as its shape.
+    def row(m):
+        if m is None or m.__class__ is int:
+            return m
+        try:
+            if m.dtype is dtype and m.nbytes == nbytes and m.is_contiguous():
+                return m.data_ptr()
+        except AttributeError:
+            pass
+        return compare(m)
+
+    def matrix(m):
+        if m is None or m.__class__ is int:
+            return m
+        try:
+            if m.dtype is dtype and m.shape == shape and m.is_contiguous():
+                return m.data_ptr()
+        except AttributeError:
+            pass
+        return compare(m)
+
+    return row if rows == 1 else matrix
 
 
 def _address(m):
-    """A matrix's device address; None stays None."""
-    if m is None:
-        return None
-    t = type(m)
-    return (_READERS.get(t) or _reader(t))(m)
+    """A workspace's device address; None stays None."""
+    if m is None or isinstance(m, int):
+        return m
+    return m.data_ptr() if hasattr(m, "data_ptr") else m.ptr
 
 
 def _bytes(m) -> int:
@@ -123,15 +201,14 @@ class _Operator:
     def _fn(self, call):
         return getattr(self.lib, "volta_op_%s_%s" % (self._name, call))
 
-    def _check(self, rc):
-        if rc != 0:
-            raise OperatorError(self.lib.volta_rt_last_error().decode())
+    def _refused(self):
+        return OperatorError(self.lib.volta_rt_last_error().decode())
 
     def workspace_bytes(self, backward: bool = False) -> int:
         """Bytes of workspace that a forward or backward call needs."""
         n = self._fn("workspace")(self._d, BACKWARD if backward else FORWARD)
         if n < 0:
-            raise OperatorError(self.lib.volta_rt_last_error().decode())
+            raise self._refused()
         return int(n)
 
 
@@ -141,19 +218,28 @@ class Linear(_Operator):
 
     def __init__(self, rows, inputs, outputs, dtype="f32", act="identity", ld_x=0, ld_w=0, ld_y=0, ld_residual=0,
                  ld_pre=0, ld_dx=0, ld_dw=0, lib=None):
-        super().__init__(LinearDesc(TYPES[dtype], ACTS[act], rows, inputs, outputs, ld_x, ld_w, ld_y, ld_residual,
-                                    ld_pre, ld_dx, ld_dw), "linear", lib)
+        t = TYPES[dtype]
+        super().__init__(LinearDesc(t, ACTS[act], rows, inputs, outputs, ld_x, ld_w, ld_y, ld_residual, ld_pre, ld_dx,
+                                    ld_dw), "linear", lib)
         self._forward, self._backward = self._fn("forward"), self._fn("backward")
+        x, w = _matrix("x", t, rows, inputs, ld_x), _matrix("w", t, inputs, outputs, ld_w)
+        pre = _matrix("pre", t, rows, outputs, ld_pre)
+        self._of_forward = (x, w, _matrix("bias", t, 1, outputs), _matrix("residual", t, rows, outputs, ld_residual),
+                            _matrix("y", t, rows, outputs, ld_y), pre)
+        self._of_backward = (_matrix("dy", t, rows, outputs, ld_y), x, w, pre, _matrix("dx", t, rows, inputs, ld_dx),
+                             _matrix("dw", t, inputs, outputs, ld_dw), _matrix("db", t, 1, outputs))
 
     def forward(self, x, w, y, bias=None, residual=None, pre=None, workspace=None, stream=0):
-        a = _address
-        self._check(self._forward(self._d, a(x), a(w), a(bias), a(residual), a(y), a(pre), a(workspace),
-                                  _bytes(workspace), stream))
+        ax, aw, ab, ar, ay, ap = self._of_forward
+        if self._forward(self._d, ax(x), aw(w), ab(bias), ar(residual), ay(y), ap(pre), _address(workspace),
+                         _bytes(workspace), stream):
+            raise self._refused()
 
     def backward(self, dy, x, w, pre=None, dx=None, dw=None, db=None, workspace=None, stream=0):
-        a = _address
-        self._check(self._backward(self._d, a(dy), a(x), a(w), a(pre), a(dx), a(dw), a(db), a(workspace),
-                                   _bytes(workspace), stream))
+        ay, ax, aw, ap, adx, adw, adb = self._of_backward
+        if self._backward(self._d, ay(dy), ax(x), aw(w), ap(pre), adx(dx), adw(dw), adb(db),
+                          _address(workspace), _bytes(workspace), stream):
+            raise self._refused()
 
 
 class GatedFF(_Operator):
@@ -161,20 +247,32 @@ class GatedFF(_Operator):
 
     def __init__(self, rows, inputs, hidden, dtype="f32", act="silu", ld_x=0, ld_w=0, ld_h=0, ld_pre=0, ld_dx=0,
                  ld_dw=0, lib=None):
-        super().__init__(GatedDesc(TYPES[dtype], ACTS[act], rows, inputs, hidden, ld_x, ld_w, ld_h, ld_pre, ld_dx,
-                                   ld_dw), "gated", lib)
+        t = TYPES[dtype]
+        super().__init__(GatedDesc(t, ACTS[act], rows, inputs, hidden, ld_x, ld_w, ld_h, ld_pre, ld_dx, ld_dw), "gated",
+                         lib)
         self._forward, self._backward = self._fn("forward"), self._fn("backward")
+        x = _matrix("x", t, rows, inputs, ld_x)
+        w = [_matrix(n, t, inputs, hidden, ld_w) for n in ("w_gate", "w_up")]
+        pre = [_matrix(n, t, rows, hidden, ld_pre) for n in ("gate", "up")]
+        self._of_forward = (x, *w, _matrix("b_gate", t, 1, hidden), _matrix("b_up", t, 1, hidden),
+                            _matrix("h", t, rows, hidden, ld_h), *pre)
+        self._of_backward = (_matrix("dh", t, rows, hidden, ld_h), x, *w, *pre, _matrix("dx", t, rows, inputs, ld_dx),
+                             _matrix("dw_gate", t, inputs, hidden, ld_dw), _matrix("dw_up", t, inputs, hidden, ld_dw),
+                             _matrix("db_gate", t, 1, hidden), _matrix("db_up", t, 1, hidden))
 
     def forward(self, x, w_gate, w_up, h, b_gate=None, b_up=None, gate=None, up=None, workspace=None, stream=0):
-        a = _address
-        self._check(self._forward(self._d, a(x), a(w_gate), a(w_up), a(b_gate), a(b_up), a(h), a(gate), a(up),
-                                  a(workspace), _bytes(workspace), stream))
+        ax, awg, awu, abg, abu, ah, ag, au = self._of_forward
+        if self._forward(self._d, ax(x), awg(w_gate), awu(w_up), abg(b_gate), abu(b_up), ah(h), ag(gate),
+                         au(up), _address(workspace), _bytes(workspace), stream):
+            raise self._refused()
 
     def backward(self, dh, x, w_gate, w_up, gate, up, dx=None, dw_gate=None, dw_up=None, db_gate=None, db_up=None,
                  workspace=None, stream=0):
-        a = _address
-        self._check(self._backward(self._d, a(dh), a(x), a(w_gate), a(w_up), a(gate), a(up), a(dx), a(dw_gate),
-                                   a(dw_up), a(db_gate), a(db_up), a(workspace), _bytes(workspace), stream))
+        ah, ax, awg, awu, ag, au, adx, adg, adu, abg, abu = self._of_backward
+        if self._backward(self._d, ah(dh), ax(x), awg(w_gate), awu(w_up), ag(gate), au(up), adx(dx),
+                          adg(dw_gate), adu(dw_up), abg(db_gate), abu(db_up), _address(workspace),
+                          _bytes(workspace), stream):
+            raise self._refused()
 
 
 class RmsNorm(_Operator):
@@ -184,18 +282,29 @@ class RmsNorm(_Operator):
 
     def __init__(self, rows, cols, dtype="f32", eps=1e-6, out="same", group=0, ld_x=0, ld_residual=0, ld_sum=0,
                  ld_y=0, ld_dx=0, lib=None):
-        super().__init__(RmsNormDesc(TYPES[dtype], TYPES[dtype if out == "same" else out], rows, cols, eps, group, ld_x,
-                                     ld_residual, ld_sum, ld_y, ld_dx), "rms_norm", lib)
+        t, to = TYPES[dtype], TYPES[dtype if out == "same" else out]
+        super().__init__(RmsNormDesc(t, to, rows, cols, eps, group, ld_x, ld_residual, ld_sum, ld_y, ld_dx), "rms_norm",
+                         lib)
         self._forward, self._backward = self._fn("forward"), self._fn("backward")
+        weight, rstd = _matrix("weight", t, 1, cols), _matrix("rstd", TYPES["f32"], 1, rows)
+        scales = _matrix("scales", TYPES["f32"], rows, -(-cols // group) if group > 0 else 1)
+        self._of_forward = (_matrix("x", t, rows, cols, ld_x), _matrix("residual", t, rows, cols, ld_residual), weight,
+                            _matrix("y", to, rows, cols, ld_y), _matrix("sum", t, rows, cols, ld_sum), rstd, scales)
+        self._of_backward = (_matrix("dy", t, rows, cols, ld_y), _matrix("s", t, rows, cols, ld_x), rstd, weight,
+                             _matrix("dsum", t, rows, cols, ld_sum), _matrix("dx", t, rows, cols, ld_dx),
+                             _matrix("dweight", t, 1, cols))
 
     def forward(self, x, y, weight=None, residual=None, sum=None, rstd=None, scales=None, stream=0):
-        a = _address
-        self._check(self._forward(self._d, a(x), a(residual), a(weight), a(y), a(sum), a(rstd), a(scales), stream))
+        ax, ar, aw, ay, asum, arstd, ascales = self._of_forward
+        if self._forward(self._d, ax(x), ar(residual), aw(weight), ay(y), asum(sum), arstd(rstd),
+                         ascales(scales), stream):
+            raise self._refused()
 
     def backward(self, dy, s, rstd, dx=None, weight=None, dsum=None, dweight=None, workspace=None, stream=0):
-        a = _address
-        self._check(self._backward(self._d, a(dy), a(s), a(rstd), a(weight), a(dsum), a(dx), a(dweight), a(workspace),
-                                   _bytes(workspace), stream))
+        ay, asum, arstd, aw, ads, adx, adw = self._of_backward
+        if self._backward(self._d, ay(dy), asum(s), arstd(rstd), aw(weight), ads(dsum), adx(dx), adw(dweight),
+                          _address(workspace), _bytes(workspace), stream):
+            raise self._refused()
 
 
 class Dropout(_Operator):
@@ -203,16 +312,23 @@ class Dropout(_Operator):
     so the backward pass is the same call on dy."""
 
     def __init__(self, rows, cols, dtype="f32", p=0.1, ld_x=0, ld_residual=0, ld_y=0, lib=None):
-        super().__init__(DropoutDesc(TYPES[dtype], p, rows, cols, ld_x, ld_residual, ld_y), "dropout", lib)
+        t = TYPES[dtype]
+        super().__init__(DropoutDesc(t, p, rows, cols, ld_x, ld_residual, ld_y), "dropout", lib)
         self._forward = self._fn("forward")
+        self._of_forward = (_matrix("x", t, rows, cols, ld_x), _matrix("residual", t, rows, cols, ld_residual),
+                            _matrix("y", t, rows, cols, ld_y))
+        self._of_backward = (_matrix("dy", t, rows, cols, ld_x), _matrix("dx", t, rows, cols, ld_y))
 
     def forward(self, x, y, residual=None, seed=0, offset=0, stream=0):
-        a = _address
-        self._check(self._forward(self._d, a(x), a(residual), a(y), seed & MASK64, offset & MASK64, stream))
+        ax, ar, ay = self._of_forward
+        if self._forward(self._d, ax(x), ar(residual), ay(y), seed & MASK64, offset & MASK64, stream):
+            raise self._refused()
 
     def backward(self, dy, dx, seed=0, offset=0, stream=0):
         """The gradient of x (the residual's is dy)."""
-        self.forward(dy, dx, seed=seed, offset=offset, stream=stream)
+        ay, ax = self._of_backward
+        if self._forward(self._d, ay(dy), None, ax(dx), seed & MASK64, offset & MASK64, stream):
+            raise self._refused()
 
     def workspace_bytes(self, backward: bool = False) -> int:
         return 0

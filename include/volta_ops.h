@@ -26,7 +26,8 @@
  *     default stream) of the current device and returns.  It allocates
  *     nothing and waits for nothing, so it can be captured into a graph.  A
  *     stream or memory of another device is refused, and so is memory that
- *     no device reads.
+ *     no device reads or that ends before the matrix does (what follows it
+ *     directly in other allocations counts as its own).
  *   - `workspace` is device memory of at least the bytes that the operator's
  *     *_workspace call gives for the same description (0: NULL is fine),
  *     16-byte aligned.  Its contents do not matter before and after.  Calls

@@ -122,16 +122,44 @@ void check_mats(std::initializer_list<Mat> list, std::initializer_list<Shared> s
       refuse(std::string(mats[i].name) + " overlaps the workspace");
   }
 }
-// Memory of another device or of the host's own would be a fault of the GPU.
-void check_memory(const char* name, const void* p, int device) {
-  hipPointerAttribute_t at{};
-  if (hipPointerGetAttributes(&at, p) != hipSuccess || at.type == hipMemoryTypeUnregistered) {
+// Memory of another device or of the host's own, and addresses behind the end
+// of all memory, would be a fault of the GPU.  A lookup takes 70 ns, so what an
+// allocation covers that this call has looked up already is not looked up again
+// (small tensors of one pool often share one).
+struct Allocation {
+  uintptr_t from = 0, to = 0;
+};
+// The allocation at `at`, or false where the runtime does not say.
+bool allocation_of(uintptr_t at, Allocation* a) {
+  hipDeviceptr_t base = nullptr;
+  size_t bytes = 0;
+  if (hipMemGetAddressRange(&base, &bytes, reinterpret_cast<hipDeviceptr_t>(at)) != hipSuccess) {
     (void)hipGetLastError();
-    refuse(std::string(name) + " is not memory that the device reads");
+    return false;
   }
-  if (at.type == hipMemoryTypeDevice && at.device != device)
-    refuse(std::string(name) + " is of device " + std::to_string(at.device) + ", the current device is " +
-           std::to_string(device));
+  *a = {(uintptr_t)base, (uintptr_t)base + bytes};
+  return a->from <= at && at < a->to;
+}
+void check_memory(const char* name, const void* p, int64_t bytes, int device, Allocation* last) {
+  uintptr_t at = (uintptr_t)p;
+  const uintptr_t end = at + (uintptr_t)bytes;
+  if (last->from <= at && end <= last->to) return;
+  // one allocation after another: memory that was mapped piece by piece lies side by side
+  for (bool first = true; at < end; first = false) {
+    hipPointerAttribute_t attr{};
+    if (hipPointerGetAttributes(&attr, reinterpret_cast<const void*>(at)) != hipSuccess ||
+        attr.type == hipMemoryTypeUnregistered) {
+      (void)hipGetLastError();
+      if (first) refuse(std::string(name) + " is not memory that the device reads");
+      refuse(std::string(name) + " ends " + std::to_string(end - at) + " bytes behind the end of its memory");
+    }
+    if (attr.type == hipMemoryTypeDevice && attr.device != device)
+      refuse(std::string(name) + " is of device " + std::to_string(attr.device) + ", the current device is " +
+             std::to_string(device));
+    // the ends of other kinds of memory (pinned, managed) are not looked up
+    if (attr.type != hipMemoryTypeDevice || !allocation_of(at, last)) return;
+    at = last->to;
+  }
 }
 
 // What every call checks of its matrices, workspace and stream.
@@ -149,9 +177,10 @@ hipStream_t check_call(std::initializer_list<Mat> mats, std::initializer_list<Sh
     if (of != device)
       refuse("the stream is of device " + std::to_string(of) + ", the current device is " + std::to_string(device));
   }
+  Allocation last;
   for (const Mat& m : mats)
-    if (m.span() > 0) check_memory(m.name, m.p, device);
-  if (workspace_bytes > 0) check_memory("the workspace", workspace, device);
+    if (m.span() > 0) check_memory(m.name, m.p, m.span(), device, &last);
+  if (workspace_bytes > 0) check_memory("the workspace", workspace, workspace_bytes, device, &last);
   return static_cast<hipStream_t>(stream);
 }
 void need(const void* p, const char* name) {

@@ -43,6 +43,12 @@
  *   - Sums are held in 32 bits; every result is rounded once, to the nearest
  *     of its type.  Runs are bit-reproducible: no sum's order depends on
  *     timing.
+ *   - rows is at most 2^30, every other size 2^21.  A product whose result is
+ *     too large for a launch is refused: more than 2^22 of the tiles that its
+ *     plan takes, so about 2^28 rows of up to 64 columns at the least.  A call
+ *     looks at the products that it runs alone; *_workspace speaks for every
+ *     gradient of a backward call and is refused where one of them would be
+ *     (the refusal of a call that lacks workspace says how much it takes).
  *   - Returns 0, or -1 with the message in volta_rt_last_error
  *     (volta_backend.h); then nothing was enqueued, unless the message names
  *     a failed launch.

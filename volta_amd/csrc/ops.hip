@@ -217,6 +217,10 @@ int64_t packed_bytes(int type, const Operand& o) {
   return align256(o.rows * packed_ld(type, o.len) * elem_bytes(type));
 }
 
+// Which of a layer's products a call runs; the others are not planned, and
+// what they would be refused for does not matter.
+enum : unsigned { RUN_FORWARD = 1, RUN_DX = 2, RUN_DW = 4 };
+
 // The shape of a product, and what follows for it from the description alone:
 // whether operands are laid out anew in rows of whole chunks, and the
 // workspace.  (Where a pointer turns out not to be 16-byte aligned, the
@@ -320,7 +324,7 @@ struct Linear {
   int64_t backward_bytes() const { return dp_bytes + sums_bytes + unit_bytes + std::max(dx.bytes(), dw.bytes()); }
 };
 
-Linear linear_of(const volta_op_linear* in) {
+Linear linear_of(const volta_op_linear* in, unsigned run) {
   need(in, "the description");
   Linear l{};
   volta_op_linear& d = l.d;
@@ -342,9 +346,9 @@ Linear linear_of(const volta_op_linear* in) {
   l.dp_bytes = d.act == VOLTA_OP_ACT_NONE ? 0 : packed_bytes(d.type, {d.rows, d.outputs, 0, 1});
   const int64_t dp_len = d.act == VOLTA_OP_ACT_NONE ? d.outputs : l.ld_dp;
   const Operand x{d.rows, d.inputs, d.ld_x, 1}, w{d.inputs, d.outputs, d.ld_w, 1}, dp{d.rows, dp_len, l.ld_dp, 1};
-  l.fwd = shape_of(d.type, OP_NN, OP_LINEAR, d.rows, d.outputs, d.inputs, 1, 1, x, w);
-  l.dx = shape_of(d.type, OP_NT, OP_STORE, d.rows, d.inputs, d.outputs, 1, 1, dp, w);
-  l.dw = shape_of(d.type, OP_TN, OP_STORE, d.inputs, d.outputs, d.rows, 1, 1, x, dp);
+  if (run & RUN_FORWARD) l.fwd = shape_of(d.type, OP_NN, OP_LINEAR, d.rows, d.outputs, d.inputs, 1, 1, x, w);
+  if (run & RUN_DX) l.dx = shape_of(d.type, OP_NT, OP_STORE, d.rows, d.inputs, d.outputs, 1, 1, dp, w);
+  if (run & RUN_DW) l.dw = shape_of(d.type, OP_TN, OP_STORE, d.inputs, d.outputs, d.rows, 1, 1, x, dp);
   l.sums_bytes = align256(4 * act_grad_strips(d.type, d.rows, d.outputs) * d.outputs);
   l.unit_bytes = d.act == VOLTA_OP_ACT_NONE ? 0 : align256(4 * act_grad_units(d.type, d.rows, d.outputs));
   return l;
@@ -358,7 +362,7 @@ struct Gated {
   int64_t backward_bytes() const { return 2 * (d_bytes + sums_bytes) + unit_bytes + std::max(dx.bytes(), dw.bytes()); }
 };
 
-Gated gated_of(const volta_op_gated* in) {
+Gated gated_of(const volta_op_gated* in, unsigned run) {
   need(in, "the description");
   Gated l{};
   volta_op_gated& d = l.d;
@@ -377,9 +381,9 @@ Gated gated_of(const volta_op_gated* in) {
   l.ld_d = packed_ld(d.type, d.hidden);
   l.d_bytes = packed_bytes(d.type, {d.rows, d.hidden, 0, 1});
   const Operand x{d.rows, d.inputs, d.ld_x, 1}, w{d.inputs, d.hidden, d.ld_w, 2}, dg{d.rows, l.ld_d, l.ld_d, 2};
-  l.fwd = shape_of(d.type, OP_NN, OP_GATED, d.rows, d.hidden, d.inputs, 1, 1, x, w);
-  l.dx = shape_of(d.type, OP_NT, OP_STORE, d.rows, d.inputs, d.hidden, 2, 1, dg, w);
-  l.dw = shape_of(d.type, OP_TN, OP_STORE, d.inputs, d.hidden, d.rows, 1, 2, x, dg);
+  if (run & RUN_FORWARD) l.fwd = shape_of(d.type, OP_NN, OP_GATED, d.rows, d.hidden, d.inputs, 1, 1, x, w);
+  if (run & RUN_DX) l.dx = shape_of(d.type, OP_NT, OP_STORE, d.rows, d.inputs, d.hidden, 2, 1, dg, w);
+  if (run & RUN_DW) l.dw = shape_of(d.type, OP_TN, OP_STORE, d.inputs, d.hidden, d.rows, 1, 2, x, dg);
   l.sums_bytes = align256(4 * act_grad_strips(d.type, d.rows, d.hidden) * d.hidden);
   l.unit_bytes = align256(4 * act_grad_units(d.type, d.rows, d.hidden));
   return l;
@@ -436,7 +440,7 @@ extern "C" {
 
 int64_t volta_op_linear_workspace(const volta_op_linear* d, int32_t direction) {
   return bytes_of("volta_op_linear_workspace", direction, [&](bool backward) {
-    const Linear l = linear_of(d);
+    const Linear l = linear_of(d, backward ? RUN_DX | RUN_DW : RUN_FORWARD);
     return backward ? l.backward_bytes() : l.forward_bytes();
   });
 }
@@ -445,7 +449,7 @@ int32_t volta_op_linear_forward(const volta_op_linear* in, const void* x, const 
                                 const void* residual, void* y, void* pre, void* workspace, int64_t workspace_bytes,
                                 void* stream) {
   return guarded("volta_op_linear_forward", [&] {
-    const Linear l = linear_of(in);
+    const Linear l = linear_of(in, RUN_FORWARD);
     const volta_op_linear& d = l.d;
     const int e = elem_bytes(d.type);
     if (d.rows > 0) {
@@ -476,7 +480,7 @@ int32_t volta_op_linear_backward(const volta_op_linear* in, const void* dy, cons
                                  const void* pre, void* dx, void* dw, void* db, void* workspace,
                                  int64_t workspace_bytes, void* stream) {
   return guarded("volta_op_linear_backward", [&] {
-    const Linear l = linear_of(in);
+    const Linear l = linear_of(in, (dx ? RUN_DX : 0) | (dw ? RUN_DW : 0));
     const volta_op_linear& d = l.d;
     const int e = elem_bytes(d.type);
     const bool act = d.act != VOLTA_OP_ACT_NONE;
@@ -532,7 +536,7 @@ int32_t volta_op_linear_backward(const volta_op_linear* in, const void* dy, cons
 
 int64_t volta_op_gated_workspace(const volta_op_gated* d, int32_t direction) {
   return bytes_of("volta_op_gated_workspace", direction, [&](bool backward) {
-    const Gated l = gated_of(d);
+    const Gated l = gated_of(d, backward ? RUN_DX | RUN_DW : RUN_FORWARD);
     return backward ? l.backward_bytes() : l.forward_bytes();
   });
 }
@@ -541,7 +545,7 @@ int32_t volta_op_gated_forward(const volta_op_gated* in, const void* x, const vo
                                const void* b_gate, const void* b_up, void* h, void* gate, void* up, void* workspace,
                                int64_t workspace_bytes, void* stream) {
   return guarded("volta_op_gated_forward", [&] {
-    const Gated l = gated_of(in);
+    const Gated l = gated_of(in, RUN_FORWARD);
     const volta_op_gated& d = l.d;
     const int e = elem_bytes(d.type);
     if (d.rows > 0) {
@@ -578,7 +582,7 @@ int32_t volta_op_gated_backward(const volta_op_gated* in, const void* dh, const 
                                 void* dw_up, void* db_gate, void* db_up, void* workspace, int64_t workspace_bytes,
                                 void* stream) {
   return guarded("volta_op_gated_backward", [&] {
-    const Gated l = gated_of(in);
+    const Gated l = gated_of(in, (dx ? RUN_DX : 0) | (dw_gate ? RUN_DW : 0));
     const volta_op_gated& d = l.d;
     const int e = elem_bytes(d.type);
     if (!dw_gate != !dw_up) refuse("dw_gate and dw_up are wanted both or neither");

@@ -184,9 +184,7 @@ def _bytes(m) -> int:
         return 0
     if isinstance(m, int):
         return (1 << 63) - 1
-    if hasattr(m, "ptr"):
-        return int(m.nbytes)
-    return int(m.numel() * m.element_size())
+    return int(m.nbytes)
 
 
 class _Operator:

@@ -1162,19 +1162,21 @@ hipError_t launch(const OpPlan& plan, OpGemm& g, hipStream_t st) {
           : plan.tile == OP_TILE_SKINNY32 ? launch_skinny<T, LAYOUT, KIND, 2, false>(g, st)
                                           : launch_skinny<T, LAYOUT, KIND, 4, false>(g, st);
     }
-  } else if (plan.tile == OP_TILE_256 && g.direct) {
-    e = launch_large<T, LAYOUT, KIND>(g, st);
   } else if (plan.tile == OP_TILE_64) {
     constexpr int WGM = KIND == OP_GATED ? 4 : 2;  // a wave has columns of both weight matrices
     e = g.direct ? launch_middle<T, LAYOUT, KIND, 64, 64, WGM, 8 / WGM, 2, 4>(g, st)
                  : launch_staged<T, LAYOUT, KIND, 64, 64>(g, st);
-  } else if (plan.tile == OP_TILE_256X128 && g.direct) {
-    e = launch_middle<T, LAYOUT, KIND, 256, 128, 4, 2, 1, 3>(g, st);
-  } else if (plan.tile == OP_TILE_64X128 && g.direct) {
-    e = launch_middle<T, LAYOUT, KIND, 64, 128, 2, 4, 1, 4>(g, st);
-  } else {
+  } else if (plan.tile == OP_TILE_128) {
     e = g.direct ? launch_middle<T, LAYOUT, KIND, 128, 128, 2, 4, 1, 4>(g, st)
                  : launch_staged<T, LAYOUT, KIND, 128, 128>(g, st);
+  } else if (!g.direct) {
+    return hipErrorInvalidValue;  // the other tiles have no form through registers
+  } else if (plan.tile == OP_TILE_256) {
+    e = launch_large<T, LAYOUT, KIND>(g, st);
+  } else if (plan.tile == OP_TILE_256X128) {
+    e = launch_middle<T, LAYOUT, KIND, 256, 128, 4, 2, 1, 3>(g, st);
+  } else {
+    e = launch_middle<T, LAYOUT, KIND, 64, 128, 2, 4, 1, 4>(g, st);
   }
   if (e != hipSuccess || g.splits <= 1) return e;
   const int64_t quads = (int64_t)g.M * ((g.N + 3) / 4);

@@ -254,7 +254,7 @@ int32_t volta_hip_op_product(int32_t type, int32_t layout, int32_t kind, int32_t
   if (direct && (ld_p % per_chunk || ld_q % per_chunk || p_len % per_chunk || q_len % per_chunk)) return -1;
   if (M < 1 || N < 1 || K < 0 || ld_p < p_len || ld_q < q_len || ld_out < N || splits < 1) return -1;
   if (tile < OP_TILE_256 || tile >= OP_TILES) return -1;
-  if ((tile == OP_TILE_256 || tile == OP_TILE_64X128) && !direct) return -1;
+  if ((tile == OP_TILE_256 || tile == OP_TILE_256X128 || tile == OP_TILE_64X128) && !direct) return -1;
   if (tile >= OP_TILE_SKINNY16 && layout == OP_TN) return -1;
   if ((pieces != 1 && (pieces != 2 || layout != OP_NT)) || (outputs != 1 && (outputs != 2 || layout != OP_TN))) return -1;
   OpPlan plan{tile, 1, stages, 0.0};

@@ -40,6 +40,9 @@ HIP_EXTRA = {
     "volta_hip_rt_graph_replays": (C.c_int64, []),
     "volta_hip_op_product": (C.c_int32, [C.c_int32] * 6 + [C.c_void_p, C.c_void_p, C.c_int64] * 3
                              + [C.c_int32] * 5),
+    "volta_hip_op_product_with": (C.c_int32, [C.c_int32] * 6 + [C.c_void_p, C.c_void_p, C.c_int64] * 3
+                                  + [C.c_int32] * 6 + [C.c_void_p] * 3 + [C.c_int64] + [C.c_void_p] * 2
+                                  + [C.c_int64, C.c_void_p]),
     "volta_hip_op_plan": (None, [C.c_int32] * 3 + [C.c_int64] * 3 + [C.c_int32] * 3 + [C.POINTER(C.c_int32)]),
 }
 

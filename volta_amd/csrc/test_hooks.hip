@@ -237,13 +237,15 @@ int32_t volta_hip_optimizer(int32_t kind, float* w, float* m, float* v, const fl
 
 // A product of the feed-forward operators on a given tile and number of
 // splits (ops_gemm.h), synchronously: D = sum over the pieces of P_i Q_i, or
-// the gated pair act(P Q_0) * (P Q_1) with the SiLU.  OP_LINEAR and OP_GATED
-// run without biases, residual and kept pre-activations.  Returns 0, or -1
-// for a plan that the operators would not make or a device error.
-int32_t volta_hip_op_product(int32_t type, int32_t layout, int32_t kind, int32_t tile, int32_t splits, int32_t direct,
-                             const void* p0, const void* p1, int64_t ld_p, const void* q0, const void* q1,
-                             int64_t ld_q, void* out0, void* out1, int64_t ld_out, int32_t M, int32_t N, int32_t K,
-                             int32_t pieces, int32_t outputs) {
+// the gated pair act(P Q_0) * (P Q_1), with the epilogue of ops_gemm.h.
+// Returns 0, or -1 for a plan that the operators would not make or a device
+// error.
+int32_t volta_hip_op_product_with(int32_t type, int32_t layout, int32_t kind, int32_t tile, int32_t splits,
+                                  int32_t direct, const void* p0, const void* p1, int64_t ld_p, const void* q0,
+                                  const void* q1, int64_t ld_q, void* out0, void* out1, int64_t ld_out, int32_t M,
+                                  int32_t N, int32_t K, int32_t pieces, int32_t outputs, int32_t act, const void* bias0,
+                                  const void* bias1, const void* residual, int64_t ld_residual, void* pre0, void* pre1,
+                                  int64_t ld_pre, const float* unit) {
   using namespace volta::ops;
   const int e = type == VOLTA_OP_F32 ? 4 : 2;
   const int per_chunk = 16 / e, stages = pieces * ((K + op_stage_k(e) - 1) / op_stage_k(e));
@@ -256,6 +258,7 @@ int32_t volta_hip_op_product(int32_t type, int32_t layout, int32_t kind, int32_t
   if (tile < OP_TILE_256 || tile >= OP_TILES) return -1;
   if ((tile == OP_TILE_256 || tile == OP_TILE_256X128 || tile == OP_TILE_64X128) && !direct) return -1;
   if (tile >= OP_TILE_SKINNY16 && layout == OP_TN) return -1;
+  if ((residual && ld_residual < N) || (pre0 && ld_pre < N) || (kind == OP_GATED && !pre0 != !pre1)) return -1;
   if ((pieces != 1 && (pieces != 2 || layout != OP_NT)) || (outputs != 1 && (outputs != 2 || layout != OP_TN))) return -1;
   OpPlan plan{tile, 1, stages, 0.0};
   if (stages > 0) {
@@ -279,16 +282,36 @@ int32_t volta_hip_op_product(int32_t type, int32_t layout, int32_t kind, int32_t
   g.outputs = outputs;
   g.direct = direct;
   g.partial = static_cast<float*>(ws);
-  g.epi.act = kind == OP_GATED ? VOLTA_ACT_SILU : VOLTA_OP_ACT_NONE;
+  g.epi.act = act;
+  g.epi.bias[0] = bias0;
+  g.epi.bias[1] = bias1;
+  g.epi.residual = residual;
   g.epi.out[0] = out0;
   g.epi.out[1] = out1;
+  g.epi.pre[0] = pre0;
+  g.epi.pre[1] = pre1;
   g.epi.ld_out = ld_out;
+  g.epi.ld_residual = ld_residual;
+  g.epi.ld_pre = ld_pre;
+  g.epi.unit = unit;
   hipError_t rc = type == VOLTA_OP_F32    ? op_gemm_f32(layout, kind, plan, g, nullptr)
                   : type == VOLTA_OP_BF16 ? op_gemm_bf16(layout, kind, plan, g, nullptr)
                                           : op_gemm_f16(layout, kind, plan, g, nullptr);
   if (rc == hipSuccess) rc = hipStreamSynchronize(nullptr);
   if (ws) (void)hipFree(ws);
   return rc == hipSuccess ? 0 : -1;
+}
+
+// The same without biases, residual, kept pre-activations and activation, but
+// the SiLU of the gated pair.
+int32_t volta_hip_op_product(int32_t type, int32_t layout, int32_t kind, int32_t tile, int32_t splits, int32_t direct,
+                             const void* p0, const void* p1, int64_t ld_p, const void* q0, const void* q1,
+                             int64_t ld_q, void* out0, void* out1, int64_t ld_out, int32_t M, int32_t N, int32_t K,
+                             int32_t pieces, int32_t outputs) {
+  return volta_hip_op_product_with(type, layout, kind, tile, splits, direct, p0, p1, ld_p, q0, q1, ld_q, out0, out1,
+                                   ld_out, M, N, K, pieces, outputs,
+                                   kind == volta::ops::OP_GATED ? VOLTA_ACT_SILU : VOLTA_OP_ACT_NONE, nullptr, nullptr,
+                                   nullptr, 0, nullptr, nullptr, 0, nullptr);
 }
 
 // The plan of such a product: {tile, splits, stages of a split}.

@@ -230,3 +230,47 @@ def test_gated_layers_on_every_tile(lib, t, form):
         check(pg.get(), g, 1.01 * eg + rounded(g, t), "gate")
         check(pu.get(), u, 1.01 * eu + rounded(u, t), "up")
         ws.check()
+
+
+@pytest.mark.parametrize("t", R.TYPES)
+def test_layers_laid_out_anew_exactly(lib, t):
+    """Operands whose rows are not whole 16-byte chunks, copied into the
+    workspace first: whole numbers, so products, gradients and what is kept are
+    exact."""
+    M, K, N = 1600, 1001, 1501
+    e = 4 if t == "f32" else 2
+    rng = np.random.default_rng(79)
+    x, wg, wu = whole(rng, M, K), whole(rng, K, N), whole(rng, K, N)
+    # a few small whole numbers, so that the gated layer's products of them stay exact
+    dh = rng.integers(-1, 2, (M, N)) * (rng.random((M, N)) < 0.05)
+
+    def exact(m, want):
+        return np.array_equal(m.get(), R.unpack(R.pack(want, t), t))
+
+    lin = ops.Linear(M, K, N, t)
+    even = ops.Linear(M, 1008, 1504, t)
+    assert lin.workspace_bytes() >= even.workspace_bytes() + (M * K + K * N) * e, "not laid out anew"
+    ws, wsb = Space(lib, lin), Space(lib, lin, True)
+    mx, mw, mdh = Mat(lib, t, M, K, x), Mat(lib, t, K, N, wg), Mat(lib, t, M, N, dh)
+    y, dx, dw = Mat(lib, t, M, N), Mat(lib, t, M, K), Mat(lib, t, K, N)
+    lin.forward(mx, mw, y, workspace=ws)
+    lin.backward(mdh, mx, mw, dx=dx, dw=dw, workspace=wsb)
+    ws.check()
+    wsb.check()
+    assert exact(y, x @ wg) and exact(dx, dh @ wg.T) and exact(dw, x.T @ dh)
+    gat = ops.GatedFF(M, K, N, t, "relu")
+    ws, wsb = Space(lib, gat), Space(lib, gat, True)
+    mu, h, g, u = Mat(lib, t, K, N, wu), Mat(lib, t, M, N), Mat(lib, t, M, N), Mat(lib, t, M, N)
+    gat.forward(mx, mw, mu, h, gate=g, up=u, workspace=ws)
+    p = [x @ wg, x @ wu]
+    with np.errstate(over="ignore"):
+        assert exact(h, np.maximum(p[0], 0) * p[1])
+    assert exact(g, p[0]) and exact(u, p[1])
+    kept = [whole(rng, M, N), whole(rng, M, N)]
+    pre = [Mat(lib, t, M, N, v) for v in kept]
+    dg, du = Mat(lib, t, K, N), Mat(lib, t, K, N)
+    gat.backward(mdh, mx, mw, mu, *pre, dx=dx, dw_gate=dg, dw_up=du, workspace=wsb)
+    d = [dh * kept[1] * (kept[0] > 0), dh * np.maximum(kept[0], 0)]
+    assert exact(dx, d[0] @ wg.T + d[1] @ wu.T) and exact(dg, x.T @ d[0]) and exact(du, x.T @ d[1])
+    ws.check()
+    wsb.check()

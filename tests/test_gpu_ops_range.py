@@ -5,12 +5,14 @@ bits, pre-activations whose square is infinite.  Bounds as in
 tests/test_gpu_ops.py."""
 from __future__ import annotations
 
+import ctypes as C
+
 import numpy as np
 import pytest
 
 from tests import ops_ref as R
 from tests.ops_ref import HALF, Mat, act, act_error, check, rounded
-from tests.test_gpu_ops import Space, U32, draws, sum_error
+from tests.test_gpu_ops import Block, Space, U32, _hip, draws, sum_error
 from volta_amd import load_hip, ops
 
 pytestmark = pytest.mark.gpu
@@ -201,3 +203,44 @@ def test_gelu_slope_of_nan_is_nan(lib, t):
     lin = ops.Linear(1, N, N, t, "gelu")
     lin.backward(m[0], m[1], w, pre=pre, db=db, workspace=Space(lib, lin, True))
     assert np.array_equal(np.isnan(db.get()[0]), np.arange(N) == 3)
+
+
+# ---------------------------------------------------------------------------
+# Float16 gradients' units, which live in the workspace, in a captured graph.
+# ---------------------------------------------------------------------------
+def test_float16_block_in_a_graph_with_other_inputs(lib):
+    """The block in float16, captured once and replayed on other values of dy,
+    eager runs of another block between the replays: each replay finds its own
+    units."""
+    hip = _hip(lib)
+    b, other = Block(lib, "f16", 70, 96, 200), Block(lib, "f16", 33, 64, 96, seed=12)
+    scales = (1.0, 2.0**-9, 64.0, 2.0**-14, 1.0)
+    dys = [R.unpack(R.pack(b.v["dy"] * s, "f16"), "f16") for s in scales]
+
+    def put(dy):
+        m = b.m["dy"]
+        host = m.before.copy()
+        m._view(host)[:, :] = R.pack(dy, "f16").view(R.BITS["f16"])
+        m.before = host
+        assert lib.lib.volta_hip_copy(m.dev.ptr, host.ctypes.data, host.nbytes, 1) == 0
+
+    want = []
+    for dy in dys:
+        put(dy)
+        b.run()
+        want.append(b.bits())
+    st, graph, run = C.c_void_p(), C.c_void_p(), C.c_void_p()
+    assert hip.hipStreamCreate(C.byref(st)) == 0
+    assert hip.hipStreamBeginCapture(st, 1) == 0  # thread-local
+    b.run(stream=st.value)
+    assert hip.hipStreamEndCapture(st, C.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(C.byref(run), graph, None, None, 0) == 0
+    for dy, w in zip(dys, want):
+        put(dy)
+        other.run()
+        assert hip.hipDeviceSynchronize() == 0
+        assert hip.hipGraphLaunch(run, st) == 0
+        assert hip.hipStreamSynchronize(st) == 0
+        assert all(np.array_equal(v, w[k]) for k, v in b.bits().items())
+    assert hip.hipGraphExecDestroy(run) == 0 and hip.hipGraphDestroy(graph) == 0
+    assert hip.hipStreamDestroy(st) == 0

@@ -127,7 +127,19 @@ void check_mats(std::initializer_list<Mat> list, std::initializer_list<Shared> s
 // allocation covers that this call has looked up already is not looked up again
 // (small tensors of one pool often share one).
 struct Allocation {
-  uintptr_t from = 0, to = 0;
+  uintptr_t from, to;
+};
+struct Known {
+  Allocation seen[8];
+  int n = 0;
+  bool covers(uintptr_t from, uintptr_t to) const {
+    for (int i = 0; i < n; ++i)
+      if (seen[i].from <= from && to <= seen[i].to) return true;
+    return false;
+  }
+  void add(const Allocation& a) {
+    if (n < 8) seen[n++] = a;
+  }
 };
 // The allocation at `at`, or false where the runtime does not say.
 bool allocation_of(uintptr_t at, Allocation* a) {
@@ -140,10 +152,10 @@ bool allocation_of(uintptr_t at, Allocation* a) {
   *a = {(uintptr_t)base, (uintptr_t)base + bytes};
   return a->from <= at && at < a->to;
 }
-void check_memory(const char* name, const void* p, int64_t bytes, int device, Allocation* last) {
+void check_memory(const char* name, const void* p, int64_t bytes, int device, Known* known) {
   uintptr_t at = (uintptr_t)p;
   const uintptr_t end = at + (uintptr_t)bytes;
-  if (last->from <= at && end <= last->to) return;
+  if (known->covers(at, end)) return;
   // one allocation after another: memory that was mapped piece by piece lies side by side
   for (bool first = true; at < end; first = false) {
     hipPointerAttribute_t attr{};
@@ -157,8 +169,10 @@ void check_memory(const char* name, const void* p, int64_t bytes, int device, Al
       refuse(std::string(name) + " is of device " + std::to_string(attr.device) + ", the current device is " +
              std::to_string(device));
     // the ends of other kinds of memory (pinned, managed) are not looked up
-    if (attr.type != hipMemoryTypeDevice || !allocation_of(at, last)) return;
-    at = last->to;
+    Allocation a;
+    if (attr.type != hipMemoryTypeDevice || !allocation_of(at, &a)) return;
+    known->add(a);
+    at = a.to;
   }
 }
 
@@ -177,10 +191,10 @@ hipStream_t check_call(std::initializer_list<Mat> mats, std::initializer_list<Sh
     if (of != device)
       refuse("the stream is of device " + std::to_string(of) + ", the current device is " + std::to_string(device));
   }
-  Allocation last;
+  Known known;
   for (const Mat& m : mats)
-    if (m.span() > 0) check_memory(m.name, m.p, m.span(), device, &last);
-  if (workspace_bytes > 0) check_memory("the workspace", workspace, workspace_bytes, device, &last);
+    if (m.span() > 0) check_memory(m.name, m.p, m.span(), device, &known);
+  if (workspace_bytes > 0) check_memory("the workspace", workspace, workspace_bytes, device, &known);
   return static_cast<hipStream_t>(stream);
 }
 void need(const void* p, const char* name) {

@@ -448,9 +448,11 @@ __device__ __forceinline__ void op_tile_of(int b, int tiles_m, int tiles_n, int*
 // Staged product, for operands whose rows direct loads cannot take: BM x BN of
 // D per block, 2 x 2 waves.  A stage goes through registers into one of two
 // places in LDS; the loads of the next are in flight while it is multiplied,
-// one stage ahead, and their latency bounds it.  bf16 2048^3: 128x128 40.8 us
-// and 64x64, of which more fit a CU, 37.1, against 23.2 of the direct
-// 128x128; so operands are laid out anew where that copy takes less.
+// one stage ahead, and their latency bounds it.  bf16 2048^3 with rows of 2049
+// elements: 128x128 43 us and 64x64 51 (rows of 2048 that start one element
+// off: 52 and 67; aligned, as the direct form takes them: 41 and 37), against
+// 23.7 of the direct 128x128; so operands are laid out anew where that copy
+// takes less.
 // ---------------------------------------------------------------------------
 template <typename T, int LAYOUT, int KIND, int BM, int BN>
 __global__ void __launch_bounds__(256) op_gemm_staged(OpGemm g) {

@@ -101,7 +101,8 @@ __device__ __forceinline__ float scale_of(float largest) {
 // registers between the sum and the output: chunk t + i TPR for i < NCH.
 // NCH = 0: rows too long for that, read again for each pass (from L2).
 // 8192 x 4096 bf16 with a residual and its sum, 268 MB: 51 us, 5.25 TB/s, a
-// large copy's rate; 512 x 65536 (NCH = 0) 30 us, 4.5 TB/s.
+// large copy's rate; the same to e4m3, 235 MB, 49 us with a scale for each 128
+// columns or for the row; 512 x 65536 (NCH = 0) 30 us, 4.5 TB/s.
 // ---------------------------------------------------------------------------
 template <typename T, bool E4M3, int TPR, int NCH>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_kernel(NormArgs a) {
@@ -262,7 +263,7 @@ hipError_t norm_launch(const NormArgs& a, hipStream_t st) {
 // rows of 1e13 or 1e-13 on, where dx is an ordinary number.  Block b takes rows
 // b, b + blocks, ... and keeps the sums of dweight of its rows in registers, a
 // partial sum for each block.
-// 8192 x 4096 bf16 with dsum, 268 MB and 17 MB of partial sums: 57 us, 5.0
+// 8192 x 4096 bf16 with dsum, 268 MB and 17 MB of partial sums: 55 us, 5.2
 // TB/s, and 5 us for the launch that adds the partial sums.
 // ---------------------------------------------------------------------------
 template <typename T, int TPR, int NCH>
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_grad_kernel(NormGr
 }
 
 // Rows too long for registers: dx row by row, read twice, and dweight column
-// by column.  512 x 65536 bf16: 50 + 23 us.
+// by column.  512 x 65536 bf16: 48 + 24 us.
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_grad_wide_dx(NormGradArgs a) {
   constexpr int E = kChunk<T>;
@@ -710,8 +711,8 @@ hipError_t norm_forward(int type, bool e4m3, const NormArgs& a, hipStream_t st) 
 int norm_grad_blocks(int type, int64_t rows, int64_t cols) {
   const int chunks = chunks_of(type, cols);
   if (chunks > kNormGradHeld) return strips_of(chunks, rows);
-  // as many blocks as the chip holds: 8192 x 4096 bf16 took 84 us with 512 blocks, 57 with 1024, 61 with 2048
-  // (and 4 us more for the sum of their partial sums)
+  // as many blocks as the chip holds: 8192 x 4096 bf16 took 84 us with 512 blocks, 57 with 1024 (55 since the cube
+  // of rstd went), 61 with 2048 (and 4 us more for the sum of their partial sums)
   const int rpb = chunks <= 128 ? 4 : 1;
   return (int)std::max<int64_t>(1, std::min<int64_t>((rows + rpb - 1) / rpb, chunks <= 512 ? 1024 : 512));
 }

@@ -89,7 +89,10 @@ __device__ __forceinline__ chunk16 load_part(const T* p, int cnt) {
 // keeps apart only a few such loads: with a ring of stages it no longer knows
 // which of them a read of LDS depends on, and waits for all before each read.
 // The kernels wait themselves (op_wait_loads), by counting: loads return in
-// order.  M0 takes a cycle to reach the load.
+// order.  M0 takes a cycle to reach the load.  The compiler warns that it does
+// not preserve M0 around asm; it has nothing there: it writes M0 for indexed
+// registers, messages and its own loads of this kind, directly before each, and
+// these kernels have none of them (their assembly has M0 in these lines alone).
 __device__ __forceinline__ void op_load_lds(const char* base, uint32_t off, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
                "v"(off), "s"(base)

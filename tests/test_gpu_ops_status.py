@@ -77,3 +77,18 @@ def test_wide_rows_and_biases_after_a_failed_call(lib, failed_call):
         lib.lib.hipGetLastError()
         got.append([v.bits() for v in (y, r, dx, dw, db)])
     assert all(np.array_equal(a, b) for a, b in zip(*got))
+
+
+def test_a_refusal_leaves_no_error_behind(lib):
+    """What a call's own lookups say is in its message alone."""
+    hip = lib.lib
+    hip.hipPeekAtLastError.restype = hip.hipGetLastError.restype = C.c_int
+    hip.hipGetLastError()
+    host = np.zeros(64, np.float32)
+    y, op = Mat(lib, "f32", 4, 8), ops.Dropout(4, 8)
+    with pytest.raises(ops.OperatorError):
+        op.forward(host.ctypes.data, y)
+    assert hip.hipPeekAtLastError() == 0
+    x = Mat(lib, "f32", 4, 8, np.ones((4, 8)))
+    op.forward(x, y)
+    assert hip.hipPeekAtLastError() == 0 and y.get().any()

@@ -176,18 +176,24 @@ void check_memory(const char* name, const void* p, int64_t bytes, int device, Kn
   }
 }
 
+// A lookup that has to succeed; its error is in the message, and not left for
+// the caller's next hipGetLastError.
+void look_up(hipError_t e, const char* what) {
+  if (e == hipSuccess) return;
+  (void)hipGetLastError();
+  refuse(std::string(what) + ": " + hipGetErrorString(e));
+}
+
 // What every call checks of its matrices, workspace and stream.
 hipStream_t check_call(std::initializer_list<Mat> mats, std::initializer_list<Shared> same, const void* workspace,
                        int64_t workspace_bytes, void* stream) {
   check_mats(mats, same, workspace, workspace_bytes);
   int device = 0;
-  hipError_t e = hipGetDevice(&device);
-  if (e != hipSuccess) refuse(std::string("the current device: ") + hipGetErrorString(e));
+  look_up(hipGetDevice(&device), "the current device");
   // NULL and the runtime's two named streams are the current device's
   if ((uintptr_t)stream > 2) {
     hipDevice_t of = 0;
-    e = hipStreamGetDevice(static_cast<hipStream_t>(stream), &of);
-    if (e != hipSuccess) refuse(std::string("the stream's device: ") + hipGetErrorString(e));
+    look_up(hipStreamGetDevice(static_cast<hipStream_t>(stream), &of), "the stream's device");
     if (of != device)
       refuse("the stream is of device " + std::to_string(of) + ", the current device is " + std::to_string(device));
   }

@@ -198,6 +198,43 @@ typedef struct volta_op_dropout {
 int32_t volta_op_dropout_forward(const volta_op_dropout* d, const void* x, const void* residual, void* y,
                                  uint64_t seed, uint64_t offset, void* stream);
 
+/* --- loss of an output layer: z = x W + b;  lse = log(sum(exp(z)));
+ *               loss = lse - z[label], over many classes, without keeping z - */
+typedef struct volta_op_cross_entropy {
+  int32_t type; /* of x, w, bias and their gradients */
+  int64_t rows, inputs, classes;
+  int64_t ld_x;         /* [rows x inputs] */
+  int64_t ld_w;         /* [inputs x classes] */
+  int64_t ld_dx, ld_dw; /* as x and w */
+} volta_op_cross_entropy;
+
+int64_t volta_op_cross_entropy_workspace(const volta_op_cross_entropy* d, int32_t direction);
+
+/* labels [rows] are class indices; a negative one is a row without a label,
+ * whose loss is 0; one of `classes` or more makes the row's loss NaN.  loss
+ * and lse [rows] are in units of the natural logarithm; each may be NULL, not
+ * both (lse alone takes no labels).  bias [classes] may be NULL; a -inf in it
+ * takes its class out.  z, its exponentials' sums and both results are held in
+ * 32 bits; a row with a z of +inf or NaN, and one whose z are all -inf, has a
+ * loss of NaN. */
+int32_t volta_op_cross_entropy_forward(const volta_op_cross_entropy* d, const void* x, const void* w,
+                                       const void* bias, const int32_t* labels, float* loss, float* lse,
+                                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/* From dloss [rows], the gradient that reaches each row's loss (1 / rows for
+ * their mean), and the forward's lse: dz = (exp(z - lse) - [label]) dloss, 0 in
+ * a row without a label, whatever else that row holds in lse and dloss; dx =
+ * dz W^T; dw = x^T dz; db = the column sums of dz.  z is formed anew, some
+ * classes at a time: as many as fit 256 MiB of dz, so that no more than that is
+ * kept at once.  dx, dw and db may be NULL where not wanted (at least one is).
+ * dz is rounded to the type before the products and the sums, half a step of
+ * each; float16 holds it in units of a power of two, which puts the largest
+ * |dloss| in [2^14, 2^15).  A label of `classes` or more makes the row's dz NaN. */
+int32_t volta_op_cross_entropy_backward(const volta_op_cross_entropy* d, const void* x, const void* w,
+                                        const void* bias, const int32_t* labels, const float* lse,
+                                        const float* dloss, void* dx, void* dw, void* db, void* workspace,
+                                        int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

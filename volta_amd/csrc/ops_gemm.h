@@ -20,8 +20,14 @@ enum OpLayout { OP_NN = 0, OP_NT = 1, OP_TN = 2 };
 enum OpKind {
   OP_LINEAR = 0,  // act(d + bias) + residual; d + bias kept on request
   OP_GATED = 1,   // two products of one P: act(d0 + b0) * (d1 + b1)
-  OP_STORE = 2    // the sums themselves
+  OP_STORE = 2,   // the sums themselves
+  // the loss of an output layer (ops_loss.hip); z = d + bias
+  OP_STATS = 3,      // of a row's z: their largest, the sum of their exponentials, the one at the row's label
+  OP_LOSS_GRAD = 4,  // (exp(z - lse) - [the label's]) dloss
+  OP_ADD = 5,        // sums of several launches, in order, in 32 bits
+  OP_BLEND = 6       // alpha d + beta r + gamma w, of several matrices (blockIdx.z)
 };
+constexpr bool op_kind_layer(int kind) { return kind == OP_LINEAR || kind == OP_GATED; }
 
 struct OpEpilogue {
   int32_t act;
@@ -31,6 +37,23 @@ struct OpEpilogue {
   void* pre[2];
   int64_t ld_out, ld_residual, ld_pre;
   const float* unit;  // OP_STORE in float16: one number on the device, what the sums are multiplied by; NULL: 1
+  // OP_STATS, OP_LOSS_GRAD.  The launch's columns are the classes class0 ..
+  // class0 + classes - 1; what D has behind them is padding: no part of the
+  // statistics, a gradient of 0.
+  const int32_t* labels;  // a row's class; < 0: none.  OP_STATS: NULL, none has one
+  int32_t class0, classes, all_classes;
+  float* stats;           // OP_STATS: [op_stats_entries][M] of {largest, sum of exp(z - largest)}
+  float* at_label;        // OP_STATS: [M]
+  const float *lse, *dloss;  // OP_LOSS_GRAD: [M]; unit[1] multiplies the float16 gradient
+  // OP_ADD: d + add (NULL: d); to sum, or where it is NULL to out
+  const float* add;
+  float* sum;
+  int64_t ld_sum;  // of both
+  // OP_BLEND; matrix z starts z strides behind the first
+  const void *blend, *w;  // r of the products' type, w of out's (NULL: none)
+  float alpha, beta, gamma;
+  int32_t out_type;       // enum volta_op_type
+  int64_t ld_blend, ld_w, stride_blend, stride_w, stride_out;
 };
 
 struct OpGemm {
@@ -39,7 +62,8 @@ struct OpGemm {
   int64_t ld_p, ld_q;
   int32_t M, N, K;   // K of one piece
   int32_t pieces;    // 1 or 2 pieces of the sum
-  int32_t outputs;   // 1 or 2 outputs (OP_STORE of OP_TN)
+  int32_t outputs;   // 1 or 2 outputs (OP_STORE of OP_TN); OP_BLEND: matrices
+  int64_t stride_p, stride_q;  // OP_BLEND: elements from one matrix to the next
   int32_t direct;    // rows of P and Q are 16-byte aligned and whole 16-byte chunks long
   // from the plan
   int32_t tiles_m, tiles_n;
@@ -91,6 +115,14 @@ int64_t op_gemm_blocks(const OpPlan& plan, int kind, int64_t M, int64_t N);
 hipError_t op_gemm_f32(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
 hipError_t op_gemm_bf16(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
 hipError_t op_gemm_f16(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
+// The kinds of an output layer's loss; and OP_BLEND, in float32 and float16.
+hipError_t op_gemm_loss_f32(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
+hipError_t op_gemm_loss_bf16(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
+hipError_t op_gemm_loss_f16(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
+hipError_t op_gemm_blend(int type, int layout, const OpPlan& plan, OpGemm g, hipStream_t st);
+
+// Entries of a row in OP_STATS' statistics.
+int64_t op_stats_entries(const OpPlan& plan, int64_t N);
 
 }  // namespace ops
 }  // namespace volta

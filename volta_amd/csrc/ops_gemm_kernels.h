@@ -216,12 +216,80 @@ struct Tile {
   }
 };
 
+template <typename T>
+__device__ __forceinline__ float op_exp(float x) {
+  if constexpr (sizeof(T) == 4) return expf(x);
+  else return fast_exp(x);
+}
+
+// Where a blend goes: in the output's type, w of which joins it last.
+template <int V>
+__device__ __forceinline__ void op_blend_out(const OpEpilogue& e, int z, int64_t m, int n, int cnt, float (&d)[V]) {
+  auto put = [&](auto like) {
+    using U = decltype(like);
+    if (e.w) {
+      float w[V];
+      load_vec(static_cast<const U*>(e.w) + z * e.stride_w + m * e.ld_w + n, cnt, w);
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i] += e.gamma * w[i];
+    }
+    store_vec(static_cast<U*>(e.out[0]) + z * e.stride_out + m * e.ld_out + n, cnt, d);
+  };
+  if (e.out_type == VOLTA_OP_F32) put(0.0f);
+  else if (e.out_type == VOLTA_OP_BF16) put((__bf16)0.0f);
+  else put((_Float16)0.0f);
+}
+
 // The epilogue of V consecutive columns n .. of row m, cnt of them in the
 // matrix: d0 (and, gated, d1) are the sums, b0 and b1 the columns' biases.
 template <typename T, int KIND, int V>
 __device__ __forceinline__ void op_epilogue(const OpEpilogue& e, int z, int64_t m, int n, int cnt, float (&d0)[V],
                                             float (&d1)[V], const float (&b0)[V], const float (&b1)[V]) {
-  if constexpr (KIND != OP_STORE) {
+  if constexpr (KIND == OP_LOSS_GRAD) {
+    // (p - [label]) dloss, p = exp(z - lse) <= 1.  Rounded to the type, half a
+    // step of each gradient, for the two products that take it; float16 in
+    // units that put the largest dloss under 2^15.  A row without a label is
+    // selected to 0, whatever z and lse are.
+    const int label = e.labels[m], at = label - e.class0 - n, valid = e.classes - n;
+    float g = e.dloss[m];
+    if constexpr (std::is_same<T, _Float16>::value) g *= e.unit[1];
+    if (label >= e.all_classes) g = __builtin_nanf("");  // no class at all: not to go unnoticed
+    const float lse = e.lse[m];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float p = op_exp<T>(d0[i] + b0[i] - lse);
+      d0[i] = label < 0 || i >= valid ? 0.0f : (p - (i == at ? 1.0f : 0.0f)) * g;
+    }
+    store_vec(static_cast<T*>(e.out[0]) + m * e.ld_out + n, cnt, d0);
+    return;
+  }
+  if constexpr (KIND == OP_ADD) {
+    if (e.add) {
+      float r[V];
+      load_vec(e.add + m * e.ld_sum + n, cnt, r);
+#pragma unroll
+      for (int i = 0; i < V; ++i) d0[i] += r[i];
+    }
+    if (e.sum) {
+      store_vec(e.sum + m * e.ld_sum + n, cnt, d0);
+    } else {
+      if constexpr (std::is_same<T, _Float16>::value) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) d0[i] *= *e.unit;
+      }
+      store_vec(static_cast<T*>(e.out[0]) + m * e.ld_out + n, cnt, d0);
+    }
+    return;
+  }
+  if constexpr (KIND == OP_BLEND) {
+    float r[V];
+    if (e.blend) load_vec(static_cast<const T*>(e.blend) + z * e.stride_blend + m * e.ld_blend + n, cnt, r);
+#pragma unroll
+    for (int i = 0; i < V; ++i) d0[i] = e.blend ? e.alpha * d0[i] + e.beta * r[i] : e.alpha * d0[i];
+    op_blend_out(e, z, m, n, cnt, d0);
+    return;
+  }
+  if constexpr (op_kind_layer(KIND)) {
     float r[V];
     const bool residual = KIND == OP_LINEAR && e.residual;
     if (residual) load_vec(static_cast<const T*>(e.residual) + m * e.ld_residual + n, cnt, r);
@@ -248,7 +316,9 @@ template <typename T, int KIND, int V>
 __device__ __forceinline__ void op_biases(const OpEpilogue& e, int n, int cnt, float (&b0)[V], float (&b1)[V]) {
 #pragma unroll
   for (int i = 0; i < V; ++i) b0[i] = b1[i] = 0.0f;
-  if constexpr (KIND != OP_STORE) {
+  if constexpr (KIND == OP_STATS || KIND == OP_LOSS_GRAD) {
+    if (e.bias[0]) load_vec(static_cast<const T*>(e.bias[0]) + n, min(cnt, e.classes - n), b0);
+  } else if constexpr (op_kind_layer(KIND)) {
     if (e.bias[0]) load_vec(static_cast<const T*>(e.bias[0]) + n, cnt, b0);
     if (KIND == OP_GATED && e.bias[1]) load_vec(static_cast<const T*>(e.bias[1]) + n, cnt, b1);
   }
@@ -295,6 +365,74 @@ __device__ __forceinline__ void op_barrier() {
   asm volatile("" ::: "memory");
 }
 
+// The statistics of 16 rows' z over a wave's 16 TN columns, from the sums as the
+// matrix instructions leave them: a lane has 4 TN columns of one row, its
+// neighbours 16, 32 and 48 lanes on the others.  A row whose z are all -inf has
+// a sum of 0.
+template <typename T, int TN>
+__device__ __forceinline__ void op_row_stats(const OpGemm& g, const floatx4 (&d)[TN], int lane, int m0, int n0, float* top_of,
+                                             float* sum_of) {
+  const OpEpilogue& e = g.epi;
+  const int m = m0 + (lane & 15), lg = lane >> 4;
+  const int label = e.labels && m < g.M ? e.labels[m] : -1;
+  float z[TN][4], top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int n = n0 + j * 16 + lg * 4, valid = e.classes - n;
+    float b0[4], b1[4];
+    op_biases<T, OP_STATS>(e, n, valid, b0, b1);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float v = d[j][r] + b0[r];
+      if (label == n + r && r < valid) e.at_label[m] = v;
+      z[j][r] = r < valid ? v : -__builtin_inff();
+      top = fmaxf(top, z[j][r]);
+    }
+  }
+  top = fmaxf(top, __shfl_xor(top, 16, kWave));
+  top = fmaxf(top, __shfl_xor(top, 32, kWave));
+  const float base = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+  for (int j = 0; j < TN; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sum += op_exp<T>(z[j][r] - base);
+  sum += __shfl_xor(sum, 16, kWave);
+  sum += __shfl_xor(sum, 32, kWave);
+  *top_of = top;
+  *sum_of = sum;
+}
+// Those of a block of WGM x WGN waves, whose waves side by side join theirs in
+// LDS: two values a row leave the block instead of its columns.  Every wave of
+// the block calls it.
+template <typename T, int TM, int TN, int WGM, int WGN>
+__device__ __forceinline__ void op_write_stats(const OpGemm& g, const floatx4 (&acc)[TM][TN], char* lds, int lane, int wm,
+                                               int wn, int m0, int n0) {
+  constexpr int kRows = WGM * TM * 16;
+  float* all = reinterpret_cast<float*>(lds);  // [wn][top, sum][rows]
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int row = (wm * TM + i) * 16;
+    float top, sum;
+    op_row_stats<T, TN>(g, acc[i], lane, m0 + row, n0 + wn * (TN * 16), &top, &sum);
+    if (lane < 16) {
+      all[(wn * 2) * kRows + row + lane] = top;
+      all[(wn * 2 + 1) * kRows + row + lane] = sum;
+    }
+  }
+  __syncthreads();
+  const int row = threadIdx.x, m = m0 + row;
+  if (row >= kRows || m >= g.M) return;
+  float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < WGN; ++w) top = fmaxf(top, all[(w * 2) * kRows + row]);
+  const float base = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+  for (int w = 0; w < WGN; ++w) sum += all[(w * 2 + 1) * kRows + row] * op_exp<T>(all[(w * 2) * kRows + row] - base);
+  float* to = g.epi.stats + 2 * ((int64_t)(n0 / (WGN * TN * 16)) * g.M + m);
+  to[0] = top;
+  to[1] = sum;
+}
+
 // A wave's sums (TM x TN blocks of 16x16; gated: the last half of the columns
 // belongs to the second matrix) to the outputs, or to the partial sums.  They
 // pass through `region`, LDS of the wave's own, 16 or 32 rows at a time, so
@@ -316,7 +454,8 @@ __device__ __forceinline__ void op_write_out(const OpGemm& g, floatx4 (&acc)[TM]
   constexpr bool kGated = KIND == OP_GATED;
   constexpr int kRows = op_out_rows<TM, TN>, RB = kRows / 16, kLd = TN * 16 + 4;
   constexpr int kCols = kGated ? TN * 8 : TN * 16, kE = 16 / (int)sizeof(T);  // columns of D
-  constexpr int V = KIND == OP_STORE || (KIND == OP_LINEAR && sizeof(T) == 4) ? kE : kCols / 4;  // of them a lane's
+  constexpr bool kFew = KIND == OP_STORE || KIND == OP_ADD || KIND == OP_BLEND || (!kGated && sizeof(T) == 4);
+  constexpr int V = kFew ? kE : kCols / 4;  // of them a lane's
   constexpr int kLanes = kCols / V, kTurn = 64 / kLanes;  // lanes of a row, rows of a turn
   static_assert(kRows % kTurn == 0, "whole turns");
   float* lds = reinterpret_cast<float*>(region);
@@ -381,8 +520,9 @@ __device__ __forceinline__ const char* op_stage_base(const void* p, int64_t ld, 
 // Where the next stage to load starts, in every operand (a block's loop takes
 // every `step`-th stage): advanced by additions, since a stage's address
 // computed anew costs a wave more time than its loads.
-template <typename T, int LAYOUT, bool GATED>
+template <typename T, int LAYOUT, int KIND>
 struct Cursor {
+  static constexpr bool GATED = KIND == OP_GATED;
   static constexpr bool P_KC = LAYOUT != OP_TN, Q_KC = LAYOUT == OP_NT;
   static constexpr int kSubs = GATED ? 2 : 1, kStageK = 128 / (int)sizeof(T);
   const char* p;
@@ -392,10 +532,15 @@ struct Cursor {
   int piece, m0, n0, z;
 
   __device__ __forceinline__ void place(const OpGemm& g) {
-    p = op_stage_base<T, P_KC>(g.p[piece], g.ld_p, m0, k);
+    if constexpr (KIND == OP_BLEND) {
+      p = op_stage_base<T, P_KC>(static_cast<const T*>(g.p[0]) + z * g.stride_p, g.ld_p, m0, k);
+      q[0] = op_stage_base<T, Q_KC>(static_cast<const T*>(g.q[0]) + z * g.stride_q, g.ld_q, n0, k);
+    } else {
+      p = op_stage_base<T, P_KC>(g.p[piece], g.ld_p, m0, k);
 #pragma unroll
-    for (int i = 0; i < kSubs; ++i)
-      q[i] = op_stage_base<T, Q_KC>(g.q[GATED ? i : LAYOUT == OP_TN ? z : piece], g.ld_q, n0, k);
+      for (int i = 0; i < kSubs; ++i)
+        q[i] = op_stage_base<T, Q_KC>(g.q[GATED ? i : LAYOUT == OP_TN ? z : piece], g.ld_q, n0, k);
+    }
   }
   __device__ __forceinline__ int piece_k(const OpGemm& g) const { return (g.K + kStageK - 1) / kStageK * kStageK; }
   __device__ __forceinline__ void init(const OpGemm& g, int m0_, int n0_, int z_, int s, int step) {
@@ -486,7 +631,7 @@ __global__ void __launch_bounds__(256) op_gemm_staged(OpGemm g) {
   const int s_begin = split * g.stages_per_split;
   const int s_end = min(per_piece * g.pieces, s_begin + g.stages_per_split);
 
-  Cursor<T, LAYOUT, kGated> next;
+  Cursor<T, LAYOUT, KIND> next;
   next.init(g, m0, n0, z, s_begin, 1);
   chunk16 rp[PT::kLoads], rq[kSubs][QT::kLoads];
   auto fetch = [&]() {  // the next stage
@@ -546,6 +691,9 @@ __global__ void __launch_bounds__(256) op_gemm_staged(OpGemm g) {
 
   __syncthreads();  // both places are free
   static_assert(NW * op_region_bytes<TM, TN> <= 2 * kStageBytes, "output regions fit");
+  if constexpr (KIND == OP_STATS) {
+    if (g.splits <= 1) return op_write_stats<T, TM, TN, 2, 2>(g, acc, lds, lane, wm, wn, m0, n0);
+  }
   op_write_out<T, KIND>(g, acc, lds + wave * op_region_bytes<TM, TN>, lane, m0 + wm * WM, n0 + wn * (TNS * 16), z, split);
 }
 
@@ -627,7 +775,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) o
   const int S = min(per_piece * g.pieces, s_begin + g.stages_per_split) - s_begin;
 
   // two cursors: the halves are loaded in different phases
-  Cursor<T, LAYOUT, kGated> next[2];
+  Cursor<T, LAYOUT, KIND> next[2];
   next[0].init(g, m0, n0, z, s_begin, 1);
   next[1].init(g, m0, n0, z, s_begin, 1);
   // P and Q halves h of the next stage of their cursor to the stage at byte
@@ -747,6 +895,9 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) o
   }
   __syncthreads();  // the regions are free
   static_assert(8 * op_region_bytes<8, 4> <= 8 * kRegion, "output regions fit");
+  if constexpr (KIND == OP_STATS) {
+    if (g.splits <= 1) return op_write_stats<T, 8, 4, 2, 4>(g, acc, lds, lane, wm, wn, m0, n0);
+  }
   op_write_out<T, KIND>(g, acc, lds + wave * op_region_bytes<8, 4>, lane, m0 + wm * 128, n0 + wn * (kGated ? 32 : 64), z,
                         split);
 }
@@ -797,7 +948,7 @@ __global__ void __launch_bounds__(512) op_gemm_middle(OpGemm g) {
   const int s_begin = split * g.stages_per_split;
   int parts = min((g.K + kStageK - 1) / kStageK * g.pieces, s_begin + g.stages_per_split) - s_begin;
   const int S = (parts + KS - 1) / KS;
-  Cursor<T, LAYOUT, kGated> next;
+  Cursor<T, LAYOUT, KIND> next;
   next.init(g, m0, n0, z, s_begin, 1);
   // The next stage to byte `to` of LDS; `whole`: it is, and in one piece.
   auto load = [&](uint32_t to, auto whole) {
@@ -890,6 +1041,9 @@ __global__ void __launch_bounds__(512) op_gemm_middle(OpGemm g) {
   }
   __syncthreads();  // the ring is free
   static_assert(8 * op_region_bytes<TM, TN> <= NST * kStageBytes, "output regions fit the ring");
+  if constexpr (KIND == OP_STATS) {
+    if (g.splits <= 1) return op_write_stats<T, TM, TN, WGM, WGN>(g, acc, lds, lane, wm, wn, m0, n0);
+  }
   op_write_out<T, KIND>(g, acc, lds + wave * op_region_bytes<TM, TN>, lane, m0 + wm * WM, n0 + wn * (TNS * 16), z, split);
 }
 
@@ -931,7 +1085,7 @@ __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
   char* mine = lds + wave * (NST * kWaveBytes);
 
   chunk16 rp[DIRECT ? 1 : PT::kLoads], rq[kSubs][DIRECT ? 1 : QT::kLoads];
-  Cursor<T, LAYOUT, kGated> next;
+  Cursor<T, LAYOUT, KIND> next;
   next.init(g, m0, n0, 0, s_begin + wave, NW);
   // This wave's next stage, to byte `to` of LDS; `whole`: it is, and in one piece.
   auto load = [&](uint32_t to, auto whole) {
@@ -1034,6 +1188,26 @@ __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
     for (int c = 0; c < TN; ++c) sums[(wave * TN + c) * 64 + lane] = acc[i][c];
     __syncthreads();
     const int m = m0 + i * 16 + l;
+    if constexpr (KIND == OP_STATS) {
+      if (g.splits <= 1) {  // 16 columns an entry, whole waves
+#pragma unroll
+        for (int u = 0; u < kTurns; ++u) {
+          const int j = wave + u * NW;
+          if (j >= TNS) continue;
+          floatx4 a[1] = {sums[j * 64 + lane]};
+#pragma unroll
+          for (int w = 1; w < NW; ++w) a[0] = a[0] + sums[(w * TN + j) * 64 + lane];
+          float top, sum;
+          op_row_stats<T, 1>(g, a, lane, m0 + i * 16, n0 + j * 16, &top, &sum);
+          if (lane < 16 && m < g.M) {
+            float* to = g.epi.stats + 2 * ((int64_t)(n0 / 16 + j) * g.M + m);
+            to[0] = top;
+            to[1] = sum;
+          }
+        }
+        continue;
+      }
+    }
     if (m >= g.M) continue;
 #pragma unroll
     for (int u = 0; u < kTurns; ++u) {
@@ -1104,6 +1278,46 @@ __global__ void __launch_bounds__(256) op_gemm_reduce(OpGemm g) {
   op_epilogue<T, KIND>(g.epi, z, m, n, cnt, d0, d1, b0, b1);
 }
 
+// OP_STATS of partial sums: a wave for 256 columns of a row.
+template <typename T>
+__global__ void __launch_bounds__(256) op_stats_reduce(OpGemm g) {
+  const OpEpilogue& e = g.epi;
+  const int lane = threadIdx.x & 63, entries = (g.N + 255) / 256;
+  const int64_t id = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t m = id / entries;
+  if (m >= g.M) return;
+  const int entry = (int)(id - m * entries), n = entry * 256 + lane * 4, cnt = g.N - n;
+  const int64_t plane = (int64_t)g.M * g.N;
+  const float* p = g.partial + m * g.N + n;
+  float z[4] = {}, b0[4], b1[4], top = -__builtin_inff(), sum = 0.0f;
+  op_biases<T, OP_STATS>(e, n, cnt, b0, b1);
+  for (int s = 0; s < g.splits; ++s) {
+    float v[4];
+    load_vec(p + (cnt > 0 ? s * plane : 0), cnt, v);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) z[r] += v[r];
+  }
+  const int label = e.labels ? e.labels[m] : -1;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    z[r] += b0[r];
+    if (r < cnt && label == n + r) e.at_label[m] = z[r];
+    if (r >= cnt) z[r] = -__builtin_inff();
+    top = fmaxf(top, z[r]);
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
+  const float base = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) sum += op_exp<T>(z[r] - base);
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, kWave);
+  if (lane == 0) {
+    e.stats[2 * (entry * (int64_t)g.M + m)] = top;
+    e.stats[2 * (entry * (int64_t)g.M + m) + 1] = sum;
+  }
+}
+
 // ---------------------------------------------------------------------------
 template <typename T, int LAYOUT, int KIND, int BM, int BN>
 hipError_t launch_staged(OpGemm& g, hipStream_t st) {
@@ -1154,26 +1368,28 @@ template <typename T, int LAYOUT, int KIND>
 hipError_t launch(const OpPlan& plan, OpGemm& g, hipStream_t st) {
   g.splits = plan.splits;
   g.stages_per_split = plan.stages_per_split;
-  hipError_t e;
+  hipError_t e = hipErrorInvalidValue;
+  constexpr bool kDirectOnly = KIND == OP_BLEND;
+  if (kDirectOnly && !g.direct) return hipErrorInvalidValue;
   if (plan.tile >= OP_TILE_SKINNY16) {
-    if constexpr (LAYOUT == OP_TN) {
+    if constexpr (LAYOUT == OP_TN || KIND == OP_BLEND) {
       return hipErrorInvalidValue;
-    } else if (g.direct) {
+    } else if (g.direct || kDirectOnly) {
       e = plan.tile == OP_TILE_SKINNY16   ? launch_skinny<T, LAYOUT, KIND, 1, true>(g, st)
           : plan.tile == OP_TILE_SKINNY32 ? launch_skinny<T, LAYOUT, KIND, 2, true>(g, st)
                                           : launch_skinny<T, LAYOUT, KIND, 4, true>(g, st);
-    } else {
+    } else if constexpr (!kDirectOnly) {
       e = plan.tile == OP_TILE_SKINNY16   ? launch_skinny<T, LAYOUT, KIND, 1, false>(g, st)
           : plan.tile == OP_TILE_SKINNY32 ? launch_skinny<T, LAYOUT, KIND, 2, false>(g, st)
                                           : launch_skinny<T, LAYOUT, KIND, 4, false>(g, st);
     }
   } else if (plan.tile == OP_TILE_64) {
     constexpr int WGM = KIND == OP_GATED ? 4 : 2;  // a wave has columns of both weight matrices
-    e = g.direct ? launch_middle<T, LAYOUT, KIND, 64, 64, WGM, 8 / WGM, 2, 4>(g, st)
-                 : launch_staged<T, LAYOUT, KIND, 64, 64>(g, st);
+    if (g.direct || kDirectOnly) e = launch_middle<T, LAYOUT, KIND, 64, 64, WGM, 8 / WGM, 2, 4>(g, st);
+    else if constexpr (!kDirectOnly) e = launch_staged<T, LAYOUT, KIND, 64, 64>(g, st);
   } else if (plan.tile == OP_TILE_128) {
-    e = g.direct ? launch_middle<T, LAYOUT, KIND, 128, 128, 2, 4, 1, 4>(g, st)
-                 : launch_staged<T, LAYOUT, KIND, 128, 128>(g, st);
+    if (g.direct || kDirectOnly) e = launch_middle<T, LAYOUT, KIND, 128, 128, 2, 4, 1, 4>(g, st);
+    else if constexpr (!kDirectOnly) e = launch_staged<T, LAYOUT, KIND, 128, 128>(g, st);
   } else if (!g.direct) {
     return hipErrorInvalidValue;  // the other tiles have no form through registers
   } else if (plan.tile == OP_TILE_256) {
@@ -1184,6 +1400,10 @@ hipError_t launch(const OpPlan& plan, OpGemm& g, hipStream_t st) {
     e = launch_middle<T, LAYOUT, KIND, 64, 128, 2, 4, 1, 4>(g, st);
   }
   if (e != hipSuccess || g.splits <= 1) return e;
+  if constexpr (KIND == OP_STATS) {
+    const int64_t blocks = ((int64_t)g.M * ((g.N + 255) / 256) + 3) / 4, x = std::min<int64_t>(blocks, int64_t{1} << 20);
+    return op_launch(op_stats_reduce<T>, dim3((unsigned)x, (unsigned)((blocks + x - 1) / x)), dim3(256), st, g);
+  }
   const int64_t quads = (int64_t)g.M * ((g.N + 3) / 4);
   const int64_t blocks = (quads + 255) / 256, x = std::min<int64_t>(blocks, int64_t{1} << 20);
   return op_launch(op_gemm_reduce<T, KIND>,
@@ -1196,6 +1416,14 @@ hipError_t op_gemm(int layout, int kind, const OpPlan& plan, OpGemm& g, hipStrea
   if (layout == OP_NN && kind == OP_GATED) return launch<T, OP_NN, OP_GATED>(plan, g, st);
   if (layout == OP_NT && kind == OP_STORE) return launch<T, OP_NT, OP_STORE>(plan, g, st);
   if (layout == OP_TN && kind == OP_STORE) return launch<T, OP_TN, OP_STORE>(plan, g, st);
+  return hipErrorInvalidValue;
+}
+
+template <typename T>
+hipError_t op_gemm_loss(int layout, int kind, const OpPlan& plan, OpGemm& g, hipStream_t st) {
+  if (layout == OP_NN && kind == OP_STATS) return launch<T, OP_NN, OP_STATS>(plan, g, st);
+  if (layout == OP_NN && kind == OP_LOSS_GRAD) return launch<T, OP_NN, OP_LOSS_GRAD>(plan, g, st);
+  if (layout == OP_NT && kind == OP_ADD) return launch<T, OP_NT, OP_ADD>(plan, g, st);
   return hipErrorInvalidValue;
 }
 

@@ -47,7 +47,7 @@ OpPlan op_gemm_plan(int elem_bytes, int layout, int kind, int64_t M, int64_t N, 
   for (int t = 0; t < OP_TILES; ++t) {
     const TileCost& c = kTiles[t];
     const bool skinny = t >= OP_TILE_SKINNY16;
-    if (skinny && (layout == OP_TN || M > 512)) continue;
+    if (skinny && (layout == OP_TN || kind == OP_BLEND || M > 512)) continue;
     if (!direct && (t == OP_TILE_256 || t == OP_TILE_256X128 || t == OP_TILE_64X128)) continue;
     const int64_t sn = skinny ? c.bn : kind == OP_GATED ? c.bn / 2 : c.bn;
     const int64_t tiles = ceil_div(M, c.bm) * ceil_div(N, sn) * outputs;
@@ -86,6 +86,13 @@ int64_t op_gemm_partial_bytes(const OpPlan& plan, int kind, int64_t M, int64_t N
   if (plan.splits <= 1) return 0;
   const int64_t planes = kind == OP_GATED ? 2 : outputs;
   return 4 * plan.splits * planes * M * N;
+}
+
+int64_t op_stats_entries(const OpPlan& plan, int64_t N) {
+  // a block's columns; 16 in the skinny tiles, a wave's in the launch that adds the splits
+  if (plan.splits > 1) return ceil_div(N, 256);
+  const int bn = kTiles[plan.tile].bn;
+  return plan.tile >= OP_TILE_SKINNY16 ? ceil_div(N, bn) * (bn / 16) : ceil_div(N, bn);
 }
 
 int64_t op_gemm_blocks(const OpPlan& plan, int kind, int64_t M, int64_t N) {

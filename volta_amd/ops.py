@@ -52,6 +52,11 @@ class RmsNormDesc(C.Structure):
         (n, C.c_int64) for n in ("ld_x", "ld_residual", "ld_sum", "ld_y", "ld_dx")]
 
 
+class CrossEntropyDesc(C.Structure):
+    _fields_ = [("type", C.c_int32)] + [
+        (n, C.c_int64) for n in ("rows", "inputs", "classes", "ld_x", "ld_w", "ld_dx", "ld_dw")]
+
+
 class DropoutDesc(C.Structure):
     _fields_ = [("type", C.c_int32), ("p", C.c_double)] + [
         (n, C.c_int64) for n in ("rows", "cols", "ld_x", "ld_residual", "ld_y")]
@@ -70,6 +75,9 @@ SIGNATURES = {
     "volta_op_rms_norm_forward": (C.c_int32, [C.POINTER(RmsNormDesc)] + [_P] * 8),
     "volta_op_rms_norm_backward": (C.c_int32, [C.POINTER(RmsNormDesc)] + [_P] * 8 + [_N, _P]),
     "volta_op_dropout_forward": (C.c_int32, [C.POINTER(DropoutDesc), _P, _P, _P, C.c_uint64, C.c_uint64, _P]),
+    "volta_op_cross_entropy_workspace": (_N, [C.POINTER(CrossEntropyDesc), C.c_int32]),
+    "volta_op_cross_entropy_forward": (C.c_int32, [C.POINTER(CrossEntropyDesc)] + [_P] * 7 + [_N, _P]),
+    "volta_op_cross_entropy_backward": (C.c_int32, [C.POINTER(CrossEntropyDesc)] + [_P] * 10 + [_N, _P]),
 }
 
 
@@ -88,9 +96,10 @@ def bind(cdll: C.CDLL) -> C.CDLL:
 
 # What torch tensors may hold a type, by the names of torch's types; what an
 # element takes.
-_TORCH = {0: ("float32",), 1: ("bfloat16",), 2: ("float16",), 3: ("float8_e4m3fn", "uint8")}
-_SIZE = {0: 4, 1: 2, 2: 2, 3: 1}
-_NAMES = {v: k for k, v in TYPES.items()}
+_I32 = 100  # whole numbers: no type of an operator's own
+_TORCH = {0: ("float32",), 1: ("bfloat16",), 2: ("float16",), 3: ("float8_e4m3fn", "uint8"), _I32: ("int32",)}
+_SIZE = {0: 4, 1: 2, 2: 2, 3: 1, _I32: 4}
+_NAMES = {**{v: k for k, v in TYPES.items()}, _I32: "int32"}
 
 
 def _lies(shape, strides, rows, cols, ld) -> bool:
@@ -330,3 +339,35 @@ class Dropout(_Operator):
 
     def workspace_bytes(self, backward: bool = False) -> int:
         return 0
+
+
+class CrossEntropy(_Operator):
+    """loss = log(sum(exp(z))) - z[label], z = x W + bias, over many classes
+    without keeping z; and its gradients from the rows' dloss.  A negative
+    label: a row without one."""
+
+    def __init__(self, rows, inputs, classes, dtype="f32", ld_x=0, ld_w=0, ld_dx=0, ld_dw=0, lib=None):
+        t = TYPES[dtype]
+        super().__init__(CrossEntropyDesc(t, rows, inputs, classes, ld_x, ld_w, ld_dx, ld_dw), "cross_entropy", lib)
+        self._forward, self._backward = self._fn("forward"), self._fn("backward")
+
+        def floats(name):
+            return _matrix(name, TYPES["f32"], 1, rows)
+
+        head = (_matrix("x", t, rows, inputs, ld_x), _matrix("w", t, inputs, classes, ld_w),
+                _matrix("bias", t, 1, classes), _matrix("labels", _I32, 1, rows))
+        self._of_forward = (*head, floats("loss"), floats("lse"))
+        self._of_backward = (*head, floats("lse"), floats("dloss"), _matrix("dx", t, rows, inputs, ld_dx),
+                             _matrix("dw", t, inputs, classes, ld_dw), _matrix("db", t, 1, classes))
+
+    def forward(self, x, w, labels, loss, lse=None, bias=None, workspace=None, stream=0):
+        ax, aw, ab, al, aloss, alse = self._of_forward
+        if self._forward(self._d, ax(x), aw(w), ab(bias), al(labels), aloss(loss), alse(lse), _address(workspace),
+                         _bytes(workspace), stream):
+            raise self._refused()
+
+    def backward(self, x, w, labels, lse, dloss, bias=None, dx=None, dw=None, db=None, workspace=None, stream=0):
+        ax, aw, ab, al, alse, ad, adx, adw, adb = self._of_backward
+        if self._backward(self._d, ax(x), aw(w), ab(bias), al(labels), alse(lse), ad(dloss), adx(dx), adw(dw), adb(db),
+                          _address(workspace), _bytes(workspace), stream):
+            raise self._refused()

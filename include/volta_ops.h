@@ -235,6 +235,53 @@ int32_t volta_op_cross_entropy_backward(const volta_op_cross_entropy* d, const v
                                         const float* dloss, void* dx, void* dw, void* db, void* workspace,
                                         int64_t workspace_bytes, void* stream);
 
+/* --- e4m3 codes of a matrix ------------------------------------------------
+ * For the values v of a group: scale = max(max|v| / 448, 2^-126) and code =
+ * e4m3(v * (1 / scale)), as the norm's output; a NaN in a group makes its scale
+ * and its codes NaN. */
+enum volta_op_groups {
+  VOLTA_OP_ROWS = 0,  /* 128 columns of a row share a scale: activations */
+  VOLTA_OP_BLOCKS = 1 /* 128 x 128 elements share one, and the codes lie transposed: weights */
+};
+typedef struct volta_op_quantize {
+  int32_t type;   /* of x: F32, BF16, F16 */
+  int32_t groups; /* enum volta_op_groups */
+  int64_t rows, cols;
+  int64_t ld_x; /* [rows x cols] */
+  int64_t ld_y; /* ROWS: [rows x cols]; BLOCKS: [cols x rows] */
+} volta_op_quantize;
+
+/* scales, packed: ROWS [rows x ceil(cols / 128)]; BLOCKS [ceil(cols / 128) x
+ * ceil(rows / 128)].  BLOCKS takes W [inputs x outputs] to what the product
+ * below reads: inputs contiguous, as its matrix instructions take them. */
+int32_t volta_op_quantize_forward(const volta_op_quantize* d, const void* x, void* y, float* scales, void* stream);
+
+/* --- linear layer of e4m3 codes: y = act(x W + bias) + residual, where
+ *     x[m][k] = code * x_scales[m][k / 128] and
+ *     W[k][n] = code[n][k] * w_scales[n / 128][k / 128] ------------------- */
+typedef struct volta_op_linear8 {
+  int32_t type; /* of bias, residual and y: F32, BF16, F16 */
+  int32_t act;  /* as the linear layer's */
+  int64_t rows, inputs, outputs;
+  int32_t group;            /* inputs that share a scale of x: 128, or 0 for the whole row (the norm's two forms) */
+  int64_t ld_x;             /* [rows x inputs] codes */
+  int64_t ld_w;             /* [outputs x inputs] codes */
+  int64_t ld_y, ld_residual; /* [rows x outputs] */
+} volta_op_linear8;
+
+int64_t volta_op_linear8_workspace(const volta_op_linear8* d);
+
+/* x_scales [rows x ceil(inputs / 128)], or [rows] for group 0, and w_scales
+ * [ceil(outputs / 128) x ceil(inputs / 128)] are packed.  The codes' products
+ * of a block of 128 inputs are summed, and the blocks' sums times their scales
+ * added, in 32 bits; with y of 16 bits the matrix instruction for codes adds
+ * eight products at a time, of which it drops what is under about 2^-17 of the
+ * largest (a hundredth of y's rounding).  bias [outputs] and residual may be NULL; residual may be
+ * y (the same pointer and ld). */
+int32_t volta_op_linear8_forward(const volta_op_linear8* d, const void* x, const float* x_scales, const void* w,
+                                 const float* w_scales, const void* bias, const void* residual, void* y,
+                                 void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

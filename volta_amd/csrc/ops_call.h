@@ -217,6 +217,10 @@ void check_workspace(const void* p, int64_t have, int64_t want) {
 }
 
 hipError_t gemm(int type, int layout, int kind, const OpPlan& plan, const OpGemm& g, hipStream_t st) {
+  if (type == VOLTA_OP_E4M3)
+    return g.epi.out_type == VOLTA_OP_F32    ? op_gemm8_f32(plan, g, st)
+           : g.epi.out_type == VOLTA_OP_BF16 ? op_gemm8_bf16(plan, g, st)
+                                             : op_gemm8_f16(plan, g, st);
   if (kind == OP_STATS || kind == OP_LOSS_GRAD || kind == OP_ADD)
     return type == VOLTA_OP_F32    ? op_gemm_loss_f32(layout, kind, plan, g, st)
            : type == VOLTA_OP_BF16 ? op_gemm_loss_bf16(layout, kind, plan, g, st)

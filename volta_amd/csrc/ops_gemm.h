@@ -49,10 +49,14 @@ struct OpEpilogue {
   const float* add;
   float* sum;
   int64_t ld_sum;  // of both
+  // products of e4m3 codes: the scale of row m and k block b at sx[m ld_sx + b
+  // step_sx], of columns n and block b at sw[n / 128 ld_sw + b]
+  const float *sx, *sw;
+  int64_t ld_sx, step_sx, ld_sw;
   // OP_BLEND; matrix z starts z strides behind the first
   const void *blend, *w;  // r of the products' type, w of out's (NULL: none)
   float alpha, beta, gamma;
-  int32_t out_type;       // enum volta_op_type
+  int32_t out_type;       // enum volta_op_type; also of a product of codes
   int64_t ld_blend, ld_w, stride_blend, stride_w, stride_out;
 };
 
@@ -120,6 +124,12 @@ hipError_t op_gemm_loss_f32(int layout, int kind, const OpPlan& plan, OpGemm g, 
 hipError_t op_gemm_loss_bf16(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
 hipError_t op_gemm_loss_f16(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
 hipError_t op_gemm_blend(int type, int layout, const OpPlan& plan, OpGemm g, hipStream_t st);
+
+// Products of e4m3 codes (OP_NT, OP_LINEAR), by the type of bias, residual and
+// result.
+hipError_t op_gemm8_f32(const OpPlan& plan, OpGemm g, hipStream_t st);
+hipError_t op_gemm8_bf16(const OpPlan& plan, OpGemm g, hipStream_t st);
+hipError_t op_gemm8_f16(const OpPlan& plan, OpGemm g, hipStream_t st);
 
 // Entries of a row in OP_STATS' statistics.
 int64_t op_stats_entries(const OpPlan& plan, int64_t N);

@@ -1,0 +1,534 @@
+// Products of e4m3 codes with scales, for one type of the result:
+//   D[m][n] = sum over k blocks of 128, b, of sx[m][b] sw[n / 128][b] *
+//             (sum over the block's k of x[m][k] w[n][k])
+// Both operands have k contiguous, and a stage of 128 bytes of a row is one
+// block, so the tiles, their order in LDS, the rings and the epilogues are
+// those of ops_gemm_kernels.h.
+//
+// v_mfma_f32_16x16x128 takes 32 codes of a row a lane and sums a whole block
+// for 16x16 of D, exactly scaled by nothing; which k a lane holds does not
+// matter as long as both operands agree, so a lane's two chunks are g and g + 4
+// of the row's eight.  Its four sums a lane are then added to the running ones,
+// times the row's and the columns' scale: 4 FMAs for the 32 cycles that the
+// instruction takes, which the vector unit has to spare (scales as powers of
+// two in the instruction itself would be free, but ours are floats).
+//
+// The rows' scales go to LDS with the stage, four bytes a lane, by one load
+// more; the columns' one (a wave's columns share their 128) is a scalar load a
+// stage ahead.
+#pragma once
+
+#include "ops_gemm_kernels.h"
+
+namespace volta {
+namespace ops {
+
+typedef int32_t intx8 __attribute__((ext_vector_type(8)));
+
+// 32 codes of a row: chunks g and g + 4.
+struct Frag8 {
+  chunk16 c[2];
+};
+__device__ __forceinline__ floatx4 mfma8(const Frag8& a, const Frag8& b) {
+  // scale operands of 0 select the instruction without scales
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(intx8, a), __builtin_bit_cast(intx8, b),
+                                                          floatx4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0, 0, 0, 0);
+}
+template <typename Tile8>
+__device__ __forceinline__ Frag8 frag8(const char* tile, int x0, int lane) {
+  return Frag8{{Tile8::frag(tile, x0, 0, lane), Tile8::frag(tile, x0, 1, lane)}};
+}
+
+// 4 bytes a lane to LDS, lane after lane (op_load_lds).
+__device__ __forceinline__ void op_load_lds4(const float* from, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
+               "v"(from)
+               : "memory", "m0");
+}
+
+// A scalar load whatever the compiler thinks of the asm around it.
+__device__ __forceinline__ float scalar_load(const float* p) {
+  return *(const __attribute__((address_space(4))) float*)p;
+}
+
+// The instruction adds eight products at a time, of which it keeps what is not
+// under about 2^-17 of the largest: normal values' sums are 1.2e-5 of their norm
+// off, which 16-bit results do not see and float32 ones do.  Those take the
+// codes as float16 (exactly) on its instructions, at half the rate or less.
+struct Frag16 {
+  chunk16 c[4];
+};
+__device__ __forceinline__ Frag16 widen(const Frag8& f) {
+  typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+  Frag16 w;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const half2_t lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(f.c[h][i], 1.0f, false);
+      const half2_t hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(f.c[h][i], 1.0f, true);
+      w.c[h * 2 + (i >> 1)][(i & 1) * 2] = __builtin_bit_cast(uint32_t, lo);
+      w.c[h * 2 + (i >> 1)][(i & 1) * 2 + 1] = __builtin_bit_cast(uint32_t, hi);
+    }
+  return w;
+}
+
+// acc += s t, of blocks TM x TN of 16x16.
+template <typename T, int TM, int TN>
+__device__ __forceinline__ void mul8(const Frag8 (&fp)[TM], const Frag8 (&fq)[TN], const float (&s)[TM],
+                                     floatx4 (&acc)[TM][TN]) {
+  if constexpr (sizeof(T) == 4) {
+    Frag16 q[TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) q[j] = widen(fq[j]);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const Frag16 p = widen(fp[i]);
+      floatx4 t[TN];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) t[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) t[j] = Mfma<_Float16>::mul(0, q[j].c[k], p.c[k], t[j]);
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(t[j][r], s[i], acc[i][j][r]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const floatx4 t = mfma8(fq[j], fp[i]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(t[r], s[i], acc[i][j][r]);
+      }
+  }
+}
+
+// The rows' scales of a block's tile: row m0 + r of k block b.
+struct RowScales {
+  const float* at;  // this lane's row, block 0
+  int64_t step;     // from a block to the next
+  int last;         // the last block
+  __device__ __forceinline__ void init(const OpGemm& g, int m0, int row) {
+    at = g.epi.sx + (int64_t)min(m0 + row, g.M - 1) * g.epi.ld_sx;
+    step = g.epi.step_sx;
+    last = (g.K + 127) / 128 - 1;
+  }
+  __device__ __forceinline__ const float* of(int b) const { return at + min(b, last) * step; }
+};
+// The columns' scales of a wave's columns from n on.
+struct ColumnScales {
+  const float* at;
+  int last;
+  __device__ __forceinline__ void init(const OpGemm& g, int n) {
+    at = g.epi.sw + (int64_t)(min(n, g.N - 1) / 128) * g.epi.ld_sw;
+    last = (g.K + 127) / 128 - 1;
+  }
+  __device__ __forceinline__ float of(int b) const { return scalar_load(at + min(b, last)); }
+};
+
+using Cursor8 = Cursor<uint8_t, OP_NT, OP_STORE>;
+
+// ---------------------------------------------------------------------------
+// BM x BN of D per block, eight waves, a ring of NST stages of KS blocks of k
+// (op_gemm_middle).
+// ---------------------------------------------------------------------------
+template <typename T, int BM, int BN, int WGM, int WGN, int KS, int NST>
+__global__ void __launch_bounds__(512) op_gemm8_middle(OpGemm g) {
+  constexpr int WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
+  using PT = Tile<uint8_t, BM, true, 8>;
+  using QT = Tile<uint8_t, BN, true, 8>;
+  constexpr int kPart = PT::kBytes + QT::kBytes + BM * 4, kStageBytes = KS * kPart;
+  constexpr int kStageLoads = KS * (PT::kLoads + QT::kLoads + 1);
+  __shared__ __attribute__((aligned(16))) char lds[NST * kStageBytes];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WGN, wn = wave % WGN;
+  int tm, tn;
+  op_tile_of(blockIdx.x, g.tiles_m, g.tiles_n, &tm, &tn);
+  const int m0 = tm * BM, n0 = tn * BN, split = blockIdx.y;
+  PT pt;
+  QT qt;
+  pt.init(g.ld_p, g.M - m0, wave, lane);
+  qt.init(g.ld_q, g.N - n0, wave, lane);
+  // every wave loads 64 rows' scales, so that all count the same loads; waves
+  // that load the same rows write the same values
+  const int scales_at = wave % (BM / 64) * 64;
+  RowScales sx;
+  sx.init(g, m0, scales_at + lane);
+  ColumnScales sw;
+  sw.init(g, n0 + wn * WN);
+  const int s_begin = split * g.stages_per_split;
+  const int blocks = (g.K + 127) / 128;
+  int parts = min(blocks, s_begin + g.stages_per_split) - s_begin;
+  const int S = (parts + KS - 1) / KS;
+  Cursor8 next;
+  next.init(g, m0, n0, 0, s_begin, 1);
+  auto load = [&](uint32_t to, auto whole) {
+    constexpr bool W = decltype(whole)::value;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      const int k_left = W ? 128 : parts > i ? g.K - next.k : 0;  // a part behind the last one is zeros
+      const uint32_t lp = to + i * kPart, lq = lp + PT::kBytes;
+      op_load_lds4(sx.of(next.k >> 7), lq + QT::kBytes + scales_at * 4);
+      if (W || k_left >= 128) {
+        qt.issue(next.q[0], lq, wave);
+        pt.issue(next.p, lp, wave);
+      } else {
+        qt.issue_tail(next.q[0], lq, wave, lane, k_left);
+        pt.issue_tail(next.p, lp, wave, lane, k_left);
+      }
+      next.step();
+    }
+    parts -= KS;
+  };
+
+  floatx4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  int from = 0, to = (NST - 1) * kStageBytes;
+  const uint32_t lds_byte = op_lds_byte(lds);
+  float w_scale[KS];
+#pragma unroll
+  for (int i = 0; i < KS; ++i) w_scale[i] = sw.of(s_begin + i);
+  auto stage = [&](int s, auto whole) {
+    constexpr bool W = decltype(whole)::value;
+    Frag8 fp[KS][TM], fq[KS][TN];
+    float sc[KS][TM], w_next[KS];
+#pragma unroll
+    for (int i = 0; i < KS; ++i) w_next[i] = sw.of(s_begin + (s + 1) * KS + i);
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) {
+      const char* part = lds + from + kk * kPart;
+      const float* scales = reinterpret_cast<const float*>(part + PT::kBytes + QT::kBytes);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) fq[kk][j] = frag8<QT>(part + PT::kBytes, wn * WN + j * 16, lane);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        fp[kk][i] = frag8<PT>(part, wm * WM + i * 16, lane);
+        sc[kk][i] = scales[wm * WM + i * 16 + (lane & 15)];
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (W || s + NST - 1 < S) {
+      load(lds_byte + to, whole);
+      op_wait_loads<(NST - 2) * kStageLoads>();  // stage s + 1 is there
+    } else {
+      op_wait_loads<0>();
+    }
+    to = from;
+    from = from == (NST - 1) * kStageBytes ? 0 : from + kStageBytes;
+    op_wait_lds();
+    op_barrier();
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) sc[kk][i] *= w_scale[kk];
+      mul8<T, TM, TN>(fp[kk], fq[kk], sc[kk], acc);
+      w_scale[kk] = w_next[kk];
+    }
+    op_barrier();
+  };
+
+  if (S > 0) {
+#pragma unroll 1
+    for (int i = 0; i < NST - 1 && i < S; ++i) load(lds_byte + i * kStageBytes, std::false_type());
+    if (S >= NST - 1) op_wait_loads<(NST - 2) * kStageLoads>();
+    else op_wait_loads<0>();
+    op_barrier();
+    if (wave >= 4) op_barrier();
+    for (int s = 0; s < S; ++s) {
+      for (int n = min(min(next.whole_steps(g), parts) / KS, S - (NST - 1) - s); n > 0; --n, ++s)
+        stage(s, std::true_type());
+      if (s < S) stage(s, std::false_type());
+    }
+    if (wave < 4) op_barrier();
+  }
+  __syncthreads();  // the ring is free
+  static_assert(8 * op_region_bytes<TM, TN> <= NST * kStageBytes, "output regions fit the ring");
+  op_write_out<T, OP_LINEAR>(g, acc, lds + wave * op_region_bytes<TM, TN>, lane, m0 + wm * WM, n0 + wn * WN, 0, split);
+}
+
+// ---------------------------------------------------------------------------
+// The same through registers, for rows that direct loads cannot take
+// (op_gemm_staged).
+// ---------------------------------------------------------------------------
+template <typename T, int BM, int BN>
+__global__ void __launch_bounds__(256) op_gemm8_staged(OpGemm g) {
+  constexpr int NW = 4, WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16;
+  using PT = Tile<uint8_t, BM, true, NW>;
+  using QT = Tile<uint8_t, BN, true, NW>;
+  constexpr int kStageBytes = PT::kBytes + QT::kBytes;
+  __shared__ __attribute__((aligned(16))) char lds[2 * kStageBytes];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+  int tm, tn;
+  op_tile_of(blockIdx.x, g.tiles_m, g.tiles_n, &tm, &tn);
+  const int m0 = tm * BM, n0 = tn * BN, split = blockIdx.y;
+  const int p_left = g.M - m0, q_left = g.N - n0;
+  PT pt;
+  QT qt;
+  pt.init(g.ld_p, p_left, wave, lane);
+  qt.init(g.ld_q, q_left, wave, lane);
+  RowScales sx[TM];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) sx[i].init(g, m0, wm * WM + i * 16 + (lane & 15));
+  ColumnScales sw;
+  sw.init(g, n0 + wn * WN);
+  const int s_begin = split * g.stages_per_split, s_end = min((g.K + 127) / 128, s_begin + g.stages_per_split);
+  Cursor8 next;
+  next.init(g, m0, n0, 0, s_begin, 1);
+  chunk16 rp[PT::kLoads], rq[QT::kLoads];
+  float scale[TM], now[TM];
+  int block = s_begin;
+  auto fetch = [&]() {
+    const int k_left = g.K - next.k;
+    pt.fetch(next.p, rp, wave, lane, p_left, k_left);
+    qt.fetch(next.q[0], rq, wave, lane, q_left, k_left);
+    const float w = sw.of(block);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) scale[i] = *sx[i].of(block) * w;
+    ++block;
+    next.step();
+  };
+  auto put = [&](char* to) {
+    pt.put(rp, to, wave, lane);
+    qt.put(rq, to + PT::kBytes, wave, lane);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) now[i] = scale[i];
+    __syncthreads();
+  };
+  floatx4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (s_begin < s_end) fetch();
+  for (int s0 = s_begin; s0 < s_end; s0 += 2) {
+    op_unroll<2>([&](auto i) {
+      const int s = s0 + i;
+      if (s >= s_end) return;
+      char* at = lds + decltype(i)::value * kStageBytes;
+      put(at);
+      if (s + 1 < s_end) fetch();
+      __builtin_amdgcn_sched_barrier(0);
+      Frag8 fp[TM], fq[TN];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) fq[j] = frag8<QT>(at + PT::kBytes, wn * WN + j * 16, lane);
+#pragma unroll
+      for (int j = 0; j < TM; ++j) fp[j] = frag8<PT>(at, wm * WM + j * 16, lane);
+      mul8<T, TM, TN>(fp, fq, now, acc);
+    });
+  }
+  __syncthreads();  // both places are free
+  static_assert(NW * op_region_bytes<TM, TN> <= 2 * kStageBytes, "output regions fit");
+  op_write_out<T, OP_LINEAR>(g, acc, lds + wave * op_region_bytes<TM, TN>, lane, m0 + wm * WM, n0 + wn * WN, 0, split);
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: 16 MT rows and 32 columns a block, whose waves take turns over the
+// blocks of k (op_gemm_skinny).
+// ---------------------------------------------------------------------------
+template <typename T, int MT, int NW, int NST, bool DIRECT>
+__global__ void __launch_bounds__(NW * 64) op_gemm8_skinny(OpGemm g) {
+  constexpr int BN = 32, TN = BN / 16;
+  using PT = Tile<uint8_t, 16 * MT, true, 1>;
+  using QT = Tile<uint8_t, BN, true, 1>;
+  constexpr int kWaveBytes = PT::kBytes + QT::kBytes + (DIRECT ? 256 : 0);
+  constexpr int kStageLoads = PT::kLoads + QT::kLoads + 1;
+  static_assert(DIRECT ? NST >= 2 : NST == 1, "ring");
+  __shared__ __attribute__((aligned(16))) char lds[NST * NW * kWaveBytes];
+
+  const int tid = threadIdx.x, lane = tid & 63, l = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int tm, tn;
+  op_tile_of(blockIdx.x, g.tiles_m, g.tiles_n, &tm, &tn);
+  const int m0 = tm * (16 * MT), n0 = tn * BN, split = blockIdx.y, p_left = g.M - m0, q_left = g.N - n0;
+  PT pt;
+  QT qt;
+  pt.init(g.ld_p, p_left, 0, lane);
+  qt.init(g.ld_q, q_left, 0, lane);
+  RowScales sx;
+  sx.init(g, m0, lane % (16 * MT));
+  ColumnScales sw;
+  sw.init(g, n0);
+  const int s_begin = split * g.stages_per_split, s_end = min((g.K + 127) / 128, s_begin + g.stages_per_split);
+  char* mine = lds + wave * (NST * kWaveBytes);
+  chunk16 rp[DIRECT ? 1 : PT::kLoads], rq[DIRECT ? 1 : QT::kLoads];
+  float held = 0.0f;  // staged: the scale of this lane's row
+  Cursor8 next;
+  next.init(g, m0, n0, 0, s_begin + wave, NW);
+  auto load = [&](uint32_t to, auto whole) {
+    constexpr bool W = decltype(whole)::value;
+    const int k_left = W ? 128 : g.K - next.k;
+    if constexpr (DIRECT) {
+      const uint32_t lq = to + PT::kBytes;
+      op_load_lds4(sx.of(next.k >> 7), lq + QT::kBytes);
+      if (W || k_left >= 128) {
+        qt.issue(next.q[0], lq, 0);
+        pt.issue(next.p, to, 0);
+      } else {
+        qt.issue_tail(next.q[0], lq, 0, lane, k_left);
+        pt.issue_tail(next.p, to, 0, lane, k_left);
+      }
+    } else {
+      held = *sx.of(next.k >> 7);
+      qt.fetch(next.q[0], rq, 0, lane, q_left, k_left);
+      pt.fetch(next.p, rp, 0, lane, p_left, k_left);
+    }
+    next.step();
+  };
+  floatx4 acc[MT][TN];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  auto compute = [&](const char* from, const float (&s)[MT]) {
+    Frag8 fq[TN], fp[MT];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) fq[j] = frag8<QT>(from + PT::kBytes, j * 16, lane);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) fp[i] = frag8<PT>(from, i * 16, lane);
+    mul8<T, MT, TN>(fp, fq, s, acc);
+  };
+  const int S = s_end > s_begin + wave ? (s_end - s_begin - wave + NW - 1) / NW : 0;
+  float w_scale = sw.of(s_begin + wave);
+  if constexpr (DIRECT) {  // NST - 1 stages in flight
+    const uint32_t lds_byte = op_lds_byte(mine);
+    int from = 0, to = (NST - 1) * kWaveBytes;
+    auto stage = [&](int s, auto whole) {
+      constexpr bool W = decltype(whole)::value;
+      op_wait_lds();  // what the next loads overwrite was read one turn ago
+      __builtin_amdgcn_sched_barrier(0);
+      const float w_next = sw.of(s_begin + wave + (s + 1) * NW);
+      if (W || s + NST - 1 < S) {
+        load(lds_byte + to, whole);
+        op_wait_loads<(NST - 1) * kStageLoads>();
+      } else {
+        op_wait_loads<0>();
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      const float* scales = reinterpret_cast<const float*>(mine + from + PT::kBytes + QT::kBytes);
+      float sc[MT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) sc[i] = scales[i * 16 + l] * w_scale;
+      compute(mine + from, sc);
+      w_scale = w_next;
+      to = from;
+      from = from == (NST - 1) * kWaveBytes ? 0 : from + kWaveBytes;
+    };
+#pragma unroll 1
+    for (int i = 0; i < NST - 1 && i < S; ++i) load(lds_byte + i * kWaveBytes, std::false_type());
+    for (int s = 0; s < S; ++s) {
+      for (int n = min(next.whole_steps(g), S - (NST - 1) - s); n > 0; --n, ++s) stage(s, std::true_type());
+      if (s < S) stage(s, std::false_type());
+    }
+  } else {
+    constexpr auto any = std::false_type();
+    if (S > 0) load(0, any);
+    for (int s = 0; s < S; ++s) {
+      pt.put(rp, mine, 0, lane);
+      qt.put(rq, mine + PT::kBytes, 0, lane);
+      float sc[MT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) sc[i] = __shfl(held, i * 16 + l, kWave) * w_scale;
+      w_scale = sw.of(s_begin + wave + (s + 1) * NW);
+      if (s + 1 < S) load(0, any);
+      __builtin_amdgcn_sched_barrier(0);
+      compute(mine, sc);
+    }
+  }
+
+  // The waves' sums, in wave order, 16 rows at a time.
+  floatx4* sums = reinterpret_cast<floatx4*>(lds);
+  static_assert(NW * TN * 1024 <= NST * NW * kWaveBytes, "sums fit the ring");
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < TN; ++c) sums[(wave * TN + c) * 64 + lane] = acc[i][c];
+    __syncthreads();
+    const int m = m0 + i * 16 + l, j = wave, n = n0 + j * 16 + lg * 4, cnt = g.N - n;
+    if (m >= g.M || j >= TN || cnt <= 0) continue;
+    floatx4 a = sums[j * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) a = a + sums[(w * TN + j) * 64 + lane];
+    float d0[4], d1[4] = {}, b0[4], b1[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) d0[r] = a[r];
+    if (g.splits > 1) {
+      store_vec(g.partial + ((int64_t)split * g.M + m) * g.N + n, cnt, d0);
+    } else {
+      op_biases<T, OP_LINEAR>(g.epi, n, cnt, b0, b1);
+      op_epilogue<T, OP_LINEAR>(g.epi, 0, m, n, cnt, d0, d1, b0, b1);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+template <typename T, int BM, int BN, int WGM, int WGN, int KS, int NST>
+hipError_t launch8_middle(OpGemm& g, hipStream_t st) {
+  g.tiles_m = (g.M + BM - 1) / BM;
+  g.tiles_n = (g.N + BN - 1) / BN;
+  return op_launch(op_gemm8_middle<T, BM, BN, WGM, WGN, KS, NST>,
+                   dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits), dim3(512), st, g);
+}
+template <typename T, int BM, int BN>
+hipError_t launch8_staged(OpGemm& g, hipStream_t st) {
+  g.tiles_m = (g.M + BM - 1) / BM;
+  g.tiles_n = (g.N + BN - 1) / BN;
+  return op_launch(op_gemm8_staged<T, BM, BN>, dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits), dim3(256),
+                   st, g);
+}
+template <typename T, int MT, bool DIRECT>
+hipError_t launch8_skinny(OpGemm& g, hipStream_t st) {
+  using S = SkinnyShape<OP_LINEAR, MT, DIRECT>;
+  g.tiles_m = (g.M + 16 * MT - 1) / (16 * MT);
+  g.tiles_n = (g.N + S::kCols - 1) / S::kCols;
+  return op_launch(op_gemm8_skinny<T, MT, S::kWaves, S::kStages, DIRECT>,
+                   dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits), dim3(S::kWaves * 64), st, g);
+}
+
+template <typename T>
+hipError_t launch8(const OpPlan& plan, OpGemm& g, hipStream_t st) {
+  g.splits = plan.splits;
+  g.stages_per_split = plan.stages_per_split;
+  hipError_t e = hipErrorInvalidValue;
+  switch (plan.tile) {
+    case OP_TILE_SKINNY16: e = g.direct ? launch8_skinny<T, 1, true>(g, st) : launch8_skinny<T, 1, false>(g, st); break;
+    case OP_TILE_SKINNY32: e = g.direct ? launch8_skinny<T, 2, true>(g, st) : launch8_skinny<T, 2, false>(g, st); break;
+    case OP_TILE_SKINNY64: e = g.direct ? launch8_skinny<T, 4, true>(g, st) : launch8_skinny<T, 4, false>(g, st); break;
+    case OP_TILE_64:
+      e = g.direct ? launch8_middle<T, 64, 64, 2, 4, 2, 4>(g, st) : launch8_staged<T, 64, 64>(g, st);
+      break;
+    case OP_TILE_128:
+      e = g.direct ? launch8_middle<T, 128, 128, 2, 4, 1, 4>(g, st) : launch8_staged<T, 128, 128>(g, st);
+      break;
+    case OP_TILE_64X128:
+      if (g.direct) e = launch8_middle<T, 64, 128, 2, 4, 1, 4>(g, st);
+      break;
+    case OP_TILE_256X128:
+      if (g.direct) e = launch8_middle<T, 256, 128, 4, 2, 1, 3>(g, st);
+      break;
+    default:  // float32's fragments take more registers than that tile has
+      if (g.direct && sizeof(T) == 4) e = launch8_middle<T, 256, 128, 4, 2, 1, 3>(g, st);
+      else if constexpr (sizeof(T) < 4) e = g.direct ? launch8_middle<T, 256, 256, 2, 4, 1, 2>(g, st) : e;
+  }
+  if (e != hipSuccess || g.splits <= 1) return e;
+  const int64_t quads = (int64_t)g.M * ((g.N + 3) / 4);
+  const int64_t blocks = (quads + 255) / 256, x = std::min<int64_t>(blocks, int64_t{1} << 20);
+  return op_launch(op_gemm_reduce<T, OP_LINEAR>, dim3((unsigned)x, 1, (unsigned)((blocks + x - 1) / x)), dim3(256), st, g);
+}
+
+}  // namespace ops
+}  // namespace volta

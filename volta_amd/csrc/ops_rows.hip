@@ -8,15 +8,13 @@
 #include <cmath>
 #include <type_traits>
 
+#include "ops_codes.h"
 #include "ops_launch.h"
 #include "ops_types.h"
 
 namespace volta {
 namespace ops {
 namespace {
-
-typedef uint32_t chunk8_by1 __attribute__((ext_vector_type(2), aligned(1)));
-typedef uint32_t chunk4_by1 __attribute__((aligned(1)));
 
 // A grid of n blocks and the block's number in it: a dimension of a grid has
 // fewer than 2^32 threads, so many blocks take two.
@@ -37,29 +35,6 @@ template <typename T>
 __device__ __forceinline__ void store_row(T* p, int cnt, const float (&f)[kChunk<T>]) {
   store_vec(p, cnt, f);
 }
-// E (4 or 8) values as e4m3 codes, to the nearest.
-template <int E>
-__device__ __forceinline__ void store_codes(uint8_t* p, int cnt, const float (&f)[E]) {
-  union { uint32_t w[E / 4]; uint8_t b[E]; } u;
-#pragma unroll
-  for (int i = 0; i < E / 4; ++i) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i], f[4 * i + 1], 0, false);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2], f[4 * i + 3], w, true);
-    u.w[i] = (uint32_t)w;
-  }
-  if (cnt >= E) {
-    if constexpr (E == 8) *(VOLTA_GLOBAL chunk8_by1*)p = chunk8_by1{u.w[0], u.w[1]};
-    else *(VOLTA_GLOBAL chunk4_by1*)p = u.w[0];
-  } else {
-#pragma unroll
-    for (int i = 0; i < E; ++i)
-      if (i < cnt) ((VOLTA_GLOBAL uint8_t*)p)[i] = u.b[i];
-  }
-}
-
-// The larger of two magnitudes; a NaN stays.
-__device__ __forceinline__ float max_or_nan(float m, float v) { return v > m || v != v ? v : m; }
-
 // Sum (or maximum) over the TPR threads of a row: over a wave by a butterfly,
 // over a block's waves through LDS, always in the same order.  `red` holds a
 // float for each wave; uses of it alternate between two arrays.
@@ -87,13 +62,6 @@ __device__ __forceinline__ float row_max(float v, float* red) {
     for (int w = 1; w < TPR / 64; ++w) v = max_or_nan(v, red[w]);
   }
   return v;
-}
-
-constexpr float kE4m3Max = 448.0f;
-constexpr float kTiny = 1.17549435e-38f;  // 2^-126
-__device__ __forceinline__ float scale_of(float largest) {
-  const float q = largest / kE4m3Max;
-  return q < kTiny ? kTiny : q;
 }
 
 // ---------------------------------------------------------------------------
@@ -621,6 +589,23 @@ __global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
   store_row(static_cast<T*>(a.to[i]) + row * a.ld_to[i] + c, E, f);
 }
 
+// The same of codes, whose rows start at any byte.
+__global__ void __launch_bounds__(256) pack_codes_kernel(PackArgs a) {
+  const int i = blockIdx.z;
+  const int64_t chunks = a.ld_to[i] / 16, id = block_id() * 256 + threadIdx.x, row = id / chunks;
+  if (row >= a.rows[i]) return;
+  const int c = (int)(id - row * chunks) * 16, cnt = a.cols[i] - c;
+  const uint8_t* from = static_cast<const uint8_t*>(a.from[i]) + row * a.ld_from[i] + c;
+  union { chunk16 v; uint8_t b[16]; } u;
+  if (cnt >= 16) {
+    u.v = *(const VOLTA_GLOBAL Access<16, 1>::type*)from;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) u.b[k] = k < cnt ? ((const VOLTA_GLOBAL uint8_t*)from)[k] : 0;
+  }
+  *reinterpret_cast<chunk16*>(static_cast<uint8_t*>(a.to[i]) + row * a.ld_to[i] + c) = u.v;
+}
+
 // ---------------------------------------------------------------------------
 // Dropout: a thread for 16 bytes of a row.  Element i's 32 bits are half of
 // output i/2 of the stream: E/2 outputs for a chunk that starts at an even i,
@@ -786,6 +771,13 @@ hipError_t act_grad(int type, bool gated, const ActGradArgs& a, hipStream_t st) 
 }
 
 hipError_t pack_rows(int type, const PackArgs& a, hipStream_t st) {
+  if (type == VOLTA_OP_E4M3) {
+    int64_t blocks = 1;
+    for (int i = 0; i < a.n; ++i) blocks = std::max(blocks, (a.rows[i] * (a.ld_to[i] / 16) + 255) / 256);
+    dim3 grid = grid_of(blocks);
+    grid.z = (unsigned)a.n;
+    return op_launch(pack_codes_kernel, grid, dim3(256), st, a);
+  }
   return with_type(type, [&](auto t) {
     using T = decltype(t);
     int64_t blocks = 1;

@@ -30,6 +30,7 @@ template <int BYTES, int ALIGN> struct Access;
   template <> struct Access<BYTES, ALIGN> { typedef BASE type __attribute__((ext_vector_type(N), aligned(ALIGN))); }
 VOLTA_ACCESS(16, 4, uint32_t, 4);
 VOLTA_ACCESS(16, 2, uint32_t, 4);
+VOLTA_ACCESS(16, 1, uint32_t, 4);
 VOLTA_ACCESS(8, 4, uint32_t, 2);
 VOLTA_ACCESS(8, 2, uint32_t, 2);
 VOLTA_ACCESS(4, 2, uint32_t, 1);

@@ -314,6 +314,50 @@ int32_t volta_hip_op_product(int32_t type, int32_t layout, int32_t kind, int32_t
                                    nullptr, 0, nullptr, nullptr, 0, nullptr);
 }
 
+// A product of e4m3 codes on a given tile and number of splits (ops_gemm8_kernels.h),
+// synchronously, without bias, activation and residual.
+int32_t volta_hip_op_product8(int32_t type, int32_t tile, int32_t splits, int32_t direct, const void* x, int64_t ld_x,
+                              const float* x_scales, int32_t group, const void* w, int64_t ld_w, const float* w_scales,
+                              void* out, int64_t ld_out, int32_t M, int32_t N, int32_t K) {
+  using namespace volta::ops;
+  if (direct && ((uintptr_t)x % 16 || (uintptr_t)w % 16 || ld_x % 16 || ld_w % 16 || K % 16)) return -1;
+  if (M < 1 || N < 1 || K < 1 || ld_x < K || ld_w < K || ld_out < N || splits < 1) return -1;
+  if (tile < OP_TILE_256 || tile >= OP_TILES) return -1;
+  if ((tile == OP_TILE_256 || tile == OP_TILE_256X128 || tile == OP_TILE_64X128) && !direct) return -1;
+  const int blocks = (K + 127) / 128;
+  OpPlan plan{tile, 1, blocks, 0.0};
+  plan.stages_per_split = (blocks + splits - 1) / splits;
+  plan.splits = (blocks + plan.stages_per_split - 1) / plan.stages_per_split;
+  const int64_t bytes = op_gemm_partial_bytes(plan, OP_LINEAR, M, N, 1);
+  void* ws = nullptr;
+  if (bytes && hipMalloc(&ws, bytes) != hipSuccess) return -1;
+  OpGemm g{};
+  g.p[0] = g.p[1] = x;
+  g.q[0] = g.q[1] = w;
+  g.ld_p = ld_x;
+  g.ld_q = ld_w;
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.pieces = g.outputs = 1;
+  g.direct = direct;
+  g.partial = static_cast<float*>(ws);
+  g.epi.act = VOLTA_OP_ACT_NONE;
+  g.epi.out[0] = out;
+  g.epi.ld_out = ld_out;
+  g.epi.sx = x_scales;
+  g.epi.sw = w_scales;
+  g.epi.ld_sx = group ? blocks : 1;
+  g.epi.step_sx = group ? 1 : 0;
+  g.epi.ld_sw = blocks;
+  hipError_t rc = type == VOLTA_OP_F32    ? op_gemm8_f32(plan, g, nullptr)
+                  : type == VOLTA_OP_BF16 ? op_gemm8_bf16(plan, g, nullptr)
+                                          : op_gemm8_f16(plan, g, nullptr);
+  if (rc == hipSuccess) rc = hipStreamSynchronize(nullptr);
+  if (ws) (void)hipFree(ws);
+  return rc == hipSuccess ? 0 : -1;
+}
+
 // The plan of such a product: {tile, splits, stages of a split}.
 void volta_hip_op_plan(int32_t elem_bytes, int32_t layout, int32_t kind, int64_t M, int64_t N, int64_t K,
                        int32_t pieces, int32_t outputs, int32_t direct, int32_t* plan) {

@@ -57,6 +57,16 @@ class CrossEntropyDesc(C.Structure):
         (n, C.c_int64) for n in ("rows", "inputs", "classes", "ld_x", "ld_w", "ld_dx", "ld_dw")]
 
 
+class QuantizeDesc(C.Structure):
+    _fields_ = [("type", C.c_int32), ("groups", C.c_int32)] + [(n, C.c_int64) for n in ("rows", "cols", "ld_x", "ld_y")]
+
+
+class Linear8Desc(C.Structure):
+    _fields_ = [("type", C.c_int32), ("act", C.c_int32), ("rows", C.c_int64), ("inputs", C.c_int64),
+                ("outputs", C.c_int64), ("group", C.c_int32)] + [
+        (n, C.c_int64) for n in ("ld_x", "ld_w", "ld_y", "ld_residual")]
+
+
 class DropoutDesc(C.Structure):
     _fields_ = [("type", C.c_int32), ("p", C.c_double)] + [
         (n, C.c_int64) for n in ("rows", "cols", "ld_x", "ld_residual", "ld_y")]
@@ -75,6 +85,9 @@ SIGNATURES = {
     "volta_op_rms_norm_forward": (C.c_int32, [C.POINTER(RmsNormDesc)] + [_P] * 8),
     "volta_op_rms_norm_backward": (C.c_int32, [C.POINTER(RmsNormDesc)] + [_P] * 8 + [_N, _P]),
     "volta_op_dropout_forward": (C.c_int32, [C.POINTER(DropoutDesc), _P, _P, _P, C.c_uint64, C.c_uint64, _P]),
+    "volta_op_quantize_forward": (C.c_int32, [C.POINTER(QuantizeDesc), _P, _P, _P, _P]),
+    "volta_op_linear8_workspace": (_N, [C.POINTER(Linear8Desc)]),
+    "volta_op_linear8_forward": (C.c_int32, [C.POINTER(Linear8Desc)] + [_P] * 8 + [_N, _P]),
     "volta_op_cross_entropy_workspace": (_N, [C.POINTER(CrossEntropyDesc), C.c_int32]),
     "volta_op_cross_entropy_forward": (C.c_int32, [C.POINTER(CrossEntropyDesc)] + [_P] * 7 + [_N, _P]),
     "volta_op_cross_entropy_backward": (C.c_int32, [C.POINTER(CrossEntropyDesc)] + [_P] * 10 + [_N, _P]),
@@ -371,3 +384,59 @@ class CrossEntropy(_Operator):
         if self._backward(self._d, ax(x), aw(w), ab(bias), al(labels), alse(lse), ad(dloss), adx(dx), adw(dw), adb(db),
                           _address(workspace), _bytes(workspace), stream):
             raise self._refused()
+
+
+class Quantize(_Operator):
+    """e4m3 codes of a matrix with a scale for each 128 columns of a row
+    (by="rows": activations), or for each block of 128 x 128, the codes
+    transposed (by="blocks": W [inputs x outputs] for Linear8)."""
+
+    def __init__(self, rows, cols, dtype="f32", by="rows", ld_x=0, ld_y=0, lib=None):
+        t, blocks = TYPES[dtype], {"rows": 0, "blocks": 1}[by]
+        super().__init__(QuantizeDesc(t, blocks, rows, cols, ld_x, ld_y), "quantize", lib)
+        self._forward = self._fn("forward")
+        y = (cols, rows) if blocks else (rows, cols)
+        scales = (-(-cols // 128), -(-rows // 128)) if blocks else (rows, -(-cols // 128))
+        self._of_forward = (_matrix("x", t, rows, cols, ld_x), _matrix("y", TYPES["e4m3"], *y, ld_y),
+                            _matrix("scales", TYPES["f32"], *scales))
+
+    def forward(self, x, y, scales, stream=0):
+        ax, ay, ascales = self._of_forward
+        if self._forward(self._d, ax(x), ay(y), ascales(scales), stream):
+            raise self._refused()
+
+    def workspace_bytes(self, backward: bool = False) -> int:
+        return 0
+
+
+class Linear8(_Operator):
+    """y = act(x W + bias) + residual of e4m3 codes: x [rows x inputs] with a
+    scale for each 128 inputs (group=128) or for the row (group=0), as RmsNorm
+    and Quantize(by="rows") leave them; w [outputs x inputs] with a scale for
+    each block of 128 x 128, as Quantize(by="blocks") leaves it."""
+
+    def __init__(self, rows, inputs, outputs, dtype="bf16", act="identity", group=128, ld_x=0, ld_w=0, ld_y=0,
+                 ld_residual=0, lib=None):
+        t, code, f32 = TYPES[dtype], TYPES["e4m3"], TYPES["f32"]
+        super().__init__(Linear8Desc(t, ACTS[act], rows, inputs, outputs, group, ld_x, ld_w, ld_y, ld_residual), "linear8",
+                         lib)
+        self._forward = self._fn("forward")
+        blocks = -(-inputs // 128)
+        self._of_forward = (_matrix("x", code, rows, inputs, ld_x),
+                            _matrix("x_scales", f32, rows, blocks if group else 1),
+                            _matrix("w", code, outputs, inputs, ld_w), _matrix("w_scales", f32, -(-outputs // 128), blocks),
+                            _matrix("bias", t, 1, outputs), _matrix("residual", t, rows, outputs, ld_residual),
+                            _matrix("y", t, rows, outputs, ld_y))
+
+    def forward(self, x, x_scales, w, w_scales, y, bias=None, residual=None, workspace=None, stream=0):
+        ax, asx, aw, asw, ab, ar, ay = self._of_forward
+        if self._forward(self._d, ax(x), asx(x_scales), aw(w), asw(w_scales), ab(bias), ar(residual), ay(y),
+                         _address(workspace), _bytes(workspace), stream):
+            raise self._refused()
+
+    def workspace_bytes(self) -> int:
+        """Bytes of workspace that a call needs."""
+        n = self._fn("workspace")(self._d)
+        if n < 0:
+            raise self._refused()
+        return int(n)

@@ -142,7 +142,7 @@ int32_t volta_op_linear_forward(const volta_op_linear* in, const void* x, const 
     const Mat mr{"residual", residual, d.rows, d.outputs, d.ld_residual, e, false};
     const Mat my{"y", y, d.rows, d.outputs, d.ld_y, e, true}, mp{"pre", pre, d.rows, d.outputs, d.ld_pre, e, true};
     check_workspace(workspace, workspace_bytes, l.forward_bytes());
-    const hipStream_t st = check_call({mx, mw, mb, mr, my, mp}, {{residual, y}}, workspace, l.forward_bytes(), stream);
+    const hipStream_t st = check_call({mx, mw, mb, mr, my, mp}, {{"residual", "y"}}, workspace, l.forward_bytes(), stream);
     OpEpilogue epi{};
     epi.act = d.act;
     epi.bias[0] = bias;
@@ -360,7 +360,7 @@ int32_t volta_op_rms_norm_forward(const volta_op_rms_norm* in, const void* x, co
          {"sum", sum, d.rows, d.cols, d.ld_sum, e, true},
          {"rstd", rstd, d.rows, 1, 1, 4, true},
          {"scales", scales, d.rows, groups, groups, 4, true}},
-        {{sum, x}, {sum, residual}}, nullptr, 0, stream);
+        {{"sum", "x"}, {"sum", "residual"}}, nullptr, 0, stream);
     NormArgs a{};
     a.x = x;
     a.residual = residual;
@@ -403,7 +403,7 @@ int32_t volta_op_rms_norm_backward(const volta_op_rms_norm* in, const void* dy, 
          {"dsum", dsum, d.rows, d.cols, d.ld_sum, e, false},
          {"dx", dx, d.rows, d.cols, d.ld_dx, e, true},
          {"dweight", dweight, 1, d.cols, d.cols, e, true}},
-        {{dsum, dx}}, workspace, dweight ? n.backward_bytes() : 0, stream);
+        {{"dsum", "dx"}}, workspace, dweight ? n.backward_bytes() : 0, stream);
     NormGradArgs a{};
     a.dy = dy;
     a.s = s;
@@ -447,7 +447,7 @@ int32_t volta_op_dropout_forward(const volta_op_dropout* in, const void* x, cons
         {{"x", x, d.rows, d.cols, d.ld_x, e, false},
          {"residual", residual, d.rows, d.cols, d.ld_residual, e, false},
          {"y", y, d.rows, d.cols, d.ld_y, e, true}},
-        {{x, y}, {residual, y}}, nullptr, 0, stream);
+        {{"x", "y"}, {"residual", "y"}}, nullptr, 0, stream);
     DropoutArgs a{};
     a.x = x;
     a.residual = residual;

@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <cstring>
 #include <exception>
 #include <initializer_list>
 #include <string>
@@ -85,8 +86,9 @@ void check_act(int act) {
     refuse("act is " + std::to_string(act) + ", must be none (-1) or relu .. gelu (0 .. 5)");
 }
 
-struct Shared {  // two matrices of a call that may be the same one
-  const void *a, *b;
+struct Shared {  // the names of two matrices of a call that may be the same one
+  const char *a, *b;
+  bool is(const Mat& x, const Mat& y) const { return std::strcmp(a, x.name) == 0 && std::strcmp(b, y.name) == 0; }
 };
 
 // Alignment of every pointer, and no output over anything else but where
@@ -116,8 +118,7 @@ void check_mats(std::initializer_list<Mat> list, std::initializer_list<Shared> s
       if (!meet(a.p, a.span(), b.p, b.span()) || beside(a, b)) continue;
       bool ok = false;
       for (const Shared& s : same)
-        if (((s.a == a.p && s.b == b.p) || (s.a == b.p && s.b == a.p)) && a.p == b.p && a.ld == b.ld &&
-            a.cols == b.cols && a.bytes == b.bytes)
+        if ((s.is(a, b) || s.is(b, a)) && a.p == b.p && a.ld == b.ld && a.cols == b.cols && a.bytes == b.bytes)
           ok = true;
       if (!ok) refuse(std::string(a.name) + " and " + b.name + " overlap");
     }

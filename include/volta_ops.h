@@ -282,6 +282,40 @@ int32_t volta_op_linear8_forward(const volta_op_linear8* d, const void* x, const
                                  const float* w_scales, const void* bias, const void* residual, void* y,
                                  void* workspace, int64_t workspace_bytes, void* stream);
 
+/* --- update by orthogonalised momentum (Newton-Schulz) ---------------------
+ * Of `batch` matrices u of one shape: X = u / (|u| + eps), |u| the root of the
+ * sum of squares; then `steps` times
+ *   X = a X + (b G + c G^2) X,  G = X X^T,  or, for more rows than columns,
+ *   X = a X + X (b G + c G^2),  G = X^T X,
+ * which moves X's singular values towards 1 and leaves its directions. */
+typedef struct volta_op_muon {
+  int32_t type;  /* of u or the gradient, the result and the weights: F32, BF16, F16 */
+  int32_t steps; /* 1 to 64; 5 is usual */
+  int64_t batch, rows, cols;
+  float a, b, c;    /* 3.4445, -4.7750, 2.0315 are usual */
+  float eps;        /* >= 0 */
+  int64_t ld_u;     /* [batch rows x cols], a matrix after the other: u or the gradient */
+  int64_t ld_m;     /* the momentum */
+  int64_t ld_o;     /* the result, or the weights before and after */
+} volta_op_muon;
+
+int64_t volta_op_muon_workspace(const volta_op_muon* d);
+
+/* o = X.  o may be u (the same pointer and ld).  F32 takes products in float32,
+ * the other types in float16, of X, G and b G + c G^2 in units that follow from
+ * the coefficients (those that let singular values grow past 1024 are refused);
+ * the sum of squares has 64 bits.  A matrix of zeros stays one; a NaN or an
+ * infinity in a matrix makes that matrix's result NaN. */
+int32_t volta_op_muon_orthogonalize(const volta_op_muon* d, const void* u, void* o, void* workspace,
+                                    int64_t workspace_bytes, void* stream);
+
+/* m_out = beta m + g;  u = g + beta m_out, or m_out without `nesterov`;  X from
+ * u as above;  w_out = (1 - lr decay) w - lr scale X.  The momentum is float
+ * whatever the type.  m_out may be m, and w_out may be w. */
+int32_t volta_op_muon_step(const volta_op_muon* d, const void* g, const float* m, const void* w, float* m_out,
+                           void* w_out, float lr, float beta, int32_t nesterov, float decay, float scale,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

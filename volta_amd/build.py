@@ -27,7 +27,7 @@ LIB = os.path.join(PKG, "libvolta_hip.so")
 SOURCES = ["gemm.hip", "skinny.hip", "step_kernels.hip", "extras.hip", "runtime.hip", "test_hooks.hip", "rt_optimizer.hip",
            "rt_graph.hip", "rt_lower.cpp", "spec.cpp", "vt_frontend.cpp", "ops.hip", "ops_rows.hip",
            "ops_gemm_f32.hip", "ops_gemm_bf16.hip", "ops_gemm_f16.hip", "ops_plan.cpp", "ops_loss.hip",
-           "ops_gemm_loss_f32.hip", "ops_gemm_loss_bf16.hip", "ops_gemm_loss_f16.hip", "ops_eight.hip",
+           "ops_gemm_loss_f32.hip", "ops_gemm_loss_bf16.hip", "ops_gemm_loss_f16.hip", "ops_eight.hip", "ops_muon.hip", "ops_gemm_blend.hip",
            "ops_gemm8_f32.hip", "ops_gemm8_bf16.hip", "ops_gemm8_f16.hip"]
 HEADERS = ["gemm.h", "skinny.h", "step_kernels.h", "extras.h", "device_common.h", "recorder.h", "spec.h",
            "narrow_dw.h", "out_head.h", "vt_frontend.h", "rt_lower.h", "ops_types.h", "ops_gemm.h",

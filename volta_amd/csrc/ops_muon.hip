@@ -1,0 +1,370 @@
+// The update by orthogonalised momentum (include/volta_ops.h): entry points,
+// and the passes before the products, which are ops_gemm_kernels.h's OP_BLEND.
+//
+// A step is three dependent products of all matrices of the batch at once: G of
+// X with itself (the smaller side), B = b G + c G^2, and X' = a X + B X (or X B
+// where the matrix is tall); the last one's epilogue writes the result, or the
+// weights.  G and B are symmetric, so the products that take them read their
+// rows where they would need columns.
+//
+// 16-bit types take float16 products.  X's singular values stay in a range that
+// follows from the coefficients, so X, G and B have fixed units that put them
+// under 2^15: all 11 bits, and no element lost that is not 2^-29 of the largest.
+// bfloat16's 8 bits instead leave the result 1.2 % of its norm off (float16:
+// 0.15 %, as much as rounding the result to bfloat16), whatever the size.
+#include "ops_call.h"
+#include "ops_launch.h"
+#include "ops_types.h"
+
+namespace volta {
+namespace ops {
+namespace {
+
+constexpr int kMaxSteps = 64;
+constexpr int64_t kMaxBatch = 65535;  // a grid's third dimension
+
+// ---------------------------------------------------------------------------
+// u and its norm.  Two passes: momentum and the sum of squares (in 64 bits:
+// gradients may be of 1e-25 or 1e25), and X = u / (norm + eps) in its unit, with
+// zeros in what pads it to whole chunks.  Bound by memory; the second pass finds
+// a few ten MB in the memory-side cache.
+// ---------------------------------------------------------------------------
+struct MuonArgs {
+  const void* g;       // u, or the gradient
+  const float* m;      // momentum, or NULL
+  float* m_out;
+  void* x;             // [batch][rows_p][ld_x]
+  double* partial;     // [batch][gridDim.x]
+  int64_t rows, cols;  // of a matrix
+  int64_t rows_p, ld_x, ld_g, ld_m;
+  float beta, eps, unit;
+  int32_t nesterov;
+};
+
+// The sum over the block's 256 threads, on every thread, in a fixed order.
+__device__ __forceinline__ double block_sum(double v, double* lds) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, kWave);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return ((lds[0] + lds[1]) + lds[2]) + lds[3];
+}
+
+// Chunks of E elements are dealt to the blocks of a matrix in turn.
+template <typename T>
+__global__ void __launch_bounds__(256) muon_norm(MuonArgs a) {
+  constexpr int E = 16 / (int)sizeof(T);
+  __shared__ double lds[4];
+  const int64_t per_row = (a.cols + E - 1) / E, chunks = per_row * a.rows, z = blockIdx.y;
+  double ss = 0.0;
+#pragma unroll 2
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per_row, row = z * a.rows + r;
+    const int c = (int)(i - r * per_row) * E, cnt = (int)min((int64_t)E, a.cols - c);
+    float u[E];
+    load_vec(static_cast<const T*>(a.g) + row * a.ld_g + c, cnt, u);
+    if (a.m) {
+      float m[E];
+      load_vec(a.m + row * a.ld_m + c, cnt, m);
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
+        m[k] = a.beta * m[k] + u[k];
+        u[k] = a.nesterov ? u[k] + a.beta * m[k] : m[k];
+      }
+      store_vec(a.m_out + row * a.ld_m + c, cnt, m);
+    }
+#pragma unroll
+    for (int k = 0; k < E; ++k) ss += (double)u[k] * (double)u[k];
+  }
+  ss = block_sum(ss, lds);
+  if (threadIdx.x == 0) a.partial[z * gridDim.x + blockIdx.x] = ss;
+}
+
+// T: of u; X: of the products.
+template <typename T, typename X>
+__global__ void __launch_bounds__(256) muon_scale(MuonArgs a, int parts) {
+  constexpr int E = 16 / (int)sizeof(X);
+  __shared__ double lds[4];
+  const int64_t z = blockIdx.y, per_row = a.ld_x / E, chunks = per_row * a.rows_p;
+  double ss = 0.0;
+  for (int i = threadIdx.x; i < parts; i += 256) ss += a.partial[z * parts + i];
+  ss = block_sum(ss, lds);
+  const double norm = sqrt(ss) + (double)a.eps;
+  const double per = norm == 0.0 ? 0.0 : (double)a.unit / norm;  // zeros stay zeros, without an eps too
+#pragma unroll 2
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per_row, row = z * a.rows + r;
+    const int c = (int)(i - r * per_row) * E;
+    const int cnt = r < a.rows ? (int)min((int64_t)E, a.cols - c) : 0;
+    float u[E];
+    load_vec(static_cast<const T*>(a.g) + (cnt > 0 ? row * a.ld_g + c : 0), cnt, u);
+    if (a.m) {
+      float m[E];
+      load_vec(static_cast<const float*>(a.m_out) + (cnt > 0 ? row * a.ld_m + c : 0), cnt, m);
+#pragma unroll
+      for (int k = 0; k < E; ++k) u[k] = a.nesterov ? u[k] + a.beta * m[k] : m[k];
+    }
+    // what is behind a row's end was read as 0; no norm makes anything else of it
+#pragma unroll
+    for (int k = 0; k < E; ++k) u[k] = k < cnt ? (float)((double)u[k] * per) : 0.0f;
+    store_vec(static_cast<X*>(a.x) + (z * a.rows_p + r) * a.ld_x + c, E, u);
+  }
+}
+
+// Blocks of a matrix in the two passes: about as many as the chip holds.
+int norm_blocks(int64_t batch, int64_t chunks) {
+  const int64_t want = std::max<int64_t>(1, 2048 / batch);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(want, (chunks + 511) / 512));
+}
+
+// ---------------------------------------------------------------------------
+struct Muon {
+  volta_op_muon d;
+  int product;             // type of the products
+  bool tall;
+  int64_t rows_p, cols_p;  // padded to whole chunks: the products run over zeros there
+  int64_t small, large;
+  int parts;
+  double x_unit[kMaxSteps], g_unit[kMaxSteps], b_unit[kMaxSteps];
+  int layout[3];           // of G, B and X'
+  OpPlan plan[3];
+  int64_t x_bytes, g_bytes, sum_bytes, partial_bytes;
+  int64_t bytes() const { return 2 * x_bytes + 2 * g_bytes + sum_bytes + partial_bytes; }
+};
+
+// The largest power of two that keeps `bound` at 2^15 or under.
+double unit_of(double bound) { return std::exp2(15.0 - std::ceil(std::log2(bound))); }
+
+Muon muon_of(const volta_op_muon* in) {
+  need(in, "the description");
+  Muon l{};
+  volta_op_muon& d = l.d;
+  d = *in;
+  check_type(d.type);
+  check_dims("steps", d.steps, 1, kMaxSteps);
+  check_dims("batch", d.batch, 1, kMaxBatch);
+  check_dims("rows", d.rows, 1, kMaxLd);
+  check_dims("cols", d.cols, 1, kMaxLd);
+  if (d.batch * d.rows > kMaxRows) refuse("batch times rows is over 2^30");
+  if (!(d.eps >= 0.0f) || !std::isfinite(d.eps)) refuse("eps is negative or not finite");
+  const double a = d.a, b = d.b, c = d.c;
+  if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) refuse("a coefficient is not finite");
+  d.ld_u = ld_of("ld_u", d.ld_u, d.cols);
+  d.ld_m = ld_of("ld_m", d.ld_m, d.cols);
+  d.ld_o = ld_of("ld_o", d.ld_o, d.cols);
+  l.product = d.type == VOLTA_OP_F32 ? VOLTA_OP_F32 : VOLTA_OP_F16;
+  const int e = elem_bytes(l.product);
+  l.rows_p = packed_ld(l.product, d.rows);
+  l.cols_p = packed_ld(l.product, d.cols);
+  l.tall = d.rows > d.cols;
+  l.small = l.tall ? l.cols_p : l.rows_p;
+  l.large = l.tall ? l.rows_p : l.cols_p;
+  // Singular values before each step are at most r: 1 at first (the sum of
+  // squares of X is at most 1), then the largest |a s + b s^3 + c s^5| on [0, r]
+  // (at the ends and between, by 4096 samples and a margin for what lies
+  // between two).  An element is at most the largest singular value.
+  double r = 1.0;
+  for (int i = 0; i < d.steps; ++i) {
+    double next = 0.0, poly = 0.0;
+    for (int k = 0; k <= 4096; ++k) {
+      const double s = r * k / 4096, q = s * s;
+      next = std::max(next, std::fabs(s * (a + b * q + c * q * q)));
+      poly = std::max(poly, std::fabs(b * q + c * q * q));
+    }
+    if (l.product == VOLTA_OP_F32) {
+      l.x_unit[i] = l.g_unit[i] = l.b_unit[i] = 1.0;
+    } else {
+      if (!(r <= 1024.0 && next <= 1024.0 && poly <= 1e6)) refuse("the coefficients let singular values grow past 1024");
+      l.x_unit[i] = unit_of(r);
+      l.g_unit[i] = unit_of(r * r);
+      l.b_unit[i] = unit_of(std::max(poly, 1e-6));
+    }
+    r = std::max(next * 1.001, 1e-6);
+  }
+  l.layout[0] = l.tall ? OP_TN : OP_NT;
+  l.layout[1] = OP_NT;
+  l.layout[2] = l.tall ? OP_NT : OP_NN;
+  const int64_t M[3] = {l.small, l.small, l.tall ? l.large : l.small};
+  const int64_t N[3] = {l.small, l.small, l.tall ? l.small : l.large};
+  const int64_t K[3] = {l.large, l.small, l.small};
+  for (int i = 0; i < 3; ++i) {
+    l.plan[i] = op_gemm_plan(e, l.layout[i], OP_BLEND, M[i], N[i], K[i], 1, (int)d.batch, true);
+    l.partial_bytes = std::max(l.partial_bytes, align256(op_gemm_partial_bytes(l.plan[i], OP_BLEND, M[i], N[i], (int)d.batch)));
+    if (op_gemm_blocks(l.plan[i], OP_BLEND, M[i], N[i]) > kMaxBlocks) refuse("the rows and columns of a product are too many");
+  }
+  l.x_bytes = align256(d.batch * l.rows_p * l.cols_p * e);
+  l.g_bytes = align256(d.batch * l.small * l.small * e);
+  l.parts = norm_blocks(d.batch, d.rows * ((d.cols + 3) / 4));
+  l.sum_bytes = align256(8 * d.batch * l.parts);
+  return l;
+}
+
+hipError_t passes(const Muon& l, MuonArgs a, hipStream_t st) {
+  const dim3 grid((unsigned)l.parts, (unsigned)l.d.batch);
+  auto run = [&](auto like) {
+    using T = decltype(like);
+    using X = typename std::conditional<sizeof(T) == 4, float, _Float16>::type;
+    const hipError_t e = op_launch(muon_norm<T>, grid, dim3(256), st, a);
+    return e != hipSuccess ? e : op_launch(muon_scale<T, X>, grid, dim3(256), st, a, l.parts);
+  };
+  return l.d.type == VOLTA_OP_F32    ? run(0.0f)
+         : l.d.type == VOLTA_OP_BF16 ? run((__bf16)0.0f)
+                                     : run((_Float16)0.0f);
+}
+
+// The passes and products of a call; `last` says what becomes of the last X:
+// out, w, gamma, and in alpha what it is multiplied by.
+void run(const Muon& l, MuonArgs a, const OpEpilogue& last, char* workspace, hipStream_t st) {
+  const volta_op_muon& d = l.d;
+  char* x[2] = {workspace, workspace + l.x_bytes};
+  char* g = workspace + 2 * l.x_bytes;
+  char* b = g + l.g_bytes;
+  a.partial = reinterpret_cast<double*>(b + l.g_bytes);
+  float* partial = reinterpret_cast<float*>(b + l.g_bytes + l.sum_bytes);
+  a.x = x[0];
+  a.rows = d.rows;
+  a.cols = d.cols;
+  a.rows_p = l.rows_p;
+  a.ld_x = l.cols_p;
+  a.ld_g = d.ld_u;
+  a.ld_m = d.ld_m;
+  a.eps = d.eps;
+  a.unit = (float)l.x_unit[0];
+  check_hip(passes(l, a, st), "norm");
+  const int64_t x_size = l.rows_p * l.cols_p, g_size = l.small * l.small;
+  auto product = [&](int which, const void* p, int64_t ld_p, int64_t stride_p, const void* q, int64_t ld_q,
+                     int64_t stride_q, int64_t M, int64_t N, int64_t K, const OpEpilogue& epi, const char* what) {
+    OpGemm m{};
+    m.p[0] = m.p[1] = p;
+    m.q[0] = m.q[1] = q;
+    m.ld_p = ld_p;
+    m.ld_q = ld_q;
+    m.stride_p = stride_p;
+    m.stride_q = stride_q;
+    m.M = (int32_t)M;
+    m.N = (int32_t)N;
+    m.K = (int32_t)K;
+    m.pieces = 1;
+    m.outputs = (int32_t)d.batch;
+    m.direct = 1;
+    m.partial = partial;
+    m.epi = epi;
+    check_hip(op_gemm_blend(l.product, l.layout[which], l.plan[which], m, st), what);
+  };
+  for (int i = 0; i < d.steps; ++i) {
+    const char* from = x[i & 1];
+    const bool end = i == d.steps - 1;
+    const double ux = l.x_unit[i], ug = l.g_unit[i], ub = l.b_unit[i];
+    OpEpilogue o{};
+    o.out[0] = g;
+    o.out_type = l.product;
+    o.ld_out = l.small;
+    o.stride_out = g_size;
+    o.alpha = (float)(ug / (ux * ux));
+    product(0, from, l.cols_p, x_size, from, l.cols_p, x_size, l.small, l.small, l.large, o, "gram");
+    o.out[0] = b;
+    o.alpha = (float)(d.c * ub / (ug * ug));
+    o.beta = (float)(d.b * ub / ug);
+    o.blend = g;
+    o.ld_blend = l.small;
+    o.stride_blend = g_size;
+    product(1, g, l.small, g_size, g, l.small, g_size, l.small, l.small, l.small, o, "polynomial");
+    // X' in the next step's unit, or the result
+    const double to = end ? (double)last.alpha : l.x_unit[i + 1];
+    OpEpilogue n{};
+    if (end) n = last;
+    n.alpha = (float)(to / (ub * ux));
+    n.beta = (float)(to * d.a / ux);
+    n.blend = from;
+    n.ld_blend = l.cols_p;
+    n.stride_blend = x_size;
+    if (!end) {
+      n.out[0] = x[(i + 1) & 1];
+      n.out_type = l.product;
+      n.ld_out = l.cols_p;
+      n.stride_out = x_size;
+    }
+    const int64_t M = end ? d.rows : l.rows_p, N = end ? d.cols : l.cols_p;
+    if (l.tall) product(2, from, l.cols_p, x_size, b, l.small, g_size, M, N, l.small, n, "step");
+    else product(2, b, l.small, g_size, from, l.cols_p, x_size, M, N, l.small, n, "step");
+  }
+}
+
+}  // namespace
+}  // namespace ops
+}  // namespace volta
+
+using namespace volta;
+using namespace volta::ops;
+
+extern "C" {
+
+int64_t volta_op_muon_workspace(const volta_op_muon* d) {
+  return bytes_of("volta_op_muon_workspace", VOLTA_OP_FORWARD, [&](bool) { return muon_of(d).bytes(); });
+}
+
+int32_t volta_op_muon_orthogonalize(const volta_op_muon* in, const void* u, void* o, void* workspace,
+                                    int64_t workspace_bytes, void* stream) {
+  return guarded("volta_op_muon_orthogonalize", [&] {
+    const Muon l = muon_of(in);
+    const volta_op_muon& d = l.d;
+    const int e = elem_bytes(d.type);
+    need(u, "u");
+    need(o, "o");
+    check_workspace(workspace, workspace_bytes, l.bytes());
+    const hipStream_t st = check_call({{"u", u, d.batch * d.rows, d.cols, d.ld_u, e, false},
+                                       {"o", o, d.batch * d.rows, d.cols, d.ld_o, e, true}},
+                                      {{"u", "o"}}, workspace, l.bytes(), stream);
+    MuonArgs a{};
+    a.g = u;
+    OpEpilogue last{};
+    last.out[0] = o;
+    last.out_type = d.type;
+    last.ld_out = d.ld_o;
+    last.stride_out = d.rows * d.ld_o;
+    last.alpha = 1.0f;
+    run(l, a, last, static_cast<char*>(workspace), st);
+  });
+}
+
+int32_t volta_op_muon_step(const volta_op_muon* in, const void* g, const float* m, const void* w, float* m_out,
+                           void* w_out, float lr, float beta, int32_t nesterov, float decay, float scale,
+                           void* workspace, int64_t workspace_bytes, void* stream) {
+  return guarded("volta_op_muon_step", [&] {
+    const Muon l = muon_of(in);
+    const volta_op_muon& d = l.d;
+    const int e = elem_bytes(d.type);
+    need(g, "g");
+    need(m, "m");
+    need(w, "w");
+    need(m_out, "m_out");
+    need(w_out, "w_out");
+    for (float v : {lr, beta, decay, scale})
+      if (!std::isfinite(v)) refuse("lr, beta, decay or scale is not finite");
+    check_workspace(workspace, workspace_bytes, l.bytes());
+    const int64_t rows = d.batch * d.rows;
+    const hipStream_t st = check_call({{"g", g, rows, d.cols, d.ld_u, e, false},
+                                       {"m", m, rows, d.cols, d.ld_m, 4, false},
+                                       {"w", w, rows, d.cols, d.ld_o, e, false},
+                                       {"m_out", m_out, rows, d.cols, d.ld_m, 4, true},
+                                       {"w_out", w_out, rows, d.cols, d.ld_o, e, true}},
+                                      {{"m", "m_out"}, {"w", "w_out"}}, workspace, l.bytes(), stream);
+    MuonArgs a{};
+    a.g = g;
+    a.m = m;
+    a.m_out = m_out;
+    a.beta = beta;
+    a.nesterov = nesterov != 0;
+    OpEpilogue last{};
+    last.out[0] = w_out;
+    last.out_type = d.type;
+    last.ld_out = last.ld_w = d.ld_o;
+    last.stride_out = last.stride_w = d.rows * d.ld_o;
+    last.w = w;
+    last.alpha = -(lr * scale);
+    last.gamma = 1.0f - lr * decay;
+    run(l, a, last, static_cast<char*>(workspace), st);
+  });
+}
+
+}  // extern "C"

@@ -358,6 +358,52 @@ int32_t volta_hip_op_product8(int32_t type, int32_t tile, int32_t splits, int32_
   return rc == hipSuccess ? 0 : -1;
 }
 
+// out = alpha P Q + beta r of `batch` matrices on a given tile and number of
+// splits (OP_BLEND), in float32 (0) or float16 (2), synchronously.  All packed,
+// rows of whole 16-byte chunks, a matrix behind the other.
+int32_t volta_hip_op_blend(int32_t type, int32_t layout, int32_t tile, int32_t splits, int32_t batch, const void* p,
+                           const void* q, const void* r, void* out, int32_t M, int32_t N, int32_t K, float alpha,
+                           float beta) {
+  using namespace volta::ops;
+  const int e = type == VOLTA_OP_F32 ? 4 : 2, per_chunk = 16 / e;
+  if ((type != VOLTA_OP_F32 && type != VOLTA_OP_F16) || M < 1 || N < 1 || K < 1 || batch < 1 || splits < 1) return -1;
+  if (M % per_chunk || N % per_chunk || K % per_chunk || tile < OP_TILE_256 || tile > OP_TILE_64) return -1;
+  for (const void* x : {p, q})
+    if ((uintptr_t)x % 16) return -1;
+  const int stages = (K + op_stage_k(e) - 1) / op_stage_k(e);
+  OpPlan plan{tile, 1, stages, 0.0};
+  plan.stages_per_split = (stages + splits - 1) / splits;
+  plan.splits = (stages + plan.stages_per_split - 1) / plan.stages_per_split;
+  const int64_t bytes = op_gemm_partial_bytes(plan, OP_BLEND, M, N, batch);
+  void* ws = nullptr;
+  if (bytes && hipMalloc(&ws, bytes) != hipSuccess) return -1;
+  OpGemm g{};
+  g.p[0] = g.p[1] = p;
+  g.q[0] = g.q[1] = q;
+  g.ld_p = layout == OP_TN ? M : K;
+  g.ld_q = layout == OP_NT ? K : N;
+  g.stride_p = (int64_t)M * K;
+  g.stride_q = (int64_t)N * K;
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.pieces = 1;
+  g.outputs = batch;
+  g.direct = 1;
+  g.partial = static_cast<float*>(ws);
+  g.epi.blend = r;
+  g.epi.ld_blend = g.epi.ld_out = N;
+  g.epi.stride_blend = g.epi.stride_out = (int64_t)M * N;
+  g.epi.out[0] = out;
+  g.epi.out_type = type;
+  g.epi.alpha = alpha;
+  g.epi.beta = beta;
+  hipError_t rc = op_gemm_blend(type, layout, plan, g, nullptr);
+  if (rc == hipSuccess) rc = hipStreamSynchronize(nullptr);
+  if (ws) (void)hipFree(ws);
+  return rc == hipSuccess ? 0 : -1;
+}
+
 // The plan of such a product: {tile, splits, stages of a split}.
 void volta_hip_op_plan(int32_t elem_bytes, int32_t layout, int32_t kind, int64_t M, int64_t N, int64_t K,
                        int32_t pieces, int32_t outputs, int32_t direct, int32_t* plan) {

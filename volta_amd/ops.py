@@ -67,6 +67,11 @@ class Linear8Desc(C.Structure):
         (n, C.c_int64) for n in ("ld_x", "ld_w", "ld_y", "ld_residual")]
 
 
+class MuonDesc(C.Structure):
+    _fields_ = [("type", C.c_int32), ("steps", C.c_int32)] + [(n, C.c_int64) for n in ("batch", "rows", "cols")] + [
+        (n, C.c_float) for n in ("a", "b", "c", "eps")] + [(n, C.c_int64) for n in ("ld_u", "ld_m", "ld_o")]
+
+
 class DropoutDesc(C.Structure):
     _fields_ = [("type", C.c_int32), ("p", C.c_double)] + [
         (n, C.c_int64) for n in ("rows", "cols", "ld_x", "ld_residual", "ld_y")]
@@ -88,6 +93,10 @@ SIGNATURES = {
     "volta_op_quantize_forward": (C.c_int32, [C.POINTER(QuantizeDesc), _P, _P, _P, _P]),
     "volta_op_linear8_workspace": (_N, [C.POINTER(Linear8Desc)]),
     "volta_op_linear8_forward": (C.c_int32, [C.POINTER(Linear8Desc)] + [_P] * 8 + [_N, _P]),
+    "volta_op_muon_workspace": (_N, [C.POINTER(MuonDesc)]),
+    "volta_op_muon_orthogonalize": (C.c_int32, [C.POINTER(MuonDesc)] + [_P] * 3 + [_N, _P]),
+    "volta_op_muon_step": (C.c_int32, [C.POINTER(MuonDesc)] + [_P] * 5 + [C.c_float, C.c_float, C.c_int32, C.c_float,
+                                                                          C.c_float, _P, _N, _P]),
     "volta_op_cross_entropy_workspace": (_N, [C.POINTER(CrossEntropyDesc), C.c_int32]),
     "volta_op_cross_entropy_forward": (C.c_int32, [C.POINTER(CrossEntropyDesc)] + [_P] * 7 + [_N, _P]),
     "volta_op_cross_entropy_backward": (C.c_int32, [C.POINTER(CrossEntropyDesc)] + [_P] * 10 + [_N, _P]),
@@ -432,6 +441,48 @@ class Linear8(_Operator):
         ax, asx, aw, asw, ab, ar, ay = self._of_forward
         if self._forward(self._d, ax(x), asx(x_scales), aw(w), asw(w_scales), ab(bias), ar(residual), ay(y),
                          _address(workspace), _bytes(workspace), stream):
+            raise self._refused()
+
+    def workspace_bytes(self) -> int:
+        """Bytes of workspace that a call needs."""
+        n = self._fn("workspace")(self._d)
+        if n < 0:
+            raise self._refused()
+        return int(n)
+
+
+class Muon(_Operator):
+    """The update by orthogonalised momentum, of `batch` matrices [rows x cols]
+    one after the other: X = u / (|u| + eps), `steps` times X = a X + (b G + c
+    G^2) X with G = X X^T (of the smaller side), coefficients = (a, b, c)."""
+
+    def __init__(self, rows, cols, dtype="f32", batch=1, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7,
+                 ld_u=0, ld_m=0, ld_o=0, lib=None):
+        t = TYPES[dtype]
+        super().__init__(MuonDesc(t, steps, batch, rows, cols, *coefficients, eps, ld_u, ld_m, ld_o), "muon", lib)
+        self._orthogonalize, self._step = self._fn("orthogonalize"), self._fn("step")
+        f32, n = TYPES["f32"], batch * rows
+        self._of_orthogonalize = (_matrix("u", t, n, cols, ld_u), _matrix("o", t, n, cols, ld_o))
+        self._of_step = (_matrix("w", t, n, cols, ld_o), _matrix("g", t, n, cols, ld_u),
+                         _matrix("momentum", f32, n, cols, ld_m), _matrix("w_out", t, n, cols, ld_o),
+                         _matrix("momentum_out", f32, n, cols, ld_m))
+
+    def orthogonalize(self, u, o, workspace=None, stream=0):
+        """o = X of u; o may be u."""
+        au, ao = self._of_orthogonalize
+        if self._orthogonalize(self._d, au(u), ao(o), _address(workspace), _bytes(workspace), stream):
+            raise self._refused()
+
+    def step(self, w, g, momentum, lr, beta=0.95, nesterov=True, decay=0.0, scale=1.0, w_out=None, momentum_out=None,
+             workspace=None, stream=0):
+        """momentum = beta momentum + g; u = g + beta momentum (nesterov) or
+        the momentum; w = (1 - lr decay) w - lr scale X of u.  In place, or to
+        w_out and momentum_out."""
+        aw, ag, am, awo, amo = self._of_step
+        w, momentum = aw(w), am(momentum)
+        if self._step(self._d, ag(g), momentum, w, momentum if momentum_out is None else amo(momentum_out),
+                      w if w_out is None else awo(w_out), lr, beta, bool(nesterov), decay, scale, _address(workspace),
+                      _bytes(workspace), stream):
             raise self._refused()
 
     def workspace_bytes(self) -> int:

@@ -91,17 +91,42 @@ def test_products_on_every_tile(lib, t):
         P, Q, r = whole(rng, batch, M, K), whole(rng, batch, K, N), whole(rng, batch, M, N)
         want = 0.5 * (P @ Q) - 2 * r
         mr = Mat(lib, t, batch * M, N, r.reshape(-1, N))
-        for layout in (0, 1, 2):
-            p, q = (P.swapaxes(1, 2) if layout == 2 else P), (Q.swapaxes(1, 2) if layout == 1 else Q)
-            mp = Mat(lib, t, batch * p.shape[1], p.shape[2], p.reshape(-1, p.shape[2]))
+        for layout in (0, 1):
+            q = Q.swapaxes(1, 2) if layout == 1 else Q
+            mp = Mat(lib, t, batch * M, K, P.reshape(-1, K))
             mq = Mat(lib, t, batch * q.shape[1], q.shape[2], q.reshape(-1, q.shape[2]))
             for tile in range(5):
                 for splits in (1, 3):
                     say(t, "batch", batch, M, N, K, "layout", layout, "tile", tile, "splits", splits)
                     out = Mat(lib, t, batch * M, N)
-                    assert lib.lib.volta_hip_op_blend(R.TYPES.index(t), layout, tile, splits, batch, C.c_void_p(mp.ptr),
-                                                      C.c_void_p(mq.ptr), C.c_void_p(mr.ptr), C.c_void_p(out.ptr), M, N, K,
-                                                      C.c_float(0.5), C.c_float(-2.0)) == 0
+                    assert _blend(lib, t, layout, 6, tile, splits, batch, mp, mq, mr, out, M, N, K) == 0
+                    assert np.array_equal(out.get().reshape(want.shape), want)
+
+
+def _blend(lib, t, layout, kind, tile, splits, batch, p, q, r, out, M, N, K):
+    return lib.lib.volta_hip_op_blend(R.TYPES.index(t), layout, kind, tile, splits, batch, C.c_void_p(p.ptr),
+                                      C.c_void_p(q.ptr), C.c_void_p(r.ptr), C.c_void_p(out.ptr), M, N, K, C.c_float(0.5),
+                                      C.c_float(-2.0))
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+def test_symmetric_products_on_every_tile(lib, t):
+    """Of X X^T: half of the tiles computed, all stored, exactly."""
+    for n, (batch, M, K) in enumerate([(1, 8, 8), (3, 72, 40), (2, 136, 264), (5, 8, 200), (1, 520, 136), (2, 304, 72),
+                                       (1, 1096, 24)]):
+        rng = np.random.default_rng(n)
+        X, r = whole(rng, batch, M, K), whole(rng, batch, M, M)
+        r = r + r.swapaxes(1, 2)
+        want = 0.5 * (X @ X.swapaxes(1, 2)) - 2 * r
+        mr = Mat(lib, t, batch * M, M, r.reshape(-1, M))
+        for layout in (1, 2):
+            x = X if layout == 1 else X.swapaxes(1, 2)
+            mx = Mat(lib, t, batch * x.shape[1], x.shape[2], x.reshape(-1, x.shape[2]))
+            for tile in (0, 2, 4):
+                for splits in (1, 3):
+                    say(t, "batch", batch, M, K, "layout", layout, "tile", tile, "splits", splits)
+                    out = Mat(lib, t, batch * M, M)
+                    assert _blend(lib, t, layout, 7, tile, splits, batch, mx, mx, mr, out, M, M, K) == 0
                     assert np.array_equal(out.get().reshape(want.shape), want)
 
 
@@ -139,7 +164,9 @@ def test_orthogonalize(lib, t, style):
 @pytest.mark.parametrize("t", TYPES)
 def test_larger(lib, t):
     """Sizes whose products take the larger tiles and split sums."""
-    for k, (batch, m, n) in enumerate([(1, 512, 2000), (2, 1100, 520), (1, 72, 9000), (1, 5000, 96)]):
+    # the last two take two steps at once, wide and tall
+    for k, (batch, m, n) in enumerate([(1, 512, 2000), (2, 1100, 520), (1, 72, 9000), (1, 5000, 96), (16, 384, 1500),
+                                       (20, 1400, 330)]):
         rng = np.random.default_rng(50 + k)
         say(t, batch, m, n)
         v = R.unpack(R.pack(gradients(rng, batch, m, n), t), t)
@@ -149,8 +176,9 @@ def test_larger(lib, t):
         op.orthogonalize(u, o, workspace=ws)
         got = o.get().reshape(batch, m, n)
         for z in range(batch):
-            want = iterate(v[z])
-            assert np.linalg.norm(got[z] - want) <= allowed(t, v[z], want), z
+            if z % 9 == 0 or batch < 16:
+                want = iterate(v[z])
+                assert np.linalg.norm(got[z] - want) <= allowed(t, v[z], want), z
         ws.check()
 
 

@@ -25,8 +25,10 @@ enum OpKind {
   OP_STATS = 3,      // of a row's z: their largest, the sum of their exponentials, the one at the row's label
   OP_LOSS_GRAD = 4,  // (exp(z - lse) - [the label's]) dloss
   OP_ADD = 5,        // sums of several launches, in order, in 32 bits
-  OP_BLEND = 6       // alpha d + beta r + gamma w, of several matrices (blockIdx.z)
+  OP_BLEND = 6,      // alpha d + beta r + gamma w, of several matrices (blockIdx.z)
+  OP_MIRROR = 7      // the same of a symmetric D and r: the tiles on and over the diagonal, stored twice
 };
+constexpr bool op_kind_blend(int kind) { return kind == OP_BLEND || kind == OP_MIRROR; }
 constexpr bool op_kind_layer(int kind) { return kind == OP_LINEAR || kind == OP_GATED; }
 
 struct OpEpilogue {
@@ -56,6 +58,7 @@ struct OpEpilogue {
   // OP_BLEND; matrix z starts z strides behind the first
   const void *blend, *w;  // r of the products' type, w of out's (NULL: none)
   float alpha, beta, gamma;
+  float diagonal;         // OP_MIRROR: added where the row is the column
   int32_t out_type;       // enum volta_op_type; also of a product of codes
   int64_t ld_blend, ld_w, stride_blend, stride_w, stride_out;
 };
@@ -119,11 +122,12 @@ int64_t op_gemm_blocks(const OpPlan& plan, int kind, int64_t M, int64_t N);
 hipError_t op_gemm_f32(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
 hipError_t op_gemm_bf16(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
 hipError_t op_gemm_f16(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
-// The kinds of an output layer's loss; and OP_BLEND, in float32 and float16.
+// The kinds of an output layer's loss; and OP_BLEND and OP_MIRROR, in float32
+// and float16.
 hipError_t op_gemm_loss_f32(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
 hipError_t op_gemm_loss_bf16(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
 hipError_t op_gemm_loss_f16(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
-hipError_t op_gemm_blend(int type, int layout, const OpPlan& plan, OpGemm g, hipStream_t st);
+hipError_t op_gemm_blend(int type, int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
 
 // Products of e4m3 codes (OP_NT, OP_LINEAR), by the type of bias, residual and
 // result.

@@ -149,9 +149,8 @@ __global__ void __launch_bounds__(512) op_gemm8_middle(OpGemm g) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WGN, wn = wave % WGN;
-  int tm, tn;
-  op_tile_of(blockIdx.x, g.tiles_m, g.tiles_n, &tm, &tn);
-  const int m0 = tm * BM, n0 = tn * BN, split = blockIdx.y;
+  const OpPlace place = op_place<true, false>(g);
+  const int m0 = place.tm * BM, n0 = place.tn * BN, split = place.split;
   PT pt;
   QT qt;
   pt.init(g.ld_p, g.M - m0, wave, lane);
@@ -258,6 +257,155 @@ __global__ void __launch_bounds__(512) op_gemm8_middle(OpGemm g) {
 }
 
 // ---------------------------------------------------------------------------
+// Large product of codes: 256x256 of D per block, in the regions, phases and
+// order of loads of op_gemm_large.  A stage is one block of k: two phases of 16
+// matrix instructions of 32 cycles, and the 64 FMAs that scale a phase's sums.
+// K is whole blocks: the code for a last part of one takes registers that the
+// loop then spills.  The rows' 256 scales are a fifth load of
+// the stage's first half, read with P0 before that half's place is loaded
+// again.
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) op_gemm8_large(OpGemm g) {
+  constexpr int kRegion = 128 * 128, kScales = 8 * kRegion;
+  using PR = Region<uint8_t, true, 64, 128>;
+  using QR = Region<uint8_t, true, 32, 64>;
+  static_assert(PR::kBytes == kRegion && PR::kLoads == 2, "two loads a wave and region");
+  __shared__ __attribute__((aligned(16))) char lds[kScales + 2 * 1024];  // [stage & 1][P0, P1, Q0, Q1], [stage & 1][256]
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 2, wn = wave & 3;
+  const OpPlace place = op_place<true, false>(g);
+  const int m0 = place.tm * 256, n0 = place.tn * 256, split = place.split;
+  PR pr[2];
+  QR qr[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    pr[h].init(g.ld_p, h * 64, g.M - m0, wave, lane);
+    qr[h].init(g.ld_q, h * 32, g.N - n0, wave, lane);
+    // opaque, or each is kept with the upper half of the product it comes from
+#pragma unroll
+    for (int i = 0; i < 2; ++i) asm volatile("" : "+v"(pr[h].off[i]), "+v"(qr[h].off[i]));
+  }
+  // every wave loads 64 rows' scales; the two that load the same rows write the same values
+  RowScales sx;
+  sx.init(g, m0, (wave & 3) * 64 + lane);
+  ColumnScales sw;
+  sw.init(g, n0 + wn * 64);
+  const int s_begin = split * g.stages_per_split;
+  const int S = min((g.K + 127) / 128, s_begin + g.stages_per_split) - s_begin;
+  Cursor8 next[2];  // the halves are loaded in different phases
+  next[0].init(g, m0, n0, 0, s_begin, 1);
+  next[1].init(g, m0, n0, 0, s_begin, 1);
+  const uint32_t lds_byte = op_lds_byte(lds);
+  auto load = [&](int to, auto half) {
+    constexpr int h = decltype(half)::value;
+    if constexpr (h == 0) op_load_lds4(sx.of(next[0].k >> 7), lds_byte + kScales + (to ? 1024 : 0) + (wave & 3) * 256);
+    qr[h].issue(next[h].q[0], lds_byte + to + (2 + h) * kRegion, wave);
+    pr[h].issue(next[h].p, lds_byte + to + h * kRegion, wave);
+    next[h].step();
+  };
+  floatx4 acc[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  Frag8 fp[4], fq[4];
+  float sc[8];
+  auto read_p = [&](const char* from) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) fp[i] = frag8<PR>(from, wm * 64 + i * 16, lane);
+  };
+  auto read_q = [&](const char* from, int h) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) fq[2 * h + j] = frag8<QR>(from, wn * 32 + j * 16, lane);
+  };
+  // Blocks (half 4 + i, j) of the phase, j in twos so that Q1 is not needed at
+  // once.  A block's sums are scaled kLate instructions behind its own, in an
+  // order that the compiler keeps: its own would wait for each of them.
+  auto mul = [&](int half) {
+    constexpr int kLate = 3;
+    floatx4 t[kLate + 1];
+#pragma unroll
+    for (int n = 0; n < 16 + kLate; ++n) {
+      if (n < 16) t[n % (kLate + 1)] = mfma8(fq[(n & 1) + (n >> 3) * 2], fp[(n >> 1) & 3]);
+      if (n >= kLate) {
+        const int o = n - kLate, i = half * 4 + ((o >> 1) & 3), j = (o & 1) + (o >> 3) * 2;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(t[o % (kLate + 1)][r], sc[i], acc[i][j][r]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  constexpr auto H0 = std::integral_constant<int, 0>();
+  constexpr auto H1 = std::integral_constant<int, 1>();
+  int from = 0;  // byte of the stage in LDS
+  float w_scale = sw.of(s_begin);
+  auto stage = [&](int s, auto behind) {
+    constexpr int left = decltype(behind)::value;  // stages behind this one: 0, 1, or more
+    const char* at = lds + from;
+    const float w_next = sw.of(s_begin + s + 1);
+    read_q(at + 2 * kRegion, 0);
+    read_p(at);
+    const float* scales = reinterpret_cast<const float*>(lds + kScales + (from ? 1024 : 0));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sc[i] = scales[wm * 128 + i * 16 + (lane & 15)];
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (left >= 1) {
+      load(from ^ 4 * kRegion, H1);
+      op_wait_loads<9>();  // P1 of s is there
+    } else {
+      op_wait_loads<0>();
+    }
+    op_wait_lds();
+    op_barrier();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sc[i] *= w_scale;
+    w_scale = w_next;
+    read_q(at + 3 * kRegion, 1);  // arrives while Q0 is multiplied
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+    mul(0);
+    __builtin_amdgcn_s_setprio(0);
+    op_barrier();
+    read_p(at + kRegion);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (left >= 2) {
+      load(from, H0);
+      op_wait_loads<7>();  // P0, Q0, Q1 and the scales of s + 1 are there
+    } else {
+      op_wait_loads<2>();
+    }
+    from ^= 4 * kRegion;
+    op_wait_lds();
+    op_barrier();
+    __builtin_amdgcn_s_setprio(1);
+    mul(1);
+    __builtin_amdgcn_s_setprio(0);
+    op_barrier();
+  };
+  load(0, H0);
+  load(0, H1);
+  if (S > 1) {
+    load(4 * kRegion, H0);
+    op_wait_loads<7>();  // P0, Q0, Q1 and the scales of the first stage are there
+  } else {
+    op_wait_loads<2>();
+  }
+  op_barrier();
+  if (wm == 1) op_barrier();
+  int s = 0;
+  for (; s < S - 2; ++s) stage(s, std::integral_constant<int, 2>());
+  if (s < S - 1) stage(s++, std::integral_constant<int, 1>());
+  stage(s, std::integral_constant<int, 0>());
+  if (wm == 0) op_barrier();
+  __syncthreads();  // the regions are free
+  static_assert(8 * op_region_bytes<8, 4> <= 8 * kRegion, "output regions fit");
+  op_write_out<T, OP_LINEAR>(g, acc, lds + wave * op_region_bytes<8, 4>, lane, m0 + wm * 128, n0 + wn * 64, 0, split);
+}
+
+// ---------------------------------------------------------------------------
 // The same through registers, for rows that direct loads cannot take
 // (op_gemm_staged).
 // ---------------------------------------------------------------------------
@@ -272,9 +420,8 @@ __global__ void __launch_bounds__(256) op_gemm8_staged(OpGemm g) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 1, wn = wave & 1;
-  int tm, tn;
-  op_tile_of(blockIdx.x, g.tiles_m, g.tiles_n, &tm, &tn);
-  const int m0 = tm * BM, n0 = tn * BN, split = blockIdx.y;
+  const OpPlace place = op_place<true, false>(g);
+  const int m0 = place.tm * BM, n0 = place.tn * BN, split = place.split;
   const int p_left = g.M - m0, q_left = g.N - n0;
   PT pt;
   QT qt;
@@ -351,9 +498,8 @@ __global__ void __launch_bounds__(NW * 64) op_gemm8_skinny(OpGemm g) {
 
   const int tid = threadIdx.x, lane = tid & 63, l = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int tm, tn;
-  op_tile_of(blockIdx.x, g.tiles_m, g.tiles_n, &tm, &tn);
-  const int m0 = tm * (16 * MT), n0 = tn * BN, split = blockIdx.y, p_left = g.M - m0, q_left = g.N - n0;
+  const OpPlace place = op_place<true, false>(g);
+  const int m0 = place.tm * (16 * MT), n0 = place.tn * BN, split = place.split, p_left = g.M - m0, q_left = g.N - n0;
   PT pt;
   QT qt;
   pt.init(g.ld_p, p_left, 0, lane);
@@ -481,13 +627,19 @@ hipError_t launch8_middle(OpGemm& g, hipStream_t st) {
   g.tiles_m = (g.M + BM - 1) / BM;
   g.tiles_n = (g.N + BN - 1) / BN;
   return op_launch(op_gemm8_middle<T, BM, BN, WGM, WGN, KS, NST>,
-                   dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits), dim3(512), st, g);
+                   op_grid<true, false>(g), dim3(512), st, g);
+}
+template <typename T>
+hipError_t launch8_large(OpGemm& g, hipStream_t st) {
+  g.tiles_m = (g.M + 255) / 256;
+  g.tiles_n = (g.N + 255) / 256;
+  return op_launch(op_gemm8_large<T>, op_grid<true, false>(g), dim3(512), st, g);
 }
 template <typename T, int BM, int BN>
 hipError_t launch8_staged(OpGemm& g, hipStream_t st) {
   g.tiles_m = (g.M + BM - 1) / BM;
   g.tiles_n = (g.N + BN - 1) / BN;
-  return op_launch(op_gemm8_staged<T, BM, BN>, dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits), dim3(256),
+  return op_launch(op_gemm8_staged<T, BM, BN>, op_grid<true, false>(g), dim3(256),
                    st, g);
 }
 template <typename T, int MT, bool DIRECT>
@@ -496,7 +648,7 @@ hipError_t launch8_skinny(OpGemm& g, hipStream_t st) {
   g.tiles_m = (g.M + 16 * MT - 1) / (16 * MT);
   g.tiles_n = (g.N + S::kCols - 1) / S::kCols;
   return op_launch(op_gemm8_skinny<T, MT, S::kWaves, S::kStages, DIRECT>,
-                   dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits), dim3(S::kWaves * 64), st, g);
+                   op_grid<true, false>(g), dim3(S::kWaves * 64), st, g);
 }
 
 template <typename T>
@@ -521,8 +673,13 @@ hipError_t launch8(const OpPlan& plan, OpGemm& g, hipStream_t st) {
       if (g.direct) e = launch8_middle<T, 256, 128, 4, 2, 1, 3>(g, st);
       break;
     default:  // float32's fragments take more registers than that tile has
-      if (g.direct && sizeof(T) == 4) e = launch8_middle<T, 256, 128, 4, 2, 1, 3>(g, st);
-      else if constexpr (sizeof(T) < 4) e = g.direct ? launch8_middle<T, 256, 256, 2, 4, 1, 2>(g, st) : e;
+      if constexpr (sizeof(T) < 4) {
+        if (g.direct && g.K % 128 == 0) {
+          e = launch8_large<T>(g, st);
+          break;
+        }
+      }
+      if (g.direct) e = launch8_middle<T, 256, 128, 4, 2, 1, 3>(g, st);
   }
   if (e != hipSuccess || g.splits <= 1) return e;
   const int64_t quads = (int64_t)g.M * ((g.N + 3) / 4);

@@ -281,11 +281,14 @@ __device__ __forceinline__ void op_epilogue(const OpEpilogue& e, int z, int64_t 
     }
     return;
   }
-  if constexpr (KIND == OP_BLEND) {
+  if constexpr (op_kind_blend(KIND)) {
     float r[V];
     if (e.blend) load_vec(static_cast<const T*>(e.blend) + z * e.stride_blend + m * e.ld_blend + n, cnt, r);
 #pragma unroll
-    for (int i = 0; i < V; ++i) d0[i] = e.blend ? e.alpha * d0[i] + e.beta * r[i] : e.alpha * d0[i];
+    for (int i = 0; i < V; ++i) {
+      d0[i] = e.blend ? e.alpha * d0[i] + e.beta * r[i] : e.alpha * d0[i];
+      if (KIND == OP_MIRROR && m == n + i) d0[i] += e.diagonal;
+    }
     op_blend_out(e, z, m, n, cnt, d0);
     return;
   }
@@ -448,13 +451,15 @@ template <int TM, int TN>
 constexpr int op_out_rows = TM % 2 == 0 ? 32 : 16;
 template <int TM, int TN>
 constexpr int op_region_bytes = op_out_rows<TM, TN> * (TN * 16 + 4) * 4;
+// `mirror`: OP_MIRROR's tile is over the diagonal, and also stored across it, by
+// lanes that take 16 bytes down a column of the region.
 template <typename T, int KIND, int TM, int TN>
 __device__ __forceinline__ void op_write_out(const OpGemm& g, floatx4 (&acc)[TM][TN], char* region, int lane, int m0,
-                                             int n0, int z, int split) {
+                                             int n0, int z, int split, bool mirror = false) {
   constexpr bool kGated = KIND == OP_GATED;
   constexpr int kRows = op_out_rows<TM, TN>, RB = kRows / 16, kLd = TN * 16 + 4;
   constexpr int kCols = kGated ? TN * 8 : TN * 16, kE = 16 / (int)sizeof(T);  // columns of D
-  constexpr bool kFew = KIND == OP_STORE || KIND == OP_ADD || KIND == OP_BLEND || (!kGated && sizeof(T) == 4);
+  constexpr bool kFew = KIND == OP_STORE || KIND == OP_ADD || op_kind_blend(KIND) || (!kGated && sizeof(T) == 4);
   constexpr int V = kFew ? kE : kCols / 4;  // of them a lane's
   constexpr int kLanes = kCols / V, kTurn = 64 / kLanes;  // lanes of a row, rows of a turn
   static_assert(kRows % kTurn == 0, "whole turns");
@@ -507,6 +512,23 @@ __device__ __forceinline__ void op_write_out(const OpGemm& g, floatx4 (&acc)[TM]
         op_epilogue<T, KIND>(g.epi, z, m, n, cnt, d0, d1, b0, b1);
       }
     }
+    if constexpr (KIND == OP_MIRROR) {
+      if (!mirror) continue;
+      constexpr int kDown = kRows / kE, kAcross = 64 / kDown;  // lanes down a column, columns of a turn
+#pragma unroll
+      for (int c0 = 0; c0 < kCols; c0 += kAcross) {
+        const int down = lane / kAcross * kE, m = m0 + ph * kRows + down, left = g.M - m;
+        const int c = c0 + lane % kAcross;
+        float d[kE], none[kE];
+#pragma unroll
+        for (int i = 0; i < kE; ++i) d[i] = lds[(down + i) * kLd + c];
+        if (left <= 0 || n0 + c >= g.N) continue;
+        if (g.splits > 1)
+          store_vec(g.partial + ((split * (int64_t)g.outputs + z) * g.M + n0 + c) * (int64_t)g.N + m, left, d);
+        else
+          op_epilogue<T, KIND>(g.epi, z, n0 + c, m, left, d, none, none, none);
+      }
+    }
   }
 }
 
@@ -532,7 +554,7 @@ struct Cursor {
   int piece, m0, n0, z;
 
   __device__ __forceinline__ void place(const OpGemm& g) {
-    if constexpr (KIND == OP_BLEND) {
+    if constexpr (op_kind_blend(KIND)) {
       p = op_stage_base<T, P_KC>(static_cast<const T*>(g.p[0]) + z * g.stride_p, g.ld_p, m0, k);
       q[0] = op_stage_base<T, Q_KC>(static_cast<const T*>(g.q[0]) + z * g.stride_q, g.ld_q, n0, k);
     } else {
@@ -592,6 +614,60 @@ __device__ __forceinline__ void op_tile_of(int b, int tiles_m, int tiles_n, int*
   *tn = in / rows;
 }
 
+// Where a block works.  The kinds from OP_STATS on count their blocks through
+// the matrices, the splits of a matrix and its tiles, and an XCD takes a run of
+// that order: tiles that read the same k of the same matrix share an L2 (16
+// matrices of 512 x 2000, G in float16: 28.4 us with each matrix's tiles on
+// every XCD, 23.7 so).
+struct OpPlace {
+  int tm, tn, split, z;
+};
+template <int KIND>
+constexpr bool kFlat = KIND >= OP_STATS;
+template <bool FLAT, bool TRIANGLE>
+__device__ __forceinline__ OpPlace op_place(const OpGemm& g) {
+  OpPlace p;
+  if constexpr (!FLAT) {
+    op_tile_of(blockIdx.x, g.tiles_m, g.tiles_n, &p.tm, &p.tn);
+    p.split = blockIdx.y;
+    p.z = g.outputs > 1 ? blockIdx.z : 0;
+    return p;
+  }
+  constexpr int kXcds = 8, kGroup = TRIANGLE ? 4 : 8;
+  const int tiles = TRIANGLE ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
+  const int total = gridDim.x, per = total / kXcds, rest = total % kXcds, x = blockIdx.x % kXcds;
+  const int id = x * per + min(x, rest) + blockIdx.x / kXcds, of = id / tiles;
+  int t = id - of * tiles;
+  p.split = of % g.splits;
+  p.z = of / g.splits;
+  if constexpr (TRIANGLE) {
+    // columns of squares of 4 x 4 tiles, each column's last one cut by the
+    // diagonal: 8 j^2 + 2 j tiles stand before column j
+    int j = (int)((sqrtf(4.0f + 32.0f * (float)t) - 2.0f) * 0.0625f);
+    while (8 * j * j + 2 * j > t) --j;
+    while (8 * (j + 1) * (j + 1) + 2 * (j + 1) <= t) ++j;
+    t -= 8 * j * j + 2 * j;
+    const int wide = min(kGroup, g.tiles_m - kGroup * j), i = t / (kGroup * wide);
+    if (i < j) {
+      t -= i * kGroup * wide;
+      p.tm = kGroup * i + t % kGroup;
+      p.tn = kGroup * j + t / kGroup;
+    } else {
+      t -= j * kGroup * wide;
+      int n = 0;
+      while ((n + 1) * (n + 2) / 2 <= t) ++n;
+      p.tm = kGroup * j + t - n * (n + 1) / 2;
+      p.tn = kGroup * j + n;
+    }
+  } else {
+    const int group = t / (kGroup * g.tiles_n), rows = min(kGroup, g.tiles_m - group * kGroup);
+    t -= group * kGroup * g.tiles_n;
+    p.tm = group * kGroup + t % rows;
+    p.tn = t / rows;
+  }
+  return p;
+}
+
 // ---------------------------------------------------------------------------
 // Staged product, for operands whose rows direct loads cannot take: BM x BN of
 // D per block, 2 x 2 waves.  A stage goes through registers into one of two
@@ -617,10 +693,10 @@ __global__ void __launch_bounds__(256) op_gemm_staged(OpGemm g) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 1, wn = wave & 1;
-  int tm, tn;
-  op_tile_of(blockIdx.x, g.tiles_m, g.tiles_n, &tm, &tn);
+  const OpPlace place = op_place<kFlat<KIND>, KIND == OP_MIRROR>(g);
+  const int tm = place.tm, tn = place.tn;
   const int m0 = tm * BM, n0 = tn * SN;
-  const int z = g.outputs > 1 ? blockIdx.z : 0, split = blockIdx.y;
+  const int z = place.z, split = place.split;
   const int p_left = g.M - m0, q_left = g.N - n0;
 
   PT pt;
@@ -759,10 +835,10 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) o
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 2, wn = wave & 3;
-  int tm, tn;
-  op_tile_of(blockIdx.x, g.tiles_m, g.tiles_n, &tm, &tn);
+  const OpPlace place = op_place<kFlat<KIND>, KIND == OP_MIRROR>(g);
+  const int tm = place.tm, tn = place.tn;
   const int m0 = tm * 256, n0 = tn * SN;
-  const int z = g.outputs > 1 ? blockIdx.z : 0, split = blockIdx.y;
+  const int z = place.z, split = place.split;
   PR pr[2];
   QR qr[2];
 #pragma unroll
@@ -899,7 +975,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) o
     if (g.splits <= 1) return op_write_stats<T, 8, 4, 2, 4>(g, acc, lds, lane, wm, wn, m0, n0);
   }
   op_write_out<T, KIND>(g, acc, lds + wave * op_region_bytes<8, 4>, lane, m0 + wm * 128, n0 + wn * (kGated ? 32 : 64), z,
-                        split);
+                        split, tm != tn);
 }
 
 // ---------------------------------------------------------------------------
@@ -937,10 +1013,10 @@ __global__ void __launch_bounds__(512) op_gemm_middle(OpGemm g) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WGN, wn = wave % WGN;
-  int tm, tn;
-  op_tile_of(blockIdx.x, g.tiles_m, g.tiles_n, &tm, &tn);
+  const OpPlace place = op_place<kFlat<KIND>, KIND == OP_MIRROR>(g);
+  const int tm = place.tm, tn = place.tn;
   const int m0 = tm * BM, n0 = tn * SN;
-  const int z = g.outputs > 1 ? blockIdx.z : 0, split = blockIdx.y;
+  const int z = place.z, split = place.split;
   PT pt;
   QT qt;
   pt.init(g.ld_p, g.M - m0, wave, lane);
@@ -1044,7 +1120,8 @@ __global__ void __launch_bounds__(512) op_gemm_middle(OpGemm g) {
   if constexpr (KIND == OP_STATS) {
     if (g.splits <= 1) return op_write_stats<T, TM, TN, WGM, WGN>(g, acc, lds, lane, wm, wn, m0, n0);
   }
-  op_write_out<T, KIND>(g, acc, lds + wave * op_region_bytes<TM, TN>, lane, m0 + wm * WM, n0 + wn * (TNS * 16), z, split);
+  op_write_out<T, KIND>(g, acc, lds + wave * op_region_bytes<TM, TN>, lane, m0 + wm * WM, n0 + wn * (TNS * 16), z, split,
+                        tm != tn);
 }
 
 // ---------------------------------------------------------------------------
@@ -1072,9 +1149,8 @@ __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
   const int tid = threadIdx.x, lane = tid & 63, l = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // blocks next to each other share cache lines of W: one XCD takes a run of them
-  int tm, tn;
-  op_tile_of(blockIdx.x, g.tiles_m, g.tiles_n, &tm, &tn);
-  const int m0 = tm * (16 * MT), n0 = tn * BN, split = blockIdx.y, p_left = g.M - m0, q_left = g.N - n0;
+  const OpPlace place = op_place<kFlat<KIND>, false>(g);
+  const int m0 = place.tm * (16 * MT), n0 = place.tn * BN, split = place.split, p_left = g.M - m0, q_left = g.N - n0;
   PT pt;
   QT qt;
   pt.init(g.ld_p, p_left, 0, lane);
@@ -1319,13 +1395,20 @@ __global__ void __launch_bounds__(256) op_stats_reduce(OpGemm g) {
 }
 
 // ---------------------------------------------------------------------------
+template <bool FLAT, bool TRIANGLE>
+dim3 op_grid(const OpGemm& g) {
+  const int64_t tiles = TRIANGLE ? (int64_t)g.tiles_m * (g.tiles_m + 1) / 2 : (int64_t)g.tiles_m * g.tiles_n;
+  return FLAT ? dim3((unsigned)(tiles * g.splits * g.outputs))
+              : dim3((unsigned)tiles, (unsigned)g.splits, (unsigned)g.outputs);
+}
+
 template <typename T, int LAYOUT, int KIND, int BM, int BN>
 hipError_t launch_staged(OpGemm& g, hipStream_t st) {
   constexpr int SN = KIND == OP_GATED ? BN / 2 : BN;
   g.tiles_m = (g.M + BM - 1) / BM;
   g.tiles_n = (g.N + SN - 1) / SN;
   return op_launch(op_gemm_staged<T, LAYOUT, KIND, BM, BN>,
-                   dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits, (unsigned)g.outputs), dim3(256), st, g);
+                   op_grid<kFlat<KIND>, false>(g), dim3(256), st, g);
 }
 
 template <typename T, int LAYOUT, int KIND, int BM, int BN, int WGM, int WGN, int KS, int NST>
@@ -1334,7 +1417,7 @@ hipError_t launch_middle(OpGemm& g, hipStream_t st) {
   g.tiles_m = (g.M + BM - 1) / BM;
   g.tiles_n = (g.N + SN - 1) / SN;
   return op_launch(op_gemm_middle<T, LAYOUT, KIND, BM, BN, WGM, WGN, KS, NST>,
-                   dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits, (unsigned)g.outputs), dim3(512), st, g);
+                   op_grid<kFlat<KIND>, KIND == OP_MIRROR>(g), dim3(512), st, g);
 }
 
 template <typename T, int LAYOUT, int KIND>
@@ -1342,8 +1425,7 @@ hipError_t launch_large(OpGemm& g, hipStream_t st) {
   constexpr int SN = KIND == OP_GATED ? 128 : 256;
   g.tiles_m = (g.M + 255) / 256;
   g.tiles_n = (g.N + SN - 1) / SN;
-  return op_launch(op_gemm_large<T, LAYOUT, KIND>,
-                   dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits, (unsigned)g.outputs), dim3(512), st, g);
+  return op_launch(op_gemm_large<T, LAYOUT, KIND>, op_grid<kFlat<KIND>, KIND == OP_MIRROR>(g), dim3(512), st, g);
 }
 
 // Columns, waves and ring of the skinny form: what fits a CU's 160 KB of LDS.
@@ -1361,7 +1443,7 @@ hipError_t launch_skinny(OpGemm& g, hipStream_t st) {
   g.tiles_m = (g.M + 16 * MT - 1) / (16 * MT);
   g.tiles_n = (g.N + S::kCols - 1) / S::kCols;
   return op_launch(op_gemm_skinny<T, LAYOUT, KIND, MT, S::kCols, S::kWaves, S::kStages, DIRECT>,
-                   dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits), dim3(S::kWaves * 64), st, g);
+                   op_grid<kFlat<KIND>, false>(g), dim3(S::kWaves * 64), st, g);
 }
 
 template <typename T, int LAYOUT, int KIND>
@@ -1369,10 +1451,10 @@ hipError_t launch(const OpPlan& plan, OpGemm& g, hipStream_t st) {
   g.splits = plan.splits;
   g.stages_per_split = plan.stages_per_split;
   hipError_t e = hipErrorInvalidValue;
-  constexpr bool kDirectOnly = KIND == OP_BLEND;
+  constexpr bool kDirectOnly = op_kind_blend(KIND);
   if (kDirectOnly && !g.direct) return hipErrorInvalidValue;
   if (plan.tile >= OP_TILE_SKINNY16) {
-    if constexpr (LAYOUT == OP_TN || KIND == OP_BLEND) {
+    if constexpr (LAYOUT == OP_TN || op_kind_blend(KIND)) {
       return hipErrorInvalidValue;
     } else if (g.direct || kDirectOnly) {
       e = plan.tile == OP_TILE_SKINNY16   ? launch_skinny<T, LAYOUT, KIND, 1, true>(g, st)
@@ -1394,10 +1476,9 @@ hipError_t launch(const OpPlan& plan, OpGemm& g, hipStream_t st) {
     return hipErrorInvalidValue;  // the other tiles have no form through registers
   } else if (plan.tile == OP_TILE_256) {
     e = launch_large<T, LAYOUT, KIND>(g, st);
-  } else if (plan.tile == OP_TILE_256X128) {
-    e = launch_middle<T, LAYOUT, KIND, 256, 128, 4, 2, 1, 3>(g, st);
-  } else {
-    e = launch_middle<T, LAYOUT, KIND, 64, 128, 2, 4, 1, 4>(g, st);
+  } else if constexpr (KIND != OP_MIRROR) {
+    e = plan.tile == OP_TILE_256X128 ? launch_middle<T, LAYOUT, KIND, 256, 128, 4, 2, 1, 3>(g, st)
+                                     : launch_middle<T, LAYOUT, KIND, 64, 128, 2, 4, 1, 4>(g, st);
   }
   if (e != hipSuccess || g.splits <= 1) return e;
   if constexpr (KIND == OP_STATS) {

@@ -99,24 +99,26 @@ __global__ void __launch_bounds__(1024) unit_kernel(const float* dloss, const in
   unit[1] = __uint_as_float((uint32_t)(127 + up) << 23);
 }
 
-// Column sums of dz: 64 lanes of 16 bytes, four waves on the rows of a strip
-// each, in order; the strips' sums are added by sum_partials.
+// Column sums of dz: 64 lanes of 16 bytes, eight waves on the rows of a strip
+// each, in order; the strips' sums are added by sum_partials.  Whole chunks are
+// read: what a row has behind its columns is dz's own memory, and its sums are
+// not stored.
+constexpr int kSumWaves = 8;
 template <typename T>
-__global__ void __launch_bounds__(256) column_sums(const T* dz, int64_t ld, int64_t rows, int cols, int64_t per,
-                                                   const float* unit, float* partial) {
+__global__ void __launch_bounds__(kSumWaves * 64) column_sums(const T* dz, int64_t ld, int64_t rows, int cols, int64_t per,
+                                                              const float* unit, float* partial) {
   constexpr int E = 16 / (int)sizeof(T);
-  __shared__ float lds[4][64][E];
+  __shared__ float lds[kSumWaves][64][E];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = (blockIdx.x * 64 + lane) * E, cnt = cols - c;
   const int64_t r0 = blockIdx.y * per, r1 = min(rows, r0 + per);
   float acc[E] = {};
-  if (cnt > 0) {
-#pragma unroll 4
-    for (int64_t r = r0 + wave; r < r1; r += 4) {
-      float v[E];
-      load_vec(dz + r * ld + c, cnt, v);
+  const T* from = dz + (cnt > 0 ? c : 0);
+#pragma unroll 8
+  for (int64_t r = r0 + wave; r < r1; r += kSumWaves) {
+    union { chunk16 v; T e[E]; } u;
+    u.v = *reinterpret_cast<const chunk16*>(from + r * ld);
 #pragma unroll
-      for (int i = 0; i < E; ++i) acc[i] += v[i];
-    }
+    for (int i = 0; i < E; ++i) acc[i] += to_f(u.e[i]);
   }
 #pragma unroll
   for (int i = 0; i < E; ++i) lds[wave][lane][i] = acc[i];
@@ -126,11 +128,12 @@ __global__ void __launch_bounds__(256) column_sums(const T* dz, int64_t ld, int6
 #pragma unroll
   for (int i = 0; i < E; ++i) {
 #pragma unroll
-    for (int w = 1; w < 4; ++w) acc[i] += lds[w][lane][i];
+    for (int w = 1; w < kSumWaves; ++w) acc[i] += lds[w][lane][i];
     acc[i] *= u;
   }
   store_vec(partial + (int64_t)blockIdx.y * cols + c, cnt, acc);
 }
+// Rows of a strip: 64 or more, so that its sums are few beside what it reads.
 int64_t strip_rows(int64_t rows) { return std::max<int64_t>(64, (rows + 63) / 64); }
 int64_t strips_of(int64_t rows) { return std::max<int64_t>(1, (rows + strip_rows(rows) - 1) / strip_rows(rows)); }
 
@@ -141,7 +144,7 @@ hipError_t sum_columns(int type, const void* dz, int64_t ld, int64_t rows, int64
   const dim3 grid((unsigned)((cols + across - 1) / across), (unsigned)strips);
   auto run = [&](auto like) {
     using T = decltype(like);
-    return op_launch(column_sums<T>, grid, dim3(256), st, static_cast<const T*>(dz), ld, rows, (int)cols, per, unit,
+    return op_launch(column_sums<T>, grid, dim3(kSumWaves * 64), st, static_cast<const T*>(dz), ld, rows, (int)cols, per, unit,
                      partial);
   };
   const hipError_t e = type == VOLTA_OP_F32    ? run(0.0f)
@@ -186,8 +189,7 @@ Piece piece_of(const Loss& l, int64_t count, unsigned run) {
   const int64_t w_ld = l.pack_w ? p.columns : d.ld_w;
   const Operand x{d.rows, x_len, x_ld, 1}, w{d.inputs, p.columns, w_ld, 1}, dz{d.rows, p.columns, l.ld_dz, 1};
   p.z = shape_of(d.type, OP_NN, OP_LOSS_GRAD, d.rows, p.columns, d.inputs, 1, 1, x, w);
-  const int kind = l.pieces > 1 ? OP_ADD : OP_STORE;
-  if (run & RUN_DX) p.dx = shape_of(d.type, OP_NT, kind, d.rows, d.inputs, count, 1, 1, dz, w);
+  if (run & RUN_DX) p.dx = shape_of(d.type, OP_NT, OP_ADD, d.rows, d.inputs, count, 1, 1, dz, w);
   if (run & RUN_DW) p.dw = shape_of(d.type, OP_TN, OP_STORE, d.inputs, count, d.rows, 1, 1, x, dz);
   return p;
 }

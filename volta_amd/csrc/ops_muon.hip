@@ -4,8 +4,22 @@
 // A step is three dependent products of all matrices of the batch at once: G of
 // X with itself (the smaller side), B = b G + c G^2, and X' = a X + B X (or X B
 // where the matrix is tall); the last one's epilogue writes the result, or the
-// weights.  G and B are symmetric, so the products that take them read their
-// rows where they would need columns.
+// weights.
+//
+// Two steps at once.  With P = a + b G + c G^2 a step is X' = P X, and G of X'
+// is P G P; P and G are polynomials of the first G, so they commute and all
+// their products are symmetric:
+//   P0 of G,  T = P0 G,  G1 = P0 T,  P1 of G1,  Q = P1 P0,  X'' = Q X
+// take 3 + 5 small / large products of small^2 large for two steps instead of 6
+// + 2, and read and write X once.  Rounded where the kernels round, two steps
+// at once leave the same error as one by one (0.9 to 1.6 times over shapes from
+// 16 x 3000 to 512 x 512 and gradients of few and many directions); three or
+// five at once lose small singular directions.  Which of the two forms is taken
+// follows from the planned products' times.
+//
+// G and the polynomials are symmetric: the tiles on and over the diagonal are
+// computed and stored twice, and the products that take them read their rows
+// where they would need columns.
 //
 // 16-bit types take float16 products.  X's singular values stay in a range that
 // follows from the coefficients, so X, G and B have fixed units that put them
@@ -118,18 +132,22 @@ int norm_blocks(int64_t batch, int64_t chunks) {
 }
 
 // ---------------------------------------------------------------------------
+// Units of what a step takes: 1 in each stands for 1 / unit.
+struct Units {
+  double x, g, b, p, t;
+};
 struct Muon {
   volta_op_muon d;
   int product;             // type of the products
-  bool tall;
+  bool tall, pairs;        // pairs: two steps at once
   int64_t rows_p, cols_p;  // padded to whole chunks: the products run over zeros there
   int64_t small, large;
   int parts;
-  double x_unit[kMaxSteps], g_unit[kMaxSteps], b_unit[kMaxSteps];
-  int layout[3];           // of G, B and X'
+  Units unit[kMaxSteps];
+  int layout[3];           // of G, the small products and X'
   OpPlan plan[3];
   int64_t x_bytes, g_bytes, sum_bytes, partial_bytes;
-  int64_t bytes() const { return 2 * x_bytes + 2 * g_bytes + sum_bytes + partial_bytes; }
+  int64_t bytes() const { return 2 * x_bytes + (pairs ? 3 : 2) * g_bytes + sum_bytes + partial_bytes; }
 };
 
 // The largest power of two that keeps `bound` at 2^15 or under.
@@ -165,19 +183,22 @@ Muon muon_of(const volta_op_muon* in) {
   // between two).  An element is at most the largest singular value.
   double r = 1.0;
   for (int i = 0; i < d.steps; ++i) {
-    double next = 0.0, poly = 0.0;
+    double next = 0.0, poly = 0.0, whole = 0.0, times = 0.0;
     for (int k = 0; k <= 4096; ++k) {
-      const double s = r * k / 4096, q = s * s;
-      next = std::max(next, std::fabs(s * (a + b * q + c * q * q)));
+      const double s = r * k / 4096, q = s * s, p = a + b * q + c * q * q;
+      next = std::max(next, std::fabs(s * p));
       poly = std::max(poly, std::fabs(b * q + c * q * q));
+      whole = std::max(whole, std::fabs(p));
+      times = std::max(times, std::fabs(q * p));
     }
+    Units& u = l.unit[i];
     if (l.product == VOLTA_OP_F32) {
-      l.x_unit[i] = l.g_unit[i] = l.b_unit[i] = 1.0;
+      u = Units{1.0, 1.0, 1.0, 1.0, 1.0};
     } else {
-      if (!(r <= 1024.0 && next <= 1024.0 && poly <= 1e6)) refuse("the coefficients let singular values grow past 1024");
-      l.x_unit[i] = unit_of(r);
-      l.g_unit[i] = unit_of(r * r);
-      l.b_unit[i] = unit_of(std::max(poly, 1e-6));
+      if (!(std::max({r, next, whole}) <= 1024.0 && std::max(poly, times) <= 1e6))
+        refuse("the coefficients let singular values grow past 1024");
+      u = Units{unit_of(r), unit_of(r * r), unit_of(std::max(poly, 1e-6)), unit_of(std::max(whole, 1e-6)),
+                unit_of(std::max(times, 1e-6))};
     }
     r = std::max(next * 1.001, 1e-6);
   }
@@ -188,10 +209,13 @@ Muon muon_of(const volta_op_muon* in) {
   const int64_t N[3] = {l.small, l.small, l.tall ? l.small : l.large};
   const int64_t K[3] = {l.large, l.small, l.small};
   for (int i = 0; i < 3; ++i) {
-    l.plan[i] = op_gemm_plan(e, l.layout[i], OP_BLEND, M[i], N[i], K[i], 1, (int)d.batch, true);
+    l.plan[i] = op_gemm_plan(e, l.layout[i], i < 2 ? OP_MIRROR : OP_BLEND, M[i], N[i], K[i], 1, (int)d.batch, true);
     l.partial_bytes = std::max(l.partial_bytes, align256(op_gemm_partial_bytes(l.plan[i], OP_BLEND, M[i], N[i], (int)d.batch)));
-    if (op_gemm_blocks(l.plan[i], OP_BLEND, M[i], N[i]) > kMaxBlocks) refuse("the rows and columns of a product are too many");
+    if (op_gemm_blocks(l.plan[i], OP_BLEND, M[i], N[i]) * d.batch > kMaxBlocks) refuse("the rows and columns of a product are too many");
   }
+  const double one = l.plan[0].us + l.plan[1].us + l.plan[2].us;
+  const double two = l.plan[0].us + 5.0 * l.plan[1].us + l.plan[2].us;
+  l.pairs = d.steps >= 2 && two < 2.0 * one;
   l.x_bytes = align256(d.batch * l.rows_p * l.cols_p * e);
   l.g_bytes = align256(d.batch * l.small * l.small * e);
   l.parts = norm_blocks(d.batch, d.rows * ((d.cols + 3) / 4));
@@ -217,10 +241,11 @@ hipError_t passes(const Muon& l, MuonArgs a, hipStream_t st) {
 void run(const Muon& l, MuonArgs a, const OpEpilogue& last, char* workspace, hipStream_t st) {
   const volta_op_muon& d = l.d;
   char* x[2] = {workspace, workspace + l.x_bytes};
-  char* g = workspace + 2 * l.x_bytes;
-  char* b = g + l.g_bytes;
-  a.partial = reinterpret_cast<double*>(b + l.g_bytes);
-  float* partial = reinterpret_cast<float*>(b + l.g_bytes + l.sum_bytes);
+  char* small[3];  // matrices of the smaller side
+  for (int i = 0; i < 3; ++i) small[i] = workspace + 2 * l.x_bytes + i * l.g_bytes;
+  char* rest = small[l.pairs ? 2 : 1] + l.g_bytes;
+  a.partial = reinterpret_cast<double*>(rest);
+  float* partial = reinterpret_cast<float*>(rest + l.sum_bytes);
   a.x = x[0];
   a.rows = d.rows;
   a.cols = d.cols;
@@ -229,10 +254,10 @@ void run(const Muon& l, MuonArgs a, const OpEpilogue& last, char* workspace, hip
   a.ld_g = d.ld_u;
   a.ld_m = d.ld_m;
   a.eps = d.eps;
-  a.unit = (float)l.x_unit[0];
+  a.unit = (float)l.unit[0].x;
   check_hip(passes(l, a, st), "norm");
   const int64_t x_size = l.rows_p * l.cols_p, g_size = l.small * l.small;
-  auto product = [&](int which, const void* p, int64_t ld_p, int64_t stride_p, const void* q, int64_t ld_q,
+  auto product = [&](int which, const char* p, int64_t ld_p, int64_t stride_p, const char* q, int64_t ld_q,
                      int64_t stride_q, int64_t M, int64_t N, int64_t K, const OpEpilogue& epi, const char* what) {
     OpGemm m{};
     m.p[0] = m.p[1] = p;
@@ -249,44 +274,81 @@ void run(const Muon& l, MuonArgs a, const OpEpilogue& last, char* workspace, hip
     m.direct = 1;
     m.partial = partial;
     m.epi = epi;
-    check_hip(op_gemm_blend(l.product, l.layout[which], l.plan[which], m, st), what);
+    check_hip(op_gemm_blend(l.product, l.layout[which], which < 2 ? OP_MIRROR : OP_BLEND, l.plan[which], m, st), what);
   };
-  for (int i = 0; i < d.steps; ++i) {
-    const char* from = x[i & 1];
-    const bool end = i == d.steps - 1;
-    const double ux = l.x_unit[i], ug = l.g_unit[i], ub = l.b_unit[i];
+  // out = alpha d, in the products' type: matrices of the smaller side
+  auto to_small = [&](char* out, double alpha) {
     OpEpilogue o{};
-    o.out[0] = g;
+    o.out[0] = out;
     o.out_type = l.product;
     o.ld_out = l.small;
     o.stride_out = g_size;
-    o.alpha = (float)(ug / (ux * ux));
-    product(0, from, l.cols_p, x_size, from, l.cols_p, x_size, l.small, l.small, l.large, o, "gram");
-    o.out[0] = b;
-    o.alpha = (float)(d.c * ub / (ug * ug));
-    o.beta = (float)(d.b * ub / ug);
+    o.alpha = (float)alpha;
+    return o;
+  };
+  auto gram = [&](const char* from, char* out, const Units& u) {
+    product(0, from, l.cols_p, x_size, from, l.cols_p, x_size, l.small, l.small, l.large,
+            to_small(out, u.g / (u.x * u.x)), "gram");
+  };
+  auto multiply = [&](const char* p, const char* q, const OpEpilogue& o) {
+    product(1, p, l.small, g_size, q, l.small, g_size, l.small, l.small, l.small, o, "polynomial");
+  };
+  // b G + c G^2 in `unit`, and a on the diagonal
+  auto polynomial = [&](const char* g, char* out, const Units& u, double unit, double diagonal) {
+    OpEpilogue o = to_small(out, d.c * unit / (u.g * u.g));
+    o.beta = (float)(d.b * unit / u.g);
     o.blend = g;
     o.ld_blend = l.small;
     o.stride_blend = g_size;
-    product(1, g, l.small, g_size, g, l.small, g_size, l.small, l.small, l.small, o, "polynomial");
+    o.diagonal = (float)(diagonal * unit);
+    multiply(g, g, o);
+  };
+  int at = 0;
+  for (int i = 0; i < d.steps;) {
+    const int n = l.pairs && i + 1 < d.steps ? 2 : 1;
+    const char *from = x[at], *by;
+    const Units &u = l.unit[i], &v = l.unit[i + n - 1];
+    double by_unit;
+    gram(from, small[0], u);
+    if (n == 2) {
+      polynomial(small[0], small[1], u, u.p, d.a);
+      multiply(small[1], small[0], to_small(small[2], u.t / (u.p * u.g)));
+      multiply(small[1], small[2], to_small(small[0], v.g / (u.p * u.t)));
+      polynomial(small[0], small[2], v, v.p, d.a);
+      // at most the product of both largest values, each at most 2^15 in its unit
+      by_unit = u.p * v.p * 0x1p-15;
+      multiply(small[2], small[1], to_small(small[0], l.product == VOLTA_OP_F32 ? 1.0 : by_unit / (u.p * v.p)));
+      if (l.product == VOLTA_OP_F32) by_unit = 1.0;
+      by = small[0];
+    } else {
+      by_unit = u.b;
+      polynomial(small[0], small[1], u, u.b, 0.0);
+      by = small[1];
+    }
+    i += n;
     // X' in the next step's unit, or the result
-    const double to = end ? (double)last.alpha : l.x_unit[i + 1];
-    OpEpilogue n{};
-    if (end) n = last;
-    n.alpha = (float)(to / (ub * ux));
-    n.beta = (float)(to * d.a / ux);
-    n.blend = from;
-    n.ld_blend = l.cols_p;
-    n.stride_blend = x_size;
-    if (!end) {
-      n.out[0] = x[(i + 1) & 1];
-      n.out_type = l.product;
-      n.ld_out = l.cols_p;
-      n.stride_out = x_size;
+    const bool end = i == d.steps;
+    const double to = end ? (double)last.alpha : l.unit[i].x;
+    OpEpilogue o{};
+    if (end) {
+      o = last;
+    } else {
+      o.out[0] = x[at ^ 1];
+      o.out_type = l.product;
+      o.ld_out = l.cols_p;
+      o.stride_out = x_size;
+    }
+    o.alpha = (float)(to / (by_unit * u.x));
+    if (n == 1) {
+      o.beta = (float)(to * d.a / u.x);
+      o.blend = from;
+      o.ld_blend = l.cols_p;
+      o.stride_blend = x_size;
     }
     const int64_t M = end ? d.rows : l.rows_p, N = end ? d.cols : l.cols_p;
-    if (l.tall) product(2, from, l.cols_p, x_size, b, l.small, g_size, M, N, l.small, n, "step");
-    else product(2, b, l.small, g_size, from, l.cols_p, x_size, M, N, l.small, n, "step");
+    if (l.tall) product(2, from, l.cols_p, x_size, by, l.small, g_size, M, N, l.small, o, "step");
+    else product(2, by, l.small, g_size, from, l.cols_p, x_size, M, N, l.small, o, "step");
+    at ^= 1;
   }
 }
 

@@ -47,10 +47,12 @@ OpPlan op_gemm_plan(int elem_bytes, int layout, int kind, int64_t M, int64_t N, 
   for (int t = 0; t < OP_TILES; ++t) {
     const TileCost& c = kTiles[t];
     const bool skinny = t >= OP_TILE_SKINNY16;
-    if (skinny && (layout == OP_TN || kind == OP_BLEND || M > 512)) continue;
+    if (skinny && (layout == OP_TN || op_kind_blend(kind) || M > 512)) continue;
+    if (kind == OP_MIRROR && c.bm != c.bn) continue;
     if (!direct && (t == OP_TILE_256 || t == OP_TILE_256X128 || t == OP_TILE_64X128)) continue;
     const int64_t sn = skinny ? c.bn : kind == OP_GATED ? c.bn / 2 : c.bn;
-    const int64_t tiles = ceil_div(M, c.bm) * ceil_div(N, sn) * outputs;
+    const int64_t side = ceil_div(M, c.bm);
+    const int64_t tiles = (kind == OP_MIRROR ? side * (side + 1) / 2 : side * ceil_div(N, sn)) * outputs;
     const int waves = !skinny ? 1 : kind == OP_GATED || c.bm > 16 ? 4 : 8;
     double stage_us = c.stage, tile_read_us = read_us;
     // half cache lines of W: whole ones are fetched (134 MB of W from memory: 40 us in 64-byte pieces, 29 in 128)

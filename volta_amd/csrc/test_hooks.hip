@@ -359,15 +359,17 @@ int32_t volta_hip_op_product8(int32_t type, int32_t tile, int32_t splits, int32_
 }
 
 // out = alpha P Q + beta r of `batch` matrices on a given tile and number of
-// splits (OP_BLEND), in float32 (0) or float16 (2), synchronously.  All packed,
-// rows of whole 16-byte chunks, a matrix behind the other.
-int32_t volta_hip_op_blend(int32_t type, int32_t layout, int32_t tile, int32_t splits, int32_t batch, const void* p,
+// splits (OP_BLEND; OP_MIRROR: of a symmetric result and r), in float32 (0) or
+// float16 (2), synchronously.  All packed, rows of whole 16-byte chunks, a matrix behind the other.
+int32_t volta_hip_op_blend(int32_t type, int32_t layout, int32_t kind, int32_t tile, int32_t splits, int32_t batch, const void* p,
                            const void* q, const void* r, void* out, int32_t M, int32_t N, int32_t K, float alpha,
                            float beta) {
   using namespace volta::ops;
   const int e = type == VOLTA_OP_F32 ? 4 : 2, per_chunk = 16 / e;
   if ((type != VOLTA_OP_F32 && type != VOLTA_OP_F16) || M < 1 || N < 1 || K < 1 || batch < 1 || splits < 1) return -1;
   if (M % per_chunk || N % per_chunk || K % per_chunk || tile < OP_TILE_256 || tile > OP_TILE_64) return -1;
+  if (kind == OP_MIRROR && (M != N || layout == OP_NN || tile == OP_TILE_256X128 || tile == OP_TILE_64X128)) return -1;
+  if (kind == OP_BLEND && layout == OP_TN) return -1;
   for (const void* x : {p, q})
     if ((uintptr_t)x % 16) return -1;
   const int stages = (K + op_stage_k(e) - 1) / op_stage_k(e);
@@ -398,7 +400,7 @@ int32_t volta_hip_op_blend(int32_t type, int32_t layout, int32_t tile, int32_t s
   g.epi.out_type = type;
   g.epi.alpha = alpha;
   g.epi.beta = beta;
-  hipError_t rc = op_gemm_blend(type, layout, plan, g, nullptr);
+  hipError_t rc = op_gemm_blend(type, layout, kind, plan, g, nullptr);
   if (rc == hipSuccess) rc = hipStreamSynchronize(nullptr);
   if (ws) (void)hipFree(ws);
   return rc == hipSuccess ? 0 : -1;

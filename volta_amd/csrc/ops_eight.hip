@@ -121,10 +121,32 @@ hipError_t quantize(int type, bool blocks, const QuantizeArgs& a, hipStream_t st
                                  : run((_Float16)0.0f);
 }
 
+// The rows' scales by blocks of k: [blocks][rows] of [rows][blocks].  A stage of a
+// product loads one block's for its rows, side by side so, and else each from a
+// cache line of its own, which costs the large tile as much as a sixth of its
+// operands.
+__global__ void __launch_bounds__(256) turn_scales(const float* from, float* to, int64_t rows, int64_t rows_p, int blocks) {
+  __shared__ float lds[32][33];
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5, b0 = blockIdx.y * 32;
+  const int64_t r0 = (int64_t)blockIdx.x * 32;
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    const int64_t r = r0 + y + i;
+    if (r < rows && b0 + x < blocks) lds[y + i][x] = from[r * blocks + b0 + x];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    if (b0 + y + i < blocks && r0 + x < rows) to[(b0 + y + i) * rows_p + r0 + x] = lds[x][y + i];
+}
+
 struct Linear8 {
   volta_op_linear8 d;
   int64_t blocks, x_groups;  // of 128 inputs; scales of a row of x
   Shape fwd;
+  int64_t turned_bytes;  // of the rows' scales by blocks, where that pays
+  int64_t rows_p;
+  int64_t bytes() const { return turned_bytes + fwd.bytes(); }
 };
 Linear8 linear8_of(const volta_op_linear8* in) {
   need(in, "the description");
@@ -145,6 +167,10 @@ Linear8 linear8_of(const volta_op_linear8* in) {
   l.x_groups = d.group ? l.blocks : 1;
   const Operand x{d.rows, d.inputs, d.ld_x, 1}, w{d.outputs, d.inputs, d.ld_w, 1};
   l.fwd = shape_of(VOLTA_OP_E4M3, OP_NT, OP_LINEAR, d.rows, d.outputs, d.inputs, 1, 1, x, w);
+  // a launch of 3 us and two passes over the scales: for products of some size
+  const OpPlan plan = plan_of(VOLTA_OP_E4M3, l.fwd, true);
+  l.rows_p = (d.rows + 31) / 32 * 32;
+  if (l.x_groups > 1 && plan.tile <= OP_TILE_128 && plan.us >= 40.0) l.turned_bytes = align256(4 * l.rows_p * l.blocks);
   return l;
 }
 
@@ -195,7 +221,7 @@ int32_t volta_op_quantize_forward(const volta_op_quantize* in, const void* x, vo
 }
 
 int64_t volta_op_linear8_workspace(const volta_op_linear8* d) {
-  return bytes_of("volta_op_linear8_workspace", VOLTA_OP_FORWARD, [&](bool) { return linear8_of(d).fwd.bytes(); });
+  return bytes_of("volta_op_linear8_workspace", VOLTA_OP_FORWARD, [&](bool) { return linear8_of(d).bytes(); });
 }
 
 int32_t volta_op_linear8_forward(const volta_op_linear8* in, const void* x, const float* x_scales, const void* w,
@@ -212,7 +238,7 @@ int32_t volta_op_linear8_forward(const volta_op_linear8* in, const void* x, cons
     }
     need(w, "w");
     need(w_scales, "w_scales");
-    const int64_t bytes = l.fwd.bytes();
+    const int64_t bytes = l.bytes();
     check_workspace(workspace, workspace_bytes, bytes);
     const hipStream_t st = check_call({{"x", x, d.rows, d.inputs, d.ld_x, 1, false},
                                        {"x_scales", x_scales, d.rows, l.x_groups, l.x_groups, 4, false},
@@ -235,7 +261,16 @@ int32_t volta_op_linear8_forward(const volta_op_linear8* in, const void* x, cons
     epi.ld_sx = l.x_groups;
     epi.step_sx = d.group ? 1 : 0;
     epi.ld_sw = l.blocks;
-    product(VOLTA_OP_E4M3, l.fwd, &x, &w, epi, static_cast<char*>(workspace), st, "product");
+    char* ws = static_cast<char*>(workspace);
+    if (l.turned_bytes && d.rows > 0) {
+      float* to = reinterpret_cast<float*>(ws);
+      const dim3 grid((unsigned)(l.rows_p / 32), (unsigned)((l.blocks + 31) / 32));
+      check_hip(op_launch(turn_scales, grid, dim3(256), st, x_scales, to, d.rows, l.rows_p, (int)l.blocks), "scales");
+      epi.sx = to;
+      epi.ld_sx = 1;
+      epi.step_sx = l.rows_p;
+    }
+    product(VOLTA_OP_E4M3, l.fwd, &x, &w, epi, ws + l.turned_bytes, st, "product");
   });
 }
 

@@ -133,6 +133,42 @@ struct ColumnScales {
 
 using Cursor8 = Cursor<uint8_t, OP_NT, OP_STORE>;
 
+// The linear layer's epilogue by op_write_swapped, one copy of the code for
+// each activation.
+template <typename T, int TM, int TN>
+__device__ __forceinline__ void write_linear8(const OpGemm& g, const floatx4 (&acc)[TM][TN], int lane, int m0, int n0) {
+  const OpEpilogue& e = g.epi;
+  float bias[TN][4], none[4];
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int n = n0 + j * 16 + (lane >> 4) * 4;
+    op_biases<T, OP_LINEAR>(e, n, g.N - n, bias[j], none);
+  }
+  const T* residual = static_cast<const T*>(e.residual);
+  auto run = [&](auto act) {
+    op_write_swapped<T>(static_cast<T*>(e.out[0]), e.ld_out, g.M, g.N, acc, lane, m0, n0,
+                        [&](int, int j, int m, const floatx4& d, float (&v)[4]) {
+                          float r[4] = {};
+                          const int n = n0 + j * 16 + (lane >> 4) * 4, cnt = m < g.M ? g.N - n : 0;
+                          if (residual) load_vec(residual + (cnt > 0 ? m * e.ld_residual + n : 0), cnt, r);
+#pragma unroll
+                          for (int k = 0; k < 4; ++k) v[k] = op_act<T>(decltype(act)::value, d[k] + bias[j][k]) + r[k];
+                        });
+  };
+#define VOLTA_ACT_CASE(A) \
+  case A: return run(std::integral_constant<int, A>())
+  switch (e.act) {
+    VOLTA_ACT_CASE(VOLTA_ACT_RELU);
+    VOLTA_ACT_CASE(VOLTA_ACT_SIGMOID);
+    VOLTA_ACT_CASE(VOLTA_ACT_TANH);
+    VOLTA_ACT_CASE(VOLTA_ACT_LEAKY_RELU);
+    VOLTA_ACT_CASE(VOLTA_ACT_SILU);
+    VOLTA_ACT_CASE(VOLTA_ACT_GELU);
+    default: return run(std::integral_constant<int, VOLTA_OP_ACT_NONE>());
+  }
+#undef VOLTA_ACT_CASE
+}
+
 // ---------------------------------------------------------------------------
 // BM x BN of D per block, eight waves, a ring of NST stages of KS blocks of k
 // (op_gemm_middle).
@@ -323,20 +359,30 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) o
   };
   // Blocks (half 4 + i, j) of the phase, j in twos so that Q1 is not needed at
   // once.  A block's sums are scaled kLate instructions behind its own, in an
-  // order that the compiler keeps: its own would wait for each of them.
+  // order that the compiler keeps: its own would wait for each of them.  The
+  // last ones' are left for the next phase, where this wave reads LDS and the
+  // other one multiplies.
+  constexpr int kLate = 3;
+  floatx4 t[kLate + 1];
+  float late[2];  // the scales of the rows of the blocks left
+  auto scale = [&](int half, int o, float by) {
+    const int i = half * 4 + ((o >> 1) & 3), j = (o & 1) + (o >> 3) * 2;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(t[o % (kLate + 1)][r], by, acc[i][j][r]);
+  };
   auto mul = [&](int half) {
-    constexpr int kLate = 3;
-    floatx4 t[kLate + 1];
 #pragma unroll
-    for (int n = 0; n < 16 + kLate; ++n) {
-      if (n < 16) t[n % (kLate + 1)] = mfma8(fq[(n & 1) + (n >> 3) * 2], fp[(n >> 1) & 3]);
-      if (n >= kLate) {
-        const int o = n - kLate, i = half * 4 + ((o >> 1) & 3), j = (o & 1) + (o >> 3) * 2;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(t[o % (kLate + 1)][r], sc[i], acc[i][j][r]);
-      }
+    for (int n = 0; n < 16; ++n) {
+      t[n % (kLate + 1)] = mfma8(fq[(n & 1) + (n >> 3) * 2], fp[(n >> 1) & 3]);
+      if (n >= kLate) scale(half, n - kLate, sc[half * 4 + (((n - kLate) >> 1) & 3)]);
       __builtin_amdgcn_sched_barrier(0);
     }
+    late[0] = sc[half * 4 + 2];
+    late[1] = sc[half * 4 + 3];
+  };
+  auto scale_late = [&](int half) {
+#pragma unroll
+    for (int o = 16 - kLate; o < 16; ++o) scale(half, o, late[((o >> 1) & 3) - 2]);
   };
   constexpr auto H0 = std::integral_constant<int, 0>();
   constexpr auto H1 = std::integral_constant<int, 1>();
@@ -351,6 +397,8 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) o
     const float* scales = reinterpret_cast<const float*>(lds + kScales + (from ? 1024 : 0));
 #pragma unroll
     for (int i = 0; i < 8; ++i) sc[i] = scales[wm * 128 + i * 16 + (lane & 15)];
+    __builtin_amdgcn_sched_barrier(0);
+    scale_late(1);  // of the stage before, while LDS is read
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (left >= 1) {
       load(from ^ 4 * kRegion, H1);
@@ -371,6 +419,8 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) o
     op_barrier();
     read_p(at + kRegion);
     __builtin_amdgcn_sched_barrier(0);
+    scale_late(0);
+    __builtin_amdgcn_sched_barrier(0);
     if constexpr (left >= 2) {
       load(from, H0);
       op_wait_loads<7>();  // P0, Q0, Q1 and the scales of s + 1 are there
@@ -385,6 +435,9 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) o
     __builtin_amdgcn_s_setprio(0);
     op_barrier();
   };
+#pragma unroll
+  for (int i = 0; i <= kLate; ++i) t[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  late[0] = late[1] = 0.0f;
   load(0, H0);
   load(0, H1);
   if (S > 1) {
@@ -399,7 +452,9 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) o
   for (; s < S - 2; ++s) stage(s, std::integral_constant<int, 2>());
   if (s < S - 1) stage(s++, std::integral_constant<int, 1>());
   stage(s, std::integral_constant<int, 0>());
+  scale_late(1);
   if (wm == 0) op_barrier();
+  if (g.splits <= 1) return write_linear8<T>(g, acc, lane, m0 + wm * 128, n0 + wn * 64);
   __syncthreads();  // the regions are free
   static_assert(8 * op_region_bytes<8, 4> <= 8 * kRegion, "output regions fit");
   op_write_out<T, OP_LINEAR>(g, acc, lds + wave * op_region_bytes<8, 4>, lane, m0 + wm * 128, n0 + wn * 64, 0, split);

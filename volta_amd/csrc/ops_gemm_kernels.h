@@ -532,6 +532,58 @@ __device__ __forceinline__ void op_write_out(const OpGemm& g, floatx4 (&acc)[TM]
   }
 }
 
+// ---------------------------------------------------------------------------
+// A wave's sums to a 16-bit output without LDS.  A lane of two blocks side by
+// side has four columns of each, 8 bytes; swapping the odd quarters of the wave
+// in the first with the even ones in the second (permlane16_swap) leaves eight
+// columns of one of them, and the quarters hold 64 bytes of a row:
+//   quarter  0: block j, columns 0..7    1: block j + 1, 0..7
+//            2: block j, 8..15           3: block j + 1, 8..15
+// `value(i, j, m, sums, out)` makes the four results of block i, j and row m.
+// ---------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ uint32_t op_pack2(float a, float b) {
+  union { T e[2]; uint32_t w; } u;
+  u.e[0] = from_f<T>(a);
+  u.e[1] = from_f<T>(b);
+  return u.w;
+}
+template <typename T, int TM, int TN, typename F>
+__device__ __forceinline__ void op_write_swapped(T* out, int64_t ld, int M, int N, const floatx4 (&acc)[TM][TN], int lane,
+                                                 int m0, int n0, F value) {
+  static_assert(sizeof(T) == 2 && TN % 2 == 0, "pairs of blocks of 16 bits");
+  const int quarter = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int m = m0 + i * 16 + (lane & 15);
+    uint32_t p[TN][2];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      float d[4];
+      value(i, j, m, acc[i][j], d);
+      p[j][0] = op_pack2<T>(d[0], d[1]);
+      p[j][1] = op_pack2<T>(d[2], d[3]);
+    }
+#pragma unroll
+    for (int j = 0; j < TN; j += 2) {
+      const auto a = __builtin_amdgcn_permlane16_swap(p[j][0], p[j + 1][0], false, false);
+      const auto b = __builtin_amdgcn_permlane16_swap(p[j][1], p[j + 1][1], false, false);
+      union { chunk16 v; T e[8]; } u;
+      u.v = chunk16{a[0], b[0], a[1], b[1]};
+      const int n = n0 + (j + (quarter & 1)) * 16 + (quarter >> 1) * 8, cnt = N - n;
+      if (m >= M || cnt <= 0) continue;
+      T* to = out + m * ld + n;
+      if (cnt >= 8) {
+        *(VOLTA_GLOBAL typename Access<16, 2>::type*)to = u.v;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < cnt) ((VOLTA_GLOBAL T*)to)[k] = u.e[k];
+      }
+    }
+  }
+}
+
 // Where a stage of an operand starts: row or column x0, k.
 template <typename T, bool KC>
 __device__ __forceinline__ const char* op_stage_base(const void* p, int64_t ld, int x0, int k) {

@@ -56,13 +56,20 @@ __global__ void __launch_bounds__(256) quantize_blocks(QuantizeArgs a) {
   const int n = nb * 128 + nc * 8, cnt = a.cols - n;
   const T* x = static_cast<const T*>(a.x);
   float v[2][4][8], m = 0.0f;
+  if (k0 + 128 <= a.rows && nb * 128 + 128 <= a.cols) {  // no branch between the loads
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int64_t k = k0 + (h * 16 + kq) * 4 + r;
-      load_vec(x + (k < a.rows ? k * a.ld_x + n : 0), k < a.rows ? cnt : 0, v[h][r]);
-    }
+      for (int r = 0; r < 4; ++r) load_vec(x + (k0 + (h * 16 + kq) * 4 + r) * a.ld_x + n, 8, v[h][r]);
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t k = k0 + (h * 16 + kq) * 4 + r;
+        load_vec(x + (k < a.rows ? k * a.ld_x + n : 0), k < a.rows ? cnt : 0, v[h][r]);
+      }
+  }
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll

@@ -301,10 +301,10 @@ typedef struct volta_op_muon {
 
 int64_t volta_op_muon_workspace(const volta_op_muon* d);
 
-/* o = X.  o may be u (the same pointer and ld).  F32 takes products in float32,
- * the other types in float16, of X, G and b G + c G^2 in units that follow from
- * the coefficients (those that let singular values grow past 1024 are refused);
- * the sum of squares has 64 bits.  A matrix of zeros stays one; a NaN or an
+/* o = X.  o may be u (the same pointer and ld).  X, G and the polynomials of it
+ * are held in float16, in units that follow from the coefficients (those that
+ * let singular values grow past 1024 are refused), for F32 in two numbers each,
+ * 23 bits; the products' sums have 32 bits, the sum of squares 64.  A matrix of zeros stays one; a NaN or an
  * infinity in a matrix makes that matrix's result NaN. */
 int32_t volta_op_muon_orthogonalize(const volta_op_muon* d, const void* u, void* o, void* workspace,
                                     int64_t workspace_bytes, void* stream);

@@ -5,15 +5,18 @@ NaN, far values, graphs.
 
 Tolerances.  The iteration amplifies errors of X's small singular directions,
 by what follows from the matrix, so the bound comes from the matrix: the same
-iteration with its products' sums and X, G and B rounded as the kernels round
-them is off by some distance, and the kernels, whose roundings are others of the
-same sizes, by up to three times it.  float16: X, G and B rounded to 11 bits in
-units of a power of two over their range; the sums' 32 bits are nothing beside
-that.  float32: a sum of K products is a chain of K / 4 additions, each rounded
-to 24 bits (of G's diagonal, whose terms all add up, that is some sqrt(K / 12)
-roundings of the sum: one rounding at the end, which the first form of this
-bound took, is too little from K = 100 on).  The result's rounding adds half a
-step.  The coefficients are floats in the call, and so in the reference."""
+iteration with X, G and the polynomials rounded as the kernels round them is off
+by some distance, and the kernels, whose roundings are others of the same sizes,
+by up to three times it.  16-bit types: to float16 in units of a power of two
+over the range; the sums' 32 bits are nothing beside that.  float32: to two such
+numbers (23 bits), and a sum of K products is a chain of K / 8 additions, each
+rounded to 24 bits (the instruction adds eight products at a time: 99 % of its
+results over random operands are those of that chain; with the smaller two of
+the three products first, those of the rests add nothing to it); the product of the two rests, which is left out, is
+2^-24 of the others; and alpha d + beta r is rounded to 24 bits three times,
+which together is as much as the two numbers' half step (the first form of this
+bound had left it out).  The result's rounding adds half a step.  The coefficients
+are floats in the call, and so in the reference."""
 from __future__ import annotations
 
 import ctypes as C
@@ -42,15 +45,22 @@ def space(lib, op):
     return _Space(lib, _NoDirection(op))
 
 
-def iterate(u, steps=5, coefficients=ABC, eps=1e-7, rounding=lambda v, kind: v, mul=lambda p, q: p @ q):
+def mixed(alpha, d, beta, r):
+    """alpha d + beta r in float32."""
+    d, r = (np.float32(k) * v.astype(np.float32) for k, v in ((alpha, d), (beta, r)))
+    return (d + r).astype(np.float64)
+
+
+def iterate(u, steps=5, coefficients=ABC, eps=1e-7, rounding=lambda v, kind: v, mul=lambda p, q: p @ q,
+            mix=lambda alpha, d, beta, r: alpha * d + beta * r):
     a, b, c = coefficients
     x = u / (np.sqrt((u**2).sum()) + eps) if u.any() else u
     x = rounding(x, 1.0)
     tall = x.shape[0] > x.shape[1]
     for i in range(steps):
         g = rounding(mul(x.T, x) if tall else mul(x, x.T), 1.5)
-        p = rounding(b * g + c * mul(g, g), 4.0)
-        x = a * x + (mul(x, p) if tall else mul(p, x))
+        p = rounding(mix(c, mul(g, g), b, g), 4.0)
+        x = mix(1.0, mul(x, p) if tall else mul(p, x), a, x)
         if i < steps - 1:
             x = rounding(x, 1.25)
     return x
@@ -62,72 +72,95 @@ def halves(v, bound):
     return (v * unit).astype(np.float16).astype(np.float64) / unit
 
 
-def singles(v, bound):
-    return v.astype(np.float32).astype(np.float64)
+def pairs(v, bound):
+    """To two float16 numbers in that unit."""
+    unit = 2.0 ** (15 - np.ceil(np.log2(bound)))
+    first = (v * unit).astype(np.float16).astype(np.float64)
+    return (first + (v * unit - first).astype(np.float16).astype(np.float64)) / unit
 
 
 def chain(p, q):
-    """p q, four products added to the sum at a time, the sum rounded to float32."""
+    """p q, eight products added to the sum at a time, the sum rounded to float32."""
     d = np.zeros((p.shape[0], q.shape[1]), np.float32)
-    for k in range(0, p.shape[1], 4):
-        d = (d + p[:, k:k + 4] @ q[k:k + 4]).astype(np.float32)
+    for k in range(0, p.shape[1], 8):
+        d = (d + p[:, k:k + 8] @ q[k:k + 8]).astype(np.float32)
     return d.astype(np.float64)
 
 
 def allowed(t, u, want, **kw):
     """The 2-norm by which a result of type t may be off."""
-    near = iterate(u, rounding=singles, mul=chain, **kw) if t == "f32" else iterate(u, rounding=halves, **kw)
+    near = iterate(u, rounding=pairs, mul=chain, mix=mixed, **kw) if t == "f32" else iterate(u, rounding=halves, **kw)
     return 3 * np.linalg.norm(near - want) + (HALF[t] + 2.0**-22) * np.linalg.norm(want) + R.FLOOR[t] * np.sqrt(want.size)
 
 
-@pytest.mark.parametrize("t", ["f32", "f16"])
-def test_products_on_every_tile(lib, t):
-    """Whole numbers: alpha P Q + beta r is exact, whatever the tile, the layout and the splits."""
-    e = 4 if t == "f32" else 8
-    for n, (batch, M, N, K) in enumerate([(1, 8, 8, 8), (3, 16, 72, 40), (2, 136, 64, 264), (5, 8, 200, 8), (1, 264, 520, 136),
+def planes(lib, v, n):
+    """Matrices of whole numbers as float16, or as two planes of it."""
+    rows = v.reshape(-1, v.shape[-1])
+    first = rows.astype(np.float16).astype(np.float64)
+    return Mat(lib, "f16", n * rows.shape[0], rows.shape[1], rows if n == 1 else np.concatenate([first, rows - first]))
+
+
+def _blend(lib, n, layout, kind, tile, splits, batch, p, q, r, out, M, N, K):
+    return lib.lib.volta_hip_op_blend(n, layout, kind, tile, splits, batch, C.c_void_p(p.ptr), C.c_void_p(q.ptr),
+                                      C.c_void_p(r.ptr), C.c_void_p(out.ptr), M, N, K, C.c_float(0.5), C.c_float(-2.0))
+
+
+def both(out, n):
+    v = out.get()
+    return v if n == 1 else v[:len(v) // 2] + v[len(v) // 2:]
+
+
+@pytest.mark.parametrize("n", [1, 2])
+def test_products_on_every_tile(lib, n):
+    """Whole numbers, with two planes some of 12 bits: alpha P Q + beta r is
+    exact, whatever the tile, the layout and the splits."""
+    for k, (batch, M, N, K) in enumerate([(1, 8, 8, 8), (3, 16, 72, 40), (2, 136, 64, 264), (5, 8, 200, 8), (1, 264, 520, 136),
                                           (2, 304, 128, 72)]):
-        rng = np.random.default_rng(n)
-        assert M % e == 0 and N % e == 0 and K % e == 0
+        rng = np.random.default_rng(k)
         P, Q, r = whole(rng, batch, M, K), whole(rng, batch, K, N), whole(rng, batch, M, N)
+        if n == 2:  # a row of P and columns of Q with a second number, none of which meet
+            P[:, 1, :] += 2049
+            Q[:, :, 2] = 0
+            Q[:, K // 2, 2] = 4097  # one: |0.5 3 4097 + 2 5001| stays in float16's range, a sum of them would not
+            P[:, 1, :] *= rng.random(K) < 0.02
+            r[:, 3, 5] = 5001
         want = 0.5 * (P @ Q) - 2 * r
-        mr = Mat(lib, t, batch * M, N, r.reshape(-1, N))
+        if n == 2:
+            want[:, 1, 2] = 0  # both have rests there
+        mp, mr = planes(lib, P, n), planes(lib, r, n)
         for layout in (0, 1):
-            q = Q.swapaxes(1, 2) if layout == 1 else Q
-            mp = Mat(lib, t, batch * M, K, P.reshape(-1, K))
-            mq = Mat(lib, t, batch * q.shape[1], q.shape[2], q.reshape(-1, q.shape[2]))
+            mq = planes(lib, np.ascontiguousarray(Q.swapaxes(1, 2)) if layout == 1 else Q, n)
             for tile in range(5):
                 for splits in (1, 3):
-                    say(t, "batch", batch, M, N, K, "layout", layout, "tile", tile, "splits", splits)
-                    out = Mat(lib, t, batch * M, N)
-                    assert _blend(lib, t, layout, 6, tile, splits, batch, mp, mq, mr, out, M, N, K) == 0
-                    assert np.array_equal(out.get().reshape(want.shape), want)
+                    say("planes", n, "batch", batch, M, N, K, "layout", layout, "tile", tile, "splits", splits)
+                    out = Mat(lib, "f16", n * batch * M, N)
+                    assert _blend(lib, n, layout, 6, tile, splits, batch, mp, mq, mr, out, M, N, K) == 0
+                    got = both(out, n).reshape(want.shape).copy()
+                    if n == 2:
+                        got[:, 1, 2] = 0
+                    assert np.array_equal(got, want)
 
 
-def _blend(lib, t, layout, kind, tile, splits, batch, p, q, r, out, M, N, K):
-    return lib.lib.volta_hip_op_blend(R.TYPES.index(t), layout, kind, tile, splits, batch, C.c_void_p(p.ptr),
-                                      C.c_void_p(q.ptr), C.c_void_p(r.ptr), C.c_void_p(out.ptr), M, N, K, C.c_float(0.5),
-                                      C.c_float(-2.0))
-
-
-@pytest.mark.parametrize("t", ["f32", "f16"])
-def test_symmetric_products_on_every_tile(lib, t):
+@pytest.mark.parametrize("n", [1, 2])
+def test_symmetric_products_on_every_tile(lib, n):
     """Of X X^T: half of the tiles computed, all stored, exactly."""
-    for n, (batch, M, K) in enumerate([(1, 8, 8), (3, 72, 40), (2, 136, 264), (5, 8, 200), (1, 520, 136), (2, 304, 72),
+    for k, (batch, M, K) in enumerate([(1, 8, 8), (3, 72, 40), (2, 136, 264), (5, 8, 200), (1, 520, 136), (2, 304, 72),
                                        (1, 1096, 24)]):
-        rng = np.random.default_rng(n)
+        rng = np.random.default_rng(k)
         X, r = whole(rng, batch, M, K), whole(rng, batch, M, M)
         r = r + r.swapaxes(1, 2)
+        if n == 2:
+            r += 4097
         want = 0.5 * (X @ X.swapaxes(1, 2)) - 2 * r
-        mr = Mat(lib, t, batch * M, M, r.reshape(-1, M))
+        mr = planes(lib, r, n)
         for layout in (1, 2):
-            x = X if layout == 1 else X.swapaxes(1, 2)
-            mx = Mat(lib, t, batch * x.shape[1], x.shape[2], x.reshape(-1, x.shape[2]))
+            mx = planes(lib, X if layout == 1 else np.ascontiguousarray(X.swapaxes(1, 2)), n)
             for tile in (0, 2, 4):
                 for splits in (1, 3):
-                    say(t, "batch", batch, M, K, "layout", layout, "tile", tile, "splits", splits)
-                    out = Mat(lib, t, batch * M, M)
-                    assert _blend(lib, t, layout, 7, tile, splits, batch, mx, mx, mr, out, M, M, K) == 0
-                    assert np.array_equal(out.get().reshape(want.shape), want)
+                    say("planes", n, "batch", batch, M, K, "layout", layout, "tile", tile, "splits", splits)
+                    out = Mat(lib, "f16", n * batch * M, M)
+                    assert _blend(lib, n, layout, 7, tile, splits, batch, mx, mx, mr, out, M, M, K) == 0
+                    assert np.array_equal(both(out, n).reshape(want.shape), want)
 
 
 SIZES = [(1, 1, 1), (3, 1, 9), (2, 9, 1), (1, 16, 16), (4, 17, 33), (2, 64, 50), (1, 100, 300), (3, 130, 70), (1, 256, 256),

@@ -16,6 +16,9 @@ namespace ops {
 // rows or columns contiguous.
 enum OpLayout { OP_NN = 0, OP_NT = 1, OP_TN = 2 };
 
+// A blend's output as two float16 planes, the value's and its rest's: 23 bits.
+constexpr int OP_PLANES = 16;
+
 // What becomes of the sums.
 enum OpKind {
   OP_LINEAR = 0,  // act(d + bias) + residual; d + bias kept on request
@@ -25,7 +28,7 @@ enum OpKind {
   OP_STATS = 3,      // of a row's z: their largest, the sum of their exponentials, the one at the row's label
   OP_LOSS_GRAD = 4,  // (exp(z - lse) - [the label's]) dloss
   OP_ADD = 5,        // sums of several launches, in order, in 32 bits
-  OP_BLEND = 6,      // alpha d + beta r + gamma w, of several matrices (blockIdx.z)
+  OP_BLEND = 6,      // alpha d + beta r + gamma w, of several matrices
   OP_MIRROR = 7      // the same of a symmetric D and r: the tiles on and over the diagonal, stored twice
 };
 constexpr bool op_kind_blend(int kind) { return kind == OP_BLEND || kind == OP_MIRROR; }
@@ -59,6 +62,7 @@ struct OpEpilogue {
   const void *blend, *w;  // r of the products' type, w of out's (NULL: none)
   float alpha, beta, gamma;
   float diagonal;         // OP_MIRROR: added where the row is the column
+  int64_t plane_blend, plane_out;  // of r and, with out_type OP_PLANES, of out: elements to the second plane; r: 0, none
   int32_t out_type;       // enum volta_op_type; also of a product of codes
   int64_t ld_blend, ld_w, stride_blend, stride_w, stride_out;
 };
@@ -68,9 +72,14 @@ struct OpGemm {
   const void* q[2];  // OP_NT: the piece's Q; OP_GATED: gate and up; OP_TN: one for each output
   int64_t ld_p, ld_q;
   int32_t M, N, K;   // K of one piece
-  int32_t pieces;    // 1 or 2 pieces of the sum
+  int32_t pieces;    // 1 or 2 pieces of the sum; OP_BLEND: 1 or 3
   int32_t outputs;   // 1 or 2 outputs (OP_STORE of OP_TN); OP_BLEND: matrices
   int64_t stride_p, stride_q;  // OP_BLEND: elements from one matrix to the next
+  // OP_BLEND with 3 pieces: P and Q are sums of two planes, the second (the
+  // rests) so many elements behind the first: second by first, first by second,
+  // then first by first, so that the small sums are rounded while they are small.
+  // One piece: 0
+  int64_t plane_p, plane_q;
   int32_t direct;    // rows of P and Q are 16-byte aligned and whole 16-byte chunks long
   // from the plan
   int32_t tiles_m, tiles_n;
@@ -122,12 +131,11 @@ int64_t op_gemm_blocks(const OpPlan& plan, int kind, int64_t M, int64_t N);
 hipError_t op_gemm_f32(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
 hipError_t op_gemm_bf16(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
 hipError_t op_gemm_f16(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
-// The kinds of an output layer's loss; and OP_BLEND and OP_MIRROR, in float32
-// and float16.
+// The kinds of an output layer's loss; and OP_BLEND and OP_MIRROR, in float16.
 hipError_t op_gemm_loss_f32(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
 hipError_t op_gemm_loss_bf16(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
 hipError_t op_gemm_loss_f16(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
-hipError_t op_gemm_blend(int type, int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
+hipError_t op_gemm_blend(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
 
 // Products of e4m3 codes (OP_NT, OP_LINEAR), by the type of bias, residual and
 // result.

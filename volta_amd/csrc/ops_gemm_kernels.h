@@ -235,7 +235,14 @@ __device__ __forceinline__ void op_blend_out(const OpEpilogue& e, int z, int64_t
     }
     store_vec(static_cast<U*>(e.out[0]) + z * e.stride_out + m * e.ld_out + n, cnt, d);
   };
-  if (e.out_type == VOLTA_OP_F32) put(0.0f);
+  if (e.out_type == OP_PLANES) {
+    _Float16* out = static_cast<_Float16*>(e.out[0]) + z * e.stride_out + m * e.ld_out + n;
+    float rest[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) rest[i] = d[i] - to_f(from_f<_Float16>(d[i]));  // exact
+    store_vec(out, cnt, d);
+    store_vec(out + e.plane_out, cnt, rest);
+  } else if (e.out_type == VOLTA_OP_F32) put(0.0f);
   else if (e.out_type == VOLTA_OP_BF16) put((__bf16)0.0f);
   else put((_Float16)0.0f);
 }
@@ -283,7 +290,16 @@ __device__ __forceinline__ void op_epilogue(const OpEpilogue& e, int z, int64_t 
   }
   if constexpr (op_kind_blend(KIND)) {
     float r[V];
-    if (e.blend) load_vec(static_cast<const T*>(e.blend) + z * e.stride_blend + m * e.ld_blend + n, cnt, r);
+    if (e.blend) {
+      const T* from = static_cast<const T*>(e.blend) + z * e.stride_blend + m * e.ld_blend + n;
+      load_vec(from, cnt, r);
+      if (e.plane_blend) {
+        float rest[V];
+        load_vec(from + e.plane_blend, cnt, rest);
+#pragma unroll
+        for (int i = 0; i < V; ++i) r[i] += rest[i];
+      }
+    }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       d0[i] = e.blend ? e.alpha * d0[i] + e.beta * r[i] : e.alpha * d0[i];
@@ -607,8 +623,10 @@ struct Cursor {
 
   __device__ __forceinline__ void place(const OpGemm& g) {
     if constexpr (op_kind_blend(KIND)) {
-      p = op_stage_base<T, P_KC>(static_cast<const T*>(g.p[0]) + z * g.stride_p, g.ld_p, m0, k);
-      q[0] = op_stage_base<T, Q_KC>(static_cast<const T*>(g.q[0]) + z * g.stride_q, g.ld_q, n0, k);
+      p = op_stage_base<T, P_KC>(static_cast<const T*>(g.p[0]) + z * g.stride_p + (piece == 0 ? g.plane_p : 0), g.ld_p,
+                                 m0, k);
+      q[0] = op_stage_base<T, Q_KC>(static_cast<const T*>(g.q[0]) + z * g.stride_q + (piece == 1 ? g.plane_q : 0), g.ld_q,
+                                    n0, k);
     } else {
       p = op_stage_base<T, P_KC>(g.p[piece], g.ld_p, m0, k);
 #pragma unroll
@@ -625,8 +643,13 @@ struct Cursor {
     dp = (P_KC ? (int64_t)dk : dk * g.ld_p) * (int64_t)sizeof(T);
     dq = (Q_KC ? (int64_t)dk : dk * g.ld_q) * (int64_t)sizeof(T);
     k = s * kStageK;
-    piece = LAYOUT == OP_NT && g.pieces > 1 && k >= piece_k(g) ? 1 : 0;
-    if (piece) k -= piece_k(g);
+    if constexpr (op_kind_blend(KIND)) {
+      piece = min(k / piece_k(g), g.pieces - 1);
+      k -= piece * piece_k(g);
+    } else {
+      piece = LAYOUT == OP_NT && g.pieces > 1 && k >= piece_k(g) ? 1 : 0;
+      if (piece) k -= piece_k(g);
+    }
     place(g);
   }
   // Inside the piece, or into the next one.
@@ -637,7 +660,12 @@ struct Cursor {
     for (int i = 0; i < kSubs; ++i) q[i] += dq;
   }
   __device__ __forceinline__ void cross(const OpGemm& g) {
-    if (LAYOUT == OP_NT && g.pieces > 1 && piece == 0 && k >= piece_k(g)) {
+    if (op_kind_blend(KIND) && piece < g.pieces - 1 && k >= piece_k(g)) {
+      ++piece;
+      k -= piece_k(g);
+      place(g);
+    }
+    if (!op_kind_blend(KIND) && LAYOUT == OP_NT && g.pieces > 1 && piece == 0 && k >= piece_k(g)) {
       piece = 1;
       k -= piece_k(g);
       place(g);

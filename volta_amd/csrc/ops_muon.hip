@@ -21,11 +21,16 @@
 // computed and stored twice, and the products that take them read their rows
 // where they would need columns.
 //
-// 16-bit types take float16 products.  X's singular values stay in a range that
-// follows from the coefficients, so X, G and B have fixed units that put them
-// under 2^15: all 11 bits, and no element lost that is not 2^-29 of the largest.
-// bfloat16's 8 bits instead leave the result 1.2 % of its norm off (float16:
-// 0.15 %, as much as rounding the result to bfloat16), whatever the size.
+// The products are float16's.  X's singular values stay in a range that follows
+// from the coefficients, so X, G and the polynomials have fixed units that put
+// them under 2^15: all 11 bits, and no element lost that is not 2^-29 of the
+// largest.  For 16-bit types that is enough: bfloat16's 8 bits instead leave the
+// result 1.2 % of its norm off (float16: 0.15 %, as much as rounding the result
+// to bfloat16), whatever the size.  float32 holds each as two such numbers, 23
+// bits, and takes three products, of all but the two rests: the product left
+// out is 2^-24 of the result, and the sums are chains of half as many additions
+// (of eight products) as those of float32's own matrix instruction, which does a
+// sixteenth of the work in the same time.
 #include "ops_call.h"
 #include "ops_launch.h"
 #include "ops_types.h"
@@ -47,7 +52,8 @@ struct MuonArgs {
   const void* g;       // u, or the gradient
   const float* m;      // momentum, or NULL
   float* m_out;
-  void* x;             // [batch][rows_p][ld_x]
+  _Float16* x;         // [batch][rows_p][ld_x]; float32: two planes of it
+  int64_t plane;
   double* partial;     // [batch][gridDim.x]
   int64_t rows, cols;  // of a matrix
   int64_t rows_p, ld_x, ld_g, ld_m;
@@ -94,10 +100,9 @@ __global__ void __launch_bounds__(256) muon_norm(MuonArgs a) {
   if (threadIdx.x == 0) a.partial[z * gridDim.x + blockIdx.x] = ss;
 }
 
-// T: of u; X: of the products.
-template <typename T, typename X>
+template <typename T>
 __global__ void __launch_bounds__(256) muon_scale(MuonArgs a, int parts) {
-  constexpr int E = 16 / (int)sizeof(X);
+  constexpr int E = 8;
   __shared__ double lds[4];
   const int64_t z = blockIdx.y, per_row = a.ld_x / E, chunks = per_row * a.rows_p;
   double ss = 0.0;
@@ -121,7 +126,13 @@ __global__ void __launch_bounds__(256) muon_scale(MuonArgs a, int parts) {
     // what is behind a row's end was read as 0; no norm makes anything else of it
 #pragma unroll
     for (int k = 0; k < E; ++k) u[k] = k < cnt ? (float)((double)u[k] * per) : 0.0f;
-    store_vec(static_cast<X*>(a.x) + (z * a.rows_p + r) * a.ld_x + c, E, u);
+    _Float16* to = a.x + (z * a.rows_p + r) * a.ld_x + c;
+    store_vec(to, E, u);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < E; ++k) u[k] -= to_f(from_f<_Float16>(u[k]));  // exact
+      store_vec(to + a.plane, E, u);
+    }
   }
 }
 
@@ -138,8 +149,8 @@ struct Units {
 };
 struct Muon {
   volta_op_muon d;
-  int product;             // type of the products
   bool tall, pairs;        // pairs: two steps at once
+  int planes;              // 2: float32
   int64_t rows_p, cols_p;  // padded to whole chunks: the products run over zeros there
   int64_t small, large;
   int parts;
@@ -170,10 +181,9 @@ Muon muon_of(const volta_op_muon* in) {
   d.ld_u = ld_of("ld_u", d.ld_u, d.cols);
   d.ld_m = ld_of("ld_m", d.ld_m, d.cols);
   d.ld_o = ld_of("ld_o", d.ld_o, d.cols);
-  l.product = d.type == VOLTA_OP_F32 ? VOLTA_OP_F32 : VOLTA_OP_F16;
-  const int e = elem_bytes(l.product);
-  l.rows_p = packed_ld(l.product, d.rows);
-  l.cols_p = packed_ld(l.product, d.cols);
+  l.planes = d.type == VOLTA_OP_F32 ? 2 : 1;
+  l.rows_p = packed_ld(VOLTA_OP_F16, d.rows);
+  l.cols_p = packed_ld(VOLTA_OP_F16, d.cols);
   l.tall = d.rows > d.cols;
   l.small = l.tall ? l.cols_p : l.rows_p;
   l.large = l.tall ? l.rows_p : l.cols_p;
@@ -191,15 +201,10 @@ Muon muon_of(const volta_op_muon* in) {
       whole = std::max(whole, std::fabs(p));
       times = std::max(times, std::fabs(q * p));
     }
-    Units& u = l.unit[i];
-    if (l.product == VOLTA_OP_F32) {
-      u = Units{1.0, 1.0, 1.0, 1.0, 1.0};
-    } else {
-      if (!(std::max({r, next, whole}) <= 1024.0 && std::max(poly, times) <= 1e6))
-        refuse("the coefficients let singular values grow past 1024");
-      u = Units{unit_of(r), unit_of(r * r), unit_of(std::max(poly, 1e-6)), unit_of(std::max(whole, 1e-6)),
-                unit_of(std::max(times, 1e-6))};
-    }
+    if (!(std::max({r, next, whole}) <= 1024.0 && std::max(poly, times) <= 1e6))
+      refuse("the coefficients let singular values grow past 1024");
+    l.unit[i] = Units{unit_of(r), unit_of(r * r), unit_of(std::max(poly, 1e-6)), unit_of(std::max(whole, 1e-6)),
+                      unit_of(std::max(times, 1e-6))};
     r = std::max(next * 1.001, 1e-6);
   }
   l.layout[0] = l.tall ? OP_TN : OP_NT;
@@ -209,15 +214,16 @@ Muon muon_of(const volta_op_muon* in) {
   const int64_t N[3] = {l.small, l.small, l.tall ? l.small : l.large};
   const int64_t K[3] = {l.large, l.small, l.small};
   for (int i = 0; i < 3; ++i) {
-    l.plan[i] = op_gemm_plan(e, l.layout[i], i < 2 ? OP_MIRROR : OP_BLEND, M[i], N[i], K[i], 1, (int)d.batch, true);
+    l.plan[i] = op_gemm_plan(2, l.layout[i], i < 2 ? OP_MIRROR : OP_BLEND, M[i], N[i], K[i], l.planes == 2 ? 3 : 1,
+                             (int)d.batch, true);
     l.partial_bytes = std::max(l.partial_bytes, align256(op_gemm_partial_bytes(l.plan[i], OP_BLEND, M[i], N[i], (int)d.batch)));
     if (op_gemm_blocks(l.plan[i], OP_BLEND, M[i], N[i]) * d.batch > kMaxBlocks) refuse("the rows and columns of a product are too many");
   }
   const double one = l.plan[0].us + l.plan[1].us + l.plan[2].us;
   const double two = l.plan[0].us + 5.0 * l.plan[1].us + l.plan[2].us;
   l.pairs = d.steps >= 2 && two < 2.0 * one;
-  l.x_bytes = align256(d.batch * l.rows_p * l.cols_p * e);
-  l.g_bytes = align256(d.batch * l.small * l.small * e);
+  l.x_bytes = align256(d.batch * l.rows_p * l.cols_p * 2 * l.planes);
+  l.g_bytes = align256(d.batch * l.small * l.small * 2 * l.planes);
   l.parts = norm_blocks(d.batch, d.rows * ((d.cols + 3) / 4));
   l.sum_bytes = align256(8 * d.batch * l.parts);
   return l;
@@ -227,9 +233,8 @@ hipError_t passes(const Muon& l, MuonArgs a, hipStream_t st) {
   const dim3 grid((unsigned)l.parts, (unsigned)l.d.batch);
   auto run = [&](auto like) {
     using T = decltype(like);
-    using X = typename std::conditional<sizeof(T) == 4, float, _Float16>::type;
     const hipError_t e = op_launch(muon_norm<T>, grid, dim3(256), st, a);
-    return e != hipSuccess ? e : op_launch(muon_scale<T, X>, grid, dim3(256), st, a, l.parts);
+    return e != hipSuccess ? e : op_launch(muon_scale<T>, grid, dim3(256), st, a, l.parts);
   };
   return l.d.type == VOLTA_OP_F32    ? run(0.0f)
          : l.d.type == VOLTA_OP_BF16 ? run((__bf16)0.0f)
@@ -246,7 +251,11 @@ void run(const Muon& l, MuonArgs a, const OpEpilogue& last, char* workspace, hip
   char* rest = small[l.pairs ? 2 : 1] + l.g_bytes;
   a.partial = reinterpret_cast<double*>(rest);
   float* partial = reinterpret_cast<float*>(rest + l.sum_bytes);
-  a.x = x[0];
+  const int64_t x_size = l.rows_p * l.cols_p, g_size = l.small * l.small;
+  const int64_t x_plane = l.planes == 2 ? d.batch * x_size : 0, g_plane = l.planes == 2 ? d.batch * g_size : 0;
+  const int out_type = l.planes == 2 ? OP_PLANES : VOLTA_OP_F16;
+  a.x = reinterpret_cast<_Float16*>(x[0]);
+  a.plane = x_plane;
   a.rows = d.rows;
   a.cols = d.cols;
   a.rows_p = l.rows_p;
@@ -256,50 +265,61 @@ void run(const Muon& l, MuonArgs a, const OpEpilogue& last, char* workspace, hip
   a.eps = d.eps;
   a.unit = (float)l.unit[0].x;
   check_hip(passes(l, a, st), "norm");
-  const int64_t x_size = l.rows_p * l.cols_p, g_size = l.small * l.small;
-  auto product = [&](int which, const char* p, int64_t ld_p, int64_t stride_p, const char* q, int64_t ld_q,
-                     int64_t stride_q, int64_t M, int64_t N, int64_t K, const OpEpilogue& epi, const char* what) {
+  struct Of {  // a matrix of each of the batch
+    const char* p;
+    int64_t ld, stride, plane;
+  };
+  auto of_x = [&](const char* p) { return Of{p, l.cols_p, x_size, x_plane}; };
+  auto of_small = [&](const char* p) { return Of{p, l.small, g_size, g_plane}; };
+  auto product = [&](int which, const Of& p, const Of& q, int64_t M, int64_t N, int64_t K, const OpEpilogue& epi,
+                     const char* what) {
     OpGemm m{};
-    m.p[0] = m.p[1] = p;
-    m.q[0] = m.q[1] = q;
-    m.ld_p = ld_p;
-    m.ld_q = ld_q;
-    m.stride_p = stride_p;
-    m.stride_q = stride_q;
+    m.p[0] = m.p[1] = p.p;
+    m.q[0] = m.q[1] = q.p;
+    m.ld_p = p.ld;
+    m.ld_q = q.ld;
+    m.stride_p = p.stride;
+    m.stride_q = q.stride;
+    m.plane_p = p.plane;
+    m.plane_q = q.plane;
     m.M = (int32_t)M;
     m.N = (int32_t)N;
     m.K = (int32_t)K;
-    m.pieces = 1;
+    m.pieces = l.planes == 2 ? 3 : 1;
     m.outputs = (int32_t)d.batch;
     m.direct = 1;
     m.partial = partial;
     m.epi = epi;
-    check_hip(op_gemm_blend(l.product, l.layout[which], which < 2 ? OP_MIRROR : OP_BLEND, l.plan[which], m, st), what);
+    check_hip(op_gemm_blend(l.layout[which], which < 2 ? OP_MIRROR : OP_BLEND, l.plan[which], m, st), what);
   };
-  // out = alpha d, in the products' type: matrices of the smaller side
+  auto blend_with = [&](OpEpilogue& o, const Of& r, double beta) {
+    o.beta = (float)beta;
+    o.blend = r.p;
+    o.ld_blend = r.ld;
+    o.stride_blend = r.stride;
+    o.plane_blend = r.plane;
+  };
+  // out = alpha d: matrices of the smaller side
   auto to_small = [&](char* out, double alpha) {
     OpEpilogue o{};
     o.out[0] = out;
-    o.out_type = l.product;
+    o.out_type = out_type;
     o.ld_out = l.small;
     o.stride_out = g_size;
+    o.plane_out = g_plane;
     o.alpha = (float)alpha;
     return o;
   };
   auto gram = [&](const char* from, char* out, const Units& u) {
-    product(0, from, l.cols_p, x_size, from, l.cols_p, x_size, l.small, l.small, l.large,
-            to_small(out, u.g / (u.x * u.x)), "gram");
+    product(0, of_x(from), of_x(from), l.small, l.small, l.large, to_small(out, u.g / (u.x * u.x)), "gram");
   };
   auto multiply = [&](const char* p, const char* q, const OpEpilogue& o) {
-    product(1, p, l.small, g_size, q, l.small, g_size, l.small, l.small, l.small, o, "polynomial");
+    product(1, of_small(p), of_small(q), l.small, l.small, l.small, o, "polynomial");
   };
   // b G + c G^2 in `unit`, and a on the diagonal
   auto polynomial = [&](const char* g, char* out, const Units& u, double unit, double diagonal) {
     OpEpilogue o = to_small(out, d.c * unit / (u.g * u.g));
-    o.beta = (float)(d.b * unit / u.g);
-    o.blend = g;
-    o.ld_blend = l.small;
-    o.stride_blend = g_size;
+    blend_with(o, of_small(g), d.b * unit / u.g);
     o.diagonal = (float)(diagonal * unit);
     multiply(g, g, o);
   };
@@ -317,8 +337,7 @@ void run(const Muon& l, MuonArgs a, const OpEpilogue& last, char* workspace, hip
       polynomial(small[0], small[2], v, v.p, d.a);
       // at most the product of both largest values, each at most 2^15 in its unit
       by_unit = u.p * v.p * 0x1p-15;
-      multiply(small[2], small[1], to_small(small[0], l.product == VOLTA_OP_F32 ? 1.0 : by_unit / (u.p * v.p)));
-      if (l.product == VOLTA_OP_F32) by_unit = 1.0;
+      multiply(small[2], small[1], to_small(small[0], by_unit / (u.p * v.p)));
       by = small[0];
     } else {
       by_unit = u.b;
@@ -334,20 +353,16 @@ void run(const Muon& l, MuonArgs a, const OpEpilogue& last, char* workspace, hip
       o = last;
     } else {
       o.out[0] = x[at ^ 1];
-      o.out_type = l.product;
+      o.out_type = out_type;
       o.ld_out = l.cols_p;
       o.stride_out = x_size;
+      o.plane_out = x_plane;
     }
     o.alpha = (float)(to / (by_unit * u.x));
-    if (n == 1) {
-      o.beta = (float)(to * d.a / u.x);
-      o.blend = from;
-      o.ld_blend = l.cols_p;
-      o.stride_blend = x_size;
-    }
+    if (n == 1) blend_with(o, of_x(from), to * d.a / u.x);
     const int64_t M = end ? d.rows : l.rows_p, N = end ? d.cols : l.cols_p;
-    if (l.tall) product(2, from, l.cols_p, x_size, by, l.small, g_size, M, N, l.small, o, "step");
-    else product(2, by, l.small, g_size, from, l.cols_p, x_size, M, N, l.small, o, "step");
+    if (l.tall) product(2, of_x(from), of_small(by), M, N, l.small, o, "step");
+    else product(2, of_small(by), of_x(from), M, N, l.small, o, "step");
     at ^= 1;
   }
 }

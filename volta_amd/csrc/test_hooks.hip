@@ -359,20 +359,20 @@ int32_t volta_hip_op_product8(int32_t type, int32_t tile, int32_t splits, int32_
 }
 
 // out = alpha P Q + beta r of `batch` matrices on a given tile and number of
-// splits (OP_BLEND; OP_MIRROR: of a symmetric result and r), in float32 (0) or
-// float16 (2), synchronously.  All packed, rows of whole 16-byte chunks, a matrix behind the other.
-int32_t volta_hip_op_blend(int32_t type, int32_t layout, int32_t kind, int32_t tile, int32_t splits, int32_t batch, const void* p,
-                           const void* q, const void* r, void* out, int32_t M, int32_t N, int32_t K, float alpha,
-                           float beta) {
+// splits (OP_BLEND; OP_MIRROR: of a symmetric result and r) in float16, or, with
+// `planes` 2, of two planes each, synchronously.  All packed, rows of whole
+// 16-byte chunks, a matrix behind the other, a plane behind the other.
+int32_t volta_hip_op_blend(int32_t planes, int32_t layout, int32_t kind, int32_t tile, int32_t splits, int32_t batch,
+                           const void* p, const void* q, const void* r, void* out, int32_t M, int32_t N, int32_t K,
+                           float alpha, float beta) {
   using namespace volta::ops;
-  const int e = type == VOLTA_OP_F32 ? 4 : 2, per_chunk = 16 / e;
-  if ((type != VOLTA_OP_F32 && type != VOLTA_OP_F16) || M < 1 || N < 1 || K < 1 || batch < 1 || splits < 1) return -1;
-  if (M % per_chunk || N % per_chunk || K % per_chunk || tile < OP_TILE_256 || tile > OP_TILE_64) return -1;
+  if ((planes != 1 && planes != 2) || M < 1 || N < 1 || K < 1 || batch < 1 || splits < 1) return -1;
+  if (M % 8 || N % 8 || K % 8 || tile < OP_TILE_256 || tile > OP_TILE_64) return -1;
   if (kind == OP_MIRROR && (M != N || layout == OP_NN || tile == OP_TILE_256X128 || tile == OP_TILE_64X128)) return -1;
   if (kind == OP_BLEND && layout == OP_TN) return -1;
   for (const void* x : {p, q})
     if ((uintptr_t)x % 16) return -1;
-  const int stages = (K + op_stage_k(e) - 1) / op_stage_k(e);
+  const int stages = (K + 63) / 64 * (planes == 2 ? 3 : 1);
   OpPlan plan{tile, 1, stages, 0.0};
   plan.stages_per_split = (stages + splits - 1) / splits;
   plan.splits = (stages + plan.stages_per_split - 1) / plan.stages_per_split;
@@ -389,7 +389,7 @@ int32_t volta_hip_op_blend(int32_t type, int32_t layout, int32_t kind, int32_t t
   g.M = M;
   g.N = N;
   g.K = K;
-  g.pieces = 1;
+  g.pieces = planes == 2 ? 3 : 1;
   g.outputs = batch;
   g.direct = 1;
   g.partial = static_cast<float*>(ws);
@@ -397,10 +397,15 @@ int32_t volta_hip_op_blend(int32_t type, int32_t layout, int32_t kind, int32_t t
   g.epi.ld_blend = g.epi.ld_out = N;
   g.epi.stride_blend = g.epi.stride_out = (int64_t)M * N;
   g.epi.out[0] = out;
-  g.epi.out_type = type;
+  g.epi.out_type = planes == 2 ? OP_PLANES : VOLTA_OP_F16;
+  if (planes == 2) {
+    g.plane_p = batch * g.stride_p;
+    g.plane_q = batch * g.stride_q;
+    g.epi.plane_blend = g.epi.plane_out = batch * g.epi.stride_out;
+  }
   g.epi.alpha = alpha;
   g.epi.beta = beta;
-  hipError_t rc = op_gemm_blend(type, layout, kind, plan, g, nullptr);
+  hipError_t rc = op_gemm_blend(layout, kind, plan, g, nullptr);
   if (rc == hipSuccess) rc = hipStreamSynchronize(nullptr);
   if (ws) (void)hipFree(ws);
   return rc == hipSuccess ? 0 : -1;

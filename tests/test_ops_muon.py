@@ -77,9 +77,9 @@ def test_both_forms_are_planned():
     wide and tall matrices the first, square ones the second."""
     for batch, m, n, pairs in ((16, 512, 2000, True), (1, 4096, 16384, True), (1, 16384, 4096, True), (1, 512, 2000, False),
                                (1, 1024, 1024, False), (1, 301, 300, False)):
-        e, sides = 2, [-(-v // 8) * 8 for v in (m, n)]
-        small = ops.Muon(m, n, "bf16", batch=batch).workspace_bytes() // batch - 2 * e * sides[0] * sides[1]
-        assert (small >= 3 * e * min(sides) ** 2) == pairs, (batch, m, n, small)
+        (m8, n8), lines = [-(-v // 8) * 8 for v in (m, n)], lambda v: -(-v // 64) * 64  # whole chunks, whole cache lines
+        small = ops.Muon(m, n, "bf16", batch=batch).workspace_bytes() // batch - 2 * 2 * m8 * lines(n8)
+        assert (small >= 3 * 2 * min(m8, n8) * lines(min(m8, n8))) == pairs, (batch, m, n, small)
     # a single step has nothing to go with
     one, two = (ops.Muon(512, 2000, "bf16", batch=16, steps=s).workspace_bytes() for s in (1, 2))
     assert one < two

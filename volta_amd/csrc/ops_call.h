@@ -245,6 +245,12 @@ int64_t packed_ld(int type, int64_t len) {
   const int64_t e = 16 / elem_bytes(type);
   return (len + e - 1) / e * e;
 }
+// Rows of a matrix of our own: whole cache lines, so that a stage's 128 bytes of
+// a row are one (16 x 512 x 2000 of float16 with rows of 4000 bytes: @@).
+int64_t line_ld(int elem, int64_t len) {
+  const int64_t e = 128 / elem;
+  return (len + e - 1) / e * e;
+}
 int64_t packed_bytes(int type, const Operand& o) {
   return align256(o.rows * packed_ld(type, o.len) * elem_bytes(type));
 }

@@ -185,8 +185,8 @@ Piece piece_of(const Loss& l, int64_t count, unsigned run) {
   Piece p{};
   p.count = count;
   p.columns = l.pack_w ? packed_ld(d.type, count) : count;
-  const int64_t x_ld = l.pack_x ? packed_ld(d.type, d.inputs) : d.ld_x, x_len = l.pack_x ? x_ld : d.inputs;
-  const int64_t w_ld = l.pack_w ? p.columns : d.ld_w;
+  const int64_t x_ld = l.pack_x ? line_ld(l.e, d.inputs) : d.ld_x, x_len = l.pack_x ? packed_ld(d.type, d.inputs) : d.inputs;
+  const int64_t w_ld = l.pack_w ? line_ld(l.e, count) : d.ld_w;
   const Operand x{d.rows, x_len, x_ld, 1}, w{d.inputs, p.columns, w_ld, 1}, dz{d.rows, p.columns, l.ld_dz, 1};
   p.z = shape_of(d.type, OP_NN, OP_LOSS_GRAD, d.rows, p.columns, d.inputs, 1, 1, x, w);
   if (run & RUN_DX) p.dx = shape_of(d.type, OP_NT, OP_ADD, d.rows, d.inputs, count, 1, 1, dz, w);
@@ -227,12 +227,12 @@ Loss loss_of(const volta_op_cross_entropy* in, unsigned run) {
     l.pieces = (d.classes + most - 1) / most;
     l.piece = l.pieces == 1 ? d.classes : ((d.classes + l.pieces - 1) / l.pieces + 255) / 256 * 256;
     l.pieces = (d.classes + l.piece - 1) / l.piece;
-    l.ld_dz = packed_ld(d.type, l.piece);
+    l.ld_dz = line_ld(l.e, l.piece);
     l.whole = piece_of(l, l.piece, run);
     l.last = piece_of(l, d.classes - (l.pieces - 1) * l.piece, run);
     l.dz_bytes = align256(d.rows * l.ld_dz * l.e);
-    l.x_bytes = l.pack_x ? packed_bytes(d.type, x) : 0;
-    l.w_bytes = l.pack_w ? align256(d.inputs * packed_ld(d.type, l.piece) * l.e) : 0;
+    l.x_bytes = l.pack_x ? align256(d.rows * line_ld(l.e, d.inputs) * l.e) : 0;
+    l.w_bytes = l.pack_w ? align256(d.inputs * line_ld(l.e, l.piece) * l.e) : 0;
     l.sum_bytes = l.pieces > 1 && (run & RUN_DX) ? align256(4 * d.rows * d.inputs) : 0;
     l.partial_bytes = align256(4 * strips_of(d.rows) * l.piece);
     l.unit_bytes = d.type == VOLTA_OP_F16 ? 256 : 0;
@@ -350,7 +350,7 @@ int32_t volta_op_cross_entropy_backward(const volta_op_cross_entropy* in, const 
     };
     if (unit)
       check_hip(op_launch(unit_kernel, dim3(1), dim3(1024), st, dloss, labels, d.rows, unit), "unit");
-    if (l.pack_x) pack(x, d.rows, d.inputs, d.ld_x, x_new, packed_ld(d.type, d.inputs));
+    if (l.pack_x) pack(x, d.rows, d.inputs, d.ld_x, x_new, line_ld(l.e, d.inputs));
     const void* px = l.pack_x ? x_new : x;
     for (int64_t i = 0; i < l.pieces; ++i) {
       const bool end = i == l.pieces - 1;
@@ -359,7 +359,7 @@ int32_t volta_op_cross_entropy_backward(const volta_op_cross_entropy* in, const 
       auto classes_from = [&](void* v) { return v ? static_cast<char*>(v) + first * l.e : nullptr; };
       const void* pw = classes_from(const_cast<void*>(w));
       if (l.pack_w) {
-        pack(pw, d.inputs, p.count, d.ld_w, w_new, packed_ld(d.type, p.count));
+        pack(pw, d.inputs, p.count, d.ld_w, w_new, line_ld(l.e, p.count));
         pw = w_new;
       }
       OpEpilogue epi{};

@@ -56,7 +56,7 @@ struct MuonArgs {
   int64_t plane;
   double* partial;     // [batch][gridDim.x]
   int64_t rows, cols;  // of a matrix
-  int64_t rows_p, ld_x, ld_g, ld_m;
+  int64_t rows_p, cols_p, ld_x, ld_g, ld_m;
   float beta, eps, unit;
   int32_t nesterov;
 };
@@ -104,7 +104,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) muon_scale(MuonArgs a, int parts) {
   constexpr int E = 8;
   __shared__ double lds[4];
-  const int64_t z = blockIdx.y, per_row = a.ld_x / E, chunks = per_row * a.rows_p;
+  const int64_t z = blockIdx.y, per_row = a.cols_p / E, chunks = per_row * a.rows_p;
   double ss = 0.0;
   for (int i = threadIdx.x; i < parts; i += 256) ss += a.partial[z * parts + i];
   ss = block_sum(ss, lds);
@@ -153,6 +153,7 @@ struct Muon {
   int planes;              // 2: float32
   int64_t rows_p, cols_p;  // padded to whole chunks: the products run over zeros there
   int64_t small, large;
+  int64_t ld_x, ld_small;
   int parts;
   Units unit[kMaxSteps];
   int layout[3];           // of G, the small products and X'
@@ -222,8 +223,10 @@ Muon muon_of(const volta_op_muon* in) {
   const double one = l.plan[0].us + l.plan[1].us + l.plan[2].us;
   const double two = l.plan[0].us + 5.0 * l.plan[1].us + l.plan[2].us;
   l.pairs = d.steps >= 2 && two < 2.0 * one;
-  l.x_bytes = align256(d.batch * l.rows_p * l.cols_p * 2 * l.planes);
-  l.g_bytes = align256(d.batch * l.small * l.small * 2 * l.planes);
+  l.ld_x = line_ld(2, l.cols_p);
+  l.ld_small = line_ld(2, l.small);
+  l.x_bytes = align256(d.batch * l.rows_p * l.ld_x * 2 * l.planes);
+  l.g_bytes = align256(d.batch * l.small * l.ld_small * 2 * l.planes);
   l.parts = norm_blocks(d.batch, d.rows * ((d.cols + 3) / 4));
   l.sum_bytes = align256(8 * d.batch * l.parts);
   return l;
@@ -251,7 +254,7 @@ void run(const Muon& l, MuonArgs a, const OpEpilogue& last, char* workspace, hip
   char* rest = small[l.pairs ? 2 : 1] + l.g_bytes;
   a.partial = reinterpret_cast<double*>(rest);
   float* partial = reinterpret_cast<float*>(rest + l.sum_bytes);
-  const int64_t x_size = l.rows_p * l.cols_p, g_size = l.small * l.small;
+  const int64_t x_size = l.rows_p * l.ld_x, g_size = l.small * l.ld_small;
   const int64_t x_plane = l.planes == 2 ? d.batch * x_size : 0, g_plane = l.planes == 2 ? d.batch * g_size : 0;
   const int out_type = l.planes == 2 ? OP_PLANES : VOLTA_OP_F16;
   a.x = reinterpret_cast<_Float16*>(x[0]);
@@ -259,7 +262,8 @@ void run(const Muon& l, MuonArgs a, const OpEpilogue& last, char* workspace, hip
   a.rows = d.rows;
   a.cols = d.cols;
   a.rows_p = l.rows_p;
-  a.ld_x = l.cols_p;
+  a.cols_p = l.cols_p;
+  a.ld_x = l.ld_x;
   a.ld_g = d.ld_u;
   a.ld_m = d.ld_m;
   a.eps = d.eps;
@@ -269,8 +273,8 @@ void run(const Muon& l, MuonArgs a, const OpEpilogue& last, char* workspace, hip
     const char* p;
     int64_t ld, stride, plane;
   };
-  auto of_x = [&](const char* p) { return Of{p, l.cols_p, x_size, x_plane}; };
-  auto of_small = [&](const char* p) { return Of{p, l.small, g_size, g_plane}; };
+  auto of_x = [&](const char* p) { return Of{p, l.ld_x, x_size, x_plane}; };
+  auto of_small = [&](const char* p) { return Of{p, l.ld_small, g_size, g_plane}; };
   auto product = [&](int which, const Of& p, const Of& q, int64_t M, int64_t N, int64_t K, const OpEpilogue& epi,
                      const char* what) {
     OpGemm m{};
@@ -304,7 +308,7 @@ void run(const Muon& l, MuonArgs a, const OpEpilogue& last, char* workspace, hip
     OpEpilogue o{};
     o.out[0] = out;
     o.out_type = out_type;
-    o.ld_out = l.small;
+    o.ld_out = l.ld_small;
     o.stride_out = g_size;
     o.plane_out = g_plane;
     o.alpha = (float)alpha;
@@ -354,7 +358,7 @@ void run(const Muon& l, MuonArgs a, const OpEpilogue& last, char* workspace, hip
     } else {
       o.out[0] = x[at ^ 1];
       o.out_type = out_type;
-      o.ld_out = l.cols_p;
+      o.ld_out = l.ld_x;
       o.stride_out = x_size;
       o.plane_out = x_plane;
     }

@@ -246,7 +246,8 @@ int64_t packed_ld(int type, int64_t len) {
   return (len + e - 1) / e * e;
 }
 // Rows of a matrix of our own: whole cache lines, so that a stage's 128 bytes of
-// a row are one (16 x 512 x 2000 of float16 with rows of 4000 bytes: @@).
+// a row are one (dx of 1000 rows of 10007 classes in float16, with rows of 20016
+// bytes: 34.1 us, and 30.0 so).
 int64_t line_ld(int elem, int64_t len) {
   const int64_t e = 128 / elem;
   return (len + e - 1) / e * e;

@@ -623,7 +623,7 @@ struct Cursor {
 
   __device__ __forceinline__ void place(const OpGemm& g) {
     if constexpr (op_kind_blend(KIND)) {
-      p = op_stage_base<T, P_KC>(static_cast<const T*>(g.p[0]) + z * g.stride_p + (piece == 0 ? g.plane_p : 0), g.ld_p,
+      p = op_stage_base<T, P_KC>(static_cast<const T*>(g.p[0]) + z * g.stride_p + (g.pieces == 3 && piece == 0 ? g.plane_p : 0), g.ld_p,
                                  m0, k);
       q[0] = op_stage_base<T, Q_KC>(static_cast<const T*>(g.q[0]) + z * g.stride_q + (piece == 1 ? g.plane_q : 0), g.ld_q,
                                     n0, k);
@@ -1205,6 +1205,129 @@ __global__ void __launch_bounds__(512) op_gemm_middle(OpGemm g) {
 }
 
 // ---------------------------------------------------------------------------
+// Small product of pairs of float16 numbers (OP_BLEND, OP_MIRROR): op_gemm_middle
+// with both planes of both operands in a stage, so that three products are made
+// of what is loaded, and read from LDS, once.  The products with a rest have a
+// sum of their own, which joins the other at the end.  64x64 of D: X' of 1024 x
+// 1024 13.4 us, 0.55 a stage from barrier to barrier, for 18.2 with the three
+// products one after the other (float32's own matrix instruction: 26.7).
+// ---------------------------------------------------------------------------
+template <int LAYOUT, int KIND, int BM, int BN, int WGM, int WGN, int NST>
+__global__ void __launch_bounds__(512) op_gemm_pairs(OpGemm g) {
+  static_assert(WGM * WGN == 8, "eight waves");
+  using T = _Float16;
+  constexpr int WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
+  constexpr bool P_KC = LAYOUT != OP_TN, Q_KC = LAYOUT == OP_NT;
+  using PT = Tile<T, BM, P_KC, 8>;
+  using QT = Tile<T, BN, Q_KC, 8>;
+  constexpr int kStageK = PT::kStageK, kStageBytes = 2 * (PT::kBytes + QT::kBytes);
+  constexpr int kStageLoads = 2 * (PT::kLoads + QT::kLoads);
+  __shared__ __attribute__((aligned(16))) char lds[NST * kStageBytes];  // [stage][P, its rests, Q, its rests]
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WGN, wn = wave % WGN;
+  const OpPlace place = op_place<true, KIND == OP_MIRROR>(g);
+  const int tm = place.tm, tn = place.tn, m0 = tm * BM, n0 = tn * BN, z = place.z, split = place.split;
+  PT pt;
+  QT qt;
+  pt.init(g.ld_p, g.M - m0, wave, lane);
+  qt.init(g.ld_q, g.N - n0, wave, lane);
+  const int64_t rest_p = g.plane_p * (int64_t)sizeof(T), rest_q = g.plane_q * (int64_t)sizeof(T);
+  const int s_begin = split * g.stages_per_split;
+  const int S = min((g.K + kStageK - 1) / kStageK, s_begin + g.stages_per_split) - s_begin;
+  Cursor<T, LAYOUT, KIND> next;
+  next.init(g, m0, n0, z, s_begin, 1);
+  auto load = [&](uint32_t to, auto whole) {
+    constexpr bool W = decltype(whole)::value;
+    const int k_left = W ? kStageK : g.K - next.k;
+    const uint32_t q = to + 2 * PT::kBytes;
+    if (W || k_left >= kStageK) {
+      qt.issue(next.q[0], q, wave);
+      pt.issue(next.p, to, wave);
+      qt.issue(next.q[0] + rest_q, q + QT::kBytes, wave);
+      pt.issue(next.p + rest_p, to + PT::kBytes, wave);
+    } else {
+      qt.issue_tail(next.q[0], q, wave, lane, k_left);
+      pt.issue_tail(next.p, to, wave, lane, k_left);
+      qt.issue_tail(next.q[0] + rest_q, q + QT::kBytes, wave, lane, k_left);
+      pt.issue_tail(next.p + rest_p, to + PT::kBytes, wave, lane, k_left);
+    }
+    next.step();
+  };
+
+  floatx4 acc[TM][TN], small[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = small[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  chunk16 fp[2][TM][2], fq[2][TN][2];  // [plane][block][half of k]
+
+  int from = 0, to = (NST - 1) * kStageBytes;
+  const uint32_t lds_byte = op_lds_byte(lds);
+  auto stage = [&](int s, auto whole) {
+    constexpr bool W = decltype(whole)::value;
+#pragma unroll
+    for (int plane = 0; plane < 2; ++plane)
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        const char* at = lds + from;
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+          fq[plane][j][kk] = QT::frag(at + 2 * PT::kBytes + plane * QT::kBytes, wn * WN + j * 16, kk, lane);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) fp[plane][i][kk] = PT::frag(at + plane * PT::kBytes, wm * WM + i * 16, kk, lane);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+    if (W || s + NST - 1 < S) {
+      load(lds_byte + to, whole);
+      op_wait_loads<(NST - 2) * kStageLoads>();  // stage s + 1 is there
+    } else {
+      op_wait_loads<0>();
+    }
+    to = from;
+    from = from == (NST - 1) * kStageBytes ? 0 : from + kStageBytes;
+    op_wait_lds();
+    op_barrier();
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          acc[i][j] = Mfma<T>::mul(0, fq[0][j][kk], fp[0][i][kk], acc[i][j]);
+          small[i][j] = Mfma<T>::mul(0, fq[0][j][kk], fp[1][i][kk], small[i][j]);
+          small[i][j] = Mfma<T>::mul(0, fq[1][j][kk], fp[0][i][kk], small[i][j]);
+        }
+    __builtin_amdgcn_s_setprio(0);
+    op_barrier();
+  };
+
+  if (S > 0) {
+#pragma unroll 1
+    for (int i = 0; i < NST - 1 && i < S; ++i) load(lds_byte + i * kStageBytes, std::false_type());
+    if (S >= NST - 1) op_wait_loads<(NST - 2) * kStageLoads>();
+    else op_wait_loads<0>();
+    op_barrier();
+    if (wave >= 4) op_barrier();
+    for (int s = 0; s < S; ++s) {
+      for (int n = min(next.whole_steps(g), S - (NST - 1) - s); n > 0; --n, ++s) stage(s, std::true_type());
+      if (s < S) stage(s, std::false_type());
+    }
+    if (wave < 4) op_barrier();
+  }
+  __syncthreads();  // the ring is free
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = acc[i][j] + small[i][j];
+  static_assert(8 * op_region_bytes<TM, TN> <= NST * kStageBytes, "output regions fit the ring");
+  op_write_out<T, KIND>(g, acc, lds + wave * op_region_bytes<TM, TN>, lane, m0 + wm * WM, n0 + wn * WN, z, split,
+                        tm != tn);
+}
+
+// ---------------------------------------------------------------------------
 // Skinny product, few rows: reading the weights bounds the time.  A block
 // takes 16 MT rows and BN columns (of each weight matrix) and its waves take turns
 // over the stages of k, each with a ring of its own in LDS for both operands
@@ -1500,6 +1623,14 @@ hipError_t launch_middle(OpGemm& g, hipStream_t st) {
                    op_grid<kFlat<KIND>, KIND == OP_MIRROR>(g), dim3(512), st, g);
 }
 
+template <int LAYOUT, int KIND>
+hipError_t launch_pairs(OpGemm g, hipStream_t st) {
+  g.tiles_m = (g.M + 63) / 64;
+  g.tiles_n = (g.N + 63) / 64;
+  g.pieces = 1;
+  return op_launch(op_gemm_pairs<LAYOUT, KIND, 64, 64, 2, 4, 4>, op_grid<true, KIND == OP_MIRROR>(g), dim3(512), st, g);
+}
+
 template <typename T, int LAYOUT, int KIND>
 hipError_t launch_large(OpGemm& g, hipStream_t st) {
   constexpr int SN = KIND == OP_GATED ? 128 : 256;
@@ -1547,7 +1678,11 @@ hipError_t launch(const OpPlan& plan, OpGemm& g, hipStream_t st) {
     }
   } else if (plan.tile == OP_TILE_64) {
     constexpr int WGM = KIND == OP_GATED ? 4 : 2;  // a wave has columns of both weight matrices
-    if (g.direct || kDirectOnly) e = launch_middle<T, LAYOUT, KIND, 64, 64, WGM, 8 / WGM, 2, 4>(g, st);
+    bool pairs = false;
+    if constexpr (op_kind_blend(KIND)) pairs = g.pieces == 3;
+    if (pairs) {
+      if constexpr (op_kind_blend(KIND)) e = launch_pairs<LAYOUT, KIND>(g, st);
+    } else if (g.direct || kDirectOnly) e = launch_middle<T, LAYOUT, KIND, 64, 64, WGM, 8 / WGM, 2, 4>(g, st);
     else if constexpr (!kDirectOnly) e = launch_staged<T, LAYOUT, KIND, 64, 64>(g, st);
   } else if (plan.tile == OP_TILE_128) {
     if (g.direct || kDirectOnly) e = launch_middle<T, LAYOUT, KIND, 128, 128, 2, 4, 1, 4>(g, st);

@@ -25,6 +25,7 @@ constexpr TileCost kTiles[OP_TILES] = {
     {256, 256, 6.0, 0.95, 0.55e6}, {256, 128, 4.4, 0.80, 0.52e6}, {128, 128, 3.2, 0.43, 0.47e6}, {64, 128, 2.4, 0.33, 0.42e6}, {64, 64, 2.2, 0.23, 0.38e6},
     {16, 32, 1.0, 0.0, 0.45e6},    {32, 32, 1.0, 0.0, 0.45e6},    {64, 32, 1.2, 0.0, 0.45e6},
 };
+constexpr double kPairStage = 0.55;                        // of op_gemm_pairs: a stage of all three products
 constexpr double kSkinnyBytes = 80e3;                      // what a CU's waves load in a microsecond
 constexpr double kReadBytes = 5.5e6;                       // what the chip reads in a microsecond
 constexpr double kLaunchUs = 2.2;                          // of a launch, whatever it does
@@ -37,10 +38,10 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 OpPlan op_gemm_plan(int elem_bytes, int layout, int kind, int64_t M, int64_t N, int64_t K, int pieces, int outputs,
                     bool direct) {
-  const int64_t stages = pieces * ceil_div(K, op_stage_k(elem_bytes));
+  const int64_t all_stages = pieces * ceil_div(K, op_stage_k(elem_bytes));
   const int planes = kind == OP_GATED ? 2 : outputs, subs = kind == OP_GATED ? 2 : 1;
-  OpPlan best{OP_TILE_128, 1, (int32_t)stages, 0.0};
-  if (stages == 0 || M == 0) return best;
+  OpPlan best{OP_TILE_128, 1, (int32_t)all_stages, 0.0};
+  if (all_stages == 0 || M == 0) return best;
   // every product reads both operands, from memory at the rate of memory
   const double read_us = (double)elem_bytes * pieces * K * ((double)M + (double)subs * N * outputs) / kReadBytes;
   double best_us = 1e30;
@@ -54,7 +55,9 @@ OpPlan op_gemm_plan(int elem_bytes, int layout, int kind, int64_t M, int64_t N, 
     const int64_t side = ceil_div(M, c.bm);
     const int64_t tiles = (kind == OP_MIRROR ? side * (side + 1) / 2 : side * ceil_div(N, sn)) * outputs;
     const int waves = !skinny ? 1 : kind == OP_GATED || c.bm > 16 ? 4 : 8;
-    double stage_us = c.stage, tile_read_us = read_us;
+    const bool pairs = pieces == 3 && t == OP_TILE_64;  // three products a stage
+    const int64_t stages = pairs ? all_stages / 3 : all_stages;
+    double stage_us = pairs ? kPairStage : c.stage, tile_read_us = read_us;
     // half cache lines of W: whole ones are fetched (134 MB of W from memory: 40 us in 64-byte pieces, 29 in 128)
     const bool halves = layout == OP_NN && sn * elem_bytes < 128;
     if (halves) tile_read_us *= 1.45;

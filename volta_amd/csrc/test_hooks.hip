@@ -372,7 +372,7 @@ int32_t volta_hip_op_blend(int32_t planes, int32_t layout, int32_t kind, int32_t
   if (kind == OP_BLEND && layout == OP_TN) return -1;
   for (const void* x : {p, q})
     if ((uintptr_t)x % 16) return -1;
-  const int stages = (K + 63) / 64 * (planes == 2 ? 3 : 1);
+  const int stages = (K + 63) / 64 * (planes == 2 && tile != OP_TILE_64 ? 3 : 1);
   OpPlan plan{tile, 1, stages, 0.0};
   plan.stages_per_split = (stages + splits - 1) / splits;
   plan.splits = (stages + plan.stages_per_split - 1) / plan.stages_per_split;

@@ -225,8 +225,8 @@ int32_t volta_op_cross_entropy_forward(const volta_op_cross_entropy* d, const vo
  * their mean), and the forward's lse: dz = (exp(z - lse) - [label]) dloss, 0 in
  * a row without a label, whatever else that row holds in lse and dloss; dx =
  * dz W^T; dw = x^T dz; db = the column sums of dz.  z is formed anew, some
- * classes at a time: as many as fit 256 MiB of dz, so that no more than that is
- * kept at once.  dx, dw and db may be NULL where not wanted (at least one is).
+ * classes at a time: as many as fit 256 MiB of dz (256 of them at least), so that
+ * no more than that is kept at once.  dx, dw and db may be NULL where not wanted (at least one is).
  * dz is rounded to the type before the products and the sums, half a step of
  * each; float16 holds it in units of a power of two, which puts the largest
  * |dloss| in [2^14, 2^15).  A label of `classes` or more makes the row's dz NaN. */

@@ -135,16 +135,18 @@ hipError_t quantize(int type, bool blocks, const QuantizeArgs& a, hipStream_t st
 __global__ void __launch_bounds__(256) turn_scales(const float* from, float* to, int64_t rows, int64_t rows_p, int blocks) {
   __shared__ float lds[32][33];
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5, b0 = blockIdx.y * 32;
-  const int64_t r0 = (int64_t)blockIdx.x * 32;
+  for (int64_t r0 = (int64_t)blockIdx.x * 32; r0 < rows; r0 += (int64_t)gridDim.x * 32) {
 #pragma unroll
-  for (int i = 0; i < 32; i += 8) {
-    const int64_t r = r0 + y + i;
-    if (r < rows && b0 + x < blocks) lds[y + i][x] = from[r * blocks + b0 + x];
+    for (int i = 0; i < 32; i += 8) {
+      const int64_t r = r0 + y + i;
+      if (r < rows && b0 + x < blocks) lds[y + i][x] = from[r * blocks + b0 + x];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+      if (b0 + y + i < blocks && r0 + x < rows) to[(b0 + y + i) * rows_p + r0 + x] = lds[x][y + i];
+    __syncthreads();
   }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 32; i += 8)
-    if (b0 + y + i < blocks && r0 + x < rows) to[(b0 + y + i) * rows_p + r0 + x] = lds[x][y + i];
 }
 
 struct Linear8 {
@@ -271,7 +273,7 @@ int32_t volta_op_linear8_forward(const volta_op_linear8* in, const void* x, cons
     char* ws = static_cast<char*>(workspace);
     if (l.turned_bytes && d.rows > 0) {
       float* to = reinterpret_cast<float*>(ws);
-      const dim3 grid((unsigned)(l.rows_p / 32), (unsigned)((l.blocks + 31) / 32));
+      const dim3 grid((unsigned)std::min<int64_t>(l.rows_p / 32, 1 << 16), (unsigned)((l.blocks + 31) / 32));
       check_hip(op_launch(turn_scales, grid, dim3(256), st, x_scales, to, d.rows, l.rows_p, (int)l.blocks), "scales");
       epi.sx = to;
       epi.ld_sx = 1;

@@ -85,8 +85,11 @@ hipError_t join_rows(const JoinArgs& a, hipStream_t st) {
 __global__ void __launch_bounds__(1024) unit_kernel(const float* dloss, const int32_t* labels, int64_t rows, float* unit) {
   __shared__ uint32_t lds[16];
   uint32_t m = 0;
-  for (int64_t i = threadIdx.x; i < rows; i += 1024)
-    if (labels[i] >= 0) m = max(m, __float_as_uint(fabsf(dloss[i])));
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < rows; i += 1024) {
+    const uint32_t v = __float_as_uint(fabsf(dloss[i]));
+    m = max(m, labels[i] >= 0 ? v : 0u);
+  }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off, kWave));
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = m;

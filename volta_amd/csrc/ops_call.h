@@ -218,17 +218,18 @@ void check_workspace(const void* p, int64_t have, int64_t want) {
 }
 
 hipError_t gemm(int type, int layout, int kind, const OpPlan& plan, const OpGemm& g, hipStream_t st) {
+  return type == VOLTA_OP_F32    ? op_gemm_f32(layout, kind, plan, g, st)
+         : type == VOLTA_OP_BF16 ? op_gemm_bf16(layout, kind, plan, g, st)
+                                 : op_gemm_f16(layout, kind, plan, g, st);
+}
+hipError_t gemm(int type, int layout, int kind, const OpPlan& plan, const OpGemmMore& g, hipStream_t st) {
   if (type == VOLTA_OP_E4M3)
     return g.epi.out_type == VOLTA_OP_F32    ? op_gemm8_f32(plan, g, st)
            : g.epi.out_type == VOLTA_OP_BF16 ? op_gemm8_bf16(plan, g, st)
                                              : op_gemm8_f16(plan, g, st);
-  if (kind == OP_STATS || kind == OP_LOSS_GRAD || kind == OP_ADD)
-    return type == VOLTA_OP_F32    ? op_gemm_loss_f32(layout, kind, plan, g, st)
-           : type == VOLTA_OP_BF16 ? op_gemm_loss_bf16(layout, kind, plan, g, st)
-                                   : op_gemm_loss_f16(layout, kind, plan, g, st);
-  return type == VOLTA_OP_F32    ? op_gemm_f32(layout, kind, plan, g, st)
-         : type == VOLTA_OP_BF16 ? op_gemm_bf16(layout, kind, plan, g, st)
-                                 : op_gemm_f16(layout, kind, plan, g, st);
+  return type == VOLTA_OP_F32    ? op_gemm_loss_f32(layout, kind, plan, g, st)
+         : type == VOLTA_OP_BF16 ? op_gemm_loss_bf16(layout, kind, plan, g, st)
+                                 : op_gemm_loss_f16(layout, kind, plan, g, st);
 }
 
 // An operand of a product as its description gives it: rows of `len`
@@ -302,10 +303,11 @@ Shape shape_of(int type, int layout, int kind, int64_t M, int64_t N, int64_t K, 
 // One product of a call: its operands' matrices (one, or p.count / q.count
 // different ones), epilogue and workspace.  Returns whether it took the direct
 // loads.
-bool product(int type, const Shape& s, const void* const* ps, const void* const* qs, const OpEpilogue& epi,
+template <typename E>
+bool product(int type, const Shape& s, const void* const* ps, const void* const* qs, const E& epi,
              char* workspace, hipStream_t st, const char* what) {
   if (s.M == 0 || s.N == 0) return true;
-  OpGemm g{};
+  OpGemmOf<E> g{};
   PackArgs pack{};
   char* at = workspace + s.partial_bytes;
   bool direct = true;

@@ -257,7 +257,7 @@ int32_t volta_op_linear8_forward(const volta_op_linear8* in, const void* x, cons
                                        {"residual", residual, d.rows, d.outputs, d.ld_residual, e, false},
                                        {"y", y, d.rows, d.outputs, d.ld_y, e, true}},
                                       {{"residual", "y"}}, workspace, bytes, stream);
-    OpEpilogue epi{};
+    OpEpilogueMore epi{};
     epi.act = d.act;
     epi.out_type = d.type;
     epi.bias[0] = bias;

@@ -42,6 +42,11 @@ struct OpEpilogue {
   void* pre[2];
   int64_t ld_out, ld_residual, ld_pre;
   const float* unit;  // OP_STORE in float16: one number on the device, what the sums are multiplied by; NULL: 1
+};
+
+// What the kinds from OP_STATS on and the products of codes take besides; the
+// others' launches are not to carry it (0.3 us of a small one).
+struct OpEpilogueMore : OpEpilogue {
   // OP_STATS, OP_LOSS_GRAD.  The launch's columns are the classes class0 ..
   // class0 + classes - 1; what D has behind them is padding: no part of the
   // statistics, a gradient of 0.
@@ -65,28 +70,31 @@ struct OpEpilogue {
   int64_t plane_blend, plane_out;  // of r and, with out_type OP_PLANES, of out: elements to the second plane; r: 0, none
   int32_t out_type;       // enum volta_op_type; also of a product of codes
   int64_t ld_blend, ld_w, stride_blend, stride_w, stride_out;
-};
-
-struct OpGemm {
-  const void* p[2];  // pieces of the sum over k (dx of the gated layer has two)
-  const void* q[2];  // OP_NT: the piece's Q; OP_GATED: gate and up; OP_TN: one for each output
-  int64_t ld_p, ld_q;
-  int32_t M, N, K;   // K of one piece
-  int32_t pieces;    // 1 or 2 pieces of the sum; OP_BLEND: 1 or 3
-  int32_t outputs;   // 1 or 2 outputs (OP_STORE of OP_TN); OP_BLEND: matrices
   int64_t stride_p, stride_q;  // OP_BLEND: elements from one matrix to the next
   // OP_BLEND with 3 pieces: P and Q are sums of two planes, the second (the
   // rests) so many elements behind the first: second by first, first by second,
   // then first by first, so that the small sums are rounded while they are small.
   // One piece: 0
   int64_t plane_p, plane_q;
+};
+
+template <typename E>
+struct OpGemmOf {
+  const void* p[2];  // pieces of the sum over k (dx of the gated layer has two)
+  const void* q[2];  // OP_NT: the piece's Q; OP_GATED: gate and up; OP_TN: one for each output
+  int64_t ld_p, ld_q;
+  int32_t M, N, K;   // K of one piece
+  int32_t pieces;    // 1 or 2 pieces of the sum; OP_BLEND: 1 or 3
+  int32_t outputs;   // 1 or 2 outputs (OP_STORE of OP_TN); OP_BLEND: matrices
   int32_t direct;    // rows of P and Q are 16-byte aligned and whole 16-byte chunks long
   // from the plan
   int32_t tiles_m, tiles_n;
   int32_t splits, stages_per_split;
   float* partial;    // splits > 1: [split][output or gate/up][M][N]
-  OpEpilogue epi;
+  E epi;
 };
+using OpGemm = OpGemmOf<OpEpilogue>;
+using OpGemmMore = OpGemmOf<OpEpilogueMore>;
 
 // Tiles, by rows x columns of D (gated: half the columns of each weight
 // matrix).  The skinny ones take 16, 32 or 64 rows and 32 columns (of each
@@ -132,16 +140,16 @@ hipError_t op_gemm_f32(int layout, int kind, const OpPlan& plan, OpGemm g, hipSt
 hipError_t op_gemm_bf16(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
 hipError_t op_gemm_f16(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
 // The kinds of an output layer's loss; and OP_BLEND and OP_MIRROR, in float16.
-hipError_t op_gemm_loss_f32(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
-hipError_t op_gemm_loss_bf16(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
-hipError_t op_gemm_loss_f16(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
-hipError_t op_gemm_blend(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st);
+hipError_t op_gemm_loss_f32(int layout, int kind, const OpPlan& plan, OpGemmMore g, hipStream_t st);
+hipError_t op_gemm_loss_bf16(int layout, int kind, const OpPlan& plan, OpGemmMore g, hipStream_t st);
+hipError_t op_gemm_loss_f16(int layout, int kind, const OpPlan& plan, OpGemmMore g, hipStream_t st);
+hipError_t op_gemm_blend(int layout, int kind, const OpPlan& plan, OpGemmMore g, hipStream_t st);
 
 // Products of e4m3 codes (OP_NT, OP_LINEAR), by the type of bias, residual and
 // result.
-hipError_t op_gemm8_f32(const OpPlan& plan, OpGemm g, hipStream_t st);
-hipError_t op_gemm8_bf16(const OpPlan& plan, OpGemm g, hipStream_t st);
-hipError_t op_gemm8_f16(const OpPlan& plan, OpGemm g, hipStream_t st);
+hipError_t op_gemm8_f32(const OpPlan& plan, OpGemmMore g, hipStream_t st);
+hipError_t op_gemm8_bf16(const OpPlan& plan, OpGemmMore g, hipStream_t st);
+hipError_t op_gemm8_f16(const OpPlan& plan, OpGemmMore g, hipStream_t st);
 
 // Entries of a row in OP_STATS' statistics.
 int64_t op_stats_entries(const OpPlan& plan, int64_t N);

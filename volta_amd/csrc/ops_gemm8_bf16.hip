@@ -3,6 +3,6 @@
 
 namespace volta {
 namespace ops {
-hipError_t op_gemm8_bf16(const OpPlan& plan, OpGemm g, hipStream_t st) { return launch8<__bf16>(plan, g, st); }
+hipError_t op_gemm8_bf16(const OpPlan& plan, OpGemmMore g, hipStream_t st) { return launch8<__bf16>(plan, g, st); }
 }  // namespace ops
 }  // namespace volta

@@ -3,6 +3,6 @@
 
 namespace volta {
 namespace ops {
-hipError_t op_gemm8_f32(const OpPlan& plan, OpGemm g, hipStream_t st) { return launch8<float>(plan, g, st); }
+hipError_t op_gemm8_f32(const OpPlan& plan, OpGemmMore g, hipStream_t st) { return launch8<float>(plan, g, st); }
 }  // namespace ops
 }  // namespace volta

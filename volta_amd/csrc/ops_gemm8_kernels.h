@@ -113,7 +113,7 @@ struct RowScales {
   const float* at;  // this lane's row, block 0
   int64_t step;     // from a block to the next
   int last;         // the last block
-  __device__ __forceinline__ void init(const OpGemm& g, int m0, int row) {
+  __device__ __forceinline__ void init(const OpGemmMore& g, int m0, int row) {
     at = g.epi.sx + (int64_t)min(m0 + row, g.M - 1) * g.epi.ld_sx;
     step = g.epi.step_sx;
     last = (g.K + 127) / 128 - 1;
@@ -124,20 +124,20 @@ struct RowScales {
 struct ColumnScales {
   const float* at;
   int last;
-  __device__ __forceinline__ void init(const OpGemm& g, int n) {
+  __device__ __forceinline__ void init(const OpGemmMore& g, int n) {
     at = g.epi.sw + (int64_t)(min(n, g.N - 1) / 128) * g.epi.ld_sw;
     last = (g.K + 127) / 128 - 1;
   }
   __device__ __forceinline__ float of(int b) const { return scalar_load(at + min(b, last)); }
 };
 
-using Cursor8 = Cursor<uint8_t, OP_NT, OP_STORE>;
+using Cursor8 = Cursor<uint8_t, OP_NT, OP_STORE, OpGemmMore>;
 
 // The linear layer's epilogue by op_write_swapped, one copy of the code for
 // each activation.
 template <typename T, int TM, int TN>
-__device__ __forceinline__ void write_linear8(const OpGemm& g, const floatx4 (&acc)[TM][TN], int lane, int m0, int n0) {
-  const OpEpilogue& e = g.epi;
+__device__ __forceinline__ void write_linear8(const OpGemmMore& g, const floatx4 (&acc)[TM][TN], int lane, int m0, int n0) {
+  const OpEpilogueMore& e = g.epi;
   float bias[TN][4], none[4];
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
@@ -174,7 +174,7 @@ __device__ __forceinline__ void write_linear8(const OpGemm& g, const floatx4 (&a
 // (op_gemm_middle).
 // ---------------------------------------------------------------------------
 template <typename T, int BM, int BN, int WGM, int WGN, int KS, int NST>
-__global__ void __launch_bounds__(512) op_gemm8_middle(OpGemm g) {
+__global__ void __launch_bounds__(512) op_gemm8_middle(OpGemmMore g) {
   constexpr int WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
   using PT = Tile<uint8_t, BM, true, 8>;
   using QT = Tile<uint8_t, BN, true, 8>;
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(512) op_gemm8_middle(OpGemm g) {
 // again.
 // ---------------------------------------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) op_gemm8_large(OpGemm g) {
+__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) op_gemm8_large(OpGemmMore g) {
   constexpr int kRegion = 128 * 128, kScales = 8 * kRegion;
   using PR = Region<uint8_t, true, 64, 128>;
   using QR = Region<uint8_t, true, 32, 64>;
@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) o
 // (op_gemm_staged).
 // ---------------------------------------------------------------------------
 template <typename T, int BM, int BN>
-__global__ void __launch_bounds__(256) op_gemm8_staged(OpGemm g) {
+__global__ void __launch_bounds__(256) op_gemm8_staged(OpGemmMore g) {
   constexpr int NW = 4, WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16;
   using PT = Tile<uint8_t, BM, true, NW>;
   using QT = Tile<uint8_t, BN, true, NW>;
@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(256) op_gemm8_staged(OpGemm g) {
 // blocks of k (op_gemm_skinny).
 // ---------------------------------------------------------------------------
 template <typename T, int MT, int NW, int NST, bool DIRECT>
-__global__ void __launch_bounds__(NW * 64) op_gemm8_skinny(OpGemm g) {
+__global__ void __launch_bounds__(NW * 64) op_gemm8_skinny(OpGemmMore g) {
   constexpr int BN = 32, TN = BN / 16;
   using PT = Tile<uint8_t, 16 * MT, true, 1>;
   using QT = Tile<uint8_t, BN, true, 1>;
@@ -678,27 +678,27 @@ __global__ void __launch_bounds__(NW * 64) op_gemm8_skinny(OpGemm g) {
 
 // ---------------------------------------------------------------------------
 template <typename T, int BM, int BN, int WGM, int WGN, int KS, int NST>
-hipError_t launch8_middle(OpGemm& g, hipStream_t st) {
+hipError_t launch8_middle(OpGemmMore& g, hipStream_t st) {
   g.tiles_m = (g.M + BM - 1) / BM;
   g.tiles_n = (g.N + BN - 1) / BN;
   return op_launch(op_gemm8_middle<T, BM, BN, WGM, WGN, KS, NST>,
                    op_grid<true, false>(g), dim3(512), st, g);
 }
 template <typename T>
-hipError_t launch8_large(OpGemm& g, hipStream_t st) {
+hipError_t launch8_large(OpGemmMore& g, hipStream_t st) {
   g.tiles_m = (g.M + 255) / 256;
   g.tiles_n = (g.N + 255) / 256;
   return op_launch(op_gemm8_large<T>, op_grid<true, false>(g), dim3(512), st, g);
 }
 template <typename T, int BM, int BN>
-hipError_t launch8_staged(OpGemm& g, hipStream_t st) {
+hipError_t launch8_staged(OpGemmMore& g, hipStream_t st) {
   g.tiles_m = (g.M + BM - 1) / BM;
   g.tiles_n = (g.N + BN - 1) / BN;
   return op_launch(op_gemm8_staged<T, BM, BN>, op_grid<true, false>(g), dim3(256),
                    st, g);
 }
 template <typename T, int MT, bool DIRECT>
-hipError_t launch8_skinny(OpGemm& g, hipStream_t st) {
+hipError_t launch8_skinny(OpGemmMore& g, hipStream_t st) {
   using S = SkinnyShape<OP_LINEAR, MT, DIRECT>;
   g.tiles_m = (g.M + 16 * MT - 1) / (16 * MT);
   g.tiles_n = (g.N + S::kCols - 1) / S::kCols;
@@ -707,7 +707,7 @@ hipError_t launch8_skinny(OpGemm& g, hipStream_t st) {
 }
 
 template <typename T>
-hipError_t launch8(const OpPlan& plan, OpGemm& g, hipStream_t st) {
+hipError_t launch8(const OpPlan& plan, OpGemmMore& g, hipStream_t st) {
   g.splits = plan.splits;
   g.stages_per_split = plan.stages_per_split;
   hipError_t e = hipErrorInvalidValue;
@@ -739,7 +739,7 @@ hipError_t launch8(const OpPlan& plan, OpGemm& g, hipStream_t st) {
   if (e != hipSuccess || g.splits <= 1) return e;
   const int64_t quads = (int64_t)g.M * ((g.N + 3) / 4);
   const int64_t blocks = (quads + 255) / 256, x = std::min<int64_t>(blocks, int64_t{1} << 20);
-  return op_launch(op_gemm_reduce<T, OP_LINEAR>, dim3((unsigned)x, 1, (unsigned)((blocks + x - 1) / x)), dim3(256), st, g);
+  return op_launch(op_gemm_reduce<T, OP_LINEAR, OpGemmMore>, dim3((unsigned)x, 1, (unsigned)((blocks + x - 1) / x)), dim3(256), st, g);
 }
 
 }  // namespace ops

@@ -4,7 +4,7 @@
 
 namespace volta {
 namespace ops {
-hipError_t op_gemm_blend(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st) {
+hipError_t op_gemm_blend(int layout, int kind, const OpPlan& plan, OpGemmMore g, hipStream_t st) {
   using T = _Float16;
   if (kind == OP_MIRROR) {
     if (layout == OP_NN || g.M != g.N) return hipErrorInvalidValue;

@@ -224,7 +224,7 @@ __device__ __forceinline__ float op_exp(float x) {
 
 // Where a blend goes: in the output's type, w of which joins it last.
 template <int V>
-__device__ __forceinline__ void op_blend_out(const OpEpilogue& e, int z, int64_t m, int n, int cnt, float (&d)[V]) {
+__device__ __forceinline__ void op_blend_out(const OpEpilogueMore& e, int z, int64_t m, int n, int cnt, float (&d)[V]) {
   auto put = [&](auto like) {
     using U = decltype(like);
     if (e.w) {
@@ -249,8 +249,8 @@ __device__ __forceinline__ void op_blend_out(const OpEpilogue& e, int z, int64_t
 
 // The epilogue of V consecutive columns n .. of row m, cnt of them in the
 // matrix: d0 (and, gated, d1) are the sums, b0 and b1 the columns' biases.
-template <typename T, int KIND, int V>
-__device__ __forceinline__ void op_epilogue(const OpEpilogue& e, int z, int64_t m, int n, int cnt, float (&d0)[V],
+template <typename T, int KIND, int V, typename E>
+__device__ __forceinline__ void op_epilogue(const E& e, int z, int64_t m, int n, int cnt, float (&d0)[V],
                                             float (&d1)[V], const float (&b0)[V], const float (&b1)[V]) {
   if constexpr (KIND == OP_LOSS_GRAD) {
     // (p - [label]) dloss, p = exp(z - lse) <= 1.  Rounded to the type, half a
@@ -331,8 +331,8 @@ __device__ __forceinline__ void op_epilogue(const OpEpilogue& e, int z, int64_t 
   }
   store_vec(static_cast<T*>(e.out[z]) + m * e.ld_out + n, cnt, d0);
 }
-template <typename T, int KIND, int V>
-__device__ __forceinline__ void op_biases(const OpEpilogue& e, int n, int cnt, float (&b0)[V], float (&b1)[V]) {
+template <typename T, int KIND, int V, typename E>
+__device__ __forceinline__ void op_biases(const E& e, int n, int cnt, float (&b0)[V], float (&b1)[V]) {
 #pragma unroll
   for (int i = 0; i < V; ++i) b0[i] = b1[i] = 0.0f;
   if constexpr (KIND == OP_STATS || KIND == OP_LOSS_GRAD) {
@@ -359,6 +359,12 @@ __device__ __forceinline__ void op_in_units(float unit, float (&d)[V]) {
     for (int i = 0; i < V; ++i) d[i] *= unit;
   }
 }
+
+// The arguments of a kind's kernels.
+template <int KIND>
+constexpr bool kFlat = KIND >= OP_STATS;  // and their order of blocks (op_place)
+template <int KIND>
+using OpArgs = typename std::conditional<kFlat<KIND>, OpGemmMore, OpGemm>::type;
 
 // A loop over 0 .. N - 1 whose index is a constant of its body.
 template <int N, int I = 0, typename F>
@@ -389,9 +395,9 @@ __device__ __forceinline__ void op_barrier() {
 // neighbours 16, 32 and 48 lanes on the others.  A row whose z are all -inf has
 // a sum of 0.
 template <typename T, int TN>
-__device__ __forceinline__ void op_row_stats(const OpGemm& g, const floatx4 (&d)[TN], int lane, int m0, int n0, float* top_of,
+__device__ __forceinline__ void op_row_stats(const OpGemmMore& g, const floatx4 (&d)[TN], int lane, int m0, int n0, float* top_of,
                                              float* sum_of) {
-  const OpEpilogue& e = g.epi;
+  const OpEpilogueMore& e = g.epi;
   const int m = m0 + (lane & 15), lg = lane >> 4;
   const int label = e.labels && m < g.M ? e.labels[m] : -1;
   float z[TN][4], top = -__builtin_inff(), sum = 0.0f;
@@ -424,7 +430,7 @@ __device__ __forceinline__ void op_row_stats(const OpGemm& g, const floatx4 (&d)
 // LDS: two values a row leave the block instead of its columns.  Every wave of
 // the block calls it.
 template <typename T, int TM, int TN, int WGM, int WGN>
-__device__ __forceinline__ void op_write_stats(const OpGemm& g, const floatx4 (&acc)[TM][TN], char* lds, int lane, int wm,
+__device__ __forceinline__ void op_write_stats(const OpGemmMore& g, const floatx4 (&acc)[TM][TN], char* lds, int lane, int wm,
                                                int wn, int m0, int n0) {
   constexpr int kRows = WGM * TM * 16;
   float* all = reinterpret_cast<float*>(lds);  // [wn][top, sum][rows]
@@ -469,8 +475,8 @@ template <int TM, int TN>
 constexpr int op_region_bytes = op_out_rows<TM, TN> * (TN * 16 + 4) * 4;
 // `mirror`: OP_MIRROR's tile is over the diagonal, and also stored across it, by
 // lanes that take 16 bytes down a column of the region.
-template <typename T, int KIND, int TM, int TN>
-__device__ __forceinline__ void op_write_out(const OpGemm& g, floatx4 (&acc)[TM][TN], char* region, int lane, int m0,
+template <typename T, int KIND, int TM, int TN, typename G>
+__device__ __forceinline__ void op_write_out(const G& g, floatx4 (&acc)[TM][TN], char* region, int lane, int m0,
                                              int n0, int z, int split, bool mirror = false) {
   constexpr bool kGated = KIND == OP_GATED;
   constexpr int kRows = op_out_rows<TM, TN>, RB = kRows / 16, kLd = TN * 16 + 4;
@@ -610,7 +616,7 @@ __device__ __forceinline__ const char* op_stage_base(const void* p, int64_t ld, 
 // Where the next stage to load starts, in every operand (a block's loop takes
 // every `step`-th stage): advanced by additions, since a stage's address
 // computed anew costs a wave more time than its loads.
-template <typename T, int LAYOUT, int KIND>
+template <typename T, int LAYOUT, int KIND, typename Args = OpArgs<KIND>>
 struct Cursor {
   static constexpr bool GATED = KIND == OP_GATED;
   static constexpr bool P_KC = LAYOUT != OP_TN, Q_KC = LAYOUT == OP_NT;
@@ -621,11 +627,11 @@ struct Cursor {
   int k, dk;       // in this piece
   int piece, m0, n0, z;
 
-  __device__ __forceinline__ void place(const OpGemm& g) {
+  __device__ __forceinline__ void place(const Args& g) {
     if constexpr (op_kind_blend(KIND)) {
-      p = op_stage_base<T, P_KC>(static_cast<const T*>(g.p[0]) + z * g.stride_p + (g.pieces == 3 && piece == 0 ? g.plane_p : 0), g.ld_p,
+      p = op_stage_base<T, P_KC>(static_cast<const T*>(g.p[0]) + z * g.epi.stride_p + (g.pieces == 3 && piece == 0 ? g.epi.plane_p : 0), g.ld_p,
                                  m0, k);
-      q[0] = op_stage_base<T, Q_KC>(static_cast<const T*>(g.q[0]) + z * g.stride_q + (piece == 1 ? g.plane_q : 0), g.ld_q,
+      q[0] = op_stage_base<T, Q_KC>(static_cast<const T*>(g.q[0]) + z * g.epi.stride_q + (piece == 1 ? g.epi.plane_q : 0), g.ld_q,
                                     n0, k);
     } else {
       p = op_stage_base<T, P_KC>(g.p[piece], g.ld_p, m0, k);
@@ -634,8 +640,8 @@ struct Cursor {
         q[i] = op_stage_base<T, Q_KC>(g.q[GATED ? i : LAYOUT == OP_TN ? z : piece], g.ld_q, n0, k);
     }
   }
-  __device__ __forceinline__ int piece_k(const OpGemm& g) const { return (g.K + kStageK - 1) / kStageK * kStageK; }
-  __device__ __forceinline__ void init(const OpGemm& g, int m0_, int n0_, int z_, int s, int step) {
+  __device__ __forceinline__ int piece_k(const Args& g) const { return (g.K + kStageK - 1) / kStageK * kStageK; }
+  __device__ __forceinline__ void init(const Args& g, int m0_, int n0_, int z_, int s, int step) {
     m0 = m0_;
     n0 = n0_;
     z = z_;
@@ -659,7 +665,7 @@ struct Cursor {
 #pragma unroll
     for (int i = 0; i < kSubs; ++i) q[i] += dq;
   }
-  __device__ __forceinline__ void cross(const OpGemm& g) {
+  __device__ __forceinline__ void cross(const Args& g) {
     if (op_kind_blend(KIND) && piece < g.pieces - 1 && k >= piece_k(g)) {
       ++piece;
       k -= piece_k(g);
@@ -672,7 +678,7 @@ struct Cursor {
     }
   }
   // Steps from here on whose stages are whole.
-  __device__ __forceinline__ int whole_steps(const OpGemm& g) const {
+  __device__ __forceinline__ int whole_steps(const Args& g) const {
     const int stages = (g.K - k) / kStageK;
     return stages > 0 ? (stages - 1) / (dk / kStageK) + 1 : 0;
   }
@@ -702,10 +708,8 @@ __device__ __forceinline__ void op_tile_of(int b, int tiles_m, int tiles_n, int*
 struct OpPlace {
   int tm, tn, split, z;
 };
-template <int KIND>
-constexpr bool kFlat = KIND >= OP_STATS;
-template <bool FLAT, bool TRIANGLE>
-__device__ __forceinline__ OpPlace op_place(const OpGemm& g) {
+template <bool FLAT, bool TRIANGLE, typename G>
+__device__ __forceinline__ OpPlace op_place(const G& g) {
   OpPlace p;
   if constexpr (!FLAT) {
     op_tile_of(blockIdx.x, g.tiles_m, g.tiles_n, &p.tm, &p.tn);
@@ -759,7 +763,7 @@ __device__ __forceinline__ OpPlace op_place(const OpGemm& g) {
 // takes less.
 // ---------------------------------------------------------------------------
 template <typename T, int LAYOUT, int KIND, int BM, int BN>
-__global__ void __launch_bounds__(256) op_gemm_staged(OpGemm g) {
+__global__ void __launch_bounds__(256) op_gemm_staged(OpArgs<KIND> g) {
   constexpr int NW = 4, WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16;
   constexpr bool kGated = KIND == OP_GATED;
   constexpr int kSubs = kGated ? 2 : 1, SN = BN / kSubs;  // gated: half the columns of each weight matrix
@@ -904,7 +908,7 @@ struct Region : Tile<T, 128, KC, 8> {
 };
 
 template <typename T, int LAYOUT, int KIND>
-__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) op_gemm_large(OpGemm g) {
+__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) op_gemm_large(OpArgs<KIND> g) {
   constexpr bool kGated = KIND == OP_GATED, P_KC = LAYOUT != OP_TN, Q_KC = LAYOUT == OP_NT;
   constexpr int kRegion = 128 * 128, kStageK = 128 / (int)sizeof(T), SN = kGated ? 128 : 256;
   using PR = Region<T, P_KC, 64, 128>;
@@ -1077,7 +1081,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) o
 // third less of LDS and pays 1 to 2 us for adding the halves.
 // ---------------------------------------------------------------------------
 template <typename T, int LAYOUT, int KIND, int BM, int BN, int WGM, int WGN, int KS, int NST>
-__global__ void __launch_bounds__(512) op_gemm_middle(OpGemm g) {
+__global__ void __launch_bounds__(512) op_gemm_middle(OpArgs<KIND> g) {
   static_assert(WGM * WGN == 8, "eight waves");
   constexpr int WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
   constexpr bool kGated = KIND == OP_GATED, P_KC = LAYOUT != OP_TN, Q_KC = LAYOUT == OP_NT;
@@ -1213,7 +1217,7 @@ __global__ void __launch_bounds__(512) op_gemm_middle(OpGemm g) {
 // products one after the other (float32's own matrix instruction: 26.7).
 // ---------------------------------------------------------------------------
 template <int LAYOUT, int KIND, int BM, int BN, int WGM, int WGN, int NST>
-__global__ void __launch_bounds__(512) op_gemm_pairs(OpGemm g) {
+__global__ void __launch_bounds__(512) op_gemm_pairs(OpGemmMore g) {
   static_assert(WGM * WGN == 8, "eight waves");
   using T = _Float16;
   constexpr int WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
@@ -1233,7 +1237,7 @@ __global__ void __launch_bounds__(512) op_gemm_pairs(OpGemm g) {
   QT qt;
   pt.init(g.ld_p, g.M - m0, wave, lane);
   qt.init(g.ld_q, g.N - n0, wave, lane);
-  const int64_t rest_p = g.plane_p * (int64_t)sizeof(T), rest_q = g.plane_q * (int64_t)sizeof(T);
+  const int64_t rest_p = g.epi.plane_p * (int64_t)sizeof(T), rest_q = g.epi.plane_q * (int64_t)sizeof(T);
   const int s_begin = split * g.stages_per_split;
   const int S = min((g.K + kStageK - 1) / kStageK, s_begin + g.stages_per_split) - s_begin;
   Cursor<T, LAYOUT, KIND> next;
@@ -1338,7 +1342,7 @@ __global__ void __launch_bounds__(512) op_gemm_pairs(OpGemm g) {
 // rows, 4096 to 16384, 134 MB: 41 us, and 29 on 64x64 tiles.
 // ---------------------------------------------------------------------------
 template <typename T, int LAYOUT, int KIND, int MT, int BN, int NW, int NST, bool DIRECT>
-__global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
+__global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpArgs<KIND> g) {
   constexpr bool kGated = KIND == OP_GATED, Q_KC = LAYOUT == OP_NT;
   constexpr int kSubs = kGated ? 2 : 1, TNS = BN / 16, TN = TNS * kSubs;
   using PT = Tile<T, 16 * MT, true, 1>;
@@ -1523,8 +1527,8 @@ __global__ void __launch_bounds__(NW * 64) op_gemm_skinny(OpGemm g) {
 // four columns of a row.  Eight splits' sums are loaded at a time.  Bound by
 // its launch and one latency of memory at few rows (8 splits of 16 x 4096:
 // 4.7 us), by memory at many.
-template <typename T, int KIND>
-__global__ void __launch_bounds__(256) op_gemm_reduce(OpGemm g) {
+template <typename T, int KIND, typename Args = OpArgs<KIND>>
+__global__ void __launch_bounds__(256) op_gemm_reduce(Args g) {
   const int quads = (g.N + 3) / 4, z = blockIdx.y;
   const int64_t t = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
   if (t >= (int64_t)g.M * quads) return;
@@ -1559,8 +1563,8 @@ __global__ void __launch_bounds__(256) op_gemm_reduce(OpGemm g) {
 
 // OP_STATS of partial sums: a wave for 256 columns of a row.
 template <typename T>
-__global__ void __launch_bounds__(256) op_stats_reduce(OpGemm g) {
-  const OpEpilogue& e = g.epi;
+__global__ void __launch_bounds__(256) op_stats_reduce(OpGemmMore g) {
+  const OpEpilogueMore& e = g.epi;
   const int lane = threadIdx.x & 63, entries = (g.N + 255) / 256;
   const int64_t id = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
   const int64_t m = id / entries;
@@ -1598,15 +1602,15 @@ __global__ void __launch_bounds__(256) op_stats_reduce(OpGemm g) {
 }
 
 // ---------------------------------------------------------------------------
-template <bool FLAT, bool TRIANGLE>
-dim3 op_grid(const OpGemm& g) {
+template <bool FLAT, bool TRIANGLE, typename G>
+dim3 op_grid(const G& g) {
   const int64_t tiles = TRIANGLE ? (int64_t)g.tiles_m * (g.tiles_m + 1) / 2 : (int64_t)g.tiles_m * g.tiles_n;
   return FLAT ? dim3((unsigned)(tiles * g.splits * g.outputs))
               : dim3((unsigned)tiles, (unsigned)g.splits, (unsigned)g.outputs);
 }
 
 template <typename T, int LAYOUT, int KIND, int BM, int BN>
-hipError_t launch_staged(OpGemm& g, hipStream_t st) {
+hipError_t launch_staged(OpArgs<KIND>& g, hipStream_t st) {
   constexpr int SN = KIND == OP_GATED ? BN / 2 : BN;
   g.tiles_m = (g.M + BM - 1) / BM;
   g.tiles_n = (g.N + SN - 1) / SN;
@@ -1615,7 +1619,7 @@ hipError_t launch_staged(OpGemm& g, hipStream_t st) {
 }
 
 template <typename T, int LAYOUT, int KIND, int BM, int BN, int WGM, int WGN, int KS, int NST>
-hipError_t launch_middle(OpGemm& g, hipStream_t st) {
+hipError_t launch_middle(OpArgs<KIND>& g, hipStream_t st) {
   constexpr int SN = KIND == OP_GATED ? BN / 2 : BN;
   g.tiles_m = (g.M + BM - 1) / BM;
   g.tiles_n = (g.N + SN - 1) / SN;
@@ -1624,7 +1628,7 @@ hipError_t launch_middle(OpGemm& g, hipStream_t st) {
 }
 
 template <int LAYOUT, int KIND>
-hipError_t launch_pairs(OpGemm g, hipStream_t st) {
+hipError_t launch_pairs(OpGemmMore g, hipStream_t st) {
   g.tiles_m = (g.M + 63) / 64;
   g.tiles_n = (g.N + 63) / 64;
   g.pieces = 1;
@@ -1632,7 +1636,7 @@ hipError_t launch_pairs(OpGemm g, hipStream_t st) {
 }
 
 template <typename T, int LAYOUT, int KIND>
-hipError_t launch_large(OpGemm& g, hipStream_t st) {
+hipError_t launch_large(OpArgs<KIND>& g, hipStream_t st) {
   constexpr int SN = KIND == OP_GATED ? 128 : 256;
   g.tiles_m = (g.M + 255) / 256;
   g.tiles_n = (g.N + SN - 1) / SN;
@@ -1649,7 +1653,7 @@ struct SkinnyShape {
   static constexpr int kStages = !DIRECT ? 1 : KIND == OP_GATED ? (MT == 4 ? 2 : 3) : (MT == 2 ? 4 : 3);
 };
 template <typename T, int LAYOUT, int KIND, int MT, bool DIRECT>
-hipError_t launch_skinny(OpGemm& g, hipStream_t st) {
+hipError_t launch_skinny(OpArgs<KIND>& g, hipStream_t st) {
   using S = SkinnyShape<KIND, MT, DIRECT>;
   g.tiles_m = (g.M + 16 * MT - 1) / (16 * MT);
   g.tiles_n = (g.N + S::kCols - 1) / S::kCols;
@@ -1658,7 +1662,7 @@ hipError_t launch_skinny(OpGemm& g, hipStream_t st) {
 }
 
 template <typename T, int LAYOUT, int KIND>
-hipError_t launch(const OpPlan& plan, OpGemm& g, hipStream_t st) {
+hipError_t launch(const OpPlan& plan, OpArgs<KIND>& g, hipStream_t st) {
   g.splits = plan.splits;
   g.stages_per_split = plan.stages_per_split;
   hipError_t e = hipErrorInvalidValue;
@@ -1716,7 +1720,7 @@ hipError_t op_gemm(int layout, int kind, const OpPlan& plan, OpGemm& g, hipStrea
 }
 
 template <typename T>
-hipError_t op_gemm_loss(int layout, int kind, const OpPlan& plan, OpGemm& g, hipStream_t st) {
+hipError_t op_gemm_loss(int layout, int kind, const OpPlan& plan, OpGemmMore& g, hipStream_t st) {
   if (layout == OP_NN && kind == OP_STATS) return launch<T, OP_NN, OP_STATS>(plan, g, st);
   if (layout == OP_NN && kind == OP_LOSS_GRAD) return launch<T, OP_NN, OP_LOSS_GRAD>(plan, g, st);
   if (layout == OP_NT && kind == OP_ADD) return launch<T, OP_NT, OP_ADD>(plan, g, st);

@@ -3,7 +3,7 @@
 
 namespace volta {
 namespace ops {
-hipError_t op_gemm_loss_bf16(int layout, int kind, const OpPlan& plan, OpGemm g, hipStream_t st) {
+hipError_t op_gemm_loss_bf16(int layout, int kind, const OpPlan& plan, OpGemmMore g, hipStream_t st) {
   return op_gemm_loss<__bf16>(layout, kind, plan, g, st);
 }
 }  // namespace ops

@@ -281,7 +281,7 @@ int32_t volta_op_cross_entropy_forward(const volta_op_cross_entropy* in, const v
                                       {}, workspace, l.forward_bytes(), stream);
     if (d.rows == 0) return;
     char* ws = static_cast<char*>(workspace);
-    OpEpilogue epi{};
+    OpEpilogueMore epi{};
     epi.bias[0] = bias;
     epi.labels = loss ? labels : nullptr;
     epi.classes = epi.all_classes = (int32_t)d.classes;
@@ -365,7 +365,7 @@ int32_t volta_op_cross_entropy_backward(const volta_op_cross_entropy* in, const 
         pack(pw, d.inputs, p.count, d.ld_w, w_new, line_ld(l.e, p.count));
         pw = w_new;
       }
-      OpEpilogue epi{};
+      OpEpilogueMore epi{};
       epi.bias[0] = classes_from(const_cast<void*>(bias));
       epi.labels = labels;
       epi.lse = lse;
@@ -380,7 +380,7 @@ int32_t volta_op_cross_entropy_backward(const volta_op_cross_entropy* in, const 
       if (db) check_hip(sum_columns(d.type, dz, l.ld_dz, d.rows, p.count, unit, partial, classes_from(db), st), "db");
       const void* pz = dz;
       if (dx) {
-        OpEpilogue o{};
+        OpEpilogueMore o{};
         o.unit = unit;
         o.out[0] = dx;
         o.ld_out = d.ld_dx;

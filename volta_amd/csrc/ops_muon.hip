@@ -246,7 +246,7 @@ hipError_t passes(const Muon& l, MuonArgs a, hipStream_t st) {
 
 // The passes and products of a call; `last` says what becomes of the last X:
 // out, w, gamma, and in alpha what it is multiplied by.
-void run(const Muon& l, MuonArgs a, const OpEpilogue& last, char* workspace, hipStream_t st) {
+void run(const Muon& l, MuonArgs a, const OpEpilogueMore& last, char* workspace, hipStream_t st) {
   const volta_op_muon& d = l.d;
   char* x[2] = {workspace, workspace + l.x_bytes};
   char* small[3];  // matrices of the smaller side
@@ -275,17 +275,18 @@ void run(const Muon& l, MuonArgs a, const OpEpilogue& last, char* workspace, hip
   };
   auto of_x = [&](const char* p) { return Of{p, l.ld_x, x_size, x_plane}; };
   auto of_small = [&](const char* p) { return Of{p, l.ld_small, g_size, g_plane}; };
-  auto product = [&](int which, const Of& p, const Of& q, int64_t M, int64_t N, int64_t K, const OpEpilogue& epi,
+  auto product = [&](int which, const Of& p, const Of& q, int64_t M, int64_t N, int64_t K, const OpEpilogueMore& epi,
                      const char* what) {
-    OpGemm m{};
+    OpGemmMore m{};
+    m.epi = epi;
     m.p[0] = m.p[1] = p.p;
     m.q[0] = m.q[1] = q.p;
     m.ld_p = p.ld;
     m.ld_q = q.ld;
-    m.stride_p = p.stride;
-    m.stride_q = q.stride;
-    m.plane_p = p.plane;
-    m.plane_q = q.plane;
+    m.epi.stride_p = p.stride;
+    m.epi.stride_q = q.stride;
+    m.epi.plane_p = p.plane;
+    m.epi.plane_q = q.plane;
     m.M = (int32_t)M;
     m.N = (int32_t)N;
     m.K = (int32_t)K;
@@ -293,10 +294,9 @@ void run(const Muon& l, MuonArgs a, const OpEpilogue& last, char* workspace, hip
     m.outputs = (int32_t)d.batch;
     m.direct = 1;
     m.partial = partial;
-    m.epi = epi;
     check_hip(op_gemm_blend(l.layout[which], which < 2 ? OP_MIRROR : OP_BLEND, l.plan[which], m, st), what);
   };
-  auto blend_with = [&](OpEpilogue& o, const Of& r, double beta) {
+  auto blend_with = [&](OpEpilogueMore& o, const Of& r, double beta) {
     o.beta = (float)beta;
     o.blend = r.p;
     o.ld_blend = r.ld;
@@ -305,7 +305,7 @@ void run(const Muon& l, MuonArgs a, const OpEpilogue& last, char* workspace, hip
   };
   // out = alpha d: matrices of the smaller side
   auto to_small = [&](char* out, double alpha) {
-    OpEpilogue o{};
+    OpEpilogueMore o{};
     o.out[0] = out;
     o.out_type = out_type;
     o.ld_out = l.ld_small;
@@ -317,12 +317,12 @@ void run(const Muon& l, MuonArgs a, const OpEpilogue& last, char* workspace, hip
   auto gram = [&](const char* from, char* out, const Units& u) {
     product(0, of_x(from), of_x(from), l.small, l.small, l.large, to_small(out, u.g / (u.x * u.x)), "gram");
   };
-  auto multiply = [&](const char* p, const char* q, const OpEpilogue& o) {
+  auto multiply = [&](const char* p, const char* q, const OpEpilogueMore& o) {
     product(1, of_small(p), of_small(q), l.small, l.small, l.small, o, "polynomial");
   };
   // b G + c G^2 in `unit`, and a on the diagonal
   auto polynomial = [&](const char* g, char* out, const Units& u, double unit, double diagonal) {
-    OpEpilogue o = to_small(out, d.c * unit / (u.g * u.g));
+    OpEpilogueMore o = to_small(out, d.c * unit / (u.g * u.g));
     blend_with(o, of_small(g), d.b * unit / u.g);
     o.diagonal = (float)(diagonal * unit);
     multiply(g, g, o);
@@ -352,7 +352,7 @@ void run(const Muon& l, MuonArgs a, const OpEpilogue& last, char* workspace, hip
     // X' in the next step's unit, or the result
     const bool end = i == d.steps;
     const double to = end ? (double)last.alpha : l.unit[i].x;
-    OpEpilogue o{};
+    OpEpilogueMore o{};
     if (end) {
       o = last;
     } else {
@@ -398,7 +398,7 @@ int32_t volta_op_muon_orthogonalize(const volta_op_muon* in, const void* u, void
                                       {{"u", "o"}}, workspace, l.bytes(), stream);
     MuonArgs a{};
     a.g = u;
-    OpEpilogue last{};
+    OpEpilogueMore last{};
     last.out[0] = o;
     last.out_type = d.type;
     last.ld_out = d.ld_o;
@@ -436,7 +436,7 @@ int32_t volta_op_muon_step(const volta_op_muon* in, const void* g, const float* 
     a.m_out = m_out;
     a.beta = beta;
     a.nesterov = nesterov != 0;
-    OpEpilogue last{};
+    OpEpilogueMore last{};
     last.out[0] = w_out;
     last.out_type = d.type;
     last.ld_out = last.ld_w = d.ld_o;

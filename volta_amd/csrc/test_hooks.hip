@@ -331,7 +331,7 @@ int32_t volta_hip_op_product8(int32_t type, int32_t tile, int32_t splits, int32_
   const int64_t bytes = op_gemm_partial_bytes(plan, OP_LINEAR, M, N, 1);
   void* ws = nullptr;
   if (bytes && hipMalloc(&ws, bytes) != hipSuccess) return -1;
-  OpGemm g{};
+  OpGemmMore g{};
   g.p[0] = g.p[1] = x;
   g.q[0] = g.q[1] = w;
   g.ld_p = ld_x;
@@ -379,13 +379,13 @@ int32_t volta_hip_op_blend(int32_t planes, int32_t layout, int32_t kind, int32_t
   const int64_t bytes = op_gemm_partial_bytes(plan, OP_BLEND, M, N, batch);
   void* ws = nullptr;
   if (bytes && hipMalloc(&ws, bytes) != hipSuccess) return -1;
-  OpGemm g{};
+  OpGemmMore g{};
   g.p[0] = g.p[1] = p;
   g.q[0] = g.q[1] = q;
   g.ld_p = layout == OP_TN ? M : K;
   g.ld_q = layout == OP_NT ? K : N;
-  g.stride_p = (int64_t)M * K;
-  g.stride_q = (int64_t)N * K;
+  g.epi.stride_p = (int64_t)M * K;
+  g.epi.stride_q = (int64_t)N * K;
   g.M = M;
   g.N = N;
   g.K = K;
@@ -399,8 +399,8 @@ int32_t volta_hip_op_blend(int32_t planes, int32_t layout, int32_t kind, int32_t
   g.epi.out[0] = out;
   g.epi.out_type = planes == 2 ? OP_PLANES : VOLTA_OP_F16;
   if (planes == 2) {
-    g.plane_p = batch * g.stride_p;
-    g.plane_q = batch * g.stride_q;
+    g.epi.plane_p = batch * g.epi.stride_p;
+    g.epi.plane_q = batch * g.epi.stride_q;
     g.epi.plane_blend = g.epi.plane_out = batch * g.epi.stride_out;
   }
   g.epi.alpha = alpha;

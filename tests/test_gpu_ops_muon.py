@@ -164,7 +164,7 @@ def test_symmetric_products_on_every_tile(lib, n):
 
 
 SIZES = [(1, 1, 1), (3, 1, 9), (2, 9, 1), (1, 16, 16), (4, 17, 33), (2, 64, 50), (1, 100, 300), (3, 130, 70), (1, 256, 256),
-         (1, 40, 1000), (2, 1000, 24), (1, 300, 301), (5, 8, 8)]
+         (1, 40, 1000), (2, 1000, 24), (1, 300, 301), (5, 8, 8), (3, 96, 97), (2, 105, 128), (1, 128, 2000), (2, 136, 129)]
 
 
 def gradients(rng, batch, m, n):

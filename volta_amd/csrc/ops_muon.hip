@@ -48,6 +48,17 @@ constexpr int64_t kMaxBatch = 65535;  // a grid's third dimension
 // zeros in what pads it to whole chunks.  Bound by memory; the second pass finds
 // a few ten MB in the memory-side cache.
 // ---------------------------------------------------------------------------
+__device__ __forceinline__ floatx4 mul16(chunk16 a, chunk16 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(halfx8, a), __builtin_bit_cast(halfx8, b), c, 0, 0, 0);
+}
+// Four numbers at an address of 8 bytes.
+__device__ __forceinline__ void store4(_Float16* to, const float (&d)[4]) {
+  union { _Float16 e[4]; uint64_t w; } u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u.e[i] = from_f<_Float16>(d[i]);
+  *reinterpret_cast<uint64_t*>(to) = u.w;
+}
+
 struct MuonArgs {
   const void* g;       // u, or the gradient
   const float* m;      // momentum, or NULL
@@ -143,6 +154,129 @@ int norm_blocks(int64_t batch, int64_t chunks) {
 }
 
 // ---------------------------------------------------------------------------
+// The small products of a step, or of two at once, in one launch: a block for a
+// matrix whose smaller side is at most S, with G and the polynomials in LDS.
+// Each product is S x S x S, one row of 16x16 blocks a wave; what bounds it is
+// one latency after another (LDS, matrix instructions, barrier): 12 us for the
+// five products of two steps at S = 128, 3.7 at 64; one launch after another
+// they take 25 and 20.
+//
+// Rows of S + 8 numbers: 16 rows' chunks of a fragment meet every bank once.  A
+// matrix's rows and columns from its side on are zeros (the diagonal's a times
+// zeros in G).
+// ---------------------------------------------------------------------------
+struct ChainArgs {
+  const _Float16* g;
+  _Float16* out;
+  int64_t plane, stride, ld;
+  int32_t side, pairs;
+  // a product's sums times alpha, the sum's other matrix times beta, the diagonal:
+  // the polynomial; T, G of the next step, its polynomial, and both together
+  float alpha[5], beta[5], diagonal[5];
+};
+template <int S, int PLANES>
+__global__ void __launch_bounds__(512) muon_chain(ChainArgs a) {
+  constexpr int LD = S + 8, kBlocks = S / 16, kRows = (kBlocks + 7) / 8;
+  __shared__ __attribute__((aligned(16))) _Float16 lds[3][PLANES][S * LD];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, lg = lane >> 4;
+  const _Float16* g = a.g + blockIdx.x * a.stride;
+  _Float16* out = a.out + blockIdx.x * a.stride;
+  // rows of whole chunks: the side is a multiple of 8
+  for (int i = threadIdx.x; i < S * (S / 8); i += 512) {
+    const int r = i / (S / 8), c = i % (S / 8) * 8;
+#pragma unroll
+    for (int p = 0; p < PLANES; ++p) {
+      chunk16 v{0, 0, 0, 0};
+      if (r < a.side && c < a.side) v = *reinterpret_cast<const chunk16*>(g + p * a.plane + r * a.ld + c);
+      *reinterpret_cast<chunk16*>(&lds[0][p][r * LD + c]) = v;
+    }
+  }
+  __syncthreads();
+  // alpha x y + beta r (r < 0: none), to a matrix in LDS or (to < 0) to the output
+  auto product = [&](int x, int y, int which, int r, int to) {
+    const float alpha = a.alpha[which], beta = a.beta[which], diagonal = a.diagonal[which];
+#pragma unroll
+    for (int row = 0; row < kRows; ++row) {
+      const int m0 = (row * 8 + wave) * 16;
+      if (m0 >= S) continue;
+      floatx4 acc[kBlocks], small[kBlocks];
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j) acc[j] = small[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < S; k += 32) {
+        chunk16 f[PLANES];
+#pragma unroll
+        for (int p = 0; p < PLANES; ++p)
+          f[p] = *reinterpret_cast<const chunk16*>(&lds[x][p][(m0 + l) * LD + k + lg * 8]);
+#pragma unroll
+        for (int j = 0; j < kBlocks; ++j) {
+          chunk16 q[PLANES];
+#pragma unroll
+          for (int p = 0; p < PLANES; ++p)
+            q[p] = *reinterpret_cast<const chunk16*>(&lds[y][p][(j * 16 + l) * LD + k + lg * 8]);
+          acc[j] = mul16(q[0], f[0], acc[j]);
+          if constexpr (PLANES == 2) {
+            small[j] = mul16(q[0], f[1], small[j]);
+            small[j] = mul16(q[1], f[0], small[j]);
+          }
+        }
+      }
+      const int m = m0 + l;
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j) {
+        const int n = j * 16 + lg * 4;
+        if constexpr (PLANES == 2) acc[j] = acc[j] + small[j];
+        float d[4], rest[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          d[i] = alpha * acc[j][i];
+          if (r >= 0) {
+            float v = to_f(lds[r][0][m * LD + n + i]);
+            if constexpr (PLANES == 2) v += to_f(lds[r][1][m * LD + n + i]);
+            d[i] += beta * v;
+          }
+          if (m == n + i) d[i] += diagonal;
+          rest[i] = d[i] - to_f(from_f<_Float16>(d[i]));  // exact
+        }
+        if (to >= 0) {
+          store4(&lds[to][0][m * LD + n], d);
+          if constexpr (PLANES == 2) store4(&lds[to][1][m * LD + n], rest);
+        } else if (m < a.side && n < a.side) {
+          store4(out + m * a.ld + n, d);
+          if constexpr (PLANES == 2) store4(out + a.plane + m * a.ld + n, rest);
+        }
+      }
+    }
+    __syncthreads();
+  };
+  if (!a.pairs) {
+    product(0, 0, 0, 0, -1);
+    return;
+  }
+  product(0, 0, 0, 0, 1);     // P0
+  product(1, 0, 1, -1, 2);    // T = P0 G
+  product(1, 2, 2, -1, 0);    // G1 = P0 T
+  product(0, 0, 3, 0, 2);     // P1
+  product(2, 1, 4, -1, -1);   // Q = P1 P0
+}
+// The largest side that the chain takes: what three matrices leave of a CU's LDS.
+int64_t chain_side(int planes) { return planes == 2 ? 96 : 128; }
+hipError_t chain(const ChainArgs& a, int planes, int64_t batch, hipStream_t st) {
+#define VOLTA_CHAIN(S, PLANES) \
+  return op_launch(muon_chain<S, PLANES>, dim3((unsigned)batch), dim3(512), st, a)
+  if (planes == 2) {
+    if (a.side <= 32) VOLTA_CHAIN(32, 2);
+    if (a.side <= 64) VOLTA_CHAIN(64, 2);
+    VOLTA_CHAIN(96, 2);
+  }
+  if (a.side <= 32) VOLTA_CHAIN(32, 1);
+  if (a.side <= 64) VOLTA_CHAIN(64, 1);
+  if (a.side <= 96) VOLTA_CHAIN(96, 1);
+  VOLTA_CHAIN(128, 1);
+#undef VOLTA_CHAIN
+}
+
+// ---------------------------------------------------------------------------
 // Units of what a step takes: 1 in each stands for 1 / unit.
 struct Units {
   double x, g, b, p, t;
@@ -150,6 +284,7 @@ struct Units {
 struct Muon {
   volta_op_muon d;
   bool tall, pairs;        // pairs: two steps at once
+  bool chain;              // the small products in one launch
   int planes;              // 2: float32
   int64_t rows_p, cols_p;  // padded to whole chunks: the products run over zeros there
   int64_t small, large;
@@ -159,7 +294,8 @@ struct Muon {
   int layout[3];           // of G, the small products and X'
   OpPlan plan[3];
   int64_t x_bytes, g_bytes, sum_bytes, partial_bytes;
-  int64_t bytes() const { return 2 * x_bytes + (pairs ? 3 : 2) * g_bytes + sum_bytes + partial_bytes; }
+  int64_t bytes() const { return 2 * x_bytes + smalls() * g_bytes + sum_bytes + partial_bytes; }
+  int smalls() const { return pairs && !chain ? 3 : 2; }  // matrices of the smaller side
 };
 
 // The largest power of two that keeps `bound` at 2^15 or under.
@@ -220,9 +356,10 @@ Muon muon_of(const volta_op_muon* in) {
     l.partial_bytes = std::max(l.partial_bytes, align256(op_gemm_partial_bytes(l.plan[i], OP_BLEND, M[i], N[i], (int)d.batch)));
     if (op_gemm_blocks(l.plan[i], OP_BLEND, M[i], N[i]) * d.batch > kMaxBlocks) refuse("the rows and columns of a product are too many");
   }
+  l.chain = l.small <= chain_side(l.planes);
   const double one = l.plan[0].us + l.plan[1].us + l.plan[2].us;
   const double two = l.plan[0].us + 5.0 * l.plan[1].us + l.plan[2].us;
-  l.pairs = d.steps >= 2 && two < 2.0 * one;
+  l.pairs = d.steps >= 2 && (l.chain || two < 2.0 * one);
   l.ld_x = line_ld(2, l.cols_p);
   l.ld_small = line_ld(2, l.small);
   l.x_bytes = align256(d.batch * l.rows_p * l.ld_x * 2 * l.planes);
@@ -251,7 +388,7 @@ void run(const Muon& l, MuonArgs a, const OpEpilogueMore& last, char* workspace,
   char* x[2] = {workspace, workspace + l.x_bytes};
   char* small[3];  // matrices of the smaller side
   for (int i = 0; i < 3; ++i) small[i] = workspace + 2 * l.x_bytes + i * l.g_bytes;
-  char* rest = small[l.pairs ? 2 : 1] + l.g_bytes;
+  char* rest = small[l.smalls() - 1] + l.g_bytes;
   a.partial = reinterpret_cast<double*>(rest);
   float* partial = reinterpret_cast<float*>(rest + l.sum_bytes);
   const int64_t x_size = l.rows_p * l.ld_x, g_size = l.small * l.ld_small;
@@ -334,7 +471,32 @@ void run(const Muon& l, MuonArgs a, const OpEpilogueMore& last, char* workspace,
     const Units &u = l.unit[i], &v = l.unit[i + n - 1];
     double by_unit;
     gram(from, small[0], u);
-    if (n == 2) {
+    if (l.chain) {
+      ChainArgs c{};
+      c.g = reinterpret_cast<const _Float16*>(small[0]);
+      c.out = reinterpret_cast<_Float16*>(small[1]);
+      c.plane = g_plane;
+      c.stride = g_size;
+      c.ld = l.ld_small;
+      c.side = (int32_t)l.small;
+      c.pairs = n == 2;
+      auto set = [&](int i, double alpha, double beta, double diagonal) {
+        c.alpha[i] = (float)alpha;
+        c.beta[i] = (float)beta;
+        c.diagonal[i] = (float)diagonal;
+      };
+      const double p = n == 2 ? u.p : u.b;
+      set(0, d.c * p / (u.g * u.g), d.b * p / u.g, n == 2 ? d.a * p : 0.0);
+      by_unit = n == 2 ? u.p * v.p * 0x1p-15 : u.b;
+      if (n == 2) {
+        set(1, u.t / (u.p * u.g), 0.0, 0.0);
+        set(2, v.g / (u.p * u.t), 0.0, 0.0);
+        set(3, d.c * v.p / (v.g * v.g), d.b * v.p / v.g, d.a * v.p);
+        set(4, by_unit / (u.p * v.p), 0.0, 0.0);
+      }
+      check_hip(chain(c, l.planes, d.batch, st), "polynomials");
+      by = small[1];
+    } else if (n == 2) {
       polynomial(small[0], small[1], u, u.p, d.a);
       multiply(small[1], small[0], to_small(small[2], u.t / (u.p * u.g)));
       multiply(small[1], small[2], to_small(small[0], v.g / (u.p * u.t)));

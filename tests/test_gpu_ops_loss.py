@@ -9,7 +9,8 @@ An exponential is off by its argument's error, by |argument| 2^-22 (its
 rounding and the factor log2 e's, in units of the result) and by 2^-21 (the
 hardware's exp2, or expf).  A sum of positive terms is off by the longest chain
 of additions times u.  lse adds the roundings of the logarithm and of the sum
-with the largest z, 2 u each.  dz is rounded to the type (half a step)."""
+with the largest z, 2 u each.  dz is rounded to the type (half a step); of up to
+128 rows it is held as two numbers of the type (half a step of half a step)."""
 from __future__ import annotations
 
 import numpy as np
@@ -57,8 +58,9 @@ def reference(x, w, b, labels):
     return z, ez, lse, 1.1 * e_lse + 1e-30, loss, 1.1 * e_loss + 1e-30
 
 
-def gradients(t, x, w, z, ez, lse, labels, dloss, pieces=1):
-    """dx, dw, db in 64 bits and their tolerances; lse is the float that the call takes."""
+def gradients(t, x, w, z, ez, lse, labels, dloss, pieces=1, rows=0):
+    """dx, dw, db in 64 bits and their tolerances; lse is the float that the call
+    takes, `rows` what the call has where x is a few of them."""
     has = labels >= 0
     g = np.where(has, dloss, 0.0)[:, None]
     p = np.exp(z - lse[:, None])
@@ -70,12 +72,14 @@ def gradients(t, x, w, z, ez, lse, labels, dloss, pieces=1):
         floor = 2.0**-25 * np.abs(g).max() * 2.0**-14
     arg = np.abs(z - lse[:, None])
     edz = (p * (ez + 3 * U * (np.abs(lse[:, None]) + np.abs(z)) + arg * 2.0**-22 + 2.0**-21) + 3 * U * np.abs(p - hit))
-    edz = 1.1 * edz * np.abs(g) + HALF[t] * np.abs(dz) * 1.01 + np.where(g != 0, floor, 0)
     C, (M, K) = w.shape[1], x.shape
+    twice = t != "f32" and max(M, rows) <= 128
+    half, terms = (HALF[t] ** 2, 2 * M) if twice else (HALF[t], M)  # terms of dw: rows of dz
+    edz = 1.1 * edz * np.abs(g) + half * np.abs(dz) * 1.01 + np.where(g != 0, floor, 0)
     dx, dw, db = dz @ w.T, x.T @ dz, dz.sum(0)
-    tx = 1.01 * (edz @ np.abs(w).T + (C + 4 + 2 * pieces) * U * ((np.abs(dz) + edz) @ np.abs(w).T)) + 1.01 * rounded(dx, t)
-    tw = 1.01 * (np.abs(x).T @ edz + (M + 4) * U * (np.abs(x).T @ (np.abs(dz) + edz))) + 1.01 * rounded(dw, t)
-    tb = 1.01 * (edz.sum(0) + (M + 4) * U * (np.abs(dz) + edz).sum(0)) + 1.01 * rounded(db, t)
+    tx = 1.01 * (edz @ np.abs(w).T + (C + 5 + 2 * pieces) * U * ((np.abs(dz) + edz) @ np.abs(w).T)) + 1.01 * rounded(dx, t)
+    tw = 1.01 * (np.abs(x).T @ edz + (terms + 4) * U * (np.abs(x).T @ (np.abs(dz) + edz))) + 1.01 * rounded(dw, t)
+    tb = 1.01 * (edz.sum(0) + (terms + 4) * U * (np.abs(dz) + edz).sum(0)) + 1.01 * rounded(db, t)
     return (dx, tx), (dw, tw), (db, tb)
 
 
@@ -181,7 +185,7 @@ def test_classes_in_several_pieces(lib, t):
     check(kept[some], want_lse, e_lse, "lse")
     check(loss.get()[0][some], want, e_loss, "loss")
     top = np.abs(np.where(labels >= 0, dloss, 0)).max()
-    (v, tol), _, _ = gradients(t, x[some], w, z, ez, kept[some], labels[some], dloss[some], pieces=3)
+    (v, tol), _, _ = gradients(t, x[some], w, z, ez, kept[some], labels[some], dloss[some], pieces=3, rows=M)
     if t == "f16":  # units are of the largest dloss of all rows
         tol = tol + 2.0**-25 * top * 2.0**-14 * np.abs(w).sum(1)
     check(dx.get()[some], v, tol, "dx")

@@ -55,6 +55,7 @@ struct OpEpilogueMore : OpEpilogue {
   float* stats;           // OP_STATS: [op_stats_entries][M] of {largest, sum of exp(z - largest)}
   float* at_label;        // OP_STATS: [M]
   const float *lse, *dloss;  // OP_LOSS_GRAD: [M]; unit[1] multiplies the float16 gradient
+  int32_t rest_rows;  // and, of 16 bits: rows behind a row that what its rounding leaves goes; 0: nowhere
   // OP_ADD: d + add (NULL: d); to sum, or where it is NULL to out
   const float* add;
   float* sum;
@@ -64,7 +65,9 @@ struct OpEpilogueMore : OpEpilogue {
   const float *sx, *sw;
   int64_t ld_sx, step_sx, ld_sw;
   // OP_BLEND; matrix z starts z strides behind the first
-  const void *blend, *w;  // r of the products' type, w of out's (NULL: none)
+  // r of the products' type, in aligned rows of whole 16-byte chunks, w of out's
+  // (NULL: none)
+  const void *blend, *w;
   float alpha, beta, gamma;
   float diagonal;         // OP_MIRROR: added where the row is the column
   int64_t plane_blend, plane_out;  // of r and, with out_type OP_PLANES, of out: elements to the second plane; r: 0, none
@@ -76,6 +79,19 @@ struct OpEpilogueMore : OpEpilogue {
   // then first by first, so that the small sums are rounded while they are small.
   // One piece: 0
   int64_t plane_p, plane_q;
+  // OP_BLEND and OP_MIRROR of one plane: what a factor's diagonal is beyond the
+  // float16 that holds it, stride_diag floats a matrix.  diag times r, the other
+  // factor, joins the sum: by rows where P's (diag_rows), by columns where Q's
+  // diagonal it is.  OP_MIRROR: diag2 times blend2, laid out as r is, too, each of
+  // them the mean of by rows and by columns (the product turned round), times
+  // diag_weight (2 for a square, which has no diag2); and r's own diagonal has
+  // diag.  diag_out: the result's.
+  const void* blend2;
+  const float *diag, *diag2;
+  float* diag_out;
+  int64_t stride_diag;
+  float diag_weight;
+  int32_t diag_rows;
 };
 
 template <typename E>

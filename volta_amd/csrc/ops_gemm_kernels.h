@@ -247,6 +247,50 @@ __device__ __forceinline__ void op_blend_out(const OpEpilogueMore& e, int z, int
   else put((_Float16)0.0f);
 }
 
+template <int V>
+struct OpHalves {
+  typedef _Float16 type __attribute__((ext_vector_type(V)));
+};
+// The sums, V columns n .. of row m, to what a blend makes of them.
+template <int KIND, int V>
+__device__ __forceinline__ void op_blend(const OpEpilogueMore& e, int z, int64_t m, int n, int cnt, float (&d)[V]) {
+  using Halves = typename OpHalves<V>::type;
+  const int64_t here = z * e.stride_blend + m * e.ld_blend + n;
+  const _Float16* from = static_cast<const _Float16*>(e.blend);
+  const _Float16* beside = e.plane_blend ? from + e.plane_blend : static_cast<const _Float16*>(e.blend2);
+  Halves first{}, second{};  // r, and its second plane or the other factor
+  if (from) first = *reinterpret_cast<const Halves*>(from + here);
+  if (beside) second = *reinterpret_cast<const Halves*>(beside + here);
+  float more = 0.0f;
+  if (e.diag) {
+    const bool columns = KIND == OP_MIRROR || !e.diag_rows;
+    const float weight = KIND == OP_MIRROR ? 0.5f * e.diag_weight : 1.0f;
+    float by[2][V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) by[0][i] = by[1][i] = 0.0f;
+    if (columns) load_vec(e.diag + z * e.stride_diag + n, cnt, by[0]);
+    if (e.diag_rows) more = e.diag[z * e.stride_diag + m];
+    float more2 = 0.0f;
+    if (e.diag2) {
+      load_vec(e.diag2 + z * e.stride_diag + n, cnt, by[1]);
+      more2 = e.diag2[z * e.stride_diag + m];
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      d[i] += weight * ((more + by[0][i]) * to_f(first[i]) + (more2 + by[1][i]) * to_f(second[i]));
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float r = to_f(first[i]);
+    if (e.plane_blend) r += to_f(second[i]);
+    d[i] = from ? e.alpha * d[i] + e.beta * r : e.alpha * d[i];
+    if (KIND == OP_MIRROR && m == n + i) {
+      d[i] += e.diagonal + e.beta * more;
+      if (e.diag_out && i < cnt) e.diag_out[z * e.stride_diag + m] = d[i] - to_f(from_f<_Float16>(d[i]));  // exact
+    }
+  }
+}
+
 // The epilogue of V consecutive columns n .. of row m, cnt of them in the
 // matrix: d0 (and, gated, d1) are the sums, b0 and b1 the columns' biases.
 template <typename T, int KIND, int V, typename E>
@@ -254,9 +298,9 @@ __device__ __forceinline__ void op_epilogue(const E& e, int z, int64_t m, int n,
                                             float (&d1)[V], const float (&b0)[V], const float (&b1)[V]) {
   if constexpr (KIND == OP_LOSS_GRAD) {
     // (p - [label]) dloss, p = exp(z - lse) <= 1.  Rounded to the type, half a
-    // step of each gradient, for the two products that take it; float16 in
-    // units that put the largest dloss under 2^15.  A row without a label is
-    // selected to 0, whatever z and lse are.
+    // step of each gradient, for the two products that take it, and with
+    // `rest_rows` the rest beside it; float16 in units that put the largest dloss
+    // under 2^15.  A row without a label is selected to 0, whatever z and lse are.
     const int label = e.labels[m], at = label - e.class0 - n, valid = e.classes - n;
     float g = e.dloss[m];
     if constexpr (std::is_same<T, _Float16>::value) g *= e.unit[1];
@@ -268,6 +312,16 @@ __device__ __forceinline__ void op_epilogue(const E& e, int z, int64_t m, int n,
       d0[i] = label < 0 || i >= valid ? 0.0f : (p - (i == at ? 1.0f : 0.0f)) * g;
     }
     store_vec(static_cast<T*>(e.out[0]) + m * e.ld_out + n, cnt, d0);
+    if constexpr (sizeof(T) == 2) {
+      if (e.rest_rows) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float held = to_f(from_f<T>(d0[i]));
+          d0[i] = fabsf(held) < __builtin_inff() ? d0[i] - held : 0.0f;  // exact
+        }
+        store_vec(static_cast<T*>(e.out[0]) + (m + e.rest_rows) * e.ld_out + n, cnt, d0);
+      }
+    }
     return;
   }
   if constexpr (KIND == OP_ADD) {
@@ -289,22 +343,7 @@ __device__ __forceinline__ void op_epilogue(const E& e, int z, int64_t m, int n,
     return;
   }
   if constexpr (op_kind_blend(KIND)) {
-    float r[V];
-    if (e.blend) {
-      const T* from = static_cast<const T*>(e.blend) + z * e.stride_blend + m * e.ld_blend + n;
-      load_vec(from, cnt, r);
-      if (e.plane_blend) {
-        float rest[V];
-        load_vec(from + e.plane_blend, cnt, rest);
-#pragma unroll
-        for (int i = 0; i < V; ++i) r[i] += rest[i];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      d0[i] = e.blend ? e.alpha * d0[i] + e.beta * r[i] : e.alpha * d0[i];
-      if (KIND == OP_MIRROR && m == n + i) d0[i] += e.diagonal;
-    }
+    op_blend<KIND>(e, z, m, n, cnt, d0);
     op_blend_out(e, z, m, n, cnt, d0);
     return;
   }
@@ -532,6 +571,11 @@ __device__ __forceinline__ void op_write_out(const G& g, floatx4 (&acc)[TM][TN],
       } else {
         op_in_units<T, KIND>(unit, d0);
         op_epilogue<T, KIND>(g.epi, z, m, n, cnt, d0, d1, b0, b1);
+        if constexpr (KIND == OP_MIRROR) {  // the results, for the other side of the diagonal
+#pragma unroll
+          for (int c = 0; c < V; c += 4)
+            *reinterpret_cast<floatx4*>(lds + (r0 + row) * kLd + col + c) = floatx4{d0[c], d0[c + 1], d0[c + 2], d0[c + 3]};
+        }
       }
     }
     if constexpr (KIND == OP_MIRROR) {
@@ -541,14 +585,14 @@ __device__ __forceinline__ void op_write_out(const G& g, floatx4 (&acc)[TM][TN],
       for (int c0 = 0; c0 < kCols; c0 += kAcross) {
         const int down = lane / kAcross * kE, m = m0 + ph * kRows + down, left = g.M - m;
         const int c = c0 + lane % kAcross;
-        float d[kE], none[kE];
+        float d[kE];
 #pragma unroll
         for (int i = 0; i < kE; ++i) d[i] = lds[(down + i) * kLd + c];
         if (left <= 0 || n0 + c >= g.N) continue;
         if (g.splits > 1)
           store_vec(g.partial + ((split * (int64_t)g.outputs + z) * g.M + n0 + c) * (int64_t)g.N + m, left, d);
         else
-          op_epilogue<T, KIND>(g.epi, z, n0 + c, m, left, d, none, none, none);
+          op_blend_out(g.epi, z, n0 + c, m, left, d);
       }
     }
   }

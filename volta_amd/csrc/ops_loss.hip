@@ -10,6 +10,14 @@
 // bits; dw's columns are the piece's own.  A piece is as many classes as 256
 // MiB of dz hold, what the memory-side cache holds: larger ones are read from
 // memory, smaller ones add dx more often.
+//
+// The roundings of dz to 16 bits average out over many rows: they add as much to
+// the gradients' error as the gradients' own rounding does (bfloat16 0.17 % each,
+// 0.24 % together).  Over few rows they do not (up to 0.39 %, where the label's
+// element is most of a sum), and the products take the time that W and dw take
+// to move.  There dz is held as two numbers of its type, the second in rows
+// behind the first: dw's product runs over both, x laid out twice; dx's halves
+// are added by a launch of their own.
 #include "ops_call.h"
 #include "ops_launch.h"
 #include "ops_types.h"
@@ -20,6 +28,7 @@ namespace {
 
 constexpr unsigned RUN_DZ = 8;  // beside those of ops_call.h
 constexpr int64_t kPieceBytes = int64_t{256} << 20;
+constexpr int64_t kTwiceRows = 128;  // dz of up to so many rows is held as two numbers
 
 // ---------------------------------------------------------------------------
 // Joins a row's entries.  A block takes 16 rows, which lie side by side in an
@@ -102,6 +111,23 @@ __global__ void __launch_bounds__(1024) unit_kernel(const float* dloss, const in
   unit[1] = __uint_as_float((uint32_t)(127 + up) << 23);
 }
 
+// dx of dz held as two numbers: the sums of the first's rows and the second's.
+template <typename T>
+__global__ void __launch_bounds__(256) add_halves(const float* sum, int64_t rows, int64_t cols, const float* unit, T* dx,
+                                                  int64_t ld) {
+  const int64_t per_row = (cols + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * per_row) return;
+  const int64_t r = i / per_row, c = i % per_row * 4;
+  const int cnt = (int)min((int64_t)4, cols - c);
+  float a[4], b[4];
+  load_vec(sum + r * cols + c, cnt, a);
+  load_vec(sum + (rows + r) * cols + c, cnt, b);
+  const float u = unit ? *unit : 1.0f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) a[k] = (a[k] + b[k]) * u;
+  store_vec(dx + r * ld + c, cnt, a);
+}
+
 // Column sums of dz: 64 lanes of 16 bytes, eight waves on the rows of a strip
 // each, in order; the strips' sums are added by sum_partials.  Whole chunks are
 // read: what a row has behind its columns is dz's own memory, and its sums are
@@ -174,6 +200,7 @@ struct Loss {
   int64_t stats_bytes, at_bytes;
   // backward
   bool pack_x, pack_w;
+  int64_t held;  // rows of dz: `rows`, or twice as many
   int64_t pieces, piece, ld_dz;
   Piece whole, last;
   int64_t dz_bytes, x_bytes, w_bytes, sum_bytes, partial_bytes, unit_bytes;
@@ -190,10 +217,13 @@ Piece piece_of(const Loss& l, int64_t count, unsigned run) {
   p.columns = l.pack_w ? packed_ld(d.type, count) : count;
   const int64_t x_ld = l.pack_x ? line_ld(l.e, d.inputs) : d.ld_x, x_len = l.pack_x ? packed_ld(d.type, d.inputs) : d.inputs;
   const int64_t w_ld = l.pack_w ? line_ld(l.e, count) : d.ld_w;
-  const Operand x{d.rows, x_len, x_ld, 1}, w{d.inputs, p.columns, w_ld, 1}, dz{d.rows, p.columns, l.ld_dz, 1};
+  const Operand x{d.rows, x_len, x_ld, 1}, w{d.inputs, p.columns, w_ld, 1}, dz{l.held, p.columns, l.ld_dz, 1};
   p.z = shape_of(d.type, OP_NN, OP_LOSS_GRAD, d.rows, p.columns, d.inputs, 1, 1, x, w);
-  if (run & RUN_DX) p.dx = shape_of(d.type, OP_NT, OP_ADD, d.rows, d.inputs, count, 1, 1, dz, w);
-  if (run & RUN_DW) p.dw = shape_of(d.type, OP_TN, OP_STORE, d.inputs, count, d.rows, 1, 1, x, dz);
+  if (run & RUN_DX) p.dx = shape_of(d.type, OP_NT, OP_ADD, l.held, d.inputs, count, 1, 1, dz, w);
+  if (run & RUN_DW) {
+    const Operand again{l.held, x_len, x_ld, 1};
+    p.dw = shape_of(d.type, OP_TN, OP_STORE, d.inputs, count, l.held, 1, 1, again, dz);
+  }
   return p;
 }
 
@@ -224,20 +254,22 @@ Loss loss_of(const volta_op_cross_entropy* in, unsigned run) {
     // Operands whose rows are not whole chunks are laid out anew once a piece,
     // for the two or three products that take them; few rows read them once
     // and a half as it is.
-    l.pack_x = d.rows >= 64 && !whole_chunks(d.type, x);
+    const bool twice = d.type != VOLTA_OP_F32 && d.rows <= kTwiceRows;
+    l.held = twice ? 2 * d.rows : d.rows;
+    l.pack_x = (twice && (run & RUN_DW)) || (d.rows >= 64 && !whole_chunks(d.type, x));
     l.pack_w = d.rows >= 64 && !whole_chunks(d.type, w);
-    const int64_t most = std::max<int64_t>(256, kPieceBytes / (l.e * std::max<int64_t>(1, d.rows)) / 256 * 256);
+    const int64_t most = std::max<int64_t>(256, kPieceBytes / (l.e * std::max<int64_t>(1, l.held)) / 256 * 256);
     l.pieces = (d.classes + most - 1) / most;
     l.piece = l.pieces == 1 ? d.classes : ((d.classes + l.pieces - 1) / l.pieces + 255) / 256 * 256;
     l.pieces = (d.classes + l.piece - 1) / l.piece;
     l.ld_dz = line_ld(l.e, l.piece);
     l.whole = piece_of(l, l.piece, run);
     l.last = piece_of(l, d.classes - (l.pieces - 1) * l.piece, run);
-    l.dz_bytes = align256(d.rows * l.ld_dz * l.e);
-    l.x_bytes = l.pack_x ? align256(d.rows * line_ld(l.e, d.inputs) * l.e) : 0;
+    l.dz_bytes = align256(l.held * l.ld_dz * l.e);
+    l.x_bytes = l.pack_x ? align256(l.held * line_ld(l.e, d.inputs) * l.e) : 0;
     l.w_bytes = l.pack_w ? align256(d.inputs * line_ld(l.e, l.piece) * l.e) : 0;
-    l.sum_bytes = l.pieces > 1 && (run & RUN_DX) ? align256(4 * d.rows * d.inputs) : 0;
-    l.partial_bytes = align256(4 * strips_of(d.rows) * l.piece);
+    l.sum_bytes = (twice || l.pieces > 1) && (run & RUN_DX) ? align256(4 * l.held * d.inputs) : 0;
+    l.partial_bytes = align256(4 * strips_of(l.held) * l.piece);
     l.unit_bytes = d.type == VOLTA_OP_F16 ? 256 : 0;
   }
   return l;
@@ -340,20 +372,24 @@ int32_t volta_op_cross_entropy_backward(const volta_op_cross_entropy* in, const 
     float* sum = reinterpret_cast<float*>(take(l.sum_bytes));
     float* partial = reinterpret_cast<float*>(take(l.partial_bytes));
     float* unit = l.unit_bytes ? reinterpret_cast<float*>(take(l.unit_bytes)) : nullptr;
-    auto pack = [&](const void* from, int64_t rows, int64_t cols, int64_t ld, void* to, int64_t ld_to) {
+    auto pack = [&](const void* from, int64_t rows, int64_t cols, int64_t ld, char* to, int64_t ld_to, int times) {
       PackArgs a{};
-      a.n = 1;
-      a.from[0] = from;
-      a.to[0] = to;
-      a.rows[0] = rows;
-      a.cols[0] = (int32_t)cols;
-      a.ld_from[0] = ld;
-      a.ld_to[0] = ld_to;
+      a.n = times;
+      for (int i = 0; i < times; ++i) {
+        a.from[i] = from;
+        a.to[i] = to + i * rows * ld_to * l.e;
+        a.rows[i] = rows;
+        a.cols[i] = (int32_t)cols;
+        a.ld_from[i] = ld;
+        a.ld_to[i] = ld_to;
+      }
       check_hip(pack_rows(d.type, a, st), "layout");
     };
     if (unit)
       check_hip(op_launch(unit_kernel, dim3(1), dim3(1024), st, dloss, labels, d.rows, unit), "unit");
-    if (l.pack_x) pack(x, d.rows, d.inputs, d.ld_x, x_new, line_ld(l.e, d.inputs));
+    const int64_t ld_new = line_ld(l.e, d.inputs);
+    const bool twice = l.held > d.rows;
+    if (l.pack_x) pack(x, d.rows, d.inputs, d.ld_x, x_new, ld_new, twice && dw ? 2 : 1);
     const void* px = l.pack_x ? x_new : x;
     for (int64_t i = 0; i < l.pieces; ++i) {
       const bool end = i == l.pieces - 1;
@@ -362,7 +398,7 @@ int32_t volta_op_cross_entropy_backward(const volta_op_cross_entropy* in, const 
       auto classes_from = [&](void* v) { return v ? static_cast<char*>(v) + first * l.e : nullptr; };
       const void* pw = classes_from(const_cast<void*>(w));
       if (l.pack_w) {
-        pack(pw, d.inputs, p.count, d.ld_w, w_new, line_ld(l.e, p.count));
+        pack(pw, d.inputs, p.count, d.ld_w, w_new, line_ld(l.e, p.count), 1);
         pw = w_new;
       }
       OpEpilogueMore epi{};
@@ -376,8 +412,9 @@ int32_t volta_op_cross_entropy_backward(const volta_op_cross_entropy* in, const 
       epi.all_classes = (int32_t)d.classes;
       epi.out[0] = dz;
       epi.ld_out = l.ld_dz;
+      epi.rest_rows = twice ? (int32_t)d.rows : 0;
       product(d.type, p.z, &px, &pw, epi, at, st, "dz");
-      if (db) check_hip(sum_columns(d.type, dz, l.ld_dz, d.rows, p.count, unit, partial, classes_from(db), st), "db");
+      if (db) check_hip(sum_columns(d.type, dz, l.ld_dz, l.held, p.count, unit, partial, classes_from(db), st), "db");
       const void* pz = dz;
       if (dx) {
         OpEpilogueMore o{};
@@ -385,9 +422,18 @@ int32_t volta_op_cross_entropy_backward(const volta_op_cross_entropy* in, const 
         o.out[0] = dx;
         o.ld_out = d.ld_dx;
         o.add = i > 0 ? sum : nullptr;
-        o.sum = end ? nullptr : sum;
+        o.sum = end && !twice ? nullptr : sum;
         o.ld_sum = d.inputs;
         product(d.type, p.dx, &pz, &pw, o, at, st, "dx");
+        if (end && twice) {
+          const dim3 grid((unsigned)((d.rows * ((d.inputs + 3) / 4) + 255) / 256));
+          check_hip(d.type == VOLTA_OP_BF16
+                        ? op_launch(add_halves<__bf16>, grid, dim3(256), st, static_cast<const float*>(sum), d.rows,
+                                    d.inputs, static_cast<const float*>(unit), static_cast<__bf16*>(dx), d.ld_dx)
+                        : op_launch(add_halves<_Float16>, grid, dim3(256), st, static_cast<const float*>(sum), d.rows,
+                                    d.inputs, static_cast<const float*>(unit), static_cast<_Float16*>(dx), d.ld_dx),
+                    "dx");
+        }
       }
       if (dw) {
         OpEpilogue o{};

@@ -24,12 +24,19 @@
 // The products are float16's.  X's singular values stay in a range that follows
 // from the coefficients, so X, G and the polynomials have fixed units that put
 // them under 2^15: all 11 bits, and no element lost that is not 2^-29 of the
-// largest.  For 16-bit types that is enough: bfloat16's 8 bits instead leave the
-// result 1.2 % of its norm off (float16: 0.15 %, as much as rounding the result
-// to bfloat16), whatever the size.  float32 holds each as two such numbers, 23
-// bits, and takes three products, of all but the two rests: the product left
-// out is 2^-24 of the result, and the sums are chains of half as many additions
-// (of eight products) as those of float32's own matrix instruction, which does a
+// largest.  For bfloat16 that is enough, with one exception: bfloat16's 8 bits
+// instead leave the result 1.2 % of its norm off, float16 0.04 to 0.17 %, where
+// rounding the result to bfloat16 is 0.17 %.  The exception are the diagonals of
+// G and the polynomials where they are far larger than what is beside them and
+// much alike, in matrices of a small side or of one many times the other: all
+// rounded one way, they make up most of the error (30 x 576: 0.40 % in all, 0.07
+// without it; 136 x 2200: 0.22 and 0.06; 512 x 2000: 0.12 and 0.08).  There, at
+// sides of up to 256 or of one to eight, what a diagonal is beyond its float16 is
+// kept as a float32 and multiplied in the epilogues, which read X once more for
+// it (16 x 512 x 2000 would take 8 % longer).  float16 and float32 hold each matrix as two such numbers, 23 bits,
+// and take three products, of all but the two rests: the product left out is
+// 2^-24 of the result, and the sums are chains of half as many additions (of
+// eight products) as those of float32's own matrix instruction, which does a
 // sixteenth of the work in the same time.
 #include "ops_call.h"
 #include "ops_launch.h"
@@ -63,8 +70,8 @@ struct MuonArgs {
   const void* g;       // u, or the gradient
   const float* m;      // momentum, or NULL
   float* m_out;
-  _Float16* x;         // [batch][rows_p][ld_x]; float32: two planes of it
-  int64_t plane;
+  _Float16* x;         // [batch][rows_p][ld_x]
+  int64_t plane;       // elements to a second plane of it; 0: there is none
   double* partial;     // [batch][gridDim.x]
   int64_t rows, cols;  // of a matrix
   int64_t rows_p, cols_p, ld_x, ld_g, ld_m;
@@ -139,7 +146,7 @@ __global__ void __launch_bounds__(256) muon_scale(MuonArgs a, int parts) {
     for (int k = 0; k < E; ++k) u[k] = k < cnt ? (float)((double)u[k] * per) : 0.0f;
     _Float16* to = a.x + (z * a.rows_p + r) * a.ld_x + c;
     store_vec(to, E, u);
-    if constexpr (sizeof(T) == 4) {
+    if (a.plane) {
 #pragma unroll
       for (int k = 0; k < E; ++k) u[k] -= to_f(from_f<_Float16>(u[k]));  // exact
       store_vec(to + a.plane, E, u);
@@ -155,11 +162,10 @@ int norm_blocks(int64_t batch, int64_t chunks) {
 
 // ---------------------------------------------------------------------------
 // The small products of a step, or of two at once, in one launch: a block for a
-// matrix whose smaller side is at most S, with G and the polynomials in LDS.
-// Each product is S x S x S, one row of 16x16 blocks a wave; what bounds it is
-// one latency after another (LDS, matrix instructions, barrier): 12 us for the
-// five products of two steps at S = 128, 3.7 at 64; one launch after another
-// they take 25 and 20.
+// matrix whose smaller side is at most S, with G and the polynomials in LDS, as
+// pairs of float16 numbers for every type (nothing else reads them).  Each
+// product is S x S x S, one row of 16x16 blocks a wave; what bounds it is one
+// latency after another (LDS, matrix instructions, barrier).
 //
 // Rows of S + 8 numbers: 16 rows' chunks of a fragment meet every bank once.  A
 // matrix's rows and columns from its side on are zeros (the diagonal's a times
@@ -168,15 +174,16 @@ int norm_blocks(int64_t batch, int64_t chunks) {
 struct ChainArgs {
   const _Float16* g;
   _Float16* out;
+  float* diag;  // what the output's diagonal is beyond its float16; NULL: the output has two planes
   int64_t plane, stride, ld;
   int32_t side, pairs;
   // a product's sums times alpha, the sum's other matrix times beta, the diagonal:
   // the polynomial; T, G of the next step, its polynomial, and both together
   float alpha[5], beta[5], diagonal[5];
 };
-template <int S, int PLANES>
+template <int S>
 __global__ void __launch_bounds__(512) muon_chain(ChainArgs a) {
-  constexpr int LD = S + 8, kBlocks = S / 16, kRows = (kBlocks + 7) / 8;
+  constexpr int PLANES = 2, LD = S + 8, kBlocks = S / 16, kRows = (kBlocks + 7) / 8;
   __shared__ __attribute__((aligned(16))) _Float16 lds[3][PLANES][S * LD];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, lg = lane >> 4;
   const _Float16* g = a.g + blockIdx.x * a.stride;
@@ -215,35 +222,32 @@ __global__ void __launch_bounds__(512) muon_chain(ChainArgs a) {
           for (int p = 0; p < PLANES; ++p)
             q[p] = *reinterpret_cast<const chunk16*>(&lds[y][p][(j * 16 + l) * LD + k + lg * 8]);
           acc[j] = mul16(q[0], f[0], acc[j]);
-          if constexpr (PLANES == 2) {
-            small[j] = mul16(q[0], f[1], small[j]);
-            small[j] = mul16(q[1], f[0], small[j]);
-          }
+          small[j] = mul16(q[0], f[1], small[j]);
+          small[j] = mul16(q[1], f[0], small[j]);
         }
       }
       const int m = m0 + l;
 #pragma unroll
       for (int j = 0; j < kBlocks; ++j) {
         const int n = j * 16 + lg * 4;
-        if constexpr (PLANES == 2) acc[j] = acc[j] + small[j];
+        acc[j] = acc[j] + small[j];
         float d[4], rest[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           d[i] = alpha * acc[j][i];
-          if (r >= 0) {
-            float v = to_f(lds[r][0][m * LD + n + i]);
-            if constexpr (PLANES == 2) v += to_f(lds[r][1][m * LD + n + i]);
-            d[i] += beta * v;
-          }
+          if (r >= 0) d[i] += beta * (to_f(lds[r][0][m * LD + n + i]) + to_f(lds[r][1][m * LD + n + i]));
           if (m == n + i) d[i] += diagonal;
           rest[i] = d[i] - to_f(from_f<_Float16>(d[i]));  // exact
         }
         if (to >= 0) {
           store4(&lds[to][0][m * LD + n], d);
-          if constexpr (PLANES == 2) store4(&lds[to][1][m * LD + n], rest);
+          store4(&lds[to][1][m * LD + n], rest);
         } else if (m < a.side && n < a.side) {
           store4(out + m * a.ld + n, d);
-          if constexpr (PLANES == 2) store4(out + a.plane + m * a.ld + n, rest);
+          if (!a.diag) store4(out + a.plane + m * a.ld + n, rest);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (a.diag && m == n + i) a.diag[blockIdx.x * (int64_t)a.side + m] = rest[i];
         }
       }
     }
@@ -260,20 +264,12 @@ __global__ void __launch_bounds__(512) muon_chain(ChainArgs a) {
   product(2, 1, 4, -1, -1);   // Q = P1 P0
 }
 // The largest side that the chain takes: what three matrices leave of a CU's LDS.
-int64_t chain_side(int planes) { return planes == 2 ? 96 : 128; }
-hipError_t chain(const ChainArgs& a, int planes, int64_t batch, hipStream_t st) {
-#define VOLTA_CHAIN(S, PLANES) \
-  return op_launch(muon_chain<S, PLANES>, dim3((unsigned)batch), dim3(512), st, a)
-  if (planes == 2) {
-    if (a.side <= 32) VOLTA_CHAIN(32, 2);
-    if (a.side <= 64) VOLTA_CHAIN(64, 2);
-    VOLTA_CHAIN(96, 2);
-  }
-  if (a.side <= 32) VOLTA_CHAIN(32, 1);
-  if (a.side <= 64) VOLTA_CHAIN(64, 1);
-  if (a.side <= 96) VOLTA_CHAIN(96, 1);
-  VOLTA_CHAIN(128, 1);
-#undef VOLTA_CHAIN
+constexpr int64_t kChainSide = 96;
+hipError_t chain(const ChainArgs& a, int64_t batch, hipStream_t st) {
+  const dim3 grid((unsigned)batch), block(512);
+  if (a.side <= 32) return op_launch(muon_chain<32>, grid, block, st, a);
+  if (a.side <= 64) return op_launch(muon_chain<64>, grid, block, st, a);
+  return op_launch(muon_chain<96>, grid, block, st, a);
 }
 
 // ---------------------------------------------------------------------------
@@ -285,7 +281,8 @@ struct Muon {
   volta_op_muon d;
   bool tall, pairs;        // pairs: two steps at once
   bool chain;              // the small products in one launch
-  int planes;              // 2: float32
+  bool diag;               // the diagonals' rests are kept
+  int planes;              // of X and the products; bfloat16: 1
   int64_t rows_p, cols_p;  // padded to whole chunks: the products run over zeros there
   int64_t small, large;
   int64_t ld_x, ld_small;
@@ -293,8 +290,8 @@ struct Muon {
   Units unit[kMaxSteps];
   int layout[3];           // of G, the small products and X'
   OpPlan plan[3];
-  int64_t x_bytes, g_bytes, sum_bytes, partial_bytes;
-  int64_t bytes() const { return 2 * x_bytes + smalls() * g_bytes + sum_bytes + partial_bytes; }
+  int64_t x_bytes, g_bytes, diag_bytes, sum_bytes, partial_bytes;
+  int64_t bytes() const { return 2 * x_bytes + smalls() * (g_bytes + diag_bytes) + sum_bytes + partial_bytes; }
   int smalls() const { return pairs && !chain ? 3 : 2; }  // matrices of the smaller side
 };
 
@@ -318,7 +315,7 @@ Muon muon_of(const volta_op_muon* in) {
   d.ld_u = ld_of("ld_u", d.ld_u, d.cols);
   d.ld_m = ld_of("ld_m", d.ld_m, d.cols);
   d.ld_o = ld_of("ld_o", d.ld_o, d.cols);
-  l.planes = d.type == VOLTA_OP_F32 ? 2 : 1;
+  l.planes = d.type == VOLTA_OP_BF16 ? 1 : 2;
   l.rows_p = packed_ld(VOLTA_OP_F16, d.rows);
   l.cols_p = packed_ld(VOLTA_OP_F16, d.cols);
   l.tall = d.rows > d.cols;
@@ -356,14 +353,16 @@ Muon muon_of(const volta_op_muon* in) {
     l.partial_bytes = std::max(l.partial_bytes, align256(op_gemm_partial_bytes(l.plan[i], OP_BLEND, M[i], N[i], (int)d.batch)));
     if (op_gemm_blocks(l.plan[i], OP_BLEND, M[i], N[i]) * d.batch > kMaxBlocks) refuse("the rows and columns of a product are too many");
   }
-  l.chain = l.small <= chain_side(l.planes);
+  l.chain = l.small <= kChainSide;
+  l.diag = l.planes == 1 && (l.small <= 256 || l.large >= 8 * l.small);
   const double one = l.plan[0].us + l.plan[1].us + l.plan[2].us;
   const double two = l.plan[0].us + 5.0 * l.plan[1].us + l.plan[2].us;
   l.pairs = d.steps >= 2 && (l.chain || two < 2.0 * one);
   l.ld_x = line_ld(2, l.cols_p);
   l.ld_small = line_ld(2, l.small);
   l.x_bytes = align256(d.batch * l.rows_p * l.ld_x * 2 * l.planes);
-  l.g_bytes = align256(d.batch * l.small * l.ld_small * 2 * l.planes);
+  l.g_bytes = align256(d.batch * l.small * l.ld_small * 2 * (l.chain ? 2 : l.planes));
+  l.diag_bytes = l.diag ? align256(d.batch * l.small * 4) : 0;
   l.parts = norm_blocks(d.batch, d.rows * ((d.cols + 3) / 4));
   l.sum_bytes = align256(8 * d.batch * l.parts);
   return l;
@@ -389,10 +388,14 @@ void run(const Muon& l, MuonArgs a, const OpEpilogueMore& last, char* workspace,
   char* small[3];  // matrices of the smaller side
   for (int i = 0; i < 3; ++i) small[i] = workspace + 2 * l.x_bytes + i * l.g_bytes;
   char* rest = small[l.smalls() - 1] + l.g_bytes;
-  a.partial = reinterpret_cast<double*>(rest);
-  float* partial = reinterpret_cast<float*>(rest + l.sum_bytes);
+  auto diag_of = [&](const char* p) -> float* {  // of one of them
+    return !l.diag ? nullptr : reinterpret_cast<float*>(rest + (p - small[0]) / l.g_bytes * l.diag_bytes);
+  };
+  char* sums = rest + l.smalls() * l.diag_bytes;
+  a.partial = reinterpret_cast<double*>(sums);
+  float* partial = reinterpret_cast<float*>(sums + l.sum_bytes);
   const int64_t x_size = l.rows_p * l.ld_x, g_size = l.small * l.ld_small;
-  const int64_t x_plane = l.planes == 2 ? d.batch * x_size : 0, g_plane = l.planes == 2 ? d.batch * g_size : 0;
+  const int64_t x_plane = l.planes == 2 ? d.batch * x_size : 0, g_plane = d.batch * g_size;
   const int out_type = l.planes == 2 ? OP_PLANES : VOLTA_OP_F16;
   a.x = reinterpret_cast<_Float16*>(x[0]);
   a.plane = x_plane;
@@ -411,7 +414,7 @@ void run(const Muon& l, MuonArgs a, const OpEpilogueMore& last, char* workspace,
     int64_t ld, stride, plane;
   };
   auto of_x = [&](const char* p) { return Of{p, l.ld_x, x_size, x_plane}; };
-  auto of_small = [&](const char* p) { return Of{p, l.ld_small, g_size, g_plane}; };
+  auto of_small = [&](const char* p) { return Of{p, l.ld_small, g_size, l.planes == 2 ? g_plane : 0}; };
   auto product = [&](int which, const Of& p, const Of& q, int64_t M, int64_t N, int64_t K, const OpEpilogueMore& epi,
                      const char* what) {
     OpGemmMore m{};
@@ -444,7 +447,9 @@ void run(const Muon& l, MuonArgs a, const OpEpilogueMore& last, char* workspace,
   auto to_small = [&](char* out, double alpha) {
     OpEpilogueMore o{};
     o.out[0] = out;
-    o.out_type = out_type;
+    o.out_type = l.chain ? OP_PLANES : out_type;
+    o.diag_out = l.chain ? nullptr : diag_of(out);
+    o.stride_diag = l.small;
     o.ld_out = l.ld_small;
     o.stride_out = g_size;
     o.plane_out = g_plane;
@@ -454,7 +459,17 @@ void run(const Muon& l, MuonArgs a, const OpEpilogueMore& last, char* workspace,
   auto gram = [&](const char* from, char* out, const Units& u) {
     product(0, of_x(from), of_x(from), l.small, l.small, l.large, to_small(out, u.g / (u.x * u.x)), "gram");
   };
-  auto multiply = [&](const char* p, const char* q, const OpEpilogueMore& o) {
+  auto multiply = [&](const char* p, const char* q, OpEpilogueMore o) {
+    o.ld_blend = l.ld_small;
+    o.stride_blend = g_size;
+    o.diag_weight = p == q ? 2.0f : 1.0f;
+    o.diag = diag_of(p);
+    o.diag_rows = 1;
+    if (o.diag) o.blend = q;
+    if (o.diag && p != q) {
+      o.diag2 = diag_of(q);
+      o.blend2 = p;
+    }
     product(1, of_small(p), of_small(q), l.small, l.small, l.small, o, "polynomial");
   };
   // b G + c G^2 in `unit`, and a on the diagonal
@@ -475,6 +490,7 @@ void run(const Muon& l, MuonArgs a, const OpEpilogueMore& last, char* workspace,
       ChainArgs c{};
       c.g = reinterpret_cast<const _Float16*>(small[0]);
       c.out = reinterpret_cast<_Float16*>(small[1]);
+      c.diag = diag_of(small[1]);
       c.plane = g_plane;
       c.stride = g_size;
       c.ld = l.ld_small;
@@ -494,7 +510,7 @@ void run(const Muon& l, MuonArgs a, const OpEpilogueMore& last, char* workspace,
         set(3, d.c * v.p / (v.g * v.g), d.b * v.p / v.g, d.a * v.p);
         set(4, by_unit / (u.p * v.p), 0.0, 0.0);
       }
-      check_hip(chain(c, l.planes, d.batch, st), "polynomials");
+      check_hip(chain(c, d.batch, st), "polynomials");
       by = small[1];
     } else if (n == 2) {
       polynomial(small[0], small[1], u, u.p, d.a);
@@ -526,6 +542,12 @@ void run(const Muon& l, MuonArgs a, const OpEpilogueMore& last, char* workspace,
     }
     o.alpha = (float)(to / (by_unit * u.x));
     if (n == 1) blend_with(o, of_x(from), to * d.a / u.x);
+    o.ld_blend = l.ld_x;
+    o.stride_blend = x_size;
+    o.stride_diag = l.small;
+    o.diag = diag_of(by);
+    o.diag_rows = !l.tall;
+    if (o.diag) o.blend = from;
     const int64_t M = end ? d.rows : l.rows_p, N = end ? d.cols : l.cols_p;
     if (l.tall) product(2, of_x(from), of_small(by), M, N, l.small, o, "step");
     else product(2, of_small(by), of_x(from), M, N, l.small, o, "step");

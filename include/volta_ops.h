@@ -1,8 +1,10 @@
 /*
- * volta_ops.h -- operators of a feed-forward block on device tensors: the
- * linear layer, the gated layer, the RMS norm with the residual's addition,
- * and dropout whose mask is drawn from a counter, each with its gradients, in
- * float32, bfloat16 and float16.
+ * volta_ops.h -- operators of a model's layers on device tensors: the linear
+ * layer, the gated layer, the RMS norm with the residual's addition, dropout
+ * whose mask is drawn from a counter, and the loss of an output layer over many
+ * classes, each with its gradients, in float32, bfloat16 and float16; the update
+ * of weight matrices by orthogonalised momentum; and, for serving, e4m3 codes of
+ * matrices and the linear layer of such codes.
  *
  * The training step (volta_train.h) and graph execution (volta_backend.h) run
  * whole MLPs in float32; these calls are single layers of the same kind on
@@ -11,6 +13,8 @@
  *
  *   s = x + r;  n = rms_norm(s);  h = act(n Wg + bg) * (n Wu + bu)
  *   y = s + dropout(h Wd + bd),  or  y = (h Wd + bd) + s in one call
+ *   loss = log(sum(exp(z))) - z[label],  z = y Wo + bo
+ *   W = (1 - lr decay) W - lr scale X,  X from the momentum of W's gradient
  *
  * Conventions, all calls:
  *   - Matrices are row-major, W is [inputs x outputs] as in the training
@@ -226,9 +230,12 @@ int32_t volta_op_cross_entropy_forward(const volta_op_cross_entropy* d, const vo
  * a row without a label, whatever else that row holds in lse and dloss; dx =
  * dz W^T; dw = x^T dz; db = the column sums of dz.  z is formed anew, some
  * classes at a time: as many as fit 256 MiB of dz (256 of them at least), so that
- * no more than that is kept at once.  dx, dw and db may be NULL where not wanted (at least one is).
+ * no more than that is kept at once.  dx, dw and db may be NULL where not wanted,
+ * but not all of them.
  * dz is rounded to the type before the products and the sums, half a step of
- * each; float16 holds it in units of a power of two, which puts the largest
+ * each, which averages out over many rows to about as much as the gradients' own
+ * rounding; of up to 128 rows it is held as two numbers of the type.  float16
+ * holds it in units of a power of two, which puts the largest
  * |dloss| in [2^14, 2^15).  A label of `classes` or more makes the row's dz NaN. */
 int32_t volta_op_cross_entropy_backward(const volta_op_cross_entropy* d, const void* x, const void* w,
                                         const void* bias, const int32_t* labels, const float* lse,
@@ -276,8 +283,8 @@ int64_t volta_op_linear8_workspace(const volta_op_linear8* d);
  * of a block of 128 inputs are summed, and the blocks' sums times their scales
  * added, in 32 bits; with y of 16 bits the matrix instruction for codes adds
  * eight products at a time, of which it drops what is under about 2^-17 of the
- * largest (a hundredth of y's rounding).  bias [outputs] and residual may be NULL; residual may be
- * y (the same pointer and ld). */
+ * largest (a hundredth of y's rounding).  bias [outputs] and residual may be
+ * NULL; residual may be y (the same pointer and ld). */
 int32_t volta_op_linear8_forward(const volta_op_linear8* d, const void* x, const float* x_scales, const void* w,
                                  const float* w_scales, const void* bias, const void* residual, void* y,
                                  void* workspace, int64_t workspace_bytes, void* stream);
@@ -303,9 +310,11 @@ int64_t volta_op_muon_workspace(const volta_op_muon* d);
 
 /* o = X.  o may be u (the same pointer and ld).  X, G and the polynomials of it
  * are held in float16, in units that follow from the coefficients (those that
- * let singular values grow past 1024 are refused), for F32 in two numbers each,
- * 23 bits; the products' sums have 32 bits, the sum of squares 64.  A matrix of zeros stays one; a NaN or an
- * infinity in a matrix makes that matrix's result NaN. */
+ * let singular values grow past 1024 are refused), for F32 and F16 in two numbers
+ * each, 23 bits; the products' sums have 32 bits, the sum of squares 64.  A BF16
+ * result is off by 0.04 to 0.17 % of its norm, where its rounding is 0.17 %.  A
+ * matrix of zeros stays one; a NaN or an infinity in a matrix makes that matrix's
+ * result NaN. */
 int32_t volta_op_muon_orthogonalize(const volta_op_muon* d, const void* u, void* o, void* workspace,
                                     int64_t workspace_bytes, void* stream);
 

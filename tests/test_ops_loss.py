@@ -3,6 +3,7 @@ without a GPU: what is refused, with which message, and what is planned."""
 from __future__ import annotations
 
 import os
+import random
 
 import pytest
 
@@ -81,3 +82,21 @@ def test_every_matrix_is_compared():
     with pytest.raises(ops.OperatorError) as e:  # torch's usual labels are of 64 bits
         op.forward(A[0], A[1], Tensor("int64", (M,)), A[2])
     assert "int32" in str(e.value)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+def test_the_workspace_does_for_every_choice_of_gradients(t):
+    """A call for some of the gradients takes no more than *_workspace says, which
+    is for all of them (another layout of x, other plans)."""
+    rng = random.Random(5)
+    for _ in range(3000):
+        M, K, C = (int(2 ** rng.uniform(0, most)) for most in (8.5, 12, 14))
+        odd = rng.choice([0, 0, 3])
+        op = ops.CrossEntropy(M, K, C, t, ld_x=K + odd, ld_w=C + rng.choice([0, 3]))
+        n = op.workspace_bytes(backward=True)
+        for wanted in range(1, 8):
+            out = [(1 + i << 52) if wanted >> i & 1 else None for i in range(3)]
+            assert op._backward(op._d, *(1 + i << 44 for i in (0, 1)), None, *(3 + i << 44 for i in range(3)), *out, 1 << 58,
+                                n, None) == -1
+            message = str(op._refused())
+            assert "needed are" not in message, (t, M, K, C, odd, wanted, message)

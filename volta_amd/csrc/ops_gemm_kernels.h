@@ -432,7 +432,8 @@ __device__ __forceinline__ void op_barrier() {
 // The statistics of 16 rows' z over a wave's 16 TN columns, from the sums as the
 // matrix instructions leave them: a lane has 4 TN columns of one row, its
 // neighbours 16, 32 and 48 lanes on the others.  A row whose z are all -inf has
-// a sum of 0.
+// a sum of 0.  An exponential for each sum: 2048 x 4096 x 131072 bfloat16 takes
+// 1600 us with them, 1.37 PFLOP/s, the matrix instructions 70 % busy.
 template <typename T, int TN>
 __device__ __forceinline__ void op_row_stats(const OpGemmMore& g, const floatx4 (&d)[TN], int lane, int m0, int n0, float* top_of,
                                              float* sum_of) {

@@ -53,7 +53,8 @@ constexpr int64_t kMaxBatch = 65535;  // a grid's third dimension
 // u and its norm.  Two passes: momentum and the sum of squares (in 64 bits:
 // gradients may be of 1e-25 or 1e25), and X = u / (norm + eps) in its unit, with
 // zeros in what pads it to whole chunks.  Bound by memory; the second pass finds
-// a few ten MB in the memory-side cache.
+// a few ten MB in the memory-side cache (16 x 512 x 2000 bfloat16 with momentum:
+// 30 and 22 us for 164 and 131 MB).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ floatx4 mul16(chunk16 a, chunk16 b, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(halfx8, a), __builtin_bit_cast(halfx8, b), c, 0, 0, 0);
@@ -165,7 +166,9 @@ int norm_blocks(int64_t batch, int64_t chunks) {
 // matrix whose smaller side is at most S, with G and the polynomials in LDS, as
 // pairs of float16 numbers for every type (nothing else reads them).  Each
 // product is S x S x S, one row of 16x16 blocks a wave; what bounds it is one
-// latency after another (LDS, matrix instructions, barrier).
+// latency after another (LDS, matrix instructions, barrier): the five products
+// of two steps take 13.7 us at S = 96, 6.6 at 64 and 4.2 at 32, one step's 5.0, 2.8
+// and 2.0; a launch for each takes 4 to 6.
 //
 // Rows of S + 8 numbers: 16 rows' chunks of a fragment meet every bank once.  A
 // matrix's rows and columns from its side on are zeros (the diagonal's a times

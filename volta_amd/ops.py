@@ -1,6 +1,8 @@
-"""Operators of a feed-forward block on device tensors, over the volta_op_* C
-ABI (include/volta_ops.h): Linear, GatedFF, RmsNorm and Dropout, forward and
-backward, in float32 ("f32"), bfloat16 ("bf16") and float16 ("f16").
+"""Operators of a model's layers on device tensors, over the volta_op_* C ABI
+(include/volta_ops.h), in float32 ("f32"), bfloat16 ("bf16") and float16
+("f16"): Linear, GatedFF, RmsNorm, Dropout and CrossEntropy, forward and
+backward; Muon, the update of weight matrices; and Quantize and Linear8, e4m3
+codes and the layer that takes them.
 
 An operator object holds the description of its matrices (sizes, types, row
 distances); a call takes the matrices themselves, as raw device addresses,
@@ -18,6 +20,11 @@ of the library, raises OperatorError with a message.
     op = Linear(rows, inputs, outputs, "bf16", act="gelu")
     op.forward(x, w, y, bias=b, pre=pre, workspace=ws)
     op.backward(dy, x, w, pre=pre, dx=dx, dw=dw, db=db, workspace=ws)
+
+    head = CrossEntropy(rows, inputs, classes, "bf16")
+    head.forward(x, w, labels, loss, lse=lse, workspace=ws)
+    head.backward(x, w, labels, lse, dloss, dx=dx, dw=dw, workspace=ws)
+    Muon(inputs, outputs, "bf16").step(w, dw, momentum, lr, workspace=ws)
 """
 from __future__ import annotations
 

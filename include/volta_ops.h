@@ -227,8 +227,9 @@ int32_t volta_op_cross_entropy_forward(const volta_op_cross_entropy* d, const vo
 
 /* From dloss [rows], the gradient that reaches each row's loss (1 / rows for
  * their mean), and the forward's lse: dz = (exp(z - lse) - [label]) dloss, 0 in
- * a row without a label, whatever else that row holds in lse and dloss; dx =
- * dz W^T; dw = x^T dz; db = the column sums of dz.  z is formed anew, some
+ * a row without a label, whatever that row holds in x, lse and dloss (its x still
+ * takes part in dw, times 0: an infinity or NaN there reaches dw); dx = dz W^T;
+ * dw = x^T dz; db = the column sums of dz.  z is formed anew, some
  * classes at a time: as many as fit 256 MiB of dz (256 of them at least), so that
  * no more than that is kept at once.  dx, dw and db may be NULL where not wanted,
  * but not all of them.

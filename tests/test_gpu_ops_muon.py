@@ -9,7 +9,7 @@ iteration with X, G and the polynomials rounded as the kernels round them is off
 by some distance, and the kernels, whose roundings are others of the same sizes,
 by up to three times it.  bfloat16: to float16 in units of a power of two over
 the range, but for the diagonals of G and the polynomials, which are kept at
-sides of up to 256 and of one to eight; the sums' 32 bits are nothing beside that.  float16 and float32: to two such numbers
+sides of up to 256 and of one to more than four; the sums' 32 bits are nothing beside that.  float16 and float32: to two such numbers
 (23 bits), and a sum of K products is a chain of K / 8 additions, each
 rounded to 24 bits (the instruction adds eight products at a time: 99 % of its
 results over random operands are those of that chain; with the smaller two of
@@ -94,7 +94,7 @@ def chain(p, q):
 def before_rounding(t, u, want, **kw):
     """The 2-norm by which the X of a result of type t may be off."""
     small, large = sorted((-n % 8 + n for n in u.shape))
-    kept = small <= 256 or large >= 8 * small  # the diagonals
+    kept = small <= 256 or large > 4 * small  # the diagonals
     half = lambda v, bound: halves(v, bound if kept else abs(bound))  # noqa: E731
     near = iterate(u, rounding=half, **kw) if t == "bf16" else iterate(u, rounding=pairs, mul=chain, mix=mixed, **kw)
     return 3 * np.linalg.norm(near - want)
@@ -211,7 +211,7 @@ def test_larger(lib, t):
     """Sizes whose products take the larger tiles and split sums."""
     # the last two take two steps at once, wide and tall
     for k, (batch, m, n) in enumerate([(1, 512, 2000), (2, 1100, 520), (1, 72, 9000), (1, 5000, 96), (16, 384, 1500),
-                                       (20, 1400, 330), (1, 136, 9000), (1, 7000, 200)]):
+                                       (20, 1400, 330), (1, 136, 9000), (1, 7000, 200), (1, 384, 2880)]):
         rng = np.random.default_rng(50 + k)
         say(t, batch, m, n)
         v = R.unpack(R.pack(gradients(rng, batch, m, n), t), t)

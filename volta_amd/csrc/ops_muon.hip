@@ -30,10 +30,11 @@
 // G and the polynomials where they are far larger than what is beside them and
 // much alike, in matrices of a small side or of one many times the other: all
 // rounded one way, they make up most of the error (30 x 576: 0.40 % in all, 0.07
-// without it; 136 x 2200: 0.22 and 0.06; 512 x 2000: 0.12 and 0.08).  There, at
-// sides of up to 256 or of one to eight, what a diagonal is beyond its float16 is
-// kept as a float32 and multiplied in the epilogues, which read X once more for
-// it (16 x 512 x 2000 would take 8 % longer).  float16 and float32 hold each matrix as two such numbers, 23 bits,
+// without it; 136 x 2200: 0.22 and 0.06; 384 x 2880: 0.18 and 0.06; 512 x 2000:
+// 0.12 and 0.08).  There, at sides of up to 256 or of one to more than four, what
+// a diagonal is beyond its float16 is kept as a float32 and multiplied in the
+// epilogues, which read X once more for it (16 x 512 x 2000 would take 8 %
+// longer).  float16 and float32 hold each matrix as two such numbers, 23 bits,
 // and take three products, of all but the two rests: the product left out is
 // 2^-24 of the result, and the sums are chains of half as many additions (of
 // eight products) as those of float32's own matrix instruction, which does a
@@ -357,7 +358,7 @@ Muon muon_of(const volta_op_muon* in) {
     if (op_gemm_blocks(l.plan[i], OP_BLEND, M[i], N[i]) * d.batch > kMaxBlocks) refuse("the rows and columns of a product are too many");
   }
   l.chain = l.small <= kChainSide;
-  l.diag = l.planes == 1 && (l.small <= 256 || l.large >= 8 * l.small);
+  l.diag = l.planes == 1 && (l.small <= 256 || l.large > 4 * l.small);
   const double one = l.plan[0].us + l.plan[1].us + l.plan[2].us;
   const double two = l.plan[0].us + 5.0 * l.plan[1].us + l.plan[2].us;
   l.pairs = d.steps >= 2 && (l.chain || two < 2.0 * one);

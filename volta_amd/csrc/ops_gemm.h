@@ -69,7 +69,7 @@ struct OpEpilogueMore : OpEpilogue {
   // (NULL: none)
   const void *blend, *w;
   float alpha, beta, gamma;
-  float diagonal;         // OP_MIRROR: added where the row is the column
+  float diagonal;         // OP_MIRROR with an r: added where the row is the column
   int64_t plane_blend, plane_out;  // of r and, with out_type OP_PLANES, of out: elements to the second plane; r: 0, none
   int32_t out_type;       // enum volta_op_type; also of a product of codes
   int64_t ld_blend, ld_w, stride_blend, stride_w, stride_out;

@@ -24,21 +24,39 @@
 // The products are float16's.  X's singular values stay in a range that follows
 // from the coefficients, so X, G and the polynomials have fixed units that put
 // them under 2^15: all 11 bits, and no element lost that is not 2^-29 of the
-// largest.  For bfloat16 that is enough, with one exception: bfloat16's 8 bits
-// instead leave the result 1.2 % of its norm off, float16 0.04 to 0.17 %, where
-// rounding the result to bfloat16 is 0.17 %.  The exception are the diagonals of
-// G and the polynomials where they are far larger than what is beside them and
-// much alike, in matrices of a small side or of one many times the other: all
-// rounded one way, they make up most of the error (30 x 576: 0.40 % in all, 0.07
-// without it; 136 x 2200: 0.22 and 0.06; 384 x 2880: 0.18 and 0.06; 512 x 2000:
-// 0.12 and 0.08).  There, at sides of up to 256 or of one to more than four, what
-// a diagonal is beyond its float16 is kept as a float32 and multiplied in the
-// epilogues, which read X once more for it (16 x 512 x 2000 would take 8 %
-// longer).  float16 and float32 hold each matrix as two such numbers, 23 bits,
-// and take three products, of all but the two rests: the product left out is
-// 2^-24 of the result, and the sums are chains of half as many additions (of
-// eight products) as those of float32's own matrix instruction, which does a
-// sixteenth of the work in the same time.
+// largest.
+//
+// float32, float16 and, with `exact`, bfloat16 hold each matrix as two such
+// numbers, 23 bits, and take three products, of all but the two rests: the product
+// left out is 2^-24 of the result, and the sums are chains of half as many
+// additions (of eight products) as those of float32's own matrix instruction, which
+// does a sixteenth of the work in the same time.
+//
+// bfloat16 without it holds them as one.  A rounding of X is noise in all
+// directions, 2^-12 / sqrt(3) of X's norm, and the steps enlarge small directions by
+// 3.4445 each.  Where u fills its directions evenly the result is 0.04 to 0.21 % of
+// its norm off, its rounding being 0.17 % (bfloat16's 8 bits in the products: 1.2 %).
+// Where it does not, the noise is what fills the others: 512 x 1024 of rank 1 9.6 %,
+// of rank 16 4.3, of rank 64 2.2, of 256 0.7; the whole of it goes by the second
+// number (0.002 % at rank 16).  That takes 4096 x 16384 from 3270 to 9150 us, 16 x
+// 512 x 2000 from 313 to 585, 1024 x 1024 from 159 to 197, so it is the caller's
+// choice.
+//
+// With one number the diagonals of G and the polynomials, nearly multiples of the
+// unit matrix, are all rounded one way, and where they are far larger than what is
+// beside them that is most of the error (noise of 30 x 576: 0.40 %, 0.07 without
+// it; 136 x 2200: 0.22 and 0.06).  At sides of up to 256 and of one to more than four
+// what a diagonal is beyond its float16 is kept as a float32 and multiplied in the
+// epilogues, which read X and G once more for it.  Percent of the norm off before
+// the result's rounding, and us, with it and without:
+//   104 x 2000   0.04 0.12   126 110       512 x 2000       0.06 0.14   156 149
+//   256 x 256    0.09 0.14   108 101       16 x 512 x 2000  0.06 0.15   362 305
+//   256 x 1000   0.07 0.14   124 115       1024 x 4096      0.05 0.10   238 219
+//   512 x 5000   0.05 0.18   186 168       2048 x 8192      0.06 0.13   697 642
+//   1024 x 8192  0.04 0.10   306 282       4096 x 16384                3370 3140
+// The left ones have it, the right ones do not: no edge in the figures asks for the
+// rule, which keeps the error without it under the result's rounding, 0.17 %, and
+// the time of large and batched matrices.
 #include "ops_call.h"
 #include "ops_launch.h"
 #include "ops_types.h"
@@ -286,7 +304,7 @@ struct Muon {
   bool tall, pairs;        // pairs: two steps at once
   bool chain;              // the small products in one launch
   bool diag;               // the diagonals' rests are kept
-  int planes;              // of X and the products; bfloat16: 1
+  int planes;              // of X and the products; bfloat16 that is not to be exact: 1
   int64_t rows_p, cols_p;  // padded to whole chunks: the products run over zeros there
   int64_t small, large;
   int64_t ld_x, ld_small;
@@ -319,7 +337,8 @@ Muon muon_of(const volta_op_muon* in) {
   d.ld_u = ld_of("ld_u", d.ld_u, d.cols);
   d.ld_m = ld_of("ld_m", d.ld_m, d.cols);
   d.ld_o = ld_of("ld_o", d.ld_o, d.cols);
-  l.planes = d.type == VOLTA_OP_BF16 ? 1 : 2;
+  if (d.exact != 0 && d.exact != 1) refuse("exact is " + std::to_string(d.exact) + ", must be 0 or 1");
+  l.planes = d.type == VOLTA_OP_BF16 && !d.exact ? 1 : 2;
   l.rows_p = packed_ld(VOLTA_OP_F16, d.rows);
   l.cols_p = packed_ld(VOLTA_OP_F16, d.cols);
   l.tall = d.rows > d.cols;

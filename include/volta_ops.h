@@ -235,9 +235,12 @@ int32_t volta_op_cross_entropy_forward(const volta_op_cross_entropy* d, const vo
  * but not all of them.
  * dz is rounded to the type before the products and the sums, half a step of
  * each, which averages out over many rows to about as much as the gradients' own
- * rounding; of up to 128 rows it is held as two numbers of the type.  float16
- * holds it in units of a power of two, which puts the largest
- * |dloss| in [2^14, 2^15).  A label of `classes` or more makes the row's dz NaN. */
+ * rounding; of up to 128 rows it is held as two numbers of the type.  16 bits hold
+ * it in units of the largest finite |dloss| of a row with a label, 2^14 of them (of
+ * two numbers: in float16 alone, of a power of two): equal dloss take no part in the
+ * rounding, rows of another one round their label's element, about -dloss, alike.
+ * float16 so keeps what is over 2^-38 of the largest, and loses bits of what is under
+ * 2^-28.  A label of `classes` or more makes the row's dz NaN. */
 int32_t volta_op_cross_entropy_backward(const volta_op_cross_entropy* d, const void* x, const void* w,
                                         const void* bias, const int32_t* labels, const float* lse,
                                         const float* dloss, void* dx, void* dw, void* db, void* workspace,

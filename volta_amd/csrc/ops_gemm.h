@@ -41,7 +41,7 @@ struct OpEpilogue {
   void* out[2];  // OP_STORE: one for each q (blockIdx.z)
   void* pre[2];
   int64_t ld_out, ld_residual, ld_pre;
-  const float* unit;  // OP_STORE in float16: one number on the device, what the sums are multiplied by; NULL: 1
+  const float* unit;  // OP_STORE in 16 bits: one number on the device, what the sums are multiplied by; NULL: 1
 };
 
 // What the kinds from OP_STATS on and the products of codes take besides; the
@@ -54,7 +54,7 @@ struct OpEpilogueMore : OpEpilogue {
   int32_t class0, classes, all_classes;
   float* stats;           // OP_STATS: [op_stats_entries][M] of {largest, sum of exp(z - largest)}
   float* at_label;        // OP_STATS: [M]
-  const float *lse, *dloss;  // OP_LOSS_GRAD: [M]; unit[1] multiplies the float16 gradient
+  const float *lse, *dloss;  // OP_LOSS_GRAD: [M]; unit[1] (NULL: 1) multiplies the 16-bit gradient
   int32_t rest_rows;  // and, of 16 bits: rows behind a row that what its rounding leaves goes; 0: nowhere
   // OP_ADD: d + add (NULL: d); to sum, or where it is NULL to out
   const float* add;

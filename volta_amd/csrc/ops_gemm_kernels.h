@@ -304,11 +304,13 @@ __device__ __forceinline__ void op_epilogue(const E& e, int z, int64_t m, int n,
   if constexpr (KIND == OP_LOSS_GRAD) {
     // (p - [label]) dloss, p = exp(z - lse) <= 1.  Rounded to the type, half a
     // step of each gradient, for the two products that take it, and with
-    // `rest_rows` the rest beside it; float16 in units that put the largest dloss
-    // under 2^15.  A row without a label is selected to 0, whatever z and lse are.
+    // `rest_rows` the rest beside it; 16 bits in units of the largest dloss.  A row
+    // without a label is selected to 0, whatever z and lse are.
     const int label = e.labels[m], at = label - e.class0 - n, valid = e.classes - n;
     float g = e.dloss[m];
-    if constexpr (std::is_same<T, _Float16>::value) g *= e.unit[1];
+    if constexpr (sizeof(T) == 2) {
+      if (e.unit) g *= e.unit[1];
+    }
     if (label >= e.all_classes) g = __builtin_nanf("");  // no class at all: not to go unnoticed
     const float lse = e.lse[m];
 #pragma unroll
@@ -339,9 +341,10 @@ __device__ __forceinline__ void op_epilogue(const E& e, int z, int64_t m, int n,
     if (e.sum) {
       store_vec(e.sum + m * e.ld_sum + n, cnt, d0);
     } else {
-      if constexpr (std::is_same<T, _Float16>::value) {
+      if constexpr (sizeof(T) == 2) {
+        const float unit = e.unit ? *e.unit : 1.0f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) d0[i] *= *e.unit;
+        for (int i = 0; i < V; ++i) d0[i] *= unit;
       }
       store_vec(static_cast<T*>(e.out[0]) + m * e.ld_out + n, cnt, d0);
     }
@@ -387,9 +390,10 @@ __device__ __forceinline__ void op_biases(const E& e, int n, int cnt, float (&b0
   }
 }
 
-// Sums alone in float16 may be in units of an operand's (act_grad_kernel).
+// Sums alone in 16 bits may be in units of an operand's (act_grad_kernel's in
+// float16; dz's).
 template <typename T, int KIND>
-constexpr bool kOpUnits = KIND == OP_STORE && std::is_same<T, _Float16>::value;
+constexpr bool kOpUnits = KIND == OP_STORE && sizeof(T) == 2;
 template <typename T, int KIND>
 __device__ __forceinline__ float op_unit(const OpEpilogue& e) {
   if constexpr (kOpUnits<T, KIND>)

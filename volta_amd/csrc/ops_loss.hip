@@ -13,9 +13,16 @@
 //
 // The roundings of dz to 16 bits average out over many rows: they add as much to
 // the gradients' error as the gradients' own rounding does (bfloat16 0.17 % each,
-// 0.24 % together).  Over few rows they do not (up to 0.39 %, where the label's
-// element is most of a sum), and the products take the time that W and dw take
-// to move.  There dz is held as two numbers of its type, the second in rows
+// 0.22 % together).  The label's element is about -dloss in every row where its p
+// is small, so dz is in units of the largest |dloss|, which the sums are multiplied
+// by in 32 bits: of a mean's equal dloss it is -1 then and exact, where 1 / 1020
+// itself would be rounded the same way in every row (0.40 % of dx, dW and db, 0.17
+// in units).  Rows of a few other dloss still round their labels' elements alike,
+// by half a step at most.
+//
+// Over few rows nothing averages out (bfloat16, 1 to 32 rows: up to 0.39 %, where
+// the label's element is most of a sum), and the products take the time that W and
+// dw take to move.  There dz is held as two numbers of its type, the second in rows
 // behind the first: dw's product runs over both, x laid out twice; dx's halves
 // are added by a launch of their own.
 #include "ops_call.h"
@@ -89,17 +96,36 @@ hipError_t join_rows(const JoinArgs& a, hipStream_t st) {
   return op_launch(per == 16 ? join_kernel<16> : per == 4 ? join_kernel<4> : join_kernel<1>, grid, dim3(1024), st, a);
 }
 
-// float16: unit[1], the power of two that puts the largest |dloss| of a row
-// with a label in [2^14, 2^15) (|dz| is at most |dloss|), and unit[0], its
-// reciprocal.  All zeros, and an infinity or a NaN among them: 1.  One block, 4.2
-// us at 1000 rows: the launch.
-__global__ void __launch_bounds__(1024) unit_kernel(const float* dloss, const int32_t* labels, int64_t rows, float* unit) {
+// The units of dz in 16 bits, from m, the largest |dloss| of a row with a label
+// (|dz| is at most |dloss|): unit[1], 2^14 / m, and unit[0], m / 2^14.  `whole`, for
+// dz held as two numbers, which need no exact m: the powers of two next to them,
+// which put m in [2^14, 2^15).  No such row, and zeros alone: 1.  Infinities and NaN
+// are left out.  An m under 2^-100 counts as that, so that no unit leaves the normal
+// numbers (float16's gradients are 0 long before).  One block for each 65536 rows and
+// at most 64; of more than one a second launch joins theirs.  4.2 us at 1000 rows:
+// the launch.
+constexpr int64_t kUnitRows = 65536;
+constexpr int kUnitBlocks = 64;
+__device__ __forceinline__ void units_of(uint32_t m, bool whole, float* unit) {
+  float u0 = 1.0f, u1 = 1.0f;
+  if (m != 0) {
+    float top = fmaxf(__uint_as_float(m), 0x1p-100f);
+    if (whole) top = __uint_as_float(__float_as_uint(top) & 0x7f800000u);
+    u0 = top * 0x1p-14f;
+    u1 = 0x1p14f / top;
+  }
+  unit[0] = u0;
+  unit[1] = u1;
+}
+// `partial` NULL: one block, to `unit`; else each block's m.
+__global__ void __launch_bounds__(1024) unit_kernel(const float* dloss, const int32_t* labels, int64_t rows, bool whole,
+                                                    uint32_t* partial, float* unit) {
   __shared__ uint32_t lds[16];
   uint32_t m = 0;
 #pragma unroll 8
-  for (int64_t i = threadIdx.x; i < rows; i += 1024) {
+  for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < rows; i += (int64_t)gridDim.x * 1024) {
     const uint32_t v = __float_as_uint(fabsf(dloss[i]));
-    m = max(m, labels[i] >= 0 ? v : 0u);
+    m = max(m, labels[i] >= 0 && v < 0x7f800000u ? v : 0u);
   }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off, kWave));
@@ -107,10 +133,21 @@ __global__ void __launch_bounds__(1024) unit_kernel(const float* dloss, const in
   __syncthreads();
   if (threadIdx.x != 0) return;
   for (int w = 0; w < 16; ++w) m = max(m, lds[w]);
-  int up = 0;
-  if (m != 0 && m < 0x7f800000u) up = min(14 - (max((int)(m >> 23), 1) - 127), 126);
-  unit[0] = __uint_as_float((uint32_t)(127 - up) << 23);
-  unit[1] = __uint_as_float((uint32_t)(127 + up) << 23);
+  if (partial) partial[blockIdx.x] = m;
+  else units_of(m, whole, unit);
+}
+__global__ void __launch_bounds__(64) unit_join(const uint32_t* partial, int n, bool whole, float* unit) {
+  uint32_t m = (int)threadIdx.x < n ? partial[threadIdx.x] : 0u;
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off, kWave));
+  if (threadIdx.x == 0) units_of(m, whole, unit);
+}
+// `unit`: 64 floats, then the blocks' maxima.
+hipError_t units(const float* dloss, const int32_t* labels, int64_t rows, bool whole, float* unit, hipStream_t st) {
+  const int blocks = (int)std::min<int64_t>(kUnitBlocks, std::max<int64_t>(1, (rows + kUnitRows - 1) / kUnitRows));
+  uint32_t* partial = blocks > 1 ? reinterpret_cast<uint32_t*>(unit + 64) : nullptr;
+  const hipError_t e = op_launch(unit_kernel, dim3(blocks), dim3(1024), st, dloss, labels, rows, whole, partial, unit);
+  return e != hipSuccess || !partial ? e : op_launch(unit_join, dim3(1), dim3(64), st, partial, blocks, whole, unit);
 }
 
 // dx of dz held as two numbers: the sums of the first's rows and the second's
@@ -276,7 +313,8 @@ Loss loss_of(const volta_op_cross_entropy* in, unsigned run) {
     l.w_bytes = l.pack_w ? align256(d.inputs * line_ld(l.e, l.piece) * l.e) : 0;
     l.sum_bytes = (twice || l.pieces > 1) && (run & RUN_DX) ? align256(4 * l.held * d.inputs) : 0;
     l.partial_bytes = align256(4 * strips_of(l.held) * l.piece);
-    l.unit_bytes = d.type == VOLTA_OP_F16 ? 256 : 0;
+    // two numbers of bfloat16 hold dz to 2^-16 in its own range: no unit
+    l.unit_bytes = d.type == VOLTA_OP_F16 || (d.type == VOLTA_OP_BF16 && !twice) ? 512 : 0;
   }
   return l;
 }
@@ -391,10 +429,9 @@ int32_t volta_op_cross_entropy_backward(const volta_op_cross_entropy* in, const 
       }
       check_hip(pack_rows(d.type, a, st), "layout");
     };
-    if (unit)
-      check_hip(op_launch(unit_kernel, dim3(1), dim3(1024), st, dloss, labels, d.rows, unit), "unit");
-    const int64_t ld_new = line_ld(l.e, d.inputs);
     const bool twice = l.held > d.rows;
+    if (unit) check_hip(units(dloss, labels, d.rows, twice, unit, st), "unit");
+    const int64_t ld_new = line_ld(l.e, d.inputs);
     if (l.pack_x) pack(x, d.rows, d.inputs, d.ld_x, x_new, ld_new, twice && dw ? 2 : 1);
     const void* px = l.pack_x ? x_new : x;
     for (int64_t i = 0; i < l.pieces; ++i) {

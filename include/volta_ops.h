@@ -41,7 +41,8 @@
  *     call names the two as allowed to be the same matrix.  Column ranges of
  *     one wider matrix (the same ld) do not overlap.
  *   - rows may be 0: nothing is read, outputs of that many rows stay as they
- *     are, and gradients of weights and biases are zero.  Elements between a
+ *     are (and may be NULL, as empty tensors are), and gradients of weights and
+ *     biases are zero.  Elements between a
  *     row's end and the next row's start (ld > length) are neither read nor
  *     written.
  *   - Sums are held in 32 bits; every result is rounded once, to the nearest

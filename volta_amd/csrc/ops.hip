@@ -164,7 +164,7 @@ int32_t volta_op_linear_backward(const volta_op_linear* in, const void* dy, cons
     const volta_op_linear& d = l.d;
     const int e = elem_bytes(d.type);
     const bool act = d.act != VOLTA_OP_ACT_NONE;
-    if (!dx && !dw && !db) refuse("dx, dw and db are all NULL");
+    if (!dx && !dw && !db && d.rows > 0) refuse("dx, dw and db are all NULL");
     if (d.rows > 0) {
       need(dy, "dy");
       if (act) need(pre, "pre");
@@ -266,7 +266,7 @@ int32_t volta_op_gated_backward(const volta_op_gated* in, const void* dh, const 
     const volta_op_gated& d = l.d;
     const int e = elem_bytes(d.type);
     if (!dw_gate != !dw_up) refuse("dw_gate and dw_up are wanted both or neither");
-    if (!dx && !dw_gate && !db_gate && !db_up) refuse("every gradient is NULL");
+    if (!dx && !dw_gate && !db_gate && !db_up && d.rows > 0) refuse("every gradient is NULL");
     if (d.rows > 0) {
       need(dh, "dh");
       need(gate, "gate");
@@ -388,7 +388,7 @@ int32_t volta_op_rms_norm_backward(const volta_op_rms_norm* in, const void* dy, 
     const Norm n = norm_of(in, true);
     const volta_op_rms_norm& d = n.d;
     const int e = elem_bytes(d.type);
-    if (!dx && !dweight) refuse("dx and dweight are both NULL");
+    if (!dx && !dweight && d.rows > 0) refuse("dx and dweight are both NULL");
     if (d.rows > 0) {
       need(dy, "dy");
       need(s, "s");

@@ -341,8 +341,8 @@ int32_t volta_op_cross_entropy_forward(const volta_op_cross_entropy* in, const v
   return guarded("volta_op_cross_entropy_forward", [&] {
     const Loss l = loss_of(in, RUN_FORWARD);
     const volta_op_cross_entropy& d = l.d;
-    if (!loss && !lse) refuse("loss and lse are both NULL");
     if (d.rows > 0) {
+      if (!loss && !lse) refuse("loss and lse are both NULL");
       need(x, "x");
       if (loss) need(labels, "labels");
     }
@@ -383,9 +383,9 @@ int32_t volta_op_cross_entropy_backward(const volta_op_cross_entropy* in, const 
                                         const float* dloss, void* dx, void* dw, void* db, void* workspace,
                                         int64_t workspace_bytes, void* stream) {
   return guarded("volta_op_cross_entropy_backward", [&] {
-    if (!dx && !dw && !db) refuse("dx, dw and db are all NULL");
     const Loss l = loss_of(in, RUN_DZ | (dx ? RUN_DX : 0) | (dw ? RUN_DW : 0));
     const volta_op_cross_entropy& d = l.d;
+    if (!dx && !dw && !db && d.rows > 0) refuse("dx, dw and db are all NULL");
     if (d.rows > 0) {
       need(x, "x");
       need(w, "w");

@@ -136,7 +136,7 @@ def _lies(shape, strides, rows, cols, ld) -> bool:
     """Whether a tensor of this shape and these strides holds `rows` rows of
     `cols` elements `ld` apart, or more of them: its last dimension is a row,
     those before it count the rows; one dimension alone is a flat buffer."""
-    if rows <= 0:
+    if rows <= 0 or cols <= 0:
         return True
     dims = [(n, s) for n, s in zip(shape, strides) if n != 1]
     if any(n == 0 for n, _ in dims):
@@ -180,7 +180,7 @@ def _matrix(name, type, rows, cols, ld=0):
                     raise OperatorError("%s has shape %s and strides %s, the description says %d rows of %d, %d apart"
                                         % (name, tuple(m.shape), tuple(m.stride()), rows, cols, ld))
             return m.data_ptr()
-        need = ((rows - 1) * ld + cols) * _SIZE.get(type, 0) if rows > 0 else 0
+        need = ((rows - 1) * ld + cols) * _SIZE.get(type, 0) if rows > 0 and cols > 0 else 0
         if getattr(m, "nbytes", need) < need:
             raise OperatorError("%s holds %d bytes, the description says %d" % (name, m.nbytes, need))
         return m.ptr

@@ -20,9 +20,9 @@
 // in units).  Rows of a few other dloss still round their labels' elements alike,
 // by half a step at most.
 //
-// Over few rows nothing averages out (bfloat16, 1 to 32 rows: up to 0.39 %, where
-// the label's element is most of a sum), and the products take the time that W and
-// dw take to move.  There dz is held as two numbers of its type, the second in rows
+// Over few rows less averages out (bfloat16, 1 to 32 rows: gradients up to 0.28 %
+// off with their own rounding, 0.17 of it), and the products take the time that W
+// and dw take to move.  There dz is held as two numbers of its type, the second in rows
 // behind the first: dw's product runs over both, x laid out twice; dx's halves
 // are added by a launch of their own.
 #include "ops_call.h"
@@ -295,9 +295,16 @@ Loss loss_of(const volta_op_cross_entropy* in, unsigned run) {
     l.held = twice ? 2 * d.rows : d.rows;
     // Operands whose rows are not whole chunks are laid out anew once a piece,
     // for the two or three products that take them.  Few rows of dz read them once
-    // and a half as it is, and a few more do where W is more than the caches hold:
-    // bfloat16, 32 rows of 1000 inputs and 10007 classes 45.6 us for 56.9, 60 of
-    // 4096 and 32769 375 for 293, 100 of them 409 for 492.
+    // and a half as it is, and so do a few more where W and its copy are more than
+    // the memory-side cache, 256 MiB.  In us, W laid out anew and not, bfloat16:
+    //   32 x 1000 x 10007   53  64      60 x 4096 x 32769   384 302
+    //   60 x 1000 x 10007   58  71      80 x 4096 x 32769   391 391
+    //   60 x 256 x 50001    66  70      100 x 4096 x 32769  415 501
+    //   64 x 4096 x 16385  178 173      1000 x 1000 x 10007 115 147
+    // Over 21 sizes of 32 to 1000 rows in three types this rule takes the faster way
+    // or one within 4 % of it, but for float32, 64 x 1000 x 10007: 88 for 82.  (The
+    // plans' own times, summed over the products, take the slower one by 16 to 24 %
+    // at 32 to 60 rows of 1000 inputs.)
     l.pack_x = (twice && (run & RUN_DW)) || (l.held >= 64 && !whole_chunks(d.type, x));
     l.pack_w = l.held >= 64 && !whole_chunks(d.type, w) &&
                (d.rows > 64 || d.inputs * d.classes * l.e <= int64_t{128} << 20);

@@ -178,10 +178,17 @@ Linear8 linear8_of(const volta_op_linear8* in) {
   l.x_groups = d.group ? l.blocks : 1;
   const Operand x{d.rows, d.inputs, d.ld_x, 1}, w{d.outputs, d.inputs, d.ld_w, 1};
   l.fwd = shape_of(VOLTA_OP_E4M3, OP_NT, OP_LINEAR, d.rows, d.outputs, d.inputs, 1, 1, x, w);
-  // a launch of 3 us and two passes over the scales: for products of some size
+  // A launch of 3 us and two passes over the scales, for less time of every stage:
+  // for products of some size and many blocks of k.  (The plan's times are made of
+  // constants of 16-bit products; those of codes take 1.1 to 2.2 times them.)  In
+  // us, turned and not, rows x inputs x outputs to bfloat16 and to float32:
+  //   2048 x 4096 x 4096     41  44    64  64      8192 x 512 x 4096    50  48    65  62
+  //   4096 x 4096 x 4096     70  70   120 124      4096 x 512 x 16384   92  90   122 118
+  //   1024 x 16384 x 4096    81  87   131 133      8192 x 1024 x 8192  117 115   168 165
+  //   8192 x 4096 x 16384   533 589   930 987      1024 x 4096 x 4096   28  28    42  39
   const OpPlan plan = plan_of(VOLTA_OP_E4M3, l.fwd, true);
   l.rows_p = (d.rows + 31) / 32 * 32;
-  if (l.x_groups > 1 && plan.tile <= OP_TILE_128 && plan.us >= 40.0) l.turned_bytes = align256(4 * l.rows_p * l.blocks);
+  if (l.x_groups >= 16 && plan.tile <= OP_TILE_128 && plan.us >= 30.0) l.turned_bytes = align256(4 * l.rows_p * l.blocks);
   return l;
 }
 

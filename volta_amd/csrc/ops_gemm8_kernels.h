@@ -732,7 +732,10 @@ hipError_t launch8(const OpPlan& plan, OpGemmMore& g, hipStream_t st) {
     case OP_TILE_256X128:
       if (g.direct) e = launch8_middle<T, 256, 128, 4, 2, 1, 3>(g, st);
       break;
-    default:  // float32's fragments take more registers than that tile has
+    default:
+      // 256x256 of float32 results, whose fragments take more registers than that
+      // tile has, and of a last part of a block of k run on 256x128, in the same
+      // splits; what the plan weighed is the larger tile's time
       if constexpr (sizeof(T) < 4) {
         if (g.direct && g.K % 128 == 0) {
           e = launch8_large<T>(g, st);

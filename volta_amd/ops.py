@@ -201,8 +201,10 @@ def _matrix(name, type, rows, cols, ld=0):
         if m is None or m.__class__ is int:
             return m
         try:
-            if m.dtype is dtype and m.shape == shape and m.is_contiguous():
-                return m.data_ptr()
+            if m.dtype is dtype and m.is_contiguous():
+                # rows of rows too: a batch's matrices
+                if m.shape == shape or (shape and len(m.shape) > 2 and m.shape[-1] == cols and m.nbytes == nbytes):
+                    return m.data_ptr()
         except AttributeError:
             pass
         return compare(m)

@@ -46,8 +46,9 @@
  *     row's end and the next row's start (ld > length) are neither read nor
  *     written.
  *   - Sums are held in 32 bits; every result is rounded once, to the nearest
- *     of its type.  Runs are bit-reproducible: no sum's order depends on
- *     timing.
+ *     of its type.  What a call holds between its products in fewer bits (dp, dg
+ *     and du, dz, the update's X and G) is said there.  Runs are bit-reproducible:
+ *     no sum's order depends on timing.
  *   - rows is at most 2^30, every other size 2^21.  A product whose result is
  *     too large for a launch is refused: more than 2^22 of the tiles that its
  *     plan takes, so about 2^28 rows of up to 64 columns at the least.  A call
@@ -72,7 +73,7 @@ enum volta_op_type {
   VOLTA_OP_F32 = 0,
   VOLTA_OP_BF16 = 1,
   VOLTA_OP_F16 = 2,
-  VOLTA_OP_E4M3 = 3 /* output of the norm only: 8 bits, 4 of exponent, largest value 448 */
+  VOLTA_OP_E4M3 = 3 /* codes: 8 bits, 4 of exponent, largest value 448; as a type, of the norm's output alone */
 };
 
 /* Activations: enum volta_activation of volta_train.h without the row
@@ -336,7 +337,8 @@ int32_t volta_op_muon_orthogonalize(const volta_op_muon* d, const void* u, void*
 
 /* m_out = beta m + g;  u = g + beta m_out, or m_out without `nesterov`;  X from
  * u as above;  w_out = (1 - lr decay) w - lr scale X.  The momentum is float
- * whatever the type.  m_out may be m, and w_out may be w. */
+ * whatever the type.  m_out may be m, and w_out may be w.  lr to scale are values of
+ * the call, and a graph keeps those it was captured with. */
 int32_t volta_op_muon_step(const volta_op_muon* d, const void* g, const float* m, const void* w, float* m_out,
                            void* w_out, float lr, float beta, int32_t nesterov, float decay, float scale,
                            void* workspace, int64_t workspace_bytes, void* stream);

@@ -310,7 +310,7 @@ typedef struct volta_op_muon {
   int64_t ld_u;     /* [batch rows x cols], a matrix after the other: u or the gradient */
   int64_t ld_m;     /* the momentum */
   int64_t ld_o;     /* the result, or the weights before and after */
-  int32_t exact;    /* BF16: 0 or 1 (below); the other types are as with 1 */
+  int32_t exact;    /* BF16: 0 or 1 (below); the other types are always as with 1 */
 } volta_op_muon;
 
 int64_t volta_op_muon_workspace(const volta_op_muon* d);
@@ -322,12 +322,12 @@ int64_t volta_op_muon_workspace(const volta_op_muon* d);
  * in all directions, and the steps enlarge small ones, the usual five up to 484
  * times: X comes out 0.003 to 0.008 % of its norm off where u is of rank 1, and
  * 0.0001 % where it is noise.
- *   BF16 without `exact` holds each as one number, 11 bits, in a third of the
- * products' time.  Of u whose singular values are alike that is enough: of noise X is
+ *   BF16 of sides over 96 without `exact` holds each as one number, 11 bits, in a
+ * third of the products' time.  Of u whose singular values are alike that is enough: of noise X is
  * 0.04 to 0.18 % off, where rounding it to BF16 is 0.17 %.  What u has in a few directions
  * alone (a batch of fewer rows than the layer is wide) comes with noise in the
  * others, in percent of X's norm up to: rank 1 10, 4 7, 16 4.5, 64 2.5, a third of
- * the directions 3 (of sides under 100) to 1; singular values that fall as 1/i 0.4,
+ * the directions 2.6 (of sides of 100) to 1; singular values that fall as 1/i 0.4,
  * as 1/i^2 2, as 1/i^4 4.6; noise and four directions 5 times stronger 0.4, 50 times
  * 2.5, 500 times 7.
  *   A norm under a millionth of eps loses bits of u.  A matrix of zeros stays one;

@@ -1,6 +1,6 @@
 """The update by orthogonalised momentum (volta_amd.ops.Muon) of matrices of few
 directions and of far apart ones, whose small directions the steps enlarge most,
-on the GPU, held in two numbers and, in bfloat16 that is not to be exact, in one.
+on the GPU, held in two numbers and, in larger bfloat16 that is not to be exact, in one.
 
 Tolerances: limits in percent of the norm, whatever the kernels round.  Of two
 numbers 0.02 % before the result's rounding (what sums in 32 bits leave of matrices
@@ -58,7 +58,7 @@ SIZES = [(64, 64), (80, 1000), (104, 128), (300, 301), (512, 1024), (1000, 136),
 def test_orthogonalize(lib, t, m, n):
     op, one = ops.Muon(m, n, t, exact=True), ops.Muon(m, n, t)
     ws, o = space(lib, op), Mat(lib, t, m, n)
-    assert t == "bf16" or one.workspace_bytes() == op.workspace_bytes()
+    assert (t == "bf16" and min(m, n) > 96) or one.workspace_bytes() == op.workspace_bytes()
     for name, v in spectra(np.random.default_rng(m + n), m, n):
         say(t, m, n, name)
         v = R.unpack(R.pack(v, t), t)
@@ -67,7 +67,7 @@ def test_orthogonalize(lib, t, m, n):
         assert np.linalg.norm(o.get() - want) <= limit(t, want), name
         before = o.bits()
         one.orthogonalize(u, o, workspace=ws)
-        if t == "bf16":
+        if t == "bf16" and min(m, n) > 96:
             assert np.linalg.norm(o.get() - want) <= limit(t, want, 1.25 * ONE[name] / 100), name
         else:
             assert np.array_equal(o.bits(), before), name

@@ -17,7 +17,10 @@ def test_exact_bfloat16_is_held_as_the_other_types_are(m, n):
         return ops.Muon(m, n, t, **kw).workspace_bytes()
 
     assert space("bf16", exact=True) == space("f16") == space("f16", exact=True) == space("f32")
-    assert space("bf16") < space("bf16", exact=True)
+    if min(m, n) > 96:  # smaller ones always are
+        assert space("bf16") < space("bf16", exact=True)
+    else:
+        assert space("bf16") == space("bf16", exact=True)
 
 
 def test_other_values_refused():

@@ -26,26 +26,28 @@
 // them under 2^15: all 11 bits, and no element lost that is not 2^-29 of the
 // largest.
 //
-// float32, float16 and, with `exact`, bfloat16 hold each matrix as two such
-// numbers, 23 bits, and take three products, of all but the two rests: the product
-// left out is 2^-24 of the result, and the sums are chains of half as many
-// additions (of eight products) as those of float32's own matrix instruction, which
-// does a sixteenth of the work in the same time.
+// float32, float16, bfloat16 with `exact` and all sides of up to 96 hold each
+// matrix as two such numbers, 23 bits, and take three products, of all but the two
+// rests: the product left out is 2^-24 of the result, and the sums are chains of
+// half as many additions (of eight products) as those of float32's own matrix
+// instruction, which does a sixteenth of the work in the same time.
 //
-// bfloat16 without it holds them as one.  A rounding of X is noise in all
+// bfloat16 else holds them as one.  A rounding of X is noise in all
 // directions, 2^-12 / sqrt(3) of X's norm, and the steps enlarge small directions by
 // 3.4445 each.  Where u fills its directions evenly the result is 0.04 to 0.21 % of
 // its norm off, its rounding being 0.17 % (bfloat16's 8 bits in the products: 1.2 %).
 // Where it does not, the noise is what fills the others: 512 x 1024 of rank 1 9.6 %,
 // of rank 16 4.3, of rank 64 2.2, of 256 0.7; the whole of it goes by the second
-// number (0.002 % at rank 16).  That takes 4096 x 16384 from 3270 to 9150 us, 16 x
-// 512 x 2000 from 313 to 585, 1024 x 1024 from 159 to 197, so it is the caller's
-// choice.
+// number (0.002 % at rank 16).  That takes 4096 x 16384 from 3200 to 8900 us, 16 x
+// 512 x 2000 from 313 to 580, 1024 x 1024 from 156 to 195, so it is the caller's
+// choice; of sides of up to 96, whose small products are one launch in pairs, 64 x
+// 64 from 62 to 63, 96 x 16384 from 102 to 113, 24 x 64 x 4096 from 119 to 136, and
+// it is none.
 //
 // With one number the diagonals of G and the polynomials, nearly multiples of the
 // unit matrix, are all rounded one way, and where they are far larger than what is
-// beside them that is most of the error (noise of 30 x 576: 0.40 %, 0.07 without
-// it; 136 x 2200: 0.22 and 0.06).  At sides of up to 256 and of one to more than four
+// beside them that is most of the error (noise of 136 x 2200: 0.22 %, 0.06 without
+// it).  At sides of up to 256 and of one to more than four
 // what a diagonal is beyond its float16 is kept as a float32 and multiplied in the
 // epilogues, which read X and G once more for it.  Percent of the norm off before
 // the result's rounding, and us, with it and without:
@@ -183,7 +185,7 @@ int norm_blocks(int64_t batch, int64_t chunks) {
 // ---------------------------------------------------------------------------
 // The small products of a step, or of two at once, in one launch: a block for a
 // matrix whose smaller side is at most S, with G and the polynomials in LDS, as
-// pairs of float16 numbers for every type (nothing else reads them).  Each
+// pairs of float16 numbers.  Each
 // product is S x S x S, one row of 16x16 blocks a wave; what bounds it is one
 // latency after another (LDS, matrix instructions, barrier): the five products
 // of two steps take 13.7 us at S = 96, 6.6 at 64 and 4.2 at 32, one step's 5.0, 2.8
@@ -196,7 +198,6 @@ int norm_blocks(int64_t batch, int64_t chunks) {
 struct ChainArgs {
   const _Float16* g;
   _Float16* out;
-  float* diag;  // what the output's diagonal is beyond its float16; NULL: the output has two planes
   int64_t plane, stride, ld;
   int32_t side, pairs;
   // a product's sums times alpha, the sum's other matrix times beta, the diagonal:
@@ -266,10 +267,7 @@ __global__ void __launch_bounds__(512) muon_chain(ChainArgs a) {
           store4(&lds[to][1][m * LD + n], rest);
         } else if (m < a.side && n < a.side) {
           store4(out + m * a.ld + n, d);
-          if (!a.diag) store4(out + a.plane + m * a.ld + n, rest);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (a.diag && m == n + i) a.diag[blockIdx.x * (int64_t)a.side + m] = rest[i];
+          store4(out + a.plane + m * a.ld + n, rest);
         }
       }
     }
@@ -304,7 +302,7 @@ struct Muon {
   bool tall, pairs;        // pairs: two steps at once
   bool chain;              // the small products in one launch
   bool diag;               // the diagonals' rests are kept
-  int planes;              // of X and the products; bfloat16 that is not to be exact: 1
+  int planes;              // of X and the products; of larger bfloat16 that is not to be exact: 1
   int64_t rows_p, cols_p;  // padded to whole chunks: the products run over zeros there
   int64_t small, large;
   int64_t ld_x, ld_small;
@@ -338,12 +336,13 @@ Muon muon_of(const volta_op_muon* in) {
   d.ld_m = ld_of("ld_m", d.ld_m, d.cols);
   d.ld_o = ld_of("ld_o", d.ld_o, d.cols);
   if (d.exact != 0 && d.exact != 1) refuse("exact is " + std::to_string(d.exact) + ", must be 0 or 1");
-  l.planes = d.type == VOLTA_OP_BF16 && !d.exact ? 1 : 2;
   l.rows_p = packed_ld(VOLTA_OP_F16, d.rows);
   l.cols_p = packed_ld(VOLTA_OP_F16, d.cols);
   l.tall = d.rows > d.cols;
   l.small = l.tall ? l.cols_p : l.rows_p;
   l.large = l.tall ? l.rows_p : l.cols_p;
+  l.chain = l.small <= kChainSide;
+  l.planes = d.type == VOLTA_OP_BF16 && !d.exact && !l.chain ? 1 : 2;
   // Singular values before each step are at most r: 1 at first (the sum of
   // squares of X is at most 1), then the largest |a s + b s^3 + c s^5| on [0, r]
   // (at the ends and between, by 4096 samples and a margin for what lies
@@ -376,7 +375,6 @@ Muon muon_of(const volta_op_muon* in) {
     l.partial_bytes = std::max(l.partial_bytes, align256(op_gemm_partial_bytes(l.plan[i], OP_BLEND, M[i], N[i], (int)d.batch)));
     if (op_gemm_blocks(l.plan[i], OP_BLEND, M[i], N[i]) * d.batch > kMaxBlocks) refuse("the rows and columns of a product are too many");
   }
-  l.chain = l.small <= kChainSide;
   l.diag = l.planes == 1 && (l.small <= 256 || l.large > 4 * l.small);
   const double one = l.plan[0].us + l.plan[1].us + l.plan[2].us;
   const double two = l.plan[0].us + 5.0 * l.plan[1].us + l.plan[2].us;
@@ -384,7 +382,7 @@ Muon muon_of(const volta_op_muon* in) {
   l.ld_x = line_ld(2, l.cols_p);
   l.ld_small = line_ld(2, l.small);
   l.x_bytes = align256(d.batch * l.rows_p * l.ld_x * 2 * l.planes);
-  l.g_bytes = align256(d.batch * l.small * l.ld_small * 2 * (l.chain ? 2 : l.planes));
+  l.g_bytes = align256(d.batch * l.small * l.ld_small * 2 * l.planes);
   l.diag_bytes = l.diag ? align256(d.batch * l.small * 4) : 0;
   l.parts = norm_blocks(d.batch, d.rows * ((d.cols + 3) / 4));
   l.sum_bytes = align256(8 * d.batch * l.parts);
@@ -470,8 +468,8 @@ void run(const Muon& l, MuonArgs a, const OpEpilogueMore& last, char* workspace,
   auto to_small = [&](char* out, double alpha) {
     OpEpilogueMore o{};
     o.out[0] = out;
-    o.out_type = l.chain ? OP_PLANES : out_type;
-    o.diag_out = l.chain ? nullptr : diag_of(out);
+    o.out_type = out_type;
+    o.diag_out = diag_of(out);
     o.stride_diag = l.small;
     o.ld_out = l.ld_small;
     o.stride_out = g_size;
@@ -513,7 +511,6 @@ void run(const Muon& l, MuonArgs a, const OpEpilogueMore& last, char* workspace,
       ChainArgs c{};
       c.g = reinterpret_cast<const _Float16*>(small[0]);
       c.out = reinterpret_cast<_Float16*>(small[1]);
-      c.diag = diag_of(small[1]);
       c.plane = g_plane;
       c.stride = g_size;
       c.ld = l.ld_small;

@@ -465,9 +465,9 @@ class Muon(_Operator):
     """The update by orthogonalised momentum, of `batch` matrices [rows x cols]
     one after the other: X = u / (|u| + eps), `steps` times X = a X + (b G + c
     G^2) X with G = X X^T (of the smaller side), coefficients = (a, b, c).
-    exact: of "bf16", whose X is otherwise some percent of its norm off where u
-    has a few directions alone, as exact as the other types, in up to three
-    times the time."""
+    exact: of "bf16" with both sides over 96, whose X is otherwise some percent of
+    its norm off where u has a few directions alone, as exact as the other types,
+    in up to three times the time."""
 
     def __init__(self, rows, cols, dtype="f32", batch=1, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7,
                  ld_u=0, ld_m=0, ld_o=0, exact=False, lib=None):

@@ -222,8 +222,8 @@ int64_t volta_op_cross_entropy_workspace(const volta_op_cross_entropy* d, int32_
  * both (lse alone takes no labels).  bias [classes] may be NULL; a -inf in it
  * takes its class out.  z, its exponentials' sums and both results are held in
  * 32 bits; of 16-bit types the exponentials are the hardware's, a few units of the
- * last place each, which leaves loss and lse some 1e-7 of themselves off.  A row with a z of +inf or NaN, and one whose z are all -inf, has a
- * loss of NaN. */
+ * last place each, which leaves loss and lse some 1e-7 of themselves off.  A row
+ * with a z of +inf or NaN, and one whose z are all -inf, has a loss of NaN. */
 int32_t volta_op_cross_entropy_forward(const volta_op_cross_entropy* d, const void* x, const void* w,
                                        const void* bias, const int32_t* labels, float* loss, float* lse,
                                        void* workspace, int64_t workspace_bytes, void* stream);

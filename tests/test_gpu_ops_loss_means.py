@@ -14,8 +14,9 @@ import pytest
 from tests import ops_ref as R
 from tests.ops_graph import Captured, put, spoil
 from tests.ops_ref import HALF, TYPES, Mat
-from tests.test_gpu_ops import Space, draws, say
+from tests.test_gpu_ops import STORE, Space, _forms, draws, say
 from tests.test_gpu_ops_loss import Words
+from tests.test_gpu_ops_tiles import SHAPES, Product
 from volta_amd import load_hip, ops
 
 pytestmark = pytest.mark.gpu
@@ -135,3 +136,17 @@ def test_the_largest_of_many_rows(lib, t):
         if t != "f16":  # subnormal gradients are rounded otherwise
             assert all(np.array_equal(m.get(), R.unpack(first[n].view(R.STORE[t]), t) * scale) for n, m in p.out.items())
     graph.close()
+
+
+def test_units_of_bfloat16_on_every_tile(lib):
+    """Sums of whole numbers times a power of two: exact up to the result's rounding."""
+    for layout, kind, tile, direct in _forms("bf16"):
+        if kind != STORE:
+            continue
+        for n, (M, K, N) in enumerate(SHAPES):
+            for splits, unit in ((1, 2.0**-7), (3, 2.0**3)):
+                say("layout", layout, "tile", tile, "direct", direct, M, K, N, "splits", splits)
+                x = Product(lib, "bf16", layout, kind, direct, M, K, N, np.random.default_rng(3000 * n + splits))
+                out = x.mat(x.dims[0], x.dims[2])
+                x.run(tile, splits, out, unit=Mat(lib, "f32", 1, 1, np.array([[unit]])))
+                x.same(out, x.sums()[0] * unit, "sums")
